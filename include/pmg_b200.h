@@ -485,6 +485,61 @@ int pmg_refiner_level_info(pmg_refiner* r, int32_t level, int64_t* capacity, int
  * "zmin", "logz", "delta", "prompt". Returns NULL for an unknown name. */
 void* pmg_refiner_debug_ptr(pmg_refiner* r, const char* what, int32_t level);
 
+/* --------------------------------------------------------------------------------------------------------------
+ * Token operators: the layers of a transformer block over packed tokens (16-bit floating point).
+ * The reference runs its encoder's blocks through torch; these entry points have no counterpart file in it.
+ *
+ * Strides are in elements.  `dtype` is a pmg_dtype.  `status` receives PMG_ERR_TIMEOUT / PMG_ERR_RANGE as above and may
+ * be NULL.  Tensors of a call do not overlap unless its comment says so.
+ * ------------------------------------------------------------------------------------------------------------ */
+enum pmg_dtype { PMG_F32 = 0, PMG_F16 = 1, PMG_BF16 = 2 };
+enum pmg_activation { PMG_ACT_NONE = 0, PMG_ACT_RELU = 1, PMG_ACT_SILU = 2, PMG_ACT_GELU = 3 /* erf form */ };
+
+/* y = act(x W^T + bias) + residual.  x [M,K] (row stride ldx), w [N,K], bias [N] or NULL, residual [M,N] or NULL, all of
+ * `dtype` (F16 or BF16); y, and the residual with it, are fp32 when out_f32 is set.  pre, when given, receives
+ * x W^T + bias in `dtype`, which pmg_linear_grad takes.  Sums are fp32.  Any M >= 0, N >= 1, K >= 1 and strides; rows of
+ * x and w that do not start on 16-byte boundaries are first copied to the workspace (pack_x / pack_w: pointer or
+ * 2 * stride not a multiple of 16).  y may be the residual itself.  workspace: 16-byte aligned. */
+size_t pmg_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t pack_x, int32_t pack_w);
+int pmg_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t dtype, int64_t M, int64_t N, int64_t K,
+               const void* bias, int32_t act, const void* residual, int64_t ldr, int32_t out_f32, void* y, int64_t ldy,
+               void* pre, int64_t ldp, void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+
+/* Gradients of pmg_linear: with dz = dy act'(pre), dx [M,K] = dz W, dw [N,K] = dz^T x, db [N] = column sums of dz, each
+ * of `dtype` and each optional (NULL).  The residual's gradient is dy.  pre is not read for PMG_ACT_NONE.  With M = 0,
+ * dw and db are zeroed.  No atomics: equal inputs give equal bits. */
+size_t pmg_linear_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t act, int32_t pack_dy, int32_t pack_x,
+                                       int32_t pack_w, int32_t bias_grad);
+int pmg_linear_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                    int32_t dtype, int64_t M, int64_t N, int64_t K, const void* pre, int64_t ldp, int32_t act, void* dx,
+                    int64_t lddx, void* dw, int64_t lddw, void* db, void* workspace, size_t workspace_bytes,
+                    int32_t* status, void* stream);
+
+/* Queries q [T,Hq,D] and keys k [T,Hk,D] (F32, F16 or BF16; strides of token and head, values of a head contiguous),
+ * each head scaled to unit root mean square (eps inside the root), times its weight [D] fp32 (NULL: ones), then the
+ * first `rot` values rotated by the angles of the token's position: cos, sin [places][rot/2] fp32, positions [T] int32
+ * (NULL: 0, 1, 2, ...).  Pairs are (i, i + rot/2), or (2i, 2i + 1) when interleaved.  A position outside
+ * [0, places) sets PMG_ERR_RANGE in `status` and is taken as 0.  Outputs may be the inputs (in place) or rows of a
+ * cache.  D <= 256, rot even. */
+int pmg_qk_norm_rope(const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok, int64_t k_head,
+                     int32_t dtype, int64_t T, int32_t Hq, int32_t Hk, int32_t D, int32_t rot, const float* q_weight,
+                     const float* k_weight, const float* cos, const float* sin, int32_t places,
+                     const int32_t* positions, float eps, int32_t interleaved, void* q_out, int64_t qo_tok,
+                     int64_t qo_head, void* k_out, int64_t ko_tok, int64_t ko_head, int32_t* status, void* stream);
+
+/* Its gradients: dq, dk are those of the outputs, q, k the inputs of the forward call; q_grad, k_grad receive the
+ * inputs' (they may be dq, dk), q_weight_grad, k_weight_grad [D] fp32 (NULL: not wanted) the weights', summed over
+ * tokens and heads in a fixed order. */
+size_t pmg_qk_norm_rope_grad_workspace_bytes(int32_t D);
+int pmg_qk_norm_rope_grad(const void* dq, int64_t dq_tok, int64_t dq_head, const void* dk, int64_t dk_tok,
+                          int64_t dk_head, const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok,
+                          int64_t k_head, int32_t dtype, int64_t T, int32_t Hq, int32_t Hk, int32_t D, int32_t rot,
+                          const float* q_weight, const float* k_weight, const float* cos, const float* sin,
+                          int32_t places, const int32_t* positions, float eps, int32_t interleaved, void* q_grad,
+                          int64_t qo_tok, int64_t qo_head, void* k_grad, int64_t ko_tok, int64_t ko_head,
+                          float* q_weight_grad, float* k_weight_grad, void* workspace, size_t workspace_bytes,
+                          int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -98,6 +98,16 @@ SIGNATURES = {
     "pmg_refiner_launches_per_step": (I32, [P]),
     "pmg_refiner_level_info": (I32, [P, I32, C.POINTER(I64), C.POINTER(I32), C.POINTER(I32), C.POINTER(I32)]),
     "pmg_refiner_debug_ptr": (P, [P, C.c_char_p, I32]),
+    "pmg_linear_workspace_bytes": (SZ, [I64, I64, I64, I32, I32]),
+    "pmg_linear": (I32, [P, I64, P, I64, I32, I64, I64, I64, P, I32, P, I64, I32, P, I64, P, I64, P, SZ, P, P]),
+    "pmg_linear_grad_workspace_bytes": (SZ, [I64, I64, I64, I32, I32, I32, I32, I32]),
+    "pmg_linear_grad": (I32, [P, I64, P, I64, P, I64, I32, I64, I64, I64, P, I64, I32, P, I64, P, I64, P, P, SZ, P,
+                              P]),
+    "pmg_qk_norm_rope": (I32, [P, I64, I64, P, I64, I64, I32, I64, I32, I32, I32, I32, P, P, P, P, I32, P, F32, I32,
+                               P, I64, I64, P, I64, I64, P, P]),
+    "pmg_qk_norm_rope_grad_workspace_bytes": (SZ, [I32]),
+    "pmg_qk_norm_rope_grad": (I32, [P, I64, I64, P, I64, I64, P, I64, I64, P, I64, I64, I32, I64, I32, I32, I32, I32,
+                                    P, P, P, P, I32, P, F32, I32, P, I64, I64, P, I64, I64, P, P, P, SZ, P, P]),
 }
 
 STATUS = {0: "ok", 1: "bad argument", 2: "CUDA runtime error", 3: "hash table full", 4: "level capacity overflow",

@@ -31,7 +31,7 @@
 #include <algorithm>
 #include <mutex>
 
-#include "tc_common.cuh"
+#include "tok_common.cuh"
 
 namespace pmg {
 
@@ -713,6 +713,25 @@ int make_tensor_map(CUtensorMap* map, const void* base, uint64_t rows, uint64_t 
     const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
                           CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? PMG_OK : PMG_ERR_BAD_ARG;
+}
+
+int make_tensor_map16(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,
+                      const uint32_t* box) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return PMG_ERR_UNSUPPORTED;
+    if (reinterpret_cast<uintptr_t>(base) & 15) return PMG_ERR_BAD_ARG;
+    cuuint64_t d[3], st[2];
+    cuuint32_t b[3], estr[3] = {1, 1, 1};
+    for (int i = 0; i < rank; ++i) {
+        if (dims[i] == 0) return PMG_ERR_BAD_ARG;
+        d[i] = dims[i];
+        b[i] = box[i];
+        if (i) st[i - 1] = strides[i - 1];
+    }
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, (cuuint32_t)rank, const_cast<void*>(base), d, st, b, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? PMG_OK : PMG_ERR_BAD_ARG;
 }
 

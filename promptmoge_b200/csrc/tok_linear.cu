@@ -1,0 +1,1022 @@
+// Linear layer with everything behind the product fused into its epilogue, and its gradients.
+//
+//   z = x W^T + b,   y = act(z) + r          x [M, K], W [N, K], r and y [M, N]; act: none, relu, silu, gelu (erf)
+//   dz = dy act'(z), dx = dz W, dW = dz^T x, db = sum over rows of dz     (dr is dy itself)
+//
+// Three kernels do the products.
+//   k_rows    up to 32 rows: bound by one read of W.  A block owns 16 output columns, its warps split K; mma.sync with W
+//             as the 16-row operand, every lane's 16-byte load feeding two instructions (a dot product does not mind the
+//             order of K, so no shuffle or shared-memory transpose is needed).
+//   k_gemm    everything larger: tcgen05 with 128 x BN tiles, TMA ring, accumulators double-buffered in tensor memory so
+//             that the epilogue of one tile runs under the next tile's products.
+//   k_split_sum   the last wave of tiles, when it would leave most SMs idle, is cut along K into fp32 partials that this
+//             kernel adds in split order (no atomics: results do not depend on timing) and takes through the epilogue.
+// dz is rounded to the operands' 16-bit type before its two products (tensor cores take no other), db is summed from the
+// unrounded fp32 values.
+#include <algorithm>
+
+#include "tok_common.cuh"
+
+namespace pmg {
+namespace {
+
+using namespace tok;
+
+// ----------------------------------------------------------------------------------------------------------------- //
+// Activations
+// ----------------------------------------------------------------------------------------------------------------- //
+
+// Phi(x) - 1/2 = x p(t), t = 2 x^2 / 25 - 1 on |x| <= 5: the degree-11 polynomial of least largest |x (p - exact)| by
+// iteratively reweighted least squares in the Chebyshev basis, constant term raised so that Phi saturates to exactly 0
+// and 1 at the ends.  |error| <= 2.1e-6 evaluated in fp32, 9.3e-6 of x Phi(x); erff in its place costs the epilogue
+// about three times as many instructions, and no output type here resolves more than 2^-11.
+__device__ constexpr float kPhi[12] = {1.41363868e-01f, -7.02976871e-02f, 5.15348489e-02f, -4.04097587e-02f,
+                                       3.12585325e-02f, -2.34790368e-02f, 1.72561175e-02f, -1.06230432e-02f,
+                                       4.62778831e-03f, -3.28729113e-03f, 3.42820314e-03f, -1.37248793e-03f};
+
+__device__ __forceinline__ float fma_sat(float a, float b, float c) {
+    float r;
+    asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+__device__ __forceinline__ void gelu_pair(float& a, float& b) {
+    const float ca = fminf(fmaxf(a, -5.0f), 5.0f), cb = fminf(fmaxf(b, -5.0f), 5.0f);
+    const uint64_t c = pack2(ca, cb);
+    const uint64_t t = fma2(mul2(c, c), pack2(0.08f, 0.08f), pack2(-1.0f, -1.0f));
+    uint64_t p = pack2(kPhi[11], kPhi[11]);
+#pragma unroll
+    for (int i = 10; i >= 0; --i) p = fma2(p, t, pack2(kPhi[i], kPhi[i]));
+    const float2 f = unpack2(p);
+    a *= fma_sat(ca, f.x, 0.5f);
+    b *= fma_sat(cb, f.y, 0.5f);
+}
+
+__device__ __forceinline__ void activate_pair(int act, float& a, float& b) {
+    if (act == PMG_ACT_GELU) {
+        gelu_pair(a, b);
+    } else if (act == PMG_ACT_SILU) {
+        a *= rcp_approx(1.0f + ex2(-a * kLog2e));
+        b *= rcp_approx(1.0f + ex2(-b * kLog2e));
+    } else if (act == PMG_ACT_RELU) {
+        a = max_nan(a, 0.0f);
+        b = max_nan(b, 0.0f);
+    }
+}
+
+__device__ __forceinline__ float act_slope(int act, float z) {
+    if (act == PMG_ACT_GELU) {
+        const float phi = 0.5f * (1.0f + erff(z * 0.70710678f));
+        return phi + z * 0.39894228f * expf(-0.5f * z * z);
+    }
+    if (act == PMG_ACT_SILU) {
+        const float g = __fdividef(1.0f, 1.0f + expf(-z));
+        return g * (1.0f + z * (1.0f - g));
+    }
+    if (act == PMG_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+    return 1.0f;
+}
+
+// ----------------------------------------------------------------------------------------------------------------- //
+// The epilogue's destination
+// ----------------------------------------------------------------------------------------------------------------- //
+struct Out {
+    const void* bias;        // [N] of the operands' type, or null
+    const void* resid;       // [M, N] of y's type, or null
+    void* y;
+    void* pre;               // z of the operands' type, or null
+    int64_t ldr, ldy, ldp;
+    int act;
+    int f32;                 // y and the residual are fp32, else the operands' type
+    int vec;                 // rows of y, resid and pre start on 16-byte boundaries
+};
+
+// 8 values z[0..7] of row m from column n on: bias, activation, residual, stores.  Used where rows are not staged.
+template <typename T>
+__device__ __forceinline__ void finish8(const Out& o, int64_t m, int n, int N, float (&z)[8]) {
+    const int cnt = min(8, N - n);
+    if (o.bias) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < cnt) z[i] += Elem<T>::to(static_cast<const T*>(o.bias)[n + i]);
+    }
+    const bool vec = o.vec && cnt == 8;
+    if (o.pre) {
+        T* p = static_cast<T*>(o.pre) + m * o.ldp + n;
+        if (vec) {
+            *reinterpret_cast<uint4*>(p) = make_uint4(Elem<T>::pack(z[0], z[1]), Elem<T>::pack(z[2], z[3]),
+                                                      Elem<T>::pack(z[4], z[5]), Elem<T>::pack(z[6], z[7]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < cnt) p[i] = Elem<T>::from(z[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) activate_pair(o.act, z[i], z[i + 1]);
+    if (o.f32) {
+        if (o.resid) {
+            const float* r = static_cast<const float*>(o.resid) + m * o.ldr + n;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < cnt) z[i] += r[i];
+        }
+        float* p = static_cast<float*>(o.y) + m * o.ldy + n;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < cnt) p[i] = z[i];
+        return;
+    }
+    if (o.resid) {
+        const T* r = static_cast<const T*>(o.resid) + m * o.ldr + n;
+        if (vec) {
+            const uint4 v = *reinterpret_cast<const uint4*>(r);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = Elem<T>::unpack(w[i]);
+                z[2 * i] += f.x;
+                z[2 * i + 1] += f.y;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < cnt) z[i] += Elem<T>::to(r[i]);
+        }
+    }
+    T* p = static_cast<T*>(o.y) + m * o.ldy + n;
+    if (vec) {
+        *reinterpret_cast<uint4*>(p) = make_uint4(Elem<T>::pack(z[0], z[1]), Elem<T>::pack(z[2], z[3]),
+                                                  Elem<T>::pack(z[4], z[5]), Elem<T>::pack(z[6], z[7]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < cnt) p[i] = Elem<T>::from(z[i]);
+    }
+}
+
+// ----------------------------------------------------------------------------------------------------------------- //
+// Few rows
+// ----------------------------------------------------------------------------------------------------------------- //
+template <typename T>
+__device__ __forceinline__ void mma_16n8k16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                            uint32_t b0, uint32_t b1) {
+    if constexpr (Elem<T>::kFmt == 1)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 8 values of a row from column k on, zero beyond K or for an absent row.
+template <bool ALIGNED>
+__device__ __forceinline__ uint4 row8(const uint16_t* row, int k, int K, bool on) {
+    if constexpr (ALIGNED) {
+        return on && k < K ? *reinterpret_cast<const uint4*>(row + k) : make_uint4(0, 0, 0, 0);
+    } else {
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (on && k + i < K) w[i >> 1] |= (uint32_t)row[k + i] << (16 * (i & 1));
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+constexpr int kRowsCols = 16;
+
+// NT groups of 8 rows; ALIGNED: K % 8 == 0 and rows on 16-byte boundaries.
+template <typename T, int NT, bool ALIGNED>
+__global__ void __launch_bounds__(512) k_rows(const uint16_t* __restrict__ x, int64_t ldx,
+                                              const uint16_t* __restrict__ w, int64_t ldw, int M, int N, int K, Out o) {
+    pdl_begin();
+    extern __shared__ float part[];                  // [warps][16 columns][8 NT rows]
+    const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, q = lane & 3;
+    const int n0 = blockIdx.x * kRowsCols;
+    const uint16_t* w0 = w + (int64_t)(n0 + g) * ldw;
+    const uint16_t* w1 = w0 + 8 * ldw;
+    const bool on0 = n0 + g < N, on1 = n0 + g + 8 < N;
+    float acc[NT][4] = {};
+    constexpr int U = NT <= 2 ? 4 : 2;
+    for (int k0 = warp * 32; k0 < K; k0 += warps * 32 * U) {
+        uint4 a[U], b[U], v[U][NT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = k0 + u * warps * 32 + 8 * q;
+            a[u] = row8<ALIGNED>(w0, k, K, on0);
+            b[u] = row8<ALIGNED>(w1, k, K, on1);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) v[u][t] = row8<ALIGNED>(x + (int64_t)(8 * t + g) * ldx, k, K, 8 * t + g < M);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                mma_16n8k16<T>(acc[t], a[u].x, b[u].x, a[u].y, b[u].y, v[u][t].x, v[u][t].y);
+                mma_16n8k16<T>(acc[t], a[u].z, b[u].z, a[u].w, b[u].w, v[u][t].z, v[u][t].w);
+            }
+    }
+    float* mine = part + warp * (kRowsCols * 8 * NT);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int m = 8 * t + 2 * q;
+        mine[m * kRowsCols + g] = acc[t][0];
+        mine[(m + 1) * kRowsCols + g] = acc[t][1];
+        mine[m * kRowsCols + g + 8] = acc[t][2];
+        mine[(m + 1) * kRowsCols + g + 8] = acc[t][3];
+    }
+    __syncthreads();
+    // one thread per row and pair of columns
+    for (int i = threadIdx.x; i < 8 * NT * (kRowsCols / 2); i += blockDim.x) {
+        const int m = i / (kRowsCols / 2), c = (i % (kRowsCols / 2)) * 2, n = n0 + c;
+        if (m >= M || n >= N) continue;
+        float z[2] = {0.0f, 0.0f};
+        for (int s = 0; s < warps; ++s) {
+            const float2 p = *reinterpret_cast<const float2*>(part + s * (kRowsCols * 8 * NT) + m * kRowsCols + c);
+            z[0] += p.x;
+            z[1] += p.y;
+        }
+        const bool two = n + 1 < N;
+        if (o.bias) {
+            z[0] += Elem<T>::to(static_cast<const T*>(o.bias)[n]);
+            if (two) z[1] += Elem<T>::to(static_cast<const T*>(o.bias)[n + 1]);
+        }
+        if (o.pre) {
+            T* p = static_cast<T*>(o.pre) + m * o.ldp + n;
+            p[0] = Elem<T>::from(z[0]);
+            if (two) p[1] = Elem<T>::from(z[1]);
+        }
+        activate_pair(o.act, z[0], z[1]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            if (e && !two) break;
+            float v = z[e];
+            if (o.f32) {
+                if (o.resid) v += static_cast<const float*>(o.resid)[m * o.ldr + n + e];
+                static_cast<float*>(o.y)[m * o.ldy + n + e] = v;
+            } else {
+                if (o.resid) v += Elem<T>::to(static_cast<const T*>(o.resid)[m * o.ldr + n + e]);
+                static_cast<T*>(o.y)[m * o.ldy + n + e] = Elem<T>::from(v);
+            }
+        }
+    }
+}
+
+// ----------------------------------------------------------------------------------------------------------------- //
+// Tiles
+// ----------------------------------------------------------------------------------------------------------------- //
+constexpr int kBM = 128, kBK = 64;
+constexpr int kEpiWarps = 8, kFirstEpi = 4;
+constexpr int kGemmThreads = 32 * (kFirstEpi + kEpiWarps);
+
+template <int BN>
+struct Cfg {
+    static constexpr int kA = kBM * kBK * 2, kB = BN * kBK * 2, kStage = kA + kB;
+    static constexpr int kStages = 196608 / kStage > 8 ? 8 : 196608 / kStage;
+    static constexpr int kStaging = kEpiWarps * 4096;          // 32 rows of 128 bytes a warp
+    static constexpr int kBias = kEpiWarps * 64 * 4;
+    static constexpr int kBars = kStages * kStage + kStaging + kBias;
+    static constexpr int kSmem = kBars + 256;
+};
+
+// What a CTA walks: units 0 .. full-1 are whole tiles, the rest (tile, split) pairs of the remaining tiles.
+struct Sched {
+    int tiles_n, tiles, full, splits, units, kblocks, kper;
+    float* part;            // [units - full][128][BN]
+};
+
+struct Unit {
+    int m0, n0, kb0, kb1, slot;      // slot < 0: a whole tile
+};
+
+template <int BN>
+__device__ __forceinline__ Unit unit_of(const Sched& s, int u) {
+    Unit r;
+    int tile = u;
+    r.kb0 = 0;
+    r.kb1 = s.kblocks;
+    r.slot = -1;
+    if (u >= s.full) {
+        r.slot = u - s.full;
+        tile = s.full + r.slot / s.splits;
+        r.kb0 = (r.slot % s.splits) * s.kper;
+        r.kb1 = min(r.kb0 + s.kper, s.kblocks);
+    }
+    r.m0 = (tile / s.tiles_n) * kBM;
+    r.n0 = (tile % s.tiles_n) * BN;
+    return r;
+}
+
+template <typename T, int BN, bool AMN, bool BMN>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+    k_gemm(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, const int M, const int N,
+           const __grid_constant__ Sched sched, const __grid_constant__ Out o, int32_t* status) {
+    using C = Cfg<BN>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::kBars);
+    uint64_t* empty = full + C::kStages;
+    uint64_t* acc_full = empty + C::kStages;       // 2
+    uint64_t* acc_empty = acc_full + 2;            // 2
+    uint64_t* drain = acc_empty + 2;
+    uint32_t* slot = reinterpret_cast<uint32_t*>(drain + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::kStages; ++i) {
+            mbar_init(full + i, 1);
+            mbar_init(empty + i, 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(acc_full + i, 1);
+            mbar_init(acc_empty + i, 32 * kEpiWarps);
+        }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 1) tmem_alloc(slot, 2 * BN);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *slot;
+    pdl_begin();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t it = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; u < sched.units && ok; u += gridDim.x) {
+                const Unit t = unit_of<BN>(sched, u);
+                for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
+                    const int st = it % C::kStages;
+                    if (!mbar_wait(empty + st, ((it / C::kStages) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                    mbar_arrive_expect_tx(full + st, C::kStage);
+                    const uint32_t a = smem_u32(smem + st * C::kStage), b = a + C::kA;
+                    if constexpr (AMN) {
+#pragma unroll
+                        for (int i = 0; i < kBM / 64; ++i) tma_tile2d(a + i * 8192, &ma, t.m0 + 64 * i, kb * kBK, full + st);
+                    } else {
+                        tma_tile2d(a, &ma, kb * kBK, t.m0, full + st);
+                    }
+                    if constexpr (BMN) {
+#pragma unroll
+                        for (int i = 0; i < BN / 64; ++i) tma_tile2d(b + i * 8192, &mb, t.n0 + 64 * i, kb * kBK, full + st);
+                    } else {
+                        tma_tile2d(b, &mb, kb * kBK, t.n0, full + st);
+                    }
+                }
+            }
+            if (!ok) {
+                *abort_flag = 1;
+                flag(status, PMG_ERR_TIMEOUT);
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = idesc16(Elem<T>::kFmt, kBM, BN, AMN, BMN);
+            uint32_t it = 0, k = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; u < sched.units && ok; u += gridDim.x, ++k) {
+                const Unit t = unit_of<BN>(sched, u);
+                const uint32_t buf = k & 1u, d = tmem + buf * BN;
+                if (!mbar_wait(acc_empty + buf, ((k >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                tc_fence_after();
+                for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
+                    const int st = it % C::kStages;
+                    if (!mbar_wait(full + st, (it / C::kStages) & 1u, abort_flag)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t a = smem_u32(smem + st * C::kStage), b = a + C::kA;
+#pragma unroll
+                    for (int kk = 0; kk < kBK / 16; ++kk)
+                        mma16(d, desc16(AMN ? a + kk * 2048 : a + kk * 32, AMN ? 8192 : 16),
+                              desc16(BMN ? b + kk * 2048 : b + kk * 32, BMN ? 8192 : 16), idesc,
+                              (kb > t.kb0 || kk > 0) ? 1u : 0u);
+                    mma_commit(empty + st);
+                }
+                if (ok) mma_commit(acc_full + buf);
+            }
+            if (!ok) flag(status, PMG_ERR_TIMEOUT);
+            if (!ok || *abort_flag) {
+                *abort_flag = 1;
+                drain_mma(drain);
+            }
+        }
+    } else if (warp >= kFirstEpi) {
+        const int ew = warp - kFirstEpi, quarter = warp & 3, group = ew >> 2;
+        uint8_t* stage = smem + C::kStages * C::kStage + ew * 4096;
+        float* bias_s = reinterpret_cast<float*>(smem + C::kStages * C::kStage + C::kStaging) + ew * 64;
+        const int srow = lane >> 3, sch = lane & 7;           // coalesced side: 4 rows x 8 chunks of 16 bytes
+        uint32_t k = 0;
+        bool ok = true;
+        for (int u = blockIdx.x; u < sched.units; u += gridDim.x, ++k) {
+            const Unit t = unit_of<BN>(sched, u);
+            const uint32_t buf = k & 1u;
+            const int mw = t.m0 + quarter * 32;               // this warp's first row
+            const bool whole = t.slot < 0;
+            const bool wide = !whole || o.f32;                // 32 columns of 4 bytes, else 64 of 2, per 128-byte row
+            const int cols = wide ? 32 : 64, n_end = min(N - t.n0, BN);
+            bool waited = false;
+            for (int c0 = group * cols; c0 < BN; c0 += 2 * cols) {
+                const int n = t.n0 + c0;
+                uint4 res[8];
+                const bool add = whole && o.resid && c0 < n_end;
+                if (add) {                                    // residual rows, coalesced, ahead of the accumulators
+                    const int esz = o.f32 ? 4 : 2, per = 16 / esz;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int m = mw + 4 * i + srow, nn = n + sch * per;
+                        res[i] = make_uint4(0, 0, 0, 0);
+                        if (m < M && nn < N) {
+                            const uint8_t* p = static_cast<const uint8_t*>(o.resid) + ((int64_t)m * o.ldr + nn) * esz;
+                            if (o.vec && nn + per <= N) {
+                                res[i] = *reinterpret_cast<const uint4*>(p);
+                            } else {
+                                uint32_t* w = reinterpret_cast<uint32_t*>(&res[i]);
+                                if (esz == 4) {
+                                    for (int e = 0; e < 4; ++e)
+                                        if (nn + e < N) w[e] = reinterpret_cast<const uint32_t*>(p)[e];
+                                } else {
+                                    for (int e = 0; e < 8; ++e)
+                                        if (nn + e < N)
+                                            w[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[e] << (16 * (e & 1));
+                                }
+                            }
+                        }
+                    }
+                }
+                if (whole && o.bias) {
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int nn = n + lane + 32 * i;
+                        bias_s[lane + 32 * i] = (lane + 32 * i < cols && nn < N) ? Elem<T>::to(static_cast<const T*>(o.bias)[nn]) : 0.0f;
+                    }
+                }
+                if (!waited) {
+                    waited = true;
+                    ok = __all_sync(0xffffffffu, mbar_wait(acc_full + buf, (k >> 1) & 1u, abort_flag));
+                    if (!ok) break;
+                    tc_fence_after();
+                }
+                if (c0 >= n_end) continue;                    // columns beyond the matrix
+                const uint32_t src = tmem + ((uint32_t)(quarter * 32) << 16) + buf * BN + c0;
+                float v[64];
+                tmem_ld32(src, reinterpret_cast<uint32_t*>(v));
+                if (!wide) tmem_ld32(src + 32, reinterpret_cast<uint32_t*>(v) + 32);
+                tmem_wait_ld();
+                if (whole && o.bias) {
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 64; i += 4) {
+                        if (i < 32 || !wide) {
+                            const float4 b4 = *reinterpret_cast<const float4*>(bias_s + i);
+                            v[i] += b4.x; v[i + 1] += b4.y; v[i + 2] += b4.z; v[i + 3] += b4.w;
+                        }
+                    }
+                }
+                // staged rows: 16-byte chunk c of row r sits at chunk c ^ (r & 7)
+                uint8_t* mine = stage + lane * 128;
+                const int sw = lane & 7;
+                auto flush = [&](void* base, int64_t ld, int esz, int row_limit, int col_limit, bool vec) {
+                    __syncwarp();
+                    const int per = 16 / esz;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = 4 * i + srow, nn = sch * per;
+                        const uint4 q = *reinterpret_cast<const uint4*>(stage + r * 128 + ((sch ^ (r & 7)) * 16));
+                        if (r < row_limit && nn < col_limit) {
+                            uint8_t* p = static_cast<uint8_t*>(base) + (r * ld + nn) * esz;
+                            if (vec && nn + per <= col_limit) {
+                                *reinterpret_cast<uint4*>(p) = q;
+                            } else {
+                                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+                                if (esz == 4) {
+                                    for (int e = 0; e < 4; ++e)
+                                        if (nn + e < col_limit) reinterpret_cast<uint32_t*>(p)[e] = w[e];
+                                } else {
+                                    for (int e = 0; e < 8; ++e)
+                                        if (nn + e < col_limit)
+                                            reinterpret_cast<uint16_t*>(p)[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+                                }
+                            }
+                        }
+                    }
+                    __syncwarp();
+                };
+                auto put16 = [&](const float* f, int half) {   // 32 values as 16-bit, chunks 4 half .. 4 half + 3
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        *reinterpret_cast<uint4*>(mine + (((4 * half + c) ^ sw) * 16)) =
+                            make_uint4(Elem<T>::pack(f[8 * c], f[8 * c + 1]), Elem<T>::pack(f[8 * c + 2], f[8 * c + 3]),
+                                       Elem<T>::pack(f[8 * c + 4], f[8 * c + 5]), Elem<T>::pack(f[8 * c + 6], f[8 * c + 7]));
+                };
+                auto put32 = [&](const float* f) {
+#pragma unroll
+                    for (int c = 0; c < 8; ++c)
+                        *reinterpret_cast<float4*>(mine + ((c ^ sw) * 16)) =
+                            make_float4(f[4 * c], f[4 * c + 1], f[4 * c + 2], f[4 * c + 3]);
+                };
+                const int rows = min(32, M - mw), left = N - n;
+                if (!whole) {
+                    put32(v);
+                    flush(sched.part + ((int64_t)t.slot * kBM + quarter * 32) * BN + c0, BN, 4, rows, cols, true);
+                    continue;
+                }
+                if (o.pre) {
+                    put16(v, 0);
+                    if (!wide) put16(v + 32, 1);
+                    flush(static_cast<T*>(o.pre) + (int64_t)mw * o.ldp + n, o.ldp, 2, rows, min(left, cols), o.vec);
+                }
+#pragma unroll
+                for (int i = 0; i < 64; i += 2)
+                    if (i < 32 || !wide) activate_pair(o.act, v[i], v[i + 1]);
+                if (add) {
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int r = 4 * i + srow;
+                        *reinterpret_cast<uint4*>(stage + r * 128 + ((sch ^ (r & 7)) * 16)) = res[i];
+                    }
+                    __syncwarp();
+                    if (wide) {
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) {
+                            const float4 f = *reinterpret_cast<const float4*>(mine + ((c ^ sw) * 16));
+                            v[4 * c] += f.x; v[4 * c + 1] += f.y; v[4 * c + 2] += f.z; v[4 * c + 3] += f.w;
+                        }
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) {
+                            const uint4 q = *reinterpret_cast<const uint4*>(mine + ((c ^ sw) * 16));
+                            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float2 f = Elem<T>::unpack(w[e]);
+                                v[8 * c + 2 * e] += f.x;
+                                v[8 * c + 2 * e + 1] += f.y;
+                            }
+                        }
+                    }
+                }
+                if (wide) {
+                    put32(v);
+                    flush(static_cast<float*>(o.y) + (int64_t)mw * o.ldy + n, o.ldy, 4, rows, min(left, cols), o.vec);
+                } else {
+                    put16(v, 0);
+                    put16(v + 32, 1);
+                    flush(static_cast<T*>(o.y) + (int64_t)mw * o.ldy + n, o.ldy, 2, rows, min(left, cols), o.vec);
+                }
+            }
+            if (!ok) break;
+            if (!waited) {                                    // a group with no columns of its own (BN = 64 in 2 bytes)
+                ok = __all_sync(0xffffffffu, mbar_wait(acc_full + buf, (k >> 1) & 1u, abort_flag));
+                if (!ok) break;
+            }
+            tc_fence_before();
+            mbar_arrive(acc_empty + buf);
+        }
+        if (!ok && lane == 0) {
+            *abort_flag = 1;
+            flag(status, PMG_ERR_TIMEOUT);
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 2 * BN);
+    }
+}
+
+template <typename T, int BN>
+__global__ void __launch_bounds__(256) k_split_sum(const __grid_constant__ Sched s, const int M, const int N,
+                                                   const __grid_constant__ Out o) {
+    pdl_begin();
+    const int per_tile = kBM * BN / 8;
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    const int rest = i / per_tile, tile = s.full + rest, e = (i % per_tile) * 8;
+    if (tile >= s.tiles) return;
+    const int r = e / BN, c = e % BN;
+    const int m = (tile / s.tiles_n) * kBM + r, n = (tile % s.tiles_n) * BN + c;
+    if (m >= M || n >= N) return;
+    float z[8] = {};
+    const float* p = s.part + ((int64_t)rest * s.splits * kBM + r) * BN + c;
+    for (int k = 0; k < s.splits; ++k) {
+        const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+        z[0] += a.x; z[1] += a.y; z[2] += a.z; z[3] += a.w;
+        z[4] += b.x; z[5] += b.y; z[6] += b.z; z[7] += b.w;
+        p += kBM * BN;
+    }
+    finish8<T>(o, m, n, N, z);
+}
+
+// ----------------------------------------------------------------------------------------------------------------- //
+// Backwards: dz and the bias gradient; row packing
+// ----------------------------------------------------------------------------------------------------------------- //
+constexpr int kStripCols = 256, kStripRows = 8;       // a block's columns; rows at a time
+
+// dz = dy act'(z) rounded to T into dst (null: not wanted) with its row padding zeroed, and this block's column sums of
+// the unrounded dz into part [row blocks][N] (null: not wanted).
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) k_act_grad(const T* __restrict__ dy, int64_t ldy, const T* __restrict__ pre,
+                                                  int64_t ldp, int64_t M, int N, int act, T* __restrict__ dst,
+                                                  int64_t ldd, int padded, int64_t rows_per_block,
+                                                  float* __restrict__ part) {
+    pdl_begin();
+    __shared__ float sm[kStripRows][kStripCols];
+    const int cg = threadIdx.x & 31, rg = threadIdx.x >> 5, n = blockIdx.x * kStripCols + cg * 8;
+    const int64_t r0 = blockIdx.y * rows_per_block, r1 = min(r0 + rows_per_block, M);
+    float acc[8] = {};
+    if (n < padded) {
+#pragma unroll 2
+        for (int64_t m = r0 + rg; m < r1; m += kStripRows) {
+            float g[8], z[8];
+            if (VEC && n + 8 <= N) {
+                const uint4 a = *reinterpret_cast<const uint4*>(dy + m * ldy + n);
+                const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = Elem<T>::unpack(w[i]);
+                    g[2 * i] = f.x;
+                    g[2 * i + 1] = f.y;
+                }
+                if (pre) {
+                    const uint4 b = *reinterpret_cast<const uint4*>(pre + m * ldp + n);
+                    const uint32_t v[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 f = Elem<T>::unpack(v[i]);
+                        z[2 * i] = f.x;
+                        z[2 * i + 1] = f.y;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    g[i] = n + i < N ? Elem<T>::to(dy[m * ldy + n + i]) : 0.0f;
+                    z[i] = pre && n + i < N ? Elem<T>::to(pre[m * ldp + n + i]) : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (pre && n + i < N) g[i] *= act_slope(act, z[i]);
+                acc[i] += g[i];
+            }
+            if (dst) {
+                *reinterpret_cast<uint4*>(dst + m * ldd + n) = make_uint4(Elem<T>::pack(g[0], g[1]), Elem<T>::pack(g[2], g[3]),
+                                                                          Elem<T>::pack(g[4], g[5]), Elem<T>::pack(g[6], g[7]));
+            }
+        }
+    }
+    if (part == nullptr) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sm[rg][cg * 8 + i] = acc[i];
+    __syncthreads();
+    const int col = blockIdx.x * kStripCols + threadIdx.x;
+    if (col < N) {
+        float v = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kStripRows; ++r) v += sm[r][threadIdx.x];
+        part[(int64_t)blockIdx.y * N + col] = v;
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) k_col_sum(const float* __restrict__ part, int blocks, int N, T* __restrict__ out) {
+    pdl_begin();
+    __shared__ float sm[8][33];
+    const int col = blockIdx.x * 32 + (threadIdx.x & 31), strand = threadIdx.x >> 5;
+    float v = 0.0f;
+    if (col < N)
+        for (int b = strand; b < blocks; b += 8) v += part[(int64_t)b * N + col];
+    sm[strand][threadIdx.x & 31] = v;
+    __syncthreads();
+    if (strand == 0 && col < N) {
+        float t = 0.0f;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) t += sm[s][threadIdx.x];
+        out[col] = Elem<T>::from(t);
+    }
+}
+
+// Rows copied to 16-byte-aligned rows of `ldd` values, padding zeroed.
+__global__ void __launch_bounds__(256) k_pack_rows(const uint16_t* __restrict__ src, int64_t lds, int64_t rows, int cols,
+                                                   uint16_t* __restrict__ dst, int64_t ldd) {
+    pdl_begin();
+    const int groups = (int)(ldd / 8);
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows * groups; i += gridDim.x * 256ll) {
+        const int64_t r = i / groups;
+        const int c = (int)(i - r * groups) * 8;
+        const uint16_t* p = src + r * lds + c;
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (c + e < cols) w[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
+        *reinterpret_cast<uint4*>(dst + r * ldd + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// ----------------------------------------------------------------------------------------------------------------- //
+// Host side
+// ----------------------------------------------------------------------------------------------------------------- //
+int64_t round8(int64_t v) { return (v + 7) & ~(int64_t)7; }
+size_t round256(size_t v) { return (v + 255) & ~(size_t)255; }
+bool tma_ok(const void* p, int64_t ld) { return !(reinterpret_cast<uintptr_t>(p) & 15) && !(ld & 7); }
+
+constexpr int kFewRows = 32;
+
+// Tile width: the widest that still gives every SM a tile, and the narrowest otherwise.
+int tile_n(int64_t M, int64_t N) {
+    const int64_t tm = (M + kBM - 1) / kBM;
+    for (int bn : {256, 128})
+        if (N > bn / 2 && tm * ((N + bn - 1) / bn) >= kNumSMs) return bn;
+    return N > 64 && tm * ((N + 63) / 64) > kNumSMs ? 128 : 64;
+}
+
+Sched schedule(int64_t M, int64_t N, int64_t K, int bn) {
+    Sched s{};
+    s.tiles_n = (int)((N + bn - 1) / bn);
+    s.tiles = (int)((M + kBM - 1) / kBM) * s.tiles_n;
+    s.kblocks = (int)((K + kBK - 1) / kBK);
+    s.full = s.tiles;
+    s.splits = 1;
+    s.kper = s.kblocks;
+    const int rest = s.tiles % kNumSMs;
+    // cut the last wave along K when at least two splits of four blocks each find an SM
+    int splits = rest ? std::min({kNumSMs / rest, s.kblocks / 4, 16}) : 1;
+    if (splits >= 2) {
+        s.full = s.tiles - rest;
+        s.kper = (s.kblocks + splits - 1) / splits;
+        s.splits = (s.kblocks + s.kper - 1) / s.kper;
+    }
+    s.units = s.full + (s.tiles - s.full) * s.splits;
+    return s;
+}
+
+size_t part_bytes(int64_t M, int64_t N, int64_t K) {
+    const int bn = tile_n(M, N);
+    const Sched s = schedule(M, N, K, bn);
+    return (size_t)(s.units - s.full) * kBM * bn * sizeof(float);
+}
+
+template <typename T, int BN, bool AMN, bool BMN>
+int gemm_bn(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N, int64_t K, const Out& o,
+            float* part, int32_t* status, cudaStream_t st) {
+    using C = Cfg<BN>;
+    static bool attr_set[64] = {};
+    int dev = 0;
+    PMG_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) return PMG_ERR_UNSUPPORTED;
+    if (!attr_set[dev]) {
+        PMG_CUDA_TRY(cudaFuncSetAttribute(k_gemm<T, BN, AMN, BMN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+        attr_set[dev] = true;
+    }
+    Sched s = schedule(M, N, K, BN);
+    s.part = part;
+    CUtensorMap ma, mb;
+    const uint64_t da[2] = {(uint64_t)(AMN ? M : K), (uint64_t)(AMN ? K : M)}, sa[1] = {(uint64_t)lda * 2};
+    const uint64_t db[2] = {(uint64_t)(BMN ? N : K), (uint64_t)(BMN ? K : N)}, sb[1] = {(uint64_t)ldb * 2};
+    const uint32_t ba[2] = {64, (uint32_t)(AMN ? kBK : kBM)}, bb[2] = {64, (uint32_t)(BMN ? kBK : BN)};
+    int rc = make_tensor_map16(&ma, A, 2, da, sa, ba);
+    if (rc != PMG_OK) return rc;
+    rc = make_tensor_map16(&mb, B, 2, db, sb, bb);
+    if (rc != PMG_OK) return rc;
+    k_gemm<T, BN, AMN, BMN><<<std::min(s.units, kNumSMs), kGemmThreads, C::kSmem, st>>>(ma, mb, (int)M, (int)N, s, o, status);
+    PMG_LAUNCH_CHECK();
+    if (s.full < s.tiles) {
+        const int64_t threads = (int64_t)(s.tiles - s.full) * (kBM * BN / 8);
+        k_split_sum<T, BN><<<(int)((threads + 255) / 256), 256, 0, st>>>(s, (int)M, (int)N, o);
+        PMG_LAUNCH_CHECK();
+    }
+    return PMG_OK;
+}
+
+template <typename T, bool AMN, bool BMN>
+int gemm(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N, int64_t K, const Out& o,
+         float* part, int32_t* status, cudaStream_t st) {
+    switch (tile_n(M, N)) {
+        case 256: return gemm_bn<T, 256, AMN, BMN>(A, lda, B, ldb, M, N, K, o, part, status, st);
+        case 128: return gemm_bn<T, 128, AMN, BMN>(A, lda, B, ldb, M, N, K, o, part, status, st);
+        default: return gemm_bn<T, 64, AMN, BMN>(A, lda, B, ldb, M, N, K, o, part, status, st);
+    }
+}
+
+int pack_rows(const void* src, int64_t ld, int64_t rows, int64_t cols, void* dst, cudaStream_t s) {
+    const int64_t n = rows * (round8(cols) / 8);
+    k_pack_rows<<<(int)std::min<int64_t>((n + 255) / 256, kNumSMs * 16), 256, 0, s>>>(
+        static_cast<const uint16_t*>(src), ld, rows, (int)cols, static_cast<uint16_t*>(dst), round8(cols));
+    PMG_LAUNCH_CHECK();
+    return PMG_OK;
+}
+
+template <typename T, int NT>
+int rows_nt(const void* x, int64_t ldx, const void* w, int64_t ldw, int M, int N, int K, const Out& o, cudaStream_t s) {
+    const bool aligned = tma_ok(x, ldx) && tma_ok(w, ldw) && K % 8 == 0;
+    int warps = std::min(16, std::max(4, (K + 127) / 128));
+    while (warps & (warps - 1)) warps &= warps - 1;
+    const size_t smem = (size_t)warps * kRowsCols * 8 * NT * sizeof(float);
+    const int grid = (N + kRowsCols - 1) / kRowsCols;
+    const uint16_t *xp = static_cast<const uint16_t*>(x), *wp = static_cast<const uint16_t*>(w);
+    if (aligned) k_rows<T, NT, true><<<grid, 32 * warps, smem, s>>>(xp, ldx, wp, ldw, M, N, K, o);
+    else k_rows<T, NT, false><<<grid, 32 * warps, smem, s>>>(xp, ldx, wp, ldw, M, N, K, o);
+    PMG_LAUNCH_CHECK();
+    return PMG_OK;
+}
+
+bool vec_ok(const Out& o) {
+    const int per = o.f32 ? 4 : 8;
+    auto ok = [](const void* p, int64_t ld, int per_) { return !p || (!(reinterpret_cast<uintptr_t>(p) & 15) && ld % per_ == 0); };
+    return ok(o.y, o.ldy, per) && ok(o.resid, o.ldr, per) && ok(o.pre, o.ldp, 8);
+}
+
+template <typename T>
+int linear(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, int64_t N, int64_t K, Out o, uint8_t* ws,
+           int32_t* status, cudaStream_t s) {
+    o.vec = vec_ok(o);
+    if (M <= 8) return rows_nt<T, 1>(x, ldx, w, ldw, (int)M, (int)N, (int)K, o, s);
+    if (M <= 16) return rows_nt<T, 2>(x, ldx, w, ldw, (int)M, (int)N, (int)K, o, s);
+    if (M <= kFewRows) return rows_nt<T, 4>(x, ldx, w, ldw, (int)M, (int)N, (int)K, o, s);
+    if (!tma_ok(x, ldx)) {
+        const int rc = pack_rows(x, ldx, M, K, ws, s);
+        if (rc != PMG_OK) return rc;
+        x = ws;
+        ldx = round8(K);
+        ws += round256((size_t)M * ldx * 2);
+    }
+    if (!tma_ok(w, ldw)) {
+        const int rc = pack_rows(w, ldw, N, K, ws, s);
+        if (rc != PMG_OK) return rc;
+        w = ws;
+        ldw = round8(K);
+        ws += round256((size_t)N * ldw * 2);
+    }
+    return gemm<T, false, false>(x, ldx, w, ldw, M, N, K, o, reinterpret_cast<float*>(ws), status, s);
+}
+
+struct GradPlan {
+    int64_t row_blocks, rows_per_block;
+    bool dz;                 // a rounded (or packed) dz is stored
+};
+
+GradPlan grad_plan(int64_t M, int64_t N, bool act, bool dy_ok) {
+    GradPlan p;
+    const int64_t strips = (N + kStripCols - 1) / kStripCols;
+    const int64_t want = std::max<int64_t>(1, kNumSMs * 8 / strips);
+    p.rows_per_block = std::max<int64_t>(kStripRows * 2, (M + want - 1) / want);
+    p.row_blocks = std::max<int64_t>(1, (M + p.rows_per_block - 1) / p.rows_per_block);
+    p.dz = act || !dy_ok;
+    return p;
+}
+
+template <typename T>
+int linear_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M,
+                int64_t N, int64_t K, const void* pre, int64_t ldp, int act, void* dx, int64_t lddx, void* dw,
+                int64_t lddw, void* db, uint8_t* ws, int32_t* status, cudaStream_t s) {
+    const bool has_act = act != PMG_ACT_NONE, products = dx || dw;
+    const GradPlan p = grad_plan(M, N, has_act, tma_ok(dy, lddy));
+    const void* dz = dy;
+    int64_t lddz = lddy;
+    if (db || (p.dz && products)) {
+        T* dst = nullptr;
+        if (p.dz && products) {
+            dst = reinterpret_cast<T*>(ws);
+            lddz = round8(N);
+            dz = dst;
+            ws += round256((size_t)M * lddz * 2);
+        }
+        float* part = nullptr;
+        if (db) {
+            part = reinterpret_cast<float*>(ws);
+            ws += round256((size_t)p.row_blocks * N * sizeof(float));
+        }
+        const dim3 grid((unsigned)((N + kStripCols - 1) / kStripCols), (unsigned)p.row_blocks);
+        const bool vec = tma_ok(dy, lddy) && (!has_act || tma_ok(pre, ldp));
+        const T *dyp = static_cast<const T*>(dy), *prep = has_act ? static_cast<const T*>(pre) : nullptr;
+        if (vec) k_act_grad<T, true><<<grid, 256, 0, s>>>(dyp, lddy, prep, ldp, M, (int)N, act, dst, lddz, (int)round8(N), p.rows_per_block, part);
+        else k_act_grad<T, false><<<grid, 256, 0, s>>>(dyp, lddy, prep, ldp, M, (int)N, act, dst, lddz, (int)round8(N), p.rows_per_block, part);
+        PMG_LAUNCH_CHECK();
+        if (db) {
+            k_col_sum<T><<<(int)((N + 31) / 32), 256, 0, s>>>(part, (int)p.row_blocks, (int)N, static_cast<T*>(db));
+            PMG_LAUNCH_CHECK();
+        }
+    }
+    Out o{};
+    if (dx) {
+        const void* wp = w;
+        int64_t ld = ldw;
+        uint8_t* left = ws;
+        if (!tma_ok(w, ldw)) {
+            const int rc = pack_rows(w, ldw, N, K, left, s);
+            if (rc != PMG_OK) return rc;
+            wp = left;
+            ld = round8(K);
+            left += round256((size_t)N * ld * 2);
+        }
+        o.y = dx;
+        o.ldy = lddx;
+        o.vec = vec_ok(o);
+        const int rc = gemm<T, false, true>(dz, lddz, wp, ld, M, K, N, o, reinterpret_cast<float*>(left), status, s);
+        if (rc != PMG_OK) return rc;
+    }
+    if (dw) {
+        const void* xp = x;
+        int64_t ld = ldx;
+        uint8_t* left = ws;
+        if (!tma_ok(x, ldx)) {
+            const int rc = pack_rows(x, ldx, M, K, left, s);
+            if (rc != PMG_OK) return rc;
+            xp = left;
+            ld = round8(K);
+            left += round256((size_t)M * ld * 2);
+        }
+        o.y = dw;
+        o.ldy = lddw;
+        o.vec = vec_ok(o);
+        const int rc = gemm<T, true, true>(dz, lddz, xp, ld, N, K, M, o, reinterpret_cast<float*>(left), status, s);
+        if (rc != PMG_OK) return rc;
+    }
+    return PMG_OK;
+}
+
+int check_linear(int dtype, int64_t M, int64_t N, int64_t K, int act) {
+    if (dtype != PMG_F16 && dtype != PMG_BF16) return PMG_ERR_UNSUPPORTED;
+    if (M < 0 || N < 1 || K < 1 || act < PMG_ACT_NONE || act > PMG_ACT_GELU) return PMG_ERR_BAD_ARG;
+    if (M > (int64_t)1 << 30 || N > 1 << 20 || K > 1 << 20) return PMG_ERR_UNSUPPORTED;
+    if (((M + kBM - 1) / kBM) * ((std::max(N, K) + 63) / 64) > (int64_t)1 << 30) return PMG_ERR_UNSUPPORTED;
+    return PMG_OK;
+}
+
+}  // namespace
+}  // namespace pmg
+
+using namespace pmg;
+
+extern "C" size_t pmg_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t pack_x, int32_t pack_w) {
+    if (M <= kFewRows || N < 1 || K < 1) return 0;
+    return (pack_x ? round256((size_t)M * round8(K) * 2) : 0) + (pack_w ? round256((size_t)N * round8(K) * 2) : 0) +
+           part_bytes(M, N, K);
+}
+
+extern "C" int pmg_linear(const void* x, int64_t ldx, const void* w, int64_t ldw, int32_t dtype, int64_t M, int64_t N,
+                          int64_t K, const void* bias, int32_t act, const void* residual, int64_t ldr, int32_t out_f32,
+                          void* y, int64_t ldy, void* pre, int64_t ldp, void* workspace, size_t workspace_bytes,
+                          int32_t* status, void* stream) {
+    const int rc = check_linear(dtype, M, N, K, act);
+    if (rc != PMG_OK) return rc;
+    if (M == 0) return PMG_OK;
+    if (!x || !w || !y || ldx < K || ldw < K || ldy < N || (residual && ldr < N) || (pre && ldp < N)) return PMG_ERR_BAD_ARG;
+    const size_t need = pmg_linear_workspace_bytes(M, N, K, !tma_ok(x, ldx), !tma_ok(w, ldw));
+    if (workspace_bytes < need || (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15)))) return PMG_ERR_BAD_ARG;
+    Out o{};
+    o.bias = bias; o.resid = residual; o.y = y; o.pre = pre;
+    o.ldr = ldr; o.ldy = ldy; o.ldp = ldp; o.act = act; o.f32 = out_f32 != 0;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    return dtype == PMG_BF16 ? linear<__nv_bfloat16>(x, ldx, w, ldw, M, N, K, o, ws, status, as_stream(stream))
+                             : linear<__half>(x, ldx, w, ldw, M, N, K, o, ws, status, as_stream(stream));
+}
+
+extern "C" size_t pmg_linear_grad_workspace_bytes(int64_t M, int64_t N, int64_t K, int32_t act, int32_t pack_dy,
+                                                  int32_t pack_x, int32_t pack_w, int32_t bias_grad) {
+    if (M < 1 || N < 1 || K < 1) return 0;
+    const GradPlan p = grad_plan(M, N, act != PMG_ACT_NONE, !pack_dy);
+    const size_t dz = p.dz ? round256((size_t)M * round8(N) * 2) : 0;
+    const size_t db = bias_grad ? round256((size_t)p.row_blocks * N * sizeof(float)) : 0;
+    const size_t wx = (pack_w ? round256((size_t)N * round8(K) * 2) : 0) + part_bytes(M, K, N);
+    const size_t ww = (pack_x ? round256((size_t)M * round8(K) * 2) : 0) + part_bytes(N, K, M);
+    return dz + db + std::max(wx, ww);
+}
+
+extern "C" int pmg_linear_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw,
+                               int32_t dtype, int64_t M, int64_t N, int64_t K, const void* pre, int64_t ldp,
+                               int32_t act, void* dx, int64_t lddx, void* dw, int64_t lddw, void* db, void* workspace,
+                               size_t workspace_bytes, int32_t* status, void* stream) {
+    const int rc = check_linear(dtype, M, N, K, act);
+    if (rc != PMG_OK) return rc;
+    cudaStream_t s = as_stream(stream);
+    if (M == 0) {                                     // no rows: the sums over rows are zero
+        if (dw) PMG_CUDA_TRY(cudaMemset2DAsync(dw, (size_t)lddw * 2, 0, (size_t)K * 2, (size_t)N, s));
+        if (db) PMG_CUDA_TRY(cudaMemsetAsync(db, 0, (size_t)N * 2, s));
+        return PMG_OK;
+    }
+    if (!dy || lddy < N || (act != PMG_ACT_NONE && (!pre || ldp < N)) || (dx && (!w || ldw < K || lddx < K)) ||
+        (dw && (!x || ldx < K || lddw < K)))
+        return PMG_ERR_BAD_ARG;
+    const size_t need = pmg_linear_grad_workspace_bytes(M, N, K, act, !tma_ok(dy, lddy), dw && !tma_ok(x, ldx),
+                                                        dx && !tma_ok(w, ldw), db != nullptr);
+    if (workspace_bytes < need || (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15)))) return PMG_ERR_BAD_ARG;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    return dtype == PMG_BF16
+               ? linear_grad<__nv_bfloat16>(dy, lddy, x, ldx, w, ldw, M, N, K, pre, ldp, act, dx, lddx, dw, lddw, db, ws, status, s)
+               : linear_grad<__half>(dy, lddy, x, ldx, w, ldw, M, N, K, pre, ldp, act, dx, lddx, dw, lddw, db, ws, status, s);
+}
