@@ -1,0 +1,741 @@
+// Attention over packed documents, forwards: rows by the tile (k_attn) and few rows over a long cache (k_attn_few).
+//
+// k_attn.  A CTA owns 256 query rows of one document and head, two tiles of 128 that share every key tile of 128.
+// Products run on tcgen05 with the scores, the probabilities (left operand of the second product) and the running
+// output in tensor memory; a warpgroup per tile holds one row a thread, so the softmax needs no shuffle.  The running
+// maximum is only renewed, and the output only rescaled, when it has grown by more than 2^8: the probabilities then lie
+// within 2^8, and the sums lose nothing to it.  Probabilities are rounded to the operands' 16-bit type for the second
+// product (its operand can be no wider); the sums are of the unrounded ones, in fp32.
+#include <algorithm>
+#include <cmath>
+
+#include "tok_attn.cuh"
+
+namespace pmg {
+
+int fill_attn(tok::Attn* a, int dtype, const int32_t* cu_q, const int32_t* cu_k, const int32_t* k_len, int docs, int64_t Tq,
+              int64_t Tk, int Hq, int Hk, int D, float scale, int causal, const int32_t* prefix, float softcap,
+              const float* slopes, int32_t* status) {
+    if (dtype != PMG_F16 && dtype != PMG_BF16) return PMG_ERR_UNSUPPORTED;
+    if (docs < 0 || Tq < 0 || Tk < 0 || Hq < 1 || Hk < 1 || Hq % Hk || D < 8 || !cu_q || !cu_k) return PMG_ERR_BAD_ARG;
+    if (!(scale > 0.0f) || !std::isfinite(scale) || !(softcap >= 0.0f) || !std::isfinite(softcap)) return PMG_ERR_BAD_ARG;
+    if (D % 8 || D > 128 || Tq > INT32_MAX - 512 || Tk > INT32_MAX - 512 || Hq > 65535) return PMG_ERR_UNSUPPORTED;
+    *a = tok::Attn{};
+    a->cu_q = cu_q; a->cu_k = cu_k; a->k_len = k_len; a->prefix = causal ? prefix : nullptr; a->slopes = slopes;
+    a->Tq = Tq; a->Tk = Tk; a->docs = docs; a->Hq = Hq; a->Hk = Hk; a->group = Hq / Hk; a->D = D; a->causal = causal != 0;
+    a->scale2 = scale * tok::kLog2e;
+    a->cap2 = softcap * tok::kLog2e;
+    a->tanh_in = softcap > 0.0f ? 2.0f * scale * tok::kLog2e / softcap : 0.0f;
+    a->status = status;
+    return PMG_OK;
+}
+
+int head_map(CUtensorMap* m, const void* p, int64_t tok, int64_t head, int64_t T, int H, int D, int rows) {
+    if ((tok & 7) || (head & 7)) return PMG_ERR_BAD_ARG;
+    const uint64_t dims[3] = {(uint64_t)D, (uint64_t)H, (uint64_t)T};
+    const uint64_t strides[2] = {(uint64_t)head * 2, (uint64_t)tok * 2};
+    const uint32_t box[3] = {64, 1, (uint32_t)rows};
+    return make_tensor_map16(m, p, 3, dims, strides, box);
+}
+
+namespace {
+
+using namespace tok;
+
+constexpr float kGrow = 8.0f;                  // log2 of how far scores may outgrow the running maximum
+
+template <typename T> constexpr float kLift = 0.0f;
+template <> constexpr float kLift<__half> = 7.0f;   // fp16 probabilities are kept times 2^7: 2^15 at most, and 7 more
+                                                    // binades before they turn subnormal
+
+template <int DP>
+struct Fwd {
+    static constexpr bool kSep = DP == 64;     // probabilities beside the scores: 2 (128 + 64 + 64) = 512 columns
+    static constexpr int kTile = 128 * DP * 2; // a tile of 128 rows
+    static constexpr int kStages = DP == 64 ? 4 : 2;
+    static constexpr int kQ = 2 * kTile;
+    static constexpr int kBars = kQ + 2 * kStages * kTile;
+    static constexpr int kSmem = kBars + 512;
+    static constexpr uint32_t S(int w) { return 128 * w; }
+    static constexpr uint32_t P(int w) { return kSep ? 256 + 64 * w : 128 * w; }
+    static constexpr uint32_t O(int w) { return kSep ? 384 + 64 * w : 256 + 128 * w; }
+};
+
+constexpr int kFwdThreads = 320;               // two softmax warpgroups, the loader, the MMA issuer
+
+#define TOK_WAIT(bar, parity)                                                                   \
+    do {                                                                                        \
+        if (!__all_sync(0xffffffffu, mbar_wait((bar), (parity), abort_flag))) { ok = false; break; } \
+    } while (0)
+
+template <typename T, int DP, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kFwdThreads, 1)
+    k_attn(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+           const __grid_constant__ CUtensorMap mv, const __grid_constant__ Attn a, T* __restrict__ o, int64_t o_tok,
+           int64_t o_head, float* __restrict__ lse) {
+    using C = Fwd<DP>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t* const sk = smem + C::kQ;
+    uint8_t* const sv = sk + C::kStages * C::kTile;
+    uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::kBars);
+    uint64_t* k_full = q_full + 2;
+    uint64_t* k_empty = k_full + C::kStages;
+    uint64_t* v_full = k_empty + C::kStages;
+    uint64_t* v_empty = v_full + C::kStages;
+    uint64_t* s_full = v_empty + C::kStages;
+    uint64_t* s_read = s_full + 2;
+    uint64_t* p_full = s_read + 2;
+    uint64_t* pv_done = p_full + 2;
+    uint64_t* drain = pv_done + 2;
+    uint32_t* slot = reinterpret_cast<uint32_t*>(drain + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
+    int* where = reinterpret_cast<int*>(slot + 2);           // document and tile
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int head = blockIdx.x % a.Hq, kvh = head / a.group;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(q_full + i, 1);
+            mbar_init(s_full + i, 1);
+            mbar_init(s_read + i, 128);
+            mbar_init(p_full + i, 128);
+            mbar_init(pv_done + i, 1);
+        }
+        for (int i = 0; i < C::kStages; ++i) {
+            mbar_init(k_full + i, 1);
+            mbar_init(k_empty + i, 1);
+            mbar_init(v_full + i, 1);
+            mbar_init(v_empty + i, 1);
+        }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 9) tmem_alloc(slot, 512);
+    pdl_begin();
+    if (warp == 8) {
+        int doc = -1, tile = 0;
+        const bool found = find_tile(a.cu_q, a.docs, 256, blockIdx.x / a.Hq, &doc, &tile);
+        if (lane == 0) {
+            where[0] = found ? doc : -1;
+            where[1] = tile;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *slot;
+    const int doc = where[0];
+    if (doc >= 0) {
+        const Span sp = span_of(a, doc);
+        // later rows of a causal document reach further: they start first
+        const int tiles = (sp.lq + 255) / 256, tile = a.causal ? tiles - 1 - where[1] : where[1];
+        const int r0 = tile * 256;
+        int n[2];
+#pragma unroll
+        for (int w = 0; w < 2; ++w) n[w] = r0 + 128 * w < sp.lq ? (key_end(a, sp, r0 + 128 * (w + 1)) + 127) / 128 : 0;
+        const int nmax = max(n[0], n[1]);
+
+        if (warp == 8) {
+            // ------------------------------------------------------------------------------------------------ loads
+            if (lane == 0) {
+                bool ok = true;
+                for (int w = 0; w < 2; ++w) {
+                    if (n[w] == 0) continue;
+                    mbar_arrive_expect_tx(q_full + w, C::kTile);
+#pragma unroll
+                    for (int c = 0; c < DP / 64; ++c)
+                        tma_tile3d(smem_u32(smem + w * C::kTile + c * 16384), &mq, 64 * c, head, sp.q0 + r0 + 128 * w, q_full + w);
+                }
+                for (int j = 0; j < nmax; ++j) {
+                    const int st = j % C::kStages;
+                    const uint32_t ph = ((j / C::kStages) & 1u) ^ 1u;
+                    if (!mbar_wait(k_empty + st, ph, abort_flag)) { ok = false; break; }
+                    mbar_arrive_expect_tx(k_full + st, C::kTile);
+#pragma unroll
+                    for (int c = 0; c < DP / 64; ++c)
+                        tma_tile3d(smem_u32(sk + st * C::kTile + c * 16384), &mk, 64 * c, kvh, sp.k0 + 128 * j, k_full + st);
+                    if (!mbar_wait(v_empty + st, ph, abort_flag)) { ok = false; break; }
+                    mbar_arrive_expect_tx(v_full + st, C::kTile);
+#pragma unroll
+                    for (int c = 0; c < DP / 64; ++c)
+                        tma_tile3d(smem_u32(sv + st * C::kTile + c * 16384), &mv, 64 * c, kvh, sp.k0 + 128 * j, v_full + st);
+                }
+                if (!ok) {
+                    *abort_flag = 1;
+                    flag(a.status, PMG_ERR_TIMEOUT);
+                }
+            }
+        } else if (warp == 9) {
+            // ------------------------------------------------------------------------------------------------ MMAs
+            const int ksteps = (a.D + 15) / 16;
+            const uint32_t id_qk = idesc16(Elem<T>::kFmt, 128, 128, false, false);
+            const uint32_t id_pv = idesc16(Elem<T>::kFmt, 128, ksteps * 16, false, true);
+            bool ok = true;
+            auto qk = [&](int w, int j) -> bool {
+                const int st = j % C::kStages;
+                if (j == 0 && !__all_sync(0xffffffffu, mbar_wait(q_full + w, 0, abort_flag))) return false;
+                if (!__all_sync(0xffffffffu, mbar_wait(k_full + st, (j / C::kStages) & 1u, abort_flag))) return false;
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint32_t qa = smem_u32(smem + w * C::kTile), kb = smem_u32(sk + st * C::kTile);
+                    for (int s = 0; s < ksteps; ++s) {
+                        const uint32_t at = (s >> 2) * 16384 + (s & 3) * 32;
+                        mma16(tmem + C::S(w), desc16(qa + at, 16), desc16(kb + at, 16), id_qk, s > 0);
+                    }
+                    mma_commit(s_full + w);
+                    if (w == 1 || j >= n[1]) mma_commit(k_empty + st);     // the tile's last reader
+                }
+                __syncwarp();
+                return true;
+            };
+            auto pv = [&](int w, int j) -> bool {
+                const int st = j % C::kStages;
+                if (!__all_sync(0xffffffffu, mbar_wait(v_full + st, (j / C::kStages) & 1u, abort_flag))) return false;
+                const int valid = sp.lk - 128 * j;
+                if (valid < 128 && (w == 0 || n[0] <= j)) {
+                    // rows behind the document's last key: whatever lies there must not reach a sum (0 * NaN)
+                    for (int c = 0; c < DP / 64; ++c)
+                        for (int b = valid * 128 + lane * 16; b < 16384; b += 512)
+                            *reinterpret_cast<uint4*>(sv + st * C::kTile + c * 16384 + b) = make_uint4(0, 0, 0, 0);
+                    fence_proxy_async();
+                    __syncwarp();
+                }
+                if (!__all_sync(0xffffffffu, mbar_wait(p_full + w, j & 1u, abort_flag))) return false;
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint32_t vb = smem_u32(sv + st * C::kTile);
+#pragma unroll
+                    for (int s = 0; s < 8; ++s)
+                        mma16_ts(tmem + C::O(w), tmem + C::P(w) + 8 * s, desc16(vb + s * 2048, 16384), id_pv, j > 0 || s > 0);
+                    mma_commit(pv_done + w);
+                    if (w == 1 || j >= n[1]) mma_commit(v_empty + st);
+                }
+                __syncwarp();
+                return true;
+            };
+            for (int w = 0; w < 2 && ok; ++w)
+                if (n[w] > 0) ok = qk(w, 0);
+            for (int j = 0; j < nmax && ok; ++j) {
+                if (C::kSep) {
+                    // the next scores as soon as these have been read, under the softmax of these
+                    for (int w = 0; w < 2 && ok; ++w)
+                        if (j + 1 < n[w]) {
+                            ok = __all_sync(0xffffffffu, mbar_wait(s_read + w, j & 1u, abort_flag));
+                            if (ok) ok = qk(w, j + 1);
+                        }
+                    for (int w = 0; w < 2 && ok; ++w)
+                        if (j < n[w]) ok = pv(w, j);
+                } else {
+                    for (int w = 0; w < 2 && ok; ++w) {
+                        if (j < n[w]) ok = pv(w, j);
+                        if (ok && j + 1 < n[w]) ok = qk(w, j + 1);
+                    }
+                }
+            }
+            if (lane == 0) {
+                if (!ok) flag(a.status, PMG_ERR_TIMEOUT);
+                if (!ok || *abort_flag) {
+                    *abort_flag = 1;
+                    drain_mma(drain);
+                }
+            }
+            __syncwarp();
+        } else {
+            // --------------------------------------------------------------------------------------------- softmax
+            const int w = warp >> 2, tiles_k = n[w];
+            const int i = r0 + 128 * w + (warp & 3) * 32 + lane;          // this thread's row in the document
+            const int lim = last_key(a, sp, i);
+            const int warp_min = __reduce_min_sync(0xffffffffu, i < sp.lq ? lim : INT32_MAX);
+            const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+            const uint32_t ts = tmem + lanes + C::S(w), tp = tmem + lanes + C::P(w), to = tmem + lanes + C::O(w);
+            const float c = (CAP || BIAS) ? 1.0f : a.scale2;              // scores to units of log 2
+            const float slope = BIAS ? a.slopes[head] * kLog2e : 0.0f;
+            const float place = (float)(i + sp.lk - sp.lq);
+            float m = -INFINITY;
+            uint64_t sum = 0;
+            float total = 0.0f;
+            bool ok = true;
+            for (int j = 0; j < tiles_k; ++j) {
+                TOK_WAIT(s_full + w, j & 1u);
+                if (!ok) break;
+                tc_fence_after();
+                float s[128];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) tmem_ld32(ts + 32 * q, reinterpret_cast<uint32_t*>(s) + 32 * q);
+                tmem_wait_ld();
+                if (C::kSep) {
+                    tc_fence_before();
+                    mbar_arrive(s_read + w);
+                }
+                const int j0 = 128 * j;
+                if (CAP) {
+#pragma unroll
+                    for (int k = 0; k < 128; ++k) s[k] = capped(a, s[k]);
+                }
+                if (BIAS) {
+                    const float far = place - (float)j0;
+#pragma unroll
+                    for (int k = 0; k < 128; ++k)
+                        s[k] = fmaf(-slope, fabsf(far - (float)k), CAP ? s[k] : s[k] * a.scale2);
+                }
+                if (j0 + 127 > warp_min) {
+#pragma unroll
+                    for (int k = 0; k < 128; ++k)
+                        if (j0 + k > lim) s[k] = -INFINITY;
+                }
+                float top = max3(s[0], s[1], s[2]);
+#pragma unroll
+                for (int k = 3; k < 127; k += 2) top = max3(top, s[k], s[k + 1]);
+                top = fmaxf(top, s[127]);
+                if (j > 0) TOK_WAIT(pv_done + w, (j - 1) & 1u);           // frees the probabilities and the output
+                if (!ok) break;
+                if (j == 0) {
+                    m = top;
+                } else if (__any_sync(0xffffffffu, (top - m) * c > kGrow)) {
+                    const float grown = fmaxf(m, top);
+                    const float f = grown == m ? 1.0f : ex2((m - grown) * c);
+                    m = grown;
+                    total *= f;
+                    const float2 s2 = unpack2(sum);
+                    sum = pack2(s2.x * f, s2.y * f);
+                    tc_fence_after();
+#pragma unroll
+                    for (int q = 0; q < DP / 32; ++q) {
+                        float v[32];
+                        tmem_ld32(to + 32 * q, reinterpret_cast<uint32_t*>(v));
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) v[k] *= f;
+                        tmem_st32(to + 32 * q, reinterpret_cast<uint32_t*>(v));
+                    }
+                    tmem_wait_st();
+                }
+                const float base = m == -INFINITY ? 0.0f : -m * c + kLift<T>;
+                const uint64_t c2 = pack2(c, c), b2 = pack2(base, base);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t p[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float2 x = unpack2(fma2(pack2(s[32 * q + 2 * k], s[32 * q + 2 * k + 1]), c2, b2));
+                        const float e0 = ex2(x.x), e1 = ex2(x.y);
+                        sum = add2(sum, pack2(e0, e1));
+                        p[k] = Elem<T>::pack(e0, e1);
+                    }
+                    tmem_st16(tp + 16 * q, p);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(p_full + w);
+            }
+            const float2 s2 = unpack2(sum);
+            total = s2.x + s2.y;
+            if (tiles_k > 0 && ok) TOK_WAIT(pv_done + w, (tiles_k - 1) & 1u);
+            if (ok) {
+                tc_fence_after();
+                const int64_t token = sp.q0 + (int64_t)i;
+                const bool mine = i < sp.lq && token < a.Tq;
+                const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;   // empty rows: zero
+                if (mine) lse[(int64_t)head * a.Tq + token] = total == 0.0f ? -INFINITY : (m * c + log2f(total) - kLift<T>) * kLn2;
+                T* row = o + token * o_tok + head * o_head;
+#pragma unroll
+                for (int q = 0; q < DP / 32; ++q) {
+                    float v[32];
+                    if (tiles_k > 0) {
+                        tmem_ld32(to + 32 * q, reinterpret_cast<uint32_t*>(v));
+                        tmem_wait_ld();
+                    }
+                    if (total == 0.0f) {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) v[k] = 0.0f;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (mine && 32 * q + 8 * k < a.D)
+                            *reinterpret_cast<uint4*>(row + 32 * q + 8 * k) =
+                                make_uint4(Elem<T>::pack(v[8 * k] * inv, v[8 * k + 1] * inv),
+                                           Elem<T>::pack(v[8 * k + 2] * inv, v[8 * k + 3] * inv),
+                                           Elem<T>::pack(v[8 * k + 4] * inv, v[8 * k + 5] * inv),
+                                           Elem<T>::pack(v[8 * k + 6] * inv, v[8 * k + 7] * inv));
+                }
+            } else if (lane == 0) {
+                *abort_flag = 1;
+                flag(a.status, PMG_ERR_TIMEOUT);
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// ----------------------------------------------------------------------------------------------------------------- //
+// Few rows over many keys
+// ----------------------------------------------------------------------------------------------------------------- //
+// Bound by one read of the keys and values.  A CTA takes one document, one key head and a stretch of the keys; the up to
+// 16 query rows that share the key head (queries x group) are the 16 rows of mma.sync, so every key is read once for all
+// of them.  A warp walks blocks of keys on its own, straight from global memory into operand registers: the order of a
+// dot product's terms is free, so lanes load 16 bytes of a key each and the queries are loaded in the same order; the
+// values' pairs of keys are joined with byte permutes, their order along the head undone when the output is stored.
+// Warps, then stretches, are joined by their maxima and sums.
+
+constexpr int kFewWarps = 8, kFewRows = 16;
+
+template <typename T>
+__device__ __forceinline__ void mma_16n8k16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                            uint32_t b0, uint32_t b1) {
+    if constexpr (Elem<T>::kFmt == 1)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+struct Heads {                    // [T, H, D]: pointer and strides in elements
+    const void* p;
+    int64_t tok, head;
+};
+
+// Partial results of a stretch: per row D unnormalised outputs, then maximum and sum (units of log 2).
+template <typename T, int DP, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(32 * kFewWarps)
+    k_attn_few(const Heads hq, const Heads hk, const Heads hv, const __grid_constant__ Attn a, int max_q, int splits,
+               float* __restrict__ part, T* __restrict__ o, int64_t o_tok, int64_t o_head, float* __restrict__ lse) {
+    constexpr int NC = DP / 32, NV = DP / 64, KB = DP == 64 ? 32 : 16;       // chunks of a key, of a value; keys a step
+    pdl_begin();
+    extern __shared__ float sm[];                  // [warps][16][DP], then [warps][16] maxima, [warps][16] sums
+    float* const sm_m = sm + kFewWarps * kFewRows * DP;
+    float* const sm_l = sm_m + kFewWarps * kFewRows;
+    const int split = blockIdx.x, kvh = blockIdx.y, doc = blockIdx.z;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    const Span sp = span_of(a, doc);
+    if (sp.lq > max_q) {
+        if (threadIdx.x == 0) flag(a.status, PMG_ERR_RANGE);
+    }
+    const int rows = min(sp.lq, max_q) * a.group;
+    if (rows == 0) return;
+    const int reach = key_end(a, sp, sp.lq);
+    const int per = ((reach + splits - 1) / splits + KB - 1) / KB * KB;
+    const int kbeg = split * per, kend = min(reach, kbeg + per);
+
+    // queries: rows g and g + 8, 16 bytes per chunk of 32
+    uint4 qa[NC], qb[NC];
+    int lim[2];
+    float place[2], slope[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int r = g + 8 * h, i = r / a.group, hd = kvh * a.group + r % a.group;
+        const bool on = r < rows;
+        lim[h] = on ? last_key(a, sp, i) : -1;
+        place[h] = (float)(i + sp.lk - sp.lq);
+        slope[h] = BIAS && on ? a.slopes[hd] * kLog2e : 0.0f;
+        const T* p = static_cast<const T*>(hq.p) + (sp.q0 + (int64_t)i) * hq.tok + hd * hq.head;
+#pragma unroll
+        for (int cidx = 0; cidx < NC; ++cidx) {
+            const int d = 32 * cidx + 8 * q;
+            (h ? qb : qa)[cidx] = on && d < a.D && sp.q0 + i < a.Tq ? *reinterpret_cast<const uint4*>(p + d) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    const T* kbase = static_cast<const T*>(hk.p) + (int64_t)sp.k0 * hk.tok + kvh * hk.head;
+    const T* vbase = static_cast<const T*>(hv.p) + (int64_t)sp.k0 * hv.tok + kvh * hv.head;
+    const int klim = min(kend, (int)min((int64_t)INT32_MAX, a.Tk - sp.k0));
+    float acc[8 * NV][4] = {};
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    const float c = (CAP || BIAS) ? 1.0f : a.scale2;
+
+    for (int j0 = kbeg + warp * KB; j0 < kend; j0 += kFewWarps * KB) {
+        uint4 kk[KB / 8][NC], vv[KB / 16][4][NV];
+#pragma unroll
+        for (int t = 0; t < KB / 8; ++t)
+#pragma unroll
+            for (int cidx = 0; cidx < NC; ++cidx) {
+                const int key = j0 + 8 * t + g, d = 32 * cidx + 8 * q;
+                kk[t][cidx] = key < klim && d < a.D ? __ldcs(reinterpret_cast<const uint4*>(kbase + (int64_t)key * hk.tok + d)) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+        for (int t = 0; t < KB / 16; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int v = 0; v < NV; ++v) {
+                    const int key = j0 + 16 * t + 2 * q + (e & 1) + 8 * (e >> 1), d = 64 * v + 8 * g;
+                    vv[t][e][v] = key < klim && d < a.D ? __ldcs(reinterpret_cast<const uint4*>(vbase + (int64_t)key * hv.tok + d)) : make_uint4(0, 0, 0, 0);
+                }
+        float s[KB / 8][4];
+#pragma unroll
+        for (int t = 0; t < KB / 8; ++t) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[t][e] = 0.0f;
+#pragma unroll
+            for (int cidx = 0; cidx < NC; ++cidx) {
+                mma_16n8k16<T>(s[t], qa[cidx].x, qb[cidx].x, qa[cidx].y, qb[cidx].y, kk[t][cidx].x, kk[t][cidx].y);
+                mma_16n8k16<T>(s[t], qa[cidx].z, qb[cidx].z, qa[cidx].w, qb[cidx].w, kk[t][cidx].z, kk[t][cidx].w);
+            }
+        }
+        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int t = 0; t < KB / 8; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int h = e >> 1, key = j0 + 8 * t + 2 * q + (e & 1);
+                float x = s[t][e];
+                if (CAP) x = capped(a, x);
+                if (BIAS) x = fmaf(-slope[h], fabsf(place[h] - (float)key), CAP ? x : x * a.scale2);
+                x = key <= lim[h] && key < kend ? x : -INFINITY;
+                s[t][e] = x;
+                top[h] = fmaxf(top[h], x);
+            }
+        float base[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+            const float grown = fmaxf(m[h], top[h]);
+            const float f = grown == m[h] ? 1.0f : ex2((m[h] - grown) * c);
+            m[h] = grown;
+            base[h] = grown == -INFINITY ? 0.0f : -grown * c + kLift<T>;
+            l[h] *= f;
+#pragma unroll
+            for (int t = 0; t < 8 * NV; ++t) {
+                acc[t][2 * h] *= f;
+                acc[t][2 * h + 1] *= f;
+            }
+        }
+        uint32_t p[KB / 8][2];
+#pragma unroll
+        for (int t = 0; t < KB / 8; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float e0 = ex2(fmaf(s[t][2 * h], c, base[h])), e1 = ex2(fmaf(s[t][2 * h + 1], c, base[h]));
+                l[h] += e0 + e1;
+                p[t][h] = Elem<T>::pack(e0, e1);
+            }
+#pragma unroll
+        for (int t = 0; t < KB / 16; ++t)
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&vv[t][0][v]);
+                const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&vv[t][1][v]);
+                const uint32_t* w2 = reinterpret_cast<const uint32_t*>(&vv[t][2][v]);
+                const uint32_t* w3 = reinterpret_cast<const uint32_t*>(&vv[t][3][v]);
+#pragma unroll
+                for (int d = 0; d < 8; ++d) {       // column g of this product is value 64 v + 8 g + d
+                    const uint32_t sel = (d & 1) ? 0x7632 : 0x5410;
+                    mma_16n8k16<T>(acc[8 * v + d], p[2 * t][0], p[2 * t][1], p[2 * t + 1][0], p[2 * t + 1][1],
+                                   __byte_perm(w0[d >> 1], w1[d >> 1], sel), __byte_perm(w2[d >> 1], w3[d >> 1], sel));
+                }
+            }
+    }
+    // this warp's rows
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        const int r = warp * kFewRows + g + 8 * h;
+        if (q == 0) {
+            sm_m[r] = m[h] * c;
+            sm_l[r] = l[h];
+        }
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int d = 0; d < 8; ++d) {
+                sm[r * DP + 64 * v + 8 * (2 * q) + d] = acc[8 * v + d][2 * h];
+                sm[r * DP + 64 * v + 8 * (2 * q + 1) + d] = acc[8 * v + d][2 * h + 1];
+            }
+    }
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < rows * (DP / 4); idx += blockDim.x) {
+        const int r = idx / (DP / 4), d = (idx % (DP / 4)) * 4;
+        float top = -INFINITY;
+        for (int w = 0; w < kFewWarps; ++w) top = fmaxf(top, sm_m[w * kFewRows + r]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+        float total = 0.0f;
+        float4 v = make_float4(0, 0, 0, 0);
+        for (int w = 0; w < kFewWarps; ++w) {
+            const float f = ex2(sm_m[w * kFewRows + r] - ref);
+            const float4 x = *reinterpret_cast<const float4*>(sm + (w * kFewRows + r) * DP + d);
+            total += f * sm_l[w * kFewRows + r];
+            v.x += f * x.x; v.y += f * x.y; v.z += f * x.z; v.w += f * x.w;
+        }
+        if (splits > 1) {
+            float* to = part + ((((int64_t)doc * a.Hk + kvh) * splits + split) * kFewRows + r) * (DP + 4);
+            *reinterpret_cast<float4*>(to + d) = v;
+            if (d == 0) {
+                to[DP] = top;
+                to[DP + 1] = total;
+            }
+            continue;
+        }
+        const int64_t token = sp.q0 + (int64_t)(r / a.group);
+        const int head = kvh * a.group + r % a.group;
+        if (token >= a.Tq || d >= a.D) continue;
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        *reinterpret_cast<uint2*>(o + token * o_tok + head * o_head + d) =
+            make_uint2(Elem<T>::pack(v.x * inv, v.y * inv), Elem<T>::pack(v.z * inv, v.w * inv));
+        if (d == 0) lse[(int64_t)head * a.Tq + token] = total == 0.0f ? -INFINITY : (top + log2f(total) - kLift<T>) * kLn2;
+    }
+}
+
+// Joins the stretches of every row, a warp a row.
+template <typename T, int DP>
+__global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ Attn a, int max_q, int splits,
+                                                   const float* __restrict__ part, T* __restrict__ o, int64_t o_tok,
+                                                   int64_t o_head, float* __restrict__ lse) {
+    pdl_begin();
+    const int lane = threadIdx.x & 31, r = blockIdx.x * 4 + (threadIdx.x >> 5), kvh = blockIdx.y, doc = blockIdx.z;
+    const int q0 = a.cu_q[doc], lq = min(max(0, a.cu_q[doc + 1] - q0), max_q);
+    if (r >= lq * a.group) return;
+    const float* from = part + (((int64_t)doc * a.Hk + kvh) * splits * kFewRows + r) * (DP + 4);
+    constexpr int64_t step = kFewRows * (DP + 4);
+    float top = -INFINITY;
+    for (int s = lane; s < splits; s += 32) top = fmaxf(top, from[s * step + DP]);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float v[DP / 32] = {}, total = 0.0f;
+    for (int s = 0; s < splits; ++s) {
+        const float f = ex2(from[s * step + DP] - ref);
+        total += f * from[s * step + DP + 1];
+#pragma unroll
+        for (int k = 0; k < DP / 32; ++k) v[k] += f * from[s * step + lane * (DP / 32) + k];
+    }
+    const int64_t token = q0 + (int64_t)(r / a.group);
+    const int head = kvh * a.group + r % a.group;
+    if (token >= a.Tq) return;
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+    for (int k = 0; k < DP / 32; k += 2) {
+        const int d = lane * (DP / 32) + k;
+        if (d < a.D)
+            *reinterpret_cast<uint32_t*>(o + token * o_tok + head * o_head + d) = Elem<T>::pack(v[k] * inv, v[k + 1] * inv);
+    }
+    if (lane == 0) lse[(int64_t)head * a.Tq + token] = total == 0.0f ? -INFINITY : (top + log2f(total) - kLift<T>) * kLn2;
+}
+
+// ----------------------------------------------------------------------------------------------------------------- //
+// Host side
+// ----------------------------------------------------------------------------------------------------------------- //
+template <auto KERNEL>
+int raise_smem(int bytes) {
+    static bool set[64] = {};
+    int dev = 0;
+    PMG_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) return PMG_ERR_UNSUPPORTED;
+    if (!set[dev]) {
+        PMG_CUDA_TRY(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        set[dev] = true;
+    }
+    return PMG_OK;
+}
+
+struct Call {
+    Heads q, k, v;
+    void* o;
+    int64_t o_tok, o_head;
+    float* lse;
+    int max_q, max_k;
+    float* part;
+};
+
+bool few_rows(int max_q, int group) { return (int64_t)max_q * group <= kFewRows; }
+
+// Stretches of the keys: enough CTAs for four on every SM, none shorter than 256 keys.
+int few_splits(int docs, int Hk, int max_k) {
+    const int64_t want = (4 * kNumSMs + (int64_t)docs * Hk - 1) / std::max<int64_t>(1, (int64_t)docs * Hk);
+    return (int)std::max<int64_t>(1, std::min<int64_t>({want, (max_k + 255) / 256, 256}));
+}
+
+template <typename T, int DP, bool CAP, bool BIAS>
+int run(const Attn& a, const Call& c, cudaStream_t s) {
+    if (few_rows(c.max_q, a.group)) {
+        const int splits = few_splits(a.docs, a.Hk, c.max_k);
+        constexpr int smem = (kFewWarps * kFewRows * (DP + 2)) * sizeof(float);
+        const int rc = raise_smem<k_attn_few<T, DP, CAP, BIAS>>(smem);
+        if (rc != PMG_OK) return rc;
+        for (int d0 = 0; d0 < a.docs; d0 += 65535) {
+            Attn b = a;
+            b.docs = std::min(65535, a.docs - d0);
+            b.cu_q += d0;
+            b.cu_k += d0;
+            if (b.k_len) b.k_len += d0;
+            if (b.prefix) b.prefix += d0;
+            k_attn_few<T, DP, CAP, BIAS><<<dim3(splits, a.Hk, b.docs), 32 * kFewWarps, smem, s>>>(
+                c.q, c.k, c.v, b, c.max_q, splits, c.part, static_cast<T*>(c.o), c.o_tok, c.o_head, c.lse);
+            PMG_LAUNCH_CHECK();
+            if (splits > 1) {
+                const int rows = c.max_q * a.group;
+                k_attn_join<T, DP><<<dim3((rows + 3) / 4, a.Hk, b.docs), 128, 0, s>>>(b, c.max_q, splits, c.part,
+                                                                                     static_cast<T*>(c.o), c.o_tok, c.o_head, c.lse);
+                PMG_LAUNCH_CHECK();
+            }
+        }
+        return PMG_OK;
+    }
+    using C = Fwd<DP>;
+    const int rc = raise_smem<k_attn<T, DP, CAP, BIAS>>(C::kSmem);
+    if (rc != PMG_OK) return rc;
+    CUtensorMap mq, mk, mv;
+    int e = head_map(&mq, c.q.p, c.q.tok, c.q.head, a.Tq, a.Hq, a.D, 128);
+    if (e == PMG_OK) e = head_map(&mk, c.k.p, c.k.tok, c.k.head, std::max<int64_t>(a.Tk, 1), a.Hk, a.D, 128);
+    if (e == PMG_OK) e = head_map(&mv, c.v.p, c.v.tok, c.v.head, std::max<int64_t>(a.Tk, 1), a.Hk, a.D, 128);
+    if (e != PMG_OK) return e;
+    const int64_t blocks = (a.Tq / 256 + a.docs) * a.Hq;
+    if (blocks > INT32_MAX) return PMG_ERR_UNSUPPORTED;
+    k_attn<T, DP, CAP, BIAS><<<(int)blocks, kFwdThreads, C::kSmem, s>>>(mq, mk, mv, a, static_cast<T*>(c.o), c.o_tok, c.o_head, c.lse);
+    PMG_LAUNCH_CHECK();
+    return PMG_OK;
+}
+
+template <typename T, int DP>
+int by_score(const Attn& a, const Call& c, cudaStream_t s) {
+    if (a.cap2 > 0.0f) return a.slopes ? run<T, DP, true, true>(a, c, s) : run<T, DP, true, false>(a, c, s);
+    return a.slopes ? run<T, DP, false, true>(a, c, s) : run<T, DP, false, false>(a, c, s);
+}
+
+}  // namespace
+}  // namespace pmg
+
+using namespace pmg;
+
+extern "C" size_t pmg_attention_workspace_bytes(int32_t docs, int32_t Hq, int32_t Hk, int32_t D, int32_t max_q,
+                                                int32_t max_k) {
+    if (docs < 1 || Hk < 1 || Hq < Hk || max_q < 1 || !few_rows(max_q, Hq / Hk)) return 0;
+    const int splits = few_splits(docs, Hk, max_k);
+    return splits > 1 ? (size_t)std::min(docs, 65535) * Hk * splits * kFewRows * ((D <= 64 ? 64 : 128) + 4) * sizeof(float) : 0;
+}
+
+extern "C" int pmg_attention(const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok,
+                             int64_t k_head, const void* v, int64_t v_tok, int64_t v_head, int32_t dtype, int64_t Tq,
+                             int64_t Tk, int32_t Hq, int32_t Hk, int32_t D, const int32_t* cu_q, const int32_t* cu_k,
+                             const int32_t* k_len, int32_t docs, int32_t max_q, int32_t max_k, float scale,
+                             int32_t causal, const int32_t* prefix, float softcap, const float* slopes, void* o,
+                             int64_t o_tok, int64_t o_head, float* lse, void* workspace, size_t workspace_bytes,
+                             int32_t* status, void* stream) {
+    Attn a;
+    const int rc = fill_attn(&a, dtype, cu_q, cu_k, k_len, docs, Tq, Tk, Hq, Hk, D, scale, causal, prefix, softcap, slopes, status);
+    if (rc != PMG_OK) return rc;
+    if (docs == 0 || Tq == 0 || max_q == 0) return PMG_OK;
+    if (Tk == 0) {                    // nothing is read of the keys: any valid place serves their tensor maps
+        k = v = q;
+        k_tok = v_tok = q_tok;
+        k_head = v_head = q_head;
+    }
+    if (!q || !k || !v || !o || !lse || max_q < 0 || max_k < 0) return PMG_ERR_BAD_ARG;
+    auto ok = [](const void* p, int64_t t, int64_t h) { return !(reinterpret_cast<uintptr_t>(p) & 15) && !(t & 7) && !(h & 7); };
+    if (!ok(q, q_tok, q_head) || !ok(k, k_tok, k_head) || !ok(v, v_tok, v_head) || !ok(o, o_tok, o_head)) return PMG_ERR_BAD_ARG;
+    const size_t need = pmg_attention_workspace_bytes(docs, Hq, Hk, D, max_q, max_k);
+    if (workspace_bytes < need || (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15)))) return PMG_ERR_BAD_ARG;
+    Call c{{q, q_tok, q_head}, {k, k_tok, k_head}, {v, v_tok, v_head}, o, o_tok, o_head, lse, max_q, max_k, static_cast<float*>(workspace)};
+    cudaStream_t s = as_stream(stream);
+    if (dtype == PMG_BF16) return D <= 64 ? by_score<__nv_bfloat16, 64>(a, c, s) : by_score<__nv_bfloat16, 128>(a, c, s);
+    return D <= 64 ? by_score<__half, 64>(a, c, s) : by_score<__half, 128>(a, c, s);
+}

@@ -2,6 +2,7 @@
 
   linear / linear_grad                  act(x W^T + b) + r in one pass, and the gradients of x, W, b
   qk_norm_rope / qk_norm_rope_grad      per-head norm of queries and keys with the position rotation, and its gradient
+  attention / attention_grad            attention within documents: causal, prefix, capped scores, distance bias
 
 Tokens of several frames (or streams) are packed one after another along the first axis.  Tensors are CUDA tensors of
 one device, floating point, with contiguous innermost axis and otherwise any strides; kernels run on that device's
@@ -306,3 +307,86 @@ def qk_norm_rope_grad(dq, dk, q, k, q_weight, k_weight, cos, sin, positions=None
               gqw.data_ptr() if gqw is not None else None, gkw.data_ptr() if gkw is not None else None,
               ws.data_ptr() if need else None, need, _status(index), stream)
     return gq, gk, gqw, gkw
+
+
+# ----------------------------------------------------------------------------------------------------------------- #
+# Attention over packed documents
+# ----------------------------------------------------------------------------------------------------------------- #
+def _aligned_heads(t, name, shape, index, dt):
+    """(pointer, token stride, head stride) of [T, H, D] on 16-byte boundaries."""
+    _dev(t, name, 3, index, (dt,))
+    if shape is not None:
+        _shape(t, shape, name)
+    T, H, D = t.shape
+    p, st, sh = t.data_ptr(), t.stride(0), t.stride(1)
+    if T <= 1:
+        st = H * D if sh == D or H <= 1 else (st + 7) // 8 * 8
+    if H <= 1:
+        sh = D
+    if p & 15 or st & 7 or sh & 7:
+        raise ValueError(f"{name}: heads must start on 16-byte boundaries (strides in multiples of 8 values)")
+    return p, st, sh
+
+
+def _packing(cu_q, cu_k, k_len, prefix, slopes, Hq, index):
+    docs = cu_q.shape[0] - 1
+    for t, name, n in ((cu_q, "cu_q", docs + 1), (cu_k, "cu_k", docs + 1), (k_len, "k_len", docs),
+                       (prefix, "prefix", docs)):
+        if t is not None:
+            _shape(_dev(t, name, 1, index, (torch.int32,)), (n,), name)
+    if docs < 0:
+        raise ValueError("cu_q must hold the documents' offsets, the total last")
+    if slopes is not None:
+        _shape(_dev(slopes, "slopes", 1, index, (torch.float32,)), (Hq,), "slopes")
+    return docs
+
+
+def _attention_shapes(q, k, v):
+    _dev(q, "q", 3, None, _HALF)
+    index, dt = q.get_device(), q.dtype
+    Tq, Hq, D = q.shape
+    _dev(k, "k", 3, index, (dt,))
+    Tk, Hk, _ = k.shape
+    if k.shape[2] != D or Hk < 1 or Hq < 1 or Hq % Hk:
+        raise ValueError(f"k must be [keys, heads, {D}] with a number of heads that divides {Hq}, got {tuple(k.shape)}")
+    _shape(v, k.shape, "v")
+    if D % 8 or not 8 <= D <= 128:
+        raise ValueError(f"heads must hold a multiple of 8 values, 8 to 128, got {D}")
+    return index, dt, Tq, Tk, Hq, Hk, D
+
+
+def attention(q, k, v, cu_q, cu_k, max_q: int, max_k: int, scale: float | None = None, causal: bool = False,
+              prefix=None, softcap: float = 0.0, slopes=None, k_len=None, out=None):
+    """Attention within documents.  q [Tq, Hq, D], k and v [Tk, Hk, D] of one 16-bit type, Hq a multiple of Hk; cu_q,
+    cu_k [documents + 1] int32: document d holds queries cu_q[d] .. cu_q[d+1] and keys cu_k[d] .. cu_k[d+1], or only
+    the first k_len[d] of these (int32: a cache with spare room).  max_q, max_k: the most queries and keys of any
+    document.  Query i stands at place p = i + Lk - Lq among its document's keys; causal: it sees keys j <= p, and j <
+    prefix[d] (int32) where prefix is given.  Scores: scale (default D ** -0.5) times q.k, through softcap *
+    tanh(. / softcap) if softcap is not 0, less slopes[h] (fp32) * |p - j| if slopes are given.
+
+    Returns (o [Tq, Hq, D], lse [Hq, Tq] fp32).  Rows that see no key give 0 and -inf.  max_q * Hq / Hk <= 16 (token by
+    token) takes the kernel that reads the keys once for all rows."""
+    index, dt, Tq, Tk, Hq, Hk, D = _attention_shapes(q, k, v)
+    docs = _packing(cu_q, cu_k, k_len, prefix, slopes, Hq, index)
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf") or not 0.0 <= softcap < float("inf"):
+        raise ValueError("scale must be positive and softcap not negative, both finite")
+    if max_q < 0 or max_k < 0:
+        raise ValueError("max_q and max_k must not be negative")
+    if prefix is not None and not causal:
+        raise ValueError("prefix needs causal (without it every key is seen)")
+    o = torch.empty((Tq, Hq, D), dtype=dt, device=q.device) if out is None else out
+    lse = torch.empty((Hq, Tq), dtype=torch.float32, device=q.device)
+    if not Tq:
+        return o, lse
+    oh = _aligned_heads(o, "out", (Tq, Hq, D), index, dt)
+    need = _query("pmg_attention_workspace_bytes", docs, Hq, Hk, D, max_q, max_k)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    with _On(index) as stream:
+        _call("pmg_attention", *_aligned_heads(q, "q", None, index, dt), *_aligned_heads(k, "k", None, index, dt),
+              *_aligned_heads(v, "v", None, index, dt), _DTYPES[dt], Tq, Tk, Hq, Hk, D, cu_q.data_ptr(),
+              cu_k.data_ptr(), k_len.data_ptr() if k_len is not None else None, docs, max_q, max_k, scale, int(causal),
+              prefix.data_ptr() if prefix is not None else None, softcap,
+              slopes.data_ptr() if slopes is not None else None, *oh, lse.data_ptr(),
+              ws.data_ptr() if need else None, need, _status(index), stream)
+    return o, lse
