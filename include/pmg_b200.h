@@ -543,8 +543,9 @@ int pmg_qk_norm_rope_grad(const void* dq, int64_t dq_tok, int64_t dq_head, const
 /* Attention over packed documents.  q, o [Tq,Hq,D]; k, v [Tk,Hk,D] (F16 or BF16; strides of token and head, values of
  * a head contiguous; pointers and strides on 16-byte boundaries; D a multiple of 8 up to 128; Hq a multiple of Hk, heads
  * h * Hq/Hk .. sharing key head h).  Document d holds queries cu_q[d] .. cu_q[d+1] and keys cu_k[d] .. cu_k[d+1] (device
- * int32 [docs+1], non-decreasing, within Tq and Tk), of the latter only the first k_len[d] where k_len is given (a cache
- * with spare room).  max_q, max_k: upper bounds of a document's queries and keys, which choose the kernel; a document
+ * int32 [docs+1], from 0 to Tq and Tk without decreasing; rows of no document are not written), of the latter only the
+ * first k_len[d] where k_len is given (a cache with spare room).  Offsets and lengths that leave the tensors or each
+ * other are cut to them and set PMG_ERR_RANGE in `status`.  max_q, max_k: upper bounds of a document's queries and keys, which choose the kernel; a document
  * with more queries sets PMG_ERR_RANGE.
  * Query i of a document stands at place p = i + Lk - Lq among its Lk keys and attends to key j if j <= p or
  * j < prefix[d] (causal; prefix may be NULL), or to all of them.  Scores: s = scale q.k; softcap > 0: s = softcap
@@ -558,6 +559,20 @@ int pmg_attention(const void* q, int64_t q_tok, int64_t q_head, const void* k, i
                   int32_t max_q, int32_t max_k, float scale, int32_t causal, const int32_t* prefix, float softcap,
                   const float* slopes, void* o, int64_t o_tok, int64_t o_head, float* lse, void* workspace,
                   size_t workspace_bytes, int32_t* status, void* stream);
+
+/* Gradients of pmg_attention: dout [Tq,Hq,D] is that of o; o and lse are the forward call's outputs, the rest its
+ * inputs (same rules).  dq [Tq,Hq,D], dk, dv [Tk,Hk,D] (shared key heads: summed over their group); rows of a cache
+ * behind k_len[d] get zeros.  No atomics: equal inputs give equal bits.  With no queries or no keys at all the outputs
+ * must be contiguous and are zeroed. */
+size_t pmg_attention_grad_workspace_bytes(int64_t Tq, int32_t Hq);
+int pmg_attention_grad(const void* dout, int64_t do_tok, int64_t do_head, const void* o, int64_t o_tok, int64_t o_head,
+                       const float* lse, const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok,
+                       int64_t k_head, const void* v, int64_t v_tok, int64_t v_head, int32_t dtype, int64_t Tq,
+                       int64_t Tk, int32_t Hq, int32_t Hk, int32_t D, const int32_t* cu_q, const int32_t* cu_k,
+                       const int32_t* k_len, int32_t docs, float scale, int32_t causal, const int32_t* prefix,
+                       float softcap, const float* slopes, void* dq, int64_t dq_tok, int64_t dq_head, void* dk,
+                       int64_t dk_tok, int64_t dk_head, void* dv, int64_t dv_tok, int64_t dv_head, void* workspace,
+                       size_t workspace_bytes, int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

@@ -106,6 +106,10 @@ SIGNATURES = {
     "pmg_attention_workspace_bytes": (SZ, [I32, I32, I32, I32, I32, I32]),
     "pmg_attention": (I32, [P, I64, I64, P, I64, I64, P, I64, I64, I32, I64, I64, I32, I32, I32, P, P, P, I32, I32, I32,
                             F32, I32, P, F32, P, P, I64, I64, P, P, SZ, P, P]),
+    "pmg_attention_grad_workspace_bytes": (SZ, [I64, I32]),
+    "pmg_attention_grad": (I32, [P, I64, I64, P, I64, I64, P, P, I64, I64, P, I64, I64, P, I64, I64, I32, I64, I64, I32,
+                                 I32, I32, P, P, P, I32, F32, I32, P, F32, P, P, I64, I64, P, I64, I64, P, I64, I64, P,
+                                 SZ, P, P]),
     "pmg_qk_norm_rope": (I32, [P, I64, I64, P, I64, I64, I32, I64, I32, I32, I32, I32, P, P, P, P, I32, P, F32, I32,
                                P, I64, I64, P, I64, I64, P, P]),
     "pmg_qk_norm_rope_grad_workspace_bytes": (SZ, [I32]),

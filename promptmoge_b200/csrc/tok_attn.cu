@@ -63,11 +63,6 @@ struct Fwd {
 
 constexpr int kFwdThreads = 320;               // two softmax warpgroups, the loader, the MMA issuer
 
-#define TOK_WAIT(bar, parity)                                                                   \
-    do {                                                                                        \
-        if (!__all_sync(0xffffffffu, mbar_wait((bar), (parity), abort_flag))) { ok = false; break; } \
-    } while (0)
-
 template <typename T, int DP, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kFwdThreads, 1)
     k_attn(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
@@ -592,8 +587,9 @@ __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ Attn 
                                                    int64_t o_head, float* __restrict__ lse) {
     pdl_begin();
     const int lane = threadIdx.x & 31, r = blockIdx.x * 4 + (threadIdx.x >> 5), kvh = blockIdx.y, doc = blockIdx.z;
-    const int q0 = a.cu_q[doc], lq = min(max(0, a.cu_q[doc + 1] - q0), max_q);
-    if (r >= lq * a.group) return;
+    const Span sp = span_of(a, doc);
+    const int q0 = sp.q0;
+    if (r >= min(sp.lq, max_q) * a.group) return;
     const float* from = part + (((int64_t)doc * a.Hk + kvh) * splits * kFewRows + r) * (DP + 4);
     constexpr int64_t step = kFewRows * (DP + 4);
     float top = -INFINITY;

@@ -10,6 +10,12 @@
 
 #include "tok_common.cuh"
 
+// A whole warp's bounded wait; clears `ok` where any lane gave up.
+#define TOK_WAIT(bar, parity)                                                                        \
+    do {                                                                                             \
+        if (!__all_sync(0xffffffffu, mbar_wait((bar), (parity), abort_flag))) { ok = false; break; } \
+    } while (0)
+
 namespace pmg {
 namespace tok {
 
@@ -26,15 +32,20 @@ struct Attn {
 
 struct Span {
     int q0, lq, k0, lk, prefix;      // first query row and count, first key row and count
+    int room;                        // key rows that belong to the document
 };
 
+// A document's span, cut to the tensors: offsets that leave them, run backwards, or lengths over the room are reported.
 __device__ __forceinline__ Span span_of(const Attn& a, int d) {
     Span s;
-    s.q0 = a.cu_q[d];
-    s.lq = max(0, a.cu_q[d + 1] - s.q0);
-    s.k0 = a.cu_k[d];
-    const int room = max(0, a.cu_k[d + 1] - s.k0);
-    s.lk = a.k_len ? max(0, min(a.k_len[d], room)) : room;
+    s.q0 = min(max(a.cu_q[d], 0), (int)a.Tq);
+    s.lq = min(max(a.cu_q[d + 1], s.q0), (int)a.Tq) - s.q0;
+    s.k0 = min(max(a.cu_k[d], 0), (int)a.Tk);
+    s.room = min(max(a.cu_k[d + 1], s.k0), (int)a.Tk) - s.k0;
+    s.lk = a.k_len ? max(0, min(a.k_len[d], s.room)) : s.room;
+    if (threadIdx.x == 0 && (s.q0 != a.cu_q[d] || s.q0 + s.lq != a.cu_q[d + 1] || s.k0 != a.cu_k[d] ||
+                             s.k0 + s.room != a.cu_k[d + 1] || (a.k_len && s.lk != a.k_len[d])))
+        flag(a.status, PMG_ERR_RANGE);
     s.prefix = a.prefix ? min(max(a.prefix[d], 0), s.lk) : 0;
     return s;
 }

@@ -1,0 +1,597 @@
+// Gradients of attention over packed documents.
+//
+//   P = exp(s - lse), dV = P^T dO, dP = dO V^T, dS = P (dP - delta), delta = rowsum(dO o),
+//   through the cap: dS (1 - (s_c / cap)^2);  dQ = scale dS K, dK = scale dS^T Q, the shared key heads' sums over their
+//   group taken by the kernel that owns the keys.
+//
+// One launch, two kinds of CTA, each with 128 stationary rows: keys (dK, dV; streams the queries of all heads that share
+// the key head) and queries (dQ; streams the keys).  Both compute scores and dP with their own rows in tensor-memory
+// lanes, so the probabilities and dS are left operands where they stand, in the columns their inputs leave, and nothing
+// is transposed or sent through shared memory.  Scores are computed twice for it (7 products a tile instead of 5), and
+// in return no gradient is summed by atomics: results do not depend on timing, and no fp32 copy of dQ is kept.
+// P and dS are rounded to the operands' 16-bit type (tensor cores take no other); fp16 values are kept times a power of
+// two, 2^15 for P (which is at most 1) and for dS the one that |dS| <= 2 max|dO| max|V| allows, so that small gradients
+// do not turn subnormal.
+#include <algorithm>
+
+#include "tok_attn.cuh"
+
+namespace pmg {
+namespace {
+
+using namespace tok;
+
+constexpr int kStatBlocks = 256;
+constexpr int kStatPad = 132;                 // columns a tile may read past the last row
+
+struct Grad {
+    Attn a;
+    float scale;
+    const float2* stat;      // [Hq][stat_ld] lse log2 e (infinite for empty rows), delta
+    const float* norms;      // fp16: [2][kStatBlocks] largest |dO|^2 and |V|^2 of each block's rows
+    int64_t stat_ld;
+    void *dq, *dk, *dv;
+    int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;      // of dq, dk, dv
+    int key_blocks;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(256)
+    k_attn_stat(const T* __restrict__ dout, int64_t do_tok, int64_t do_head, const T* __restrict__ o, int64_t o_tok,
+                int64_t o_head, const float* __restrict__ lse, const T* __restrict__ v, int64_t v_tok, int64_t v_head,
+                int64_t Tq, int64_t Tk, int Hq, int Hk, int D, float2* __restrict__ stat, int64_t stat_ld,
+                float* __restrict__ norms) {
+    pdl_begin();
+    constexpr int G = DP / 8, kRows = 256 / G;            // lanes a row
+    const int gl = threadIdx.x % G;
+    const bool in = 8 * gl < D;
+    float big_do = 0.0f, big_v = 0.0f;
+    const int64_t rows = Tq * Hq;
+    for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < rows; r0 += (int64_t)gridDim.x * kRows) {
+        const int64_t r = r0 + threadIdx.x / G, t = r / Hq;
+        const int h = (int)(r - t * Hq);
+        float dot = 0.0f, sq = 0.0f;
+        if (r < rows && in) {
+            const uint4 x = *reinterpret_cast<const uint4*>(dout + t * do_tok + h * do_head + 8 * gl);
+            const uint4 y = *reinterpret_cast<const uint4*>(o + t * o_tok + h * o_head + 8 * gl);
+            const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 a = Elem<T>::unpack(xs[i]), b = Elem<T>::unpack(ys[i]);
+                dot += a.x * b.x + a.y * b.y;
+                sq += a.x * a.x + a.y * a.y;
+            }
+        }
+#pragma unroll
+        for (int x = G / 2; x > 0; x >>= 1) {
+            dot += __shfl_xor_sync(0xffffffffu, dot, x);
+            sq += __shfl_xor_sync(0xffffffffu, sq, x);
+        }
+        if (sq < INFINITY) big_do = fmaxf(big_do, sq);
+        if (r < rows && gl == 0) {
+            const float l = lse[(int64_t)h * Tq + t];
+            stat[h * stat_ld + t] = make_float2(l == -INFINITY ? INFINITY : l * kLog2e, dot);
+        }
+    }
+    if constexpr (Elem<T>::kFmt == 0) {
+        const int64_t vrows = Tk * Hk;
+        for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < vrows; r0 += (int64_t)gridDim.x * kRows) {
+            const int64_t r = r0 + threadIdx.x / G, t = r / Hk;
+            const int h = (int)(r - t * Hk);
+            float sq = 0.0f;
+            if (r < vrows && in) {
+                const uint4 x = *reinterpret_cast<const uint4*>(v + t * v_tok + h * v_head + 8 * gl);
+                const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 a = Elem<T>::unpack(xs[i]);
+                    sq += a.x * a.x + a.y * a.y;
+                }
+            }
+#pragma unroll
+            for (int x = G / 2; x > 0; x >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, x);
+            if (sq < INFINITY) big_v = fmaxf(big_v, sq);
+        }
+        __shared__ float sm[2][8];
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) {
+            big_do = fmaxf(big_do, __shfl_xor_sync(0xffffffffu, big_do, x));
+            big_v = fmaxf(big_v, __shfl_xor_sync(0xffffffffu, big_v, x));
+        }
+        if ((threadIdx.x & 31) == 0) {
+            sm[0][threadIdx.x >> 5] = big_do;
+            sm[1][threadIdx.x >> 5] = big_v;
+        }
+        __syncthreads();
+        if (threadIdx.x < 2) {
+            float m = 0.0f;
+            for (int i = 0; i < 8; ++i) m = fmaxf(m, sm[threadIdx.x][i]);
+            norms[threadIdx.x * kStatBlocks + blockIdx.x] = m;
+        }
+    }
+}
+
+template <int DP>
+struct Bwd {
+    static constexpr int kTile = 128 * DP * 2;
+    static constexpr int kStages = DP == 64 ? 4 : 2;
+    static constexpr int kStat = 130 * 8;                     // bytes of a tile's stats: from an even column on
+    static constexpr int kStatRoom = 1152;
+    static constexpr int kStream = 2 * kTile;                 // offset of the ring
+    static constexpr int kStats = kStream + kStages * 2 * kTile;
+    static constexpr int kBars = kStats + kStages * kStatRoom;
+    static constexpr int kSmem = kBars + 512;
+    static constexpr uint32_t kS = 0, kDP = 128, kOut0 = 256, kOut1 = 256 + DP;
+};
+
+constexpr int kBwdThreads = 320;              // two compute warpgroups (halves of the columns), the loader, the issuer
+
+struct Bars {
+    uint64_t *a_full, *b_full, *b_empty, *s_full, *dp_full, *p_full, *ds_full, *done, *drain;
+    volatile int* abort_flag;
+};
+
+// The factor that dS carries before it is rounded.
+template <typename T>
+__device__ __forceinline__ float ds_lift(const float* norms) {
+    if constexpr (Elem<T>::kFmt == 1) {
+        return 1.0f;
+    } else {
+        const int lane = threadIdx.x & 31;
+        float a = 0.0f, b = 0.0f;
+        for (int i = lane; i < kStatBlocks; i += 32) {
+            a = fmaxf(a, norms[i]);
+            b = fmaxf(b, norms[kStatBlocks + i]);
+        }
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) {
+            a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, x));
+            b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, x));
+        }
+        // log2 (2 max|dO| max|V|) = 1 + (log2 a + log2 b) / 2
+        const float l = 1.0f + 0.5f * (log2f(a) + log2f(b));
+        return a > 0.0f && b > 0.0f ? exp2f(fminf(fmaxf(floorf(14.0f - l), -60.0f), 60.0f)) : 1.0f;
+    }
+}
+
+template <typename T, int DP, bool KEYS, bool CAP, bool BIAS>
+__device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorMap& ma1, const CUtensorMap& mb0,
+                                         const CUtensorMap& mb1, const Grad& g, uint8_t* smem, const Bars& b,
+                                         uint32_t tmem, int block, int doc, int tile) {
+    using C = Bwd<DP>;
+    const Attn& a = g.a;
+    volatile int* abort_flag = b.abort_flag;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Span sp = span_of(a, doc);
+    const int off = sp.lk - sp.lq;
+    const int head = KEYS ? 0 : block % a.Hq;                       // query CTAs: their head
+    const int kvh = KEYS ? block % a.Hk : head / a.group;
+    const int r0 = tile * 128;                                      // first stationary row within the document
+    // streamed tiles of 128: queries t0 .. t1 - 1 of each head of the group, or keys
+    int t0 = 0, t1 = 0;
+    if (KEYS) {
+        if (r0 < sp.lk) {
+            t1 = (sp.lq + 127) / 128;
+            if (a.causal && r0 >= sp.prefix) t0 = min(t1, max(0, r0 - off) / 128);
+        }
+    } else {
+        t1 = (key_end(a, sp, r0 + 128) + 127) / 128;
+    }
+    const int per = t1 - t0, total = KEYS ? per * a.group : per;
+
+    if (warp == 8) {
+        if (lane == 0 && total > 0) {
+            bool ok = true;
+            const int row = (KEYS ? sp.k0 : sp.q0) + r0, h = KEYS ? kvh : head;
+            mbar_arrive_expect_tx(b.a_full, 2 * C::kTile);
+#pragma unroll
+            for (int c = 0; c < DP / 64; ++c) {
+                tma_tile3d(smem_u32(smem + c * 16384), &ma0, 64 * c, h, row, b.a_full);
+                tma_tile3d(smem_u32(smem + C::kTile + c * 16384), &ma1, 64 * c, h, row, b.a_full);
+            }
+            for (int i = 0; i < total; ++i) {
+                const int st = i % C::kStages;
+                if (!mbar_wait(b.b_empty + st, ((i / C::kStages) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                const int t = t0 + i % per, bh = KEYS ? kvh * a.group + i / per : kvh;
+                const int brow = (KEYS ? sp.q0 : sp.k0) + 128 * t;
+                uint8_t* to = smem + C::kStream + st * 2 * C::kTile;
+                mbar_arrive_expect_tx(b.b_full + st, 2 * C::kTile + (KEYS ? C::kStat : 0));
+#pragma unroll
+                for (int c = 0; c < DP / 64; ++c) {
+                    tma_tile3d(smem_u32(to + c * 16384), &mb0, 64 * c, bh, brow, b.b_full + st);
+                    tma_tile3d(smem_u32(to + C::kTile + c * 16384), &mb1, 64 * c, bh, brow, b.b_full + st);
+                }
+                if (KEYS)
+                    bulk_g2s(smem_u32(smem + C::kStats + st * C::kStatRoom), g.stat + bh * g.stat_ld + (brow & ~1), C::kStat,
+                             b.b_full + st);
+            }
+            if (!ok) {
+                *abort_flag = 1;
+                flag(a.status, PMG_ERR_TIMEOUT);
+            }
+        }
+    } else if (warp == 9) {
+        const int ksteps = (a.D + 15) / 16;
+        const uint32_t id_s = idesc16(Elem<T>::kFmt, 128, 128, false, false);
+        const uint32_t id_o = idesc16(Elem<T>::kFmt, 128, ksteps * 16, false, true);
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t ph) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, ph, abort_flag)); };
+        auto stage = [&](int i) { return smem + C::kStream + (i % C::kStages) * 2 * C::kTile; };
+        // a streamed tile has landed; rows behind the document's last must not reach a sum over rows (0 * NaN)
+        auto landed = [&](int i) {
+            if (!wait(b.b_full + i % C::kStages, (i / C::kStages) & 1u)) return false;
+            const int valid = (KEYS ? sp.lq : sp.lk) - 128 * (t0 + i % per);
+            if (valid < 128) {
+                uint8_t* s = stage(i);
+                for (int c = 0; c < (KEYS ? 2 : 1) * (DP / 64); ++c)
+                    for (int x = valid * 128 + lane * 16; x < 16384; x += 512)
+                        *reinterpret_cast<uint4*>(s + c * 16384 + x) = make_uint4(0, 0, 0, 0);
+                fence_proxy_async();
+                __syncwarp();
+            }
+            return true;
+        };
+        auto square = [&](int i, int which) {           // scores (0) or dP (1) of tile i
+            tc_fence_after();
+            if (lane == 0) {
+                const uint32_t x = smem_u32(smem + which * C::kTile), y = smem_u32(stage(i) + which * C::kTile);
+                for (int s = 0; s < ksteps; ++s) {
+                    const uint32_t at = (s >> 2) * 16384 + (s & 3) * 32;
+                    mma16(tmem + (which ? C::kDP : C::kS), desc16(x + at, 16), desc16(y + at, 16), id_s, s > 0);
+                }
+                mma_commit(which ? b.dp_full : b.s_full);
+            }
+            __syncwarp();
+        };
+        auto sum = [&](int i, int which) {              // out0 += dS B0, out1 += P B1
+            tc_fence_after();
+            if (lane == 0) {
+                const uint32_t x = tmem + (which ? C::kS : C::kDP), y = smem_u32(stage(i) + which * C::kTile);
+#pragma unroll
+                for (int s = 0; s < 8; ++s)             // each warpgroup's half lies in its own columns
+                    mma16_ts(tmem + (which ? C::kOut1 : C::kOut0), x + (s >> 2) * 64 + (s & 3) * 8, desc16(y + s * 2048, 16384),
+                             id_o, i > 0 || s > 0);
+            }
+            __syncwarp();
+        };
+        if (total > 0) {
+            ok = wait(b.a_full, 0) && landed(0);
+            if (ok) {
+                square(0, 0);
+                square(0, 1);
+            }
+            for (int i = 0; i < total && ok; ++i) {
+                ok = wait(b.p_full, i & 1u);
+                if (!ok) break;
+                if (KEYS) sum(i, 1);
+                if (i + 1 < total) {
+                    ok = landed(i + 1);
+                    if (!ok) break;
+                    square(i + 1, 0);
+                }
+                ok = wait(b.ds_full, i & 1u);
+                if (!ok) break;
+                sum(i, 0);
+                if (lane == 0) mma_commit(b.b_empty + i % C::kStages);
+                if (i + 1 < total) square(i + 1, 1);
+            }
+            if (lane == 0) {
+                if (ok) mma_commit(b.done);
+                else flag(a.status, PMG_ERR_TIMEOUT);
+                if (!ok || *abort_flag) {
+                    *abort_flag = 1;
+                    drain_mma(b.drain);
+                }
+            }
+            __syncwarp();
+        }
+    } else {
+        const int w = warp >> 2, row = r0 + (warp & 3) * 32 + lane;        // column half; stationary row in the document
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + lanes + C::kS + 64 * w, td = tmem + lanes + C::kDP + 64 * w;
+        constexpr float kP = Elem<T>::kFmt == 0 ? 15.0f : 0.0f;            // log2 of the factor P carries
+        const float lift = ds_lift<T>(g.norms);
+        const float pd = Elem<T>::kFmt == 0 ? lift * exp2f(-kP) : 1.0f;
+        const float c = (CAP || BIAS) ? 1.0f : a.scale2;
+        // columns [lo, hi) of the streamed side take part in this row
+        int lo = 0, hi;
+        if (KEYS) {
+            hi = sp.lq;
+            if (a.causal && row >= sp.prefix) lo = max(0, row - off);
+        } else {
+            hi = last_key(a, sp, row) + 1;
+        }
+        const bool live = row < (KEYS ? sp.lk : sp.lq);
+        const int lo_max = __reduce_max_sync(0xffffffffu, live ? lo : 0), hi_min = __reduce_min_sync(0xffffffffu, live ? hi : INT32_MAX);
+        float my_lse = INFINITY, my_delta = 0.0f;
+        if (!KEYS && live && sp.q0 + (int64_t)row < a.Tq) {
+            const float2 s = g.stat[head * g.stat_ld + sp.q0 + row];
+            my_lse = s.x;
+            my_delta = s.y;
+        }
+        bool ok = true;
+        for (int i = 0; i < total; ++i) {
+            const int t = t0 + i % per, c0 = 128 * t + 64 * w;             // first column within the document
+            const int h = KEYS ? kvh * a.group + i / per : head;
+            const float slope = BIAS ? a.slopes[h] * kLog2e : 0.0f;
+            const float far = KEYS ? (float)(c0 + off - row) : (float)(c0 - (row + off));
+            const bool masked = c0 < lo_max || c0 + 64 > hi_min;
+            const float2* st = reinterpret_cast<const float2*>(smem + C::kStats + (i % C::kStages) * C::kStatRoom) +
+                               ((sp.q0 + 128 * t) & 1) + 64 * w;
+            if (KEYS) TOK_WAIT(b.b_full + i % C::kStages, (i / C::kStages) & 1u);
+            if (!ok) break;
+            TOK_WAIT(b.s_full, i & 1u);
+            if (!ok) break;
+            tc_fence_after();
+            float p[64], u[CAP ? 64 : 1];
+            tmem_ld32(ts, reinterpret_cast<uint32_t*>(p));
+            tmem_ld32(ts + 32, reinterpret_cast<uint32_t*>(p) + 32);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 64; ++k) {
+                float x = p[k];
+                if (CAP) {
+                    u[k] = fmaf(-2.0f, rcp_approx(ex2(x * a.tanh_in) + 1.0f), 1.0f);
+                    x = a.cap2 * u[k];
+                } else if (BIAS) {
+                    x *= a.scale2;
+                }
+                if (BIAS) x = fmaf(-slope, fabsf(far + (float)k), x);
+                p[k] = ex2(fmaf(x, c, kP - (KEYS ? st[k].x : my_lse)));
+            }
+            if (masked) {
+#pragma unroll
+                for (int k = 0; k < 64; ++k)
+                    if (c0 + k < lo || c0 + k >= hi) p[k] = 0.0f;
+            }
+            if (KEYS) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    uint32_t r[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) r[k] = Elem<T>::pack(p[32 * q + 2 * k], p[32 * q + 2 * k + 1]);
+                    tmem_st16(ts + 16 * q, r);
+                }
+                tmem_wait_st();
+            }
+            tc_fence_before();
+            mbar_arrive(b.p_full);
+            TOK_WAIT(b.dp_full, i & 1u);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                float d[32];
+                uint32_t r[16];
+                tmem_ld32(td + 32 * q, reinterpret_cast<uint32_t*>(d));
+                tmem_wait_ld();
+#pragma unroll
+                for (int k = 0; k < 32; ++k) {
+                    float x = p[32 * q + k] * (d[k] - (KEYS ? st[32 * q + k].y : my_delta));
+                    if (Elem<T>::kFmt == 0) x *= pd;
+                    if (CAP) x *= fmaf(-u[32 * q + k], u[32 * q + k], 1.0f);
+                    d[k] = x;
+                }
+                if (masked) {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k)
+                        if (c0 + 32 * q + k < lo || c0 + 32 * q + k >= hi) d[k] = 0.0f;
+                }
+#pragma unroll
+                for (int k = 0; k < 16; ++k) r[k] = Elem<T>::pack(d[2 * k], d[2 * k + 1]);
+                tmem_st16(td + 16 * q, r);        // behind what this warp has read: columns 32 q .. 32 q + 31
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(b.ds_full);
+        }
+        if (ok && total > 0) TOK_WAIT(b.done, 0);
+        if (ok) {
+            tc_fence_after();
+            const float f0 = g.scale / lift, f1 = Elem<T>::kFmt == 0 ? exp2f(-kP) : 1.0f;
+            const int room = KEYS ? sp.room : sp.lq;        // rows behind k_len get zeros
+            const int64_t at = (KEYS ? sp.k0 : sp.q0) + (int64_t)row;
+            const bool mine = row < room && at < (KEYS ? a.Tk : a.Tq);
+            const bool zero = total == 0 || !live;
+#pragma unroll
+            for (int which = 0; which < (KEYS ? 2 : 1); ++which) {
+                T* base = KEYS ? static_cast<T*>(which ? g.dv : g.dk) + at * (which ? g.v_tok : g.k_tok) + kvh * (which ? g.v_head : g.k_head)
+                               : static_cast<T*>(g.dq) + at * g.q_tok + head * g.q_head;
+                const float f = which ? f1 : f0;
+#pragma unroll
+                for (int q = 0; q < DP / 64; ++q) {
+                    const int c1 = w * (DP / 2) + 32 * q;
+                    float v[32];
+                    if (total > 0) {
+                        tmem_ld32(tmem + lanes + (which ? C::kOut1 : C::kOut0) + c1, reinterpret_cast<uint32_t*>(v));
+                        tmem_wait_ld();
+                    }
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) v[k] = zero ? 0.0f : v[k] * f;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (mine && c1 + 8 * k < a.D)
+                            *reinterpret_cast<uint4*>(base + c1 + 8 * k) =
+                                make_uint4(Elem<T>::pack(v[8 * k], v[8 * k + 1]), Elem<T>::pack(v[8 * k + 2], v[8 * k + 3]),
+                                           Elem<T>::pack(v[8 * k + 4], v[8 * k + 5]), Elem<T>::pack(v[8 * k + 6], v[8 * k + 7]));
+                }
+            }
+        } else if (lane == 0) {
+            *abort_flag = 1;
+            flag(a.status, PMG_ERR_TIMEOUT);
+        }
+    }
+}
+
+template <typename T, int DP, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+    k_attn_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo, const __grid_constant__ Grad g) {
+    using C = Bwd<DP>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    Bars b;
+    b.a_full = reinterpret_cast<uint64_t*>(smem + C::kBars);
+    b.b_full = b.a_full + 1;
+    b.b_empty = b.b_full + C::kStages;
+    b.s_full = b.b_empty + C::kStages;
+    b.dp_full = b.s_full + 1;
+    b.p_full = b.dp_full + 1;
+    b.ds_full = b.p_full + 1;
+    b.done = b.ds_full + 1;
+    b.drain = b.done + 1;
+    uint32_t* slot = reinterpret_cast<uint32_t*>(b.drain + 1);
+    b.abort_flag = reinterpret_cast<volatile int*>(slot + 1);
+    int* where = reinterpret_cast<int*>(slot + 2);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const bool keys = (int)blockIdx.x < g.key_blocks;
+    const int block = keys ? blockIdx.x : blockIdx.x - g.key_blocks;
+
+    if (threadIdx.x == 0) {
+        mbar_init(b.a_full, 1);
+        for (int i = 0; i < C::kStages; ++i) {
+            mbar_init(b.b_full + i, 1);
+            mbar_init(b.b_empty + i, 1);
+        }
+        mbar_init(b.s_full, 1);
+        mbar_init(b.dp_full, 1);
+        mbar_init(b.p_full, 256);
+        mbar_init(b.ds_full, 256);
+        mbar_init(b.done, 1);
+        mbar_init(b.drain, 1);
+        *b.abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == 9) tmem_alloc(slot, 512);
+    pdl_begin();
+    if (warp == 8) {
+        int doc = -1, tile = 0;
+        const bool found = find_tile(keys ? g.a.cu_k : g.a.cu_q, g.a.docs, 128, block / (keys ? g.a.Hk : g.a.Hq), &doc, &tile);
+        if (lane == 0) {
+            where[0] = found ? doc : -1;
+            where[1] = tile;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *slot;
+    if (where[0] >= 0) {
+        if (keys) grad_cta<T, DP, true, CAP, BIAS>(mk, mv, mq, mdo, g, smem, b, tmem, block, where[0], where[1]);
+        else grad_cta<T, DP, false, CAP, BIAS>(mq, mdo, mk, mv, g, smem, b, tmem, block, where[0], where[1]);
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+template <auto KERNEL>
+int raise_smem(int bytes) {
+    static bool set[64] = {};
+    int dev = 0;
+    PMG_CUDA_TRY(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) return PMG_ERR_UNSUPPORTED;
+    if (!set[dev]) {
+        PMG_CUDA_TRY(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+        set[dev] = true;
+    }
+    return PMG_OK;
+}
+
+struct Heads {
+    const void* p;
+    int64_t tok, head;
+};
+
+struct Ins {
+    Heads dout, o, q, k, v;
+    const float* lse;
+    float* ws;
+};
+
+template <typename T, int DP, bool CAP, bool BIAS>
+int run(Grad g, const Ins& in, cudaStream_t s) {
+    using C = Bwd<DP>;
+    const Attn& a = g.a;
+    const int rc = raise_smem<k_attn_grad<T, DP, CAP, BIAS>>(C::kSmem);
+    if (rc != PMG_OK) return rc;
+    float2* stat = reinterpret_cast<float2*>(in.ws + 2 * kStatBlocks);
+    k_attn_stat<T, DP><<<kStatBlocks, 256, 0, s>>>(static_cast<const T*>(in.dout.p), in.dout.tok, in.dout.head,
+                                                   static_cast<const T*>(in.o.p), in.o.tok, in.o.head, in.lse,
+                                                   static_cast<const T*>(in.v.p), in.v.tok, in.v.head, a.Tq, a.Tk, a.Hq, a.Hk,
+                                                   a.D, stat, g.stat_ld, in.ws);
+    PMG_LAUNCH_CHECK();
+    g.stat = stat;
+    g.norms = in.ws;
+    const int64_t key_blocks = (a.Tk / 128 + a.docs) * a.Hk, query_blocks = (a.Tq / 128 + a.docs) * a.Hq;
+    if (key_blocks + query_blocks > INT32_MAX) return PMG_ERR_UNSUPPORTED;
+    g.key_blocks = (int)key_blocks;
+    CUtensorMap mq, mk, mv, mdo;
+    int e = head_map(&mq, in.q.p, in.q.tok, in.q.head, a.Tq, a.Hq, a.D, 128);
+    if (e == PMG_OK) e = head_map(&mdo, in.dout.p, in.dout.tok, in.dout.head, a.Tq, a.Hq, a.D, 128);
+    if (e == PMG_OK) e = head_map(&mk, in.k.p, in.k.tok, in.k.head, a.Tk, a.Hk, a.D, 128);
+    if (e == PMG_OK) e = head_map(&mv, in.v.p, in.v.tok, in.v.head, a.Tk, a.Hk, a.D, 128);
+    if (e != PMG_OK) return e;
+    k_attn_grad<T, DP, CAP, BIAS><<<(int)(key_blocks + query_blocks), kBwdThreads, C::kSmem, s>>>(mq, mk, mv, mdo, g);
+    PMG_LAUNCH_CHECK();
+    return PMG_OK;
+}
+
+template <typename T, int DP>
+int by_score(const Grad& g, const Ins& in, cudaStream_t s) {
+    if (g.a.cap2 > 0.0f) return g.a.slopes ? run<T, DP, true, true>(g, in, s) : run<T, DP, true, false>(g, in, s);
+    return g.a.slopes ? run<T, DP, false, true>(g, in, s) : run<T, DP, false, false>(g, in, s);
+}
+
+}  // namespace
+}  // namespace pmg
+
+using namespace pmg;
+
+extern "C" size_t pmg_attention_grad_workspace_bytes(int64_t Tq, int32_t Hq) {
+    if (Tq < 0 || Hq < 0) return 0;
+    return 2 * kStatBlocks * sizeof(float) + ((size_t)(Tq + 1) / 2 * 2 * Hq + kStatPad) * sizeof(float2);
+}
+
+extern "C" int pmg_attention_grad(const void* dout, int64_t do_tok, int64_t do_head, const void* o, int64_t o_tok,
+                                  int64_t o_head, const float* lse, const void* q, int64_t q_tok, int64_t q_head,
+                                  const void* k, int64_t k_tok, int64_t k_head, const void* v, int64_t v_tok,
+                                  int64_t v_head, int32_t dtype, int64_t Tq, int64_t Tk, int32_t Hq, int32_t Hk,
+                                  int32_t D, const int32_t* cu_q, const int32_t* cu_k, const int32_t* k_len,
+                                  int32_t docs, float scale, int32_t causal, const int32_t* prefix, float softcap,
+                                  const float* slopes, void* dq, int64_t dq_tok, int64_t dq_head, void* dk,
+                                  int64_t dk_tok, int64_t dk_head, void* dv, int64_t dv_tok, int64_t dv_head,
+                                  void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+    Grad g{};
+    const int rc = fill_attn(&g.a, dtype, cu_q, cu_k, k_len, docs, Tq, Tk, Hq, Hk, D, scale, causal, prefix, softcap, slopes, status);
+    if (rc != PMG_OK) return rc;
+    auto ok = [](const void* p, int64_t t, int64_t h) { return p && !(reinterpret_cast<uintptr_t>(p) & 15) && !(t & 7) && !(h & 7); };
+    cudaStream_t s = as_stream(stream);
+    // without queries or keys every gradient that has rows is zero
+    if (docs == 0 || Tq == 0 || Tk == 0) {
+        if (Tq > 0 && (!ok(dq, dq_tok, dq_head) || dq_head != D || dq_tok != (int64_t)Hq * D)) return PMG_ERR_BAD_ARG;
+        if (Tk > 0 && (!ok(dk, dk_tok, dk_head) || dk_head != D || dk_tok != (int64_t)Hk * D || !ok(dv, dv_tok, dv_head) ||
+                       dv_head != D || dv_tok != (int64_t)Hk * D))
+            return PMG_ERR_BAD_ARG;
+        if (Tq > 0) PMG_CUDA_TRY(cudaMemsetAsync(dq, 0, (size_t)Tq * Hq * D * 2, s));
+        if (Tk > 0) PMG_CUDA_TRY(cudaMemsetAsync(dk, 0, (size_t)Tk * Hk * D * 2, s));
+        if (Tk > 0) PMG_CUDA_TRY(cudaMemsetAsync(dv, 0, (size_t)Tk * Hk * D * 2, s));
+        return PMG_OK;
+    }
+    if (!lse || !ok(dout, do_tok, do_head) || !ok(o, o_tok, o_head) || !ok(q, q_tok, q_head) || !ok(k, k_tok, k_head) ||
+        !ok(v, v_tok, v_head) || !ok(dq, dq_tok, dq_head) || !ok(dk, dk_tok, dk_head) || !ok(dv, dv_tok, dv_head))
+        return PMG_ERR_BAD_ARG;
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < pmg_attention_grad_workspace_bytes(Tq, Hq))
+        return PMG_ERR_BAD_ARG;
+    g.scale = scale;
+    g.stat_ld = (Tq + 1) / 2 * 2;
+    g.dq = dq; g.dk = dk; g.dv = dv;
+    g.q_tok = dq_tok; g.q_head = dq_head; g.k_tok = dk_tok; g.k_head = dk_head; g.v_tok = dv_tok; g.v_head = dv_head;
+    const Ins in{{dout, do_tok, do_head}, {o, o_tok, o_head}, {q, q_tok, q_head}, {k, k_tok, k_head}, {v, v_tok, v_head}, lse,
+                 static_cast<float*>(workspace)};
+    if (dtype == PMG_BF16) return D <= 64 ? by_score<__nv_bfloat16, 64>(g, in, s) : by_score<__nv_bfloat16, 128>(g, in, s);
+    return D <= 64 ? by_score<__half, 64>(g, in, s) : by_score<__half, 128>(g, in, s);
+}

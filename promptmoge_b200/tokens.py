@@ -355,6 +355,17 @@ def _attention_shapes(q, k, v):
     return index, dt, Tq, Tk, Hq, Hk, D
 
 
+def _score(scale, D, softcap, causal, prefix, max_q, max_k):
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf") or not 0.0 <= softcap < float("inf"):
+        raise ValueError("scale must be positive and softcap not negative, both finite")
+    if max_q < 0 or max_k < 0:
+        raise ValueError("max_q and max_k must not be negative")
+    if prefix is not None and not causal:
+        raise ValueError("prefix needs causal (without it every key is seen)")
+    return scale
+
+
 def attention(q, k, v, cu_q, cu_k, max_q: int, max_k: int, scale: float | None = None, causal: bool = False,
               prefix=None, softcap: float = 0.0, slopes=None, k_len=None, out=None):
     """Attention within documents.  q [Tq, Hq, D], k and v [Tk, Hk, D] of one 16-bit type, Hq a multiple of Hk; cu_q,
@@ -368,13 +379,7 @@ def attention(q, k, v, cu_q, cu_k, max_q: int, max_k: int, scale: float | None =
     token) takes the kernel that reads the keys once for all rows."""
     index, dt, Tq, Tk, Hq, Hk, D = _attention_shapes(q, k, v)
     docs = _packing(cu_q, cu_k, k_len, prefix, slopes, Hq, index)
-    scale = D ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf") or not 0.0 <= softcap < float("inf"):
-        raise ValueError("scale must be positive and softcap not negative, both finite")
-    if max_q < 0 or max_k < 0:
-        raise ValueError("max_q and max_k must not be negative")
-    if prefix is not None and not causal:
-        raise ValueError("prefix needs causal (without it every key is seen)")
+    scale = _score(scale, D, softcap, causal, prefix, max_q, max_k)
     o = torch.empty((Tq, Hq, D), dtype=dt, device=q.device) if out is None else out
     lse = torch.empty((Hq, Tq), dtype=torch.float32, device=q.device)
     if not Tq:
@@ -390,3 +395,29 @@ def attention(q, k, v, cu_q, cu_k, max_q: int, max_k: int, scale: float | None =
               slopes.data_ptr() if slopes is not None else None, *oh, lse.data_ptr(),
               ws.data_ptr() if need else None, need, _status(index), stream)
     return o, lse
+
+
+def attention_grad(do, o, lse, q, k, v, cu_q, cu_k, max_q: int, max_k: int, scale: float | None = None,
+                   causal: bool = False, prefix=None, softcap: float = 0.0, slopes=None, k_len=None):
+    """Gradients (dq, dk, dv) of attention() for do, the gradient of its output: o and lse are what it returned, the
+    rest its arguments.  The slopes are constants of the score and get no gradient.  Key rows behind k_len get zeros."""
+    index, dt, Tq, Tk, Hq, Hk, D = _attention_shapes(q, k, v)
+    docs = _packing(cu_q, cu_k, k_len, prefix, slopes, Hq, index)
+    scale = _score(scale, D, softcap, causal, prefix, max_q, max_k)
+    _shape(_dev(lse, "lse", 2, index, (torch.float32,)), (Hq, Tq), "lse")
+    if not lse.is_contiguous():
+        raise ValueError("lse must be contiguous")
+    doh = _aligned_heads(do, "do", q.shape, index, dt)
+    oh = _aligned_heads(o, "o", q.shape, index, dt)
+    dq, dk, dv = (torch.empty(t.shape, dtype=dt, device=q.device) for t in (q, k, v))
+    need = _query("pmg_attention_grad_workspace_bytes", Tq, Hq)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    ks = (Hk * D, D)
+    with _On(index) as stream:
+        _call("pmg_attention_grad", *doh, *oh, lse.data_ptr(), *_aligned_heads(q, "q", None, index, dt),
+              *_aligned_heads(k, "k", None, index, dt), *_aligned_heads(v, "v", None, index, dt), _DTYPES[dt], Tq, Tk,
+              Hq, Hk, D, cu_q.data_ptr(), cu_k.data_ptr(), k_len.data_ptr() if k_len is not None else None, docs, scale,
+              int(causal), prefix.data_ptr() if prefix is not None else None, softcap,
+              slopes.data_ptr() if slopes is not None else None, dq.data_ptr(), Hq * D, D, dk.data_ptr(), *ks,
+              dv.data_ptr(), *ks, ws.data_ptr(), need, _status(index), stream)
+    return dq, dk, dv
