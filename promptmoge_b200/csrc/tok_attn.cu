@@ -8,6 +8,7 @@
 // product (its operand can be no wider); the sums are of the unrounded ones, in fp32.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "tok_attn.cuh"
 
@@ -26,6 +27,7 @@ int fill_attn(tok::Attn* a, int dtype, const int32_t* cu_q, const int32_t* cu_k,
     a->scale2 = scale * tok::kLog2e;
     a->cap2 = softcap * tok::kLog2e;
     a->tanh_in = softcap > 0.0f ? 2.0f * scale * tok::kLog2e / softcap : 0.0f;
+    a->cap_in = softcap > 0.0f ? scale / softcap : 0.0f;
     a->status = status;
     return PMG_OK;
 }
@@ -55,13 +57,20 @@ struct Fwd {
     static constexpr int kStages = DP == 64 ? 4 : 2;
     static constexpr int kQ = 2 * kTile;
     static constexpr int kBars = kQ + 2 * kStages * kTile;
-    static constexpr int kSmem = kBars + 512;
+    static constexpr int kSmem = kBars + 1024;
     static constexpr uint32_t S(int w) { return 128 * w; }
     static constexpr uint32_t P(int w) { return kSep ? 256 + 64 * w : 128 * w; }
     static constexpr uint32_t O(int w) { return kSep ? 384 + 64 * w : 256 + 128 * w; }
 };
 
-constexpr int kFwdThreads = 320;               // two softmax warpgroups, the loader, the MMA issuer
+constexpr int kFwdThreads = 384;               // two softmax warpgroups, then the loader, the MMA issuer and two spare warps
+constexpr int kItems = 4;                      // items described ahead
+
+// One item of a CTA's walk: 256 query rows of a document and head.
+struct Item {
+    int doc, head, r0, n0, n1;                 // doc < 0: the walk ends; n: key tiles of each half
+    Span sp;
+};
 
 template <typename T, int DP, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kFwdThreads, 1)
@@ -72,29 +81,36 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* const sk = smem + C::kQ;
     uint8_t* const sv = sk + C::kStages * C::kTile;
-    uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + C::kBars);
-    uint64_t* k_full = q_full + 2;
-    uint64_t* k_empty = k_full + C::kStages;
-    uint64_t* v_full = k_empty + C::kStages;
-    uint64_t* v_empty = v_full + C::kStages;
-    uint64_t* s_full = v_empty + C::kStages;
-    uint64_t* s_read = s_full + 2;
-    uint64_t* p_full = s_read + 2;
-    uint64_t* pv_done = p_full + 2;
-    uint64_t* drain = pv_done + 2;
-    uint32_t* slot = reinterpret_cast<uint32_t*>(drain + 1);
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
-    int* where = reinterpret_cast<int*>(slot + 2);           // document and tile
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int head = blockIdx.x % a.Hq, kvh = head / a.group;
+    uint64_t* const next_slot = reinterpret_cast<uint64_t*>(smem + C::kBars);      // 16 bytes: the answer to a claim
+    uint64_t* const next_bar = next_slot + 2;
+    uint64_t* const q_full = next_bar + 1;
+    uint64_t* const q_empty = q_full + 2;
+    uint64_t* const k_full = q_empty + 2;
+    uint64_t* const k_empty = k_full + C::kStages;
+    uint64_t* const v_full = k_empty + C::kStages;
+    uint64_t* const v_empty = v_full + C::kStages;
+    uint64_t* const s_full = v_empty + C::kStages;
+    uint64_t* const s_read = s_full + 2;
+    uint64_t* const p_full = s_read + 2;
+    uint64_t* const pv_done = p_full + 2;
+    uint64_t* const o_read = pv_done + 2;
+    uint64_t* const item_full = o_read + 2;
+    uint64_t* const item_empty = item_full + kItems;
+    uint64_t* const drain = item_empty + kItems;
+    Item* const items = reinterpret_cast<Item*>(drain + 1);
+    uint32_t* const slot = reinterpret_cast<uint32_t*>(items + kItems);
+    volatile int* const abort_flag = reinterpret_cast<volatile int*>(slot + 1);
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(q_full + i, 1);
+            mbar_init(q_empty + i, 1);
             mbar_init(s_full + i, 1);
             mbar_init(s_read + i, 128);
             mbar_init(p_full + i, 128);
             mbar_init(pv_done + i, 1);
+            mbar_init(o_read + i, 128);
         }
         for (int i = 0; i < C::kStages; ++i) {
             mbar_init(k_full + i, 1);
@@ -102,130 +118,187 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             mbar_init(v_full + i, 1);
             mbar_init(v_empty + i, 1);
         }
+        for (int i = 0; i < kItems; ++i) {
+            mbar_init(item_full + i, 1);
+            mbar_init(item_empty + i, 9);            // eight softmax warps and the issuer
+        }
+        mbar_init(next_bar, 1);
         mbar_init(drain, 1);
         *abort_flag = 0;
         fence_mbar_init();
     }
     if (warp == 9) tmem_alloc(slot, 512);
-    pdl_begin();
-    if (warp == 8) {
-        int doc = -1, tile = 0;
-        const bool found = find_tile(a.cu_q, a.docs, 256, blockIdx.x / a.Hq, &doc, &tile);
-        if (lane == 0) {
-            where[0] = found ? doc : -1;
-            where[1] = tile;
-        }
-    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *slot;
-    const int doc = where[0];
-    if (doc >= 0) {
-        const Span sp = span_of(a, doc);
-        // later rows of a causal document reach further: they start first
-        const int tiles = (sp.lq + 255) / 256, tile = a.causal ? tiles - 1 - where[1] : where[1];
-        const int r0 = tile * 256;
-        int n[2];
-#pragma unroll
-        for (int w = 0; w < 2; ++w) n[w] = r0 + 128 * w < sp.lq ? (key_end(a, sp, r0 + 128 * (w + 1)) + 127) / 128 : 0;
-        const int nmax = max(n[0], n[1]);
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *slot, 0);
+    pdl_begin();
 
+    // Every warp but the loader reads the items in order through this.
+    auto next_item = [&](uint32_t it, Item& x) -> bool {
+        const int at = it % kItems;
+        if (!__all_sync(0xffffffffu, mbar_wait(item_full + at, (it / kItems) & 1u, abort_flag))) return false;
+        x = items[at];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(item_empty + at);
+        return true;
+    };
+
+    if (warp >= 8) {
+        reg_dealloc<kAttnRegsFew>();
         if (warp == 8) {
             // ------------------------------------------------------------------------------------------------ loads
-            if (lane == 0) {
-                bool ok = true;
-                for (int w = 0; w < 2; ++w) {
-                    if (n[w] == 0) continue;
-                    mbar_arrive_expect_tx(q_full + w, C::kTile);
+            bool ok = true;
+            uint32_t it = 0, kt = 0, qc[2] = {0, 0};
+            int block = blockIdx.x;
+            for (uint32_t claim = 0; block >= 0 && ok; ++claim) {
+                if (lane == 0) claim_block(next_slot, next_bar);          // answered while this block is loaded
+                Item x;
+                x.doc = -1;
+                int tile = 0;
+                const bool found = find_tile(a.cu_q, a.docs, 256, block / a.Hq, &x.doc, &tile);
+                if (found) {
+                    x.sp = span_of(a, x.doc);
+                    x.head = block % a.Hq;
+                    // later rows of a causal document reach further: they start first
+                    x.r0 = 256 * (a.causal ? (x.sp.lq + 255) / 256 - 1 - tile : tile);
+                    if (x.r0 < 0) x.r0 = 1 << 30;                     // offsets that had to be cut: no such rows
+                    x.n0 = x.r0 < x.sp.lq ? (key_end(a, x.sp, x.r0 + 128) + 127) / 128 : 0;
+                    x.n1 = x.r0 + 128 < x.sp.lq ? (key_end(a, x.sp, x.r0 + 256) + 127) / 128 : 0;
+                    const int at = it % kItems;
+                    ok = __all_sync(0xffffffffu, mbar_wait(item_empty + at, ((it / kItems) & 1u) ^ 1u, abort_flag));
+                    if (!ok) break;
+                    if (lane == 0) {
+                        items[at] = x;
+                        mbar_arrive(item_full + at);
+                        const int kvh = x.head / a.group, nmax = max(x.n0, x.n1);
+                        for (int w = 0; w < 2 && ok; ++w) {
+                            if ((w ? x.n1 : x.n0) == 0) continue;
+                            ok = mbar_wait(q_empty + w, (qc[w] & 1u) ^ 1u, abort_flag);
+                            if (!ok) break;
+                            mbar_arrive_expect_tx(q_full + w, C::kTile);
 #pragma unroll
-                    for (int c = 0; c < DP / 64; ++c)
-                        tma_tile3d(smem_u32(smem + w * C::kTile + c * 16384), &mq, 64 * c, head, sp.q0 + r0 + 128 * w, q_full + w);
-                }
-                for (int j = 0; j < nmax; ++j) {
-                    const int st = j % C::kStages;
-                    const uint32_t ph = ((j / C::kStages) & 1u) ^ 1u;
-                    if (!mbar_wait(k_empty + st, ph, abort_flag)) { ok = false; break; }
-                    mbar_arrive_expect_tx(k_full + st, C::kTile);
+                            for (int c = 0; c < DP / 64; ++c)
+                                tma_tile3d(smem_u32(smem + w * C::kTile + c * 16384), &mq, 64 * c, x.head, x.sp.q0 + x.r0 + 128 * w, q_full + w);
+                            ++qc[w];
+                        }
+                        for (int j = 0; j < nmax && ok; ++j, ++kt) {
+                            const int st = kt % C::kStages;
+                            const uint32_t ph = ((kt / C::kStages) & 1u) ^ 1u;
+                            ok = mbar_wait(k_empty + st, ph, abort_flag);
+                            if (!ok) break;
+                            mbar_arrive_expect_tx(k_full + st, C::kTile);
 #pragma unroll
-                    for (int c = 0; c < DP / 64; ++c)
-                        tma_tile3d(smem_u32(sk + st * C::kTile + c * 16384), &mk, 64 * c, kvh, sp.k0 + 128 * j, k_full + st);
-                    if (!mbar_wait(v_empty + st, ph, abort_flag)) { ok = false; break; }
-                    mbar_arrive_expect_tx(v_full + st, C::kTile);
+                            for (int c = 0; c < DP / 64; ++c)
+                                tma_tile3d(smem_u32(sk + st * C::kTile + c * 16384), &mk, 64 * c, kvh, x.sp.k0 + 128 * j, k_full + st);
+                            ok = mbar_wait(v_empty + st, ph, abort_flag);
+                            if (!ok) break;
+                            mbar_arrive_expect_tx(v_full + st, C::kTile);
 #pragma unroll
-                    for (int c = 0; c < DP / 64; ++c)
-                        tma_tile3d(smem_u32(sv + st * C::kTile + c * 16384), &mv, 64 * c, kvh, sp.k0 + 128 * j, v_full + st);
+                            for (int c = 0; c < DP / 64; ++c)
+                                tma_tile3d(smem_u32(sv + st * C::kTile + c * 16384), &mv, 64 * c, kvh, x.sp.k0 + 128 * j, v_full + st);
+                        }
+                    }
+                    ++it;
+                    ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+                    if (!ok) break;
                 }
-                if (!ok) {
-                    *abort_flag = 1;
-                    flag(a.status, PMG_ERR_TIMEOUT);
+                ok = __all_sync(0xffffffffu, mbar_wait(next_bar, claim & 1u, abort_flag));
+                if (!ok) break;
+                block = claimed_block(next_slot);
+                __syncwarp();
+                fence_proxy_async();
+            }
+            if (ok) {
+                const int at = it % kItems;
+                ok = __all_sync(0xffffffffu, mbar_wait(item_empty + at, ((it / kItems) & 1u) ^ 1u, abort_flag));
+                if (ok && lane == 0) {
+                    items[at].doc = -1;
+                    mbar_arrive(item_full + at);
                 }
+            }
+            if (!ok && lane == 0) {
+                *abort_flag = 1;
+                flag(a.status, PMG_ERR_TIMEOUT);
             }
         } else if (warp == 9) {
             // ------------------------------------------------------------------------------------------------ MMAs
             const int ksteps = (a.D + 15) / 16;
             const uint32_t id_qk = idesc16(Elem<T>::kFmt, 128, 128, false, false);
             const uint32_t id_pv = idesc16(Elem<T>::kFmt, 128, ksteps * 16, false, true);
+            const uint32_t lead = elect_one();
             bool ok = true;
-            auto qk = [&](int w, int j) -> bool {
-                const int st = j % C::kStages;
-                if (j == 0 && !__all_sync(0xffffffffu, mbar_wait(q_full + w, 0, abort_flag))) return false;
-                if (!__all_sync(0xffffffffu, mbar_wait(k_full + st, (j / C::kStages) & 1u, abort_flag))) return false;
-                tc_fence_after();
-                if (lane == 0) {
-                    const uint32_t qa = smem_u32(smem + w * C::kTile), kb = smem_u32(sk + st * C::kTile);
-                    for (int s = 0; s < ksteps; ++s) {
-                        const uint32_t at = (s >> 2) * 16384 + (s & 3) * 32;
-                        mma16(tmem + C::S(w), desc16(qa + at, 16), desc16(kb + at, 16), id_qk, s > 0);
+            uint32_t kt = 0, qc[2] = {0, 0}, sc[2] = {0, 0};    // key tiles; items and tiles of each half so far
+            auto wait = [&](uint64_t* bar, uint32_t ph) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, ph & 1u, abort_flag)); };
+            Item x;
+            for (uint32_t it = 0;; ++it) {
+                ok = next_item(it, x);
+                if (!ok || x.doc < 0) break;
+                const int n[2] = {__shfl_sync(0xffffffffu, x.n0, 0), __shfl_sync(0xffffffffu, x.n1, 0)}, nmax = max(n[0], n[1]);
+                auto qk = [&](int w, int j) -> bool {
+                    const uint32_t t = kt + j, st = t % C::kStages;
+                    if (j == 0 && !wait(q_full + w, qc[w])) return false;
+                    if (!wait(k_full + st, t / C::kStages)) return false;
+                    tc_fence_after();
+                    const uint32_t qa = desc_lo(smem_u32(smem + w * C::kTile), 16), kb = desc_lo(smem_u32(sk + st * C::kTile), 16);
+#pragma unroll
+                    for (int s = 0; s < DP / 16; ++s)
+                        if (s < ksteps) {
+                            const uint32_t at = ((s >> 2) * 16384 + (s & 3) * 32) >> 4;
+                            mma16(lead, tmem + C::S(w), qa + at, kb + at, id_qk, s > 0);
+                        }
+                    mma_commit_if(lead, s_full + w);
+                    if (w == 1 || j >= n[1]) mma_commit_if(lead, k_empty + st);     // the tile's last reader
+                    if (j + 1 == n[w]) mma_commit_if(lead, q_empty + w);
+                    return true;
+                };
+                auto pv = [&](int w, int j) -> bool {
+                    const uint32_t t = kt + j, st = t % C::kStages;
+                    if (!wait(v_full + st, t / C::kStages)) return false;
+                    const int valid = x.sp.lk - 128 * j;
+                    if (valid < 128 && (w == 0 || n[0] <= j)) {
+                        // rows behind the document's last key: whatever lies there must not reach a sum (0 * NaN)
+                        for (int c = 0; c < DP / 64; ++c)
+                            for (int b = valid * 128 + lane * 16; b < 16384; b += 512)
+                                *reinterpret_cast<uint4*>(sv + st * C::kTile + c * 16384 + b) = make_uint4(0, 0, 0, 0);
+                        fence_proxy_async();
+                        __syncwarp();
                     }
-                    mma_commit(s_full + w);
-                    if (w == 1 || j >= n[1]) mma_commit(k_empty + st);     // the tile's last reader
-                }
-                __syncwarp();
-                return true;
-            };
-            auto pv = [&](int w, int j) -> bool {
-                const int st = j % C::kStages;
-                if (!__all_sync(0xffffffffu, mbar_wait(v_full + st, (j / C::kStages) & 1u, abort_flag))) return false;
-                const int valid = sp.lk - 128 * j;
-                if (valid < 128 && (w == 0 || n[0] <= j)) {
-                    // rows behind the document's last key: whatever lies there must not reach a sum (0 * NaN)
-                    for (int c = 0; c < DP / 64; ++c)
-                        for (int b = valid * 128 + lane * 16; b < 16384; b += 512)
-                            *reinterpret_cast<uint4*>(sv + st * C::kTile + c * 16384 + b) = make_uint4(0, 0, 0, 0);
-                    fence_proxy_async();
-                    __syncwarp();
-                }
-                if (!__all_sync(0xffffffffu, mbar_wait(p_full + w, j & 1u, abort_flag))) return false;
-                tc_fence_after();
-                if (lane == 0) {
-                    const uint32_t vb = smem_u32(sv + st * C::kTile);
+                    if (!wait(p_full + w, sc[w] + j)) return false;
+                    if (j == 0 && !wait(o_read + w, qc[w] ^ 1u)) return false;    // the last item's output is out
+                    tc_fence_after();
+                    const uint32_t vb = desc_lo(smem_u32(sv + st * C::kTile), 16384);
 #pragma unroll
                     for (int s = 0; s < 8; ++s)
-                        mma16_ts(tmem + C::O(w), tmem + C::P(w) + 8 * s, desc16(vb + s * 2048, 16384), id_pv, j > 0 || s > 0);
-                    mma_commit(pv_done + w);
-                    if (w == 1 || j >= n[1]) mma_commit(v_empty + st);
-                }
-                __syncwarp();
-                return true;
-            };
-            for (int w = 0; w < 2 && ok; ++w)
-                if (n[w] > 0) ok = qk(w, 0);
-            for (int j = 0; j < nmax && ok; ++j) {
-                if (C::kSep) {
-                    // the next scores as soon as these have been read, under the softmax of these
-                    for (int w = 0; w < 2 && ok; ++w)
-                        if (j + 1 < n[w]) {
-                            ok = __all_sync(0xffffffffu, mbar_wait(s_read + w, j & 1u, abort_flag));
-                            if (ok) ok = qk(w, j + 1);
+                        mma16_ts(lead, tmem + C::O(w), tmem + C::P(w) + 8 * s, vb + s * 128, id_pv, j > 0 || s > 0);
+                    mma_commit_if(lead, pv_done + w);
+                    if (w == 1 || j >= n[1]) mma_commit_if(lead, v_empty + st);
+                    return true;
+                };
+                for (int w = 0; w < 2 && ok; ++w)
+                    if (n[w] > 0) ok = qk(w, 0);
+                for (int j = 0; j < nmax && ok; ++j) {
+                    if (C::kSep) {
+                        // the next scores as soon as these have been read, under the softmax of these
+                        for (int w = 0; w < 2 && ok; ++w)
+                            if (j + 1 < n[w]) {
+                                ok = wait(s_read + w, sc[w] + j);
+                                if (ok) ok = qk(w, j + 1);
+                            }
+                        for (int w = 0; w < 2 && ok; ++w)
+                            if (j < n[w]) ok = pv(w, j);
+                    } else {
+                        for (int w = 0; w < 2 && ok; ++w) {
+                            if (j < n[w]) ok = pv(w, j);
+                            if (ok && j + 1 < n[w]) ok = qk(w, j + 1);
                         }
-                    for (int w = 0; w < 2 && ok; ++w)
-                        if (j < n[w]) ok = pv(w, j);
-                } else {
-                    for (int w = 0; w < 2 && ok; ++w) {
-                        if (j < n[w]) ok = pv(w, j);
-                        if (ok && j + 1 < n[w]) ok = qk(w, j + 1);
                     }
+                }
+                if (!ok) break;
+                kt += nmax;
+                for (int w = 0; w < 2; ++w) {
+                    sc[w] += n[w];
+                    qc[w] += n[w] > 0;
                 }
             }
             if (lane == 0) {
@@ -236,23 +309,30 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                 }
             }
             __syncwarp();
-        } else {
-            // --------------------------------------------------------------------------------------------- softmax
-            const int w = warp >> 2, tiles_k = n[w];
-            const int i = r0 + 128 * w + (warp & 3) * 32 + lane;          // this thread's row in the document
-            const int lim = last_key(a, sp, i);
-            const int warp_min = __reduce_min_sync(0xffffffffu, i < sp.lq ? lim : INT32_MAX);
-            const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-            const uint32_t ts = tmem + lanes + C::S(w), tp = tmem + lanes + C::P(w), to = tmem + lanes + C::O(w);
-            const float c = (CAP || BIAS) ? 1.0f : a.scale2;              // scores to units of log 2
-            const float slope = BIAS ? a.slopes[head] * kLog2e : 0.0f;
-            const float place = (float)(i + sp.lk - sp.lq);
+        }
+    } else {
+        // ------------------------------------------------------------------------------------------------- softmax
+        reg_alloc<kAttnRegsMany>();
+        const int w = warp >> 2;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + lanes + C::S(w), tp = tmem + lanes + C::P(w), to = tmem + lanes + C::O(w);
+        const float c = (CAP || BIAS) ? 1.0f : a.scale2;                  // scores to units of log 2
+        uint32_t sc = 0;
+        bool ok = true;
+        Item x;
+        for (uint32_t it = 0;; ++it) {
+            ok = next_item(it, x);
+            if (!ok || x.doc < 0) break;
+            const int tiles_k = w ? x.n1 : x.n0;
+            const int i = x.r0 + 128 * w + (warp & 3) * 32 + lane;        // this thread's row in the document
+            const int lim = last_key(a, x.sp, i);
+            const int warp_min = __reduce_min_sync(0xffffffffu, i < x.sp.lq ? lim : INT32_MAX);
+            const float slope = BIAS ? a.slopes[x.head] * kLog2e : 0.0f;
+            const float place = (float)(i + x.sp.lk - x.sp.lq);
             float m = -INFINITY;
             uint64_t sum = 0;
-            float total = 0.0f;
-            bool ok = true;
-            for (int j = 0; j < tiles_k; ++j) {
-                TOK_WAIT(s_full + w, j & 1u);
+            for (int j = 0; j < tiles_k; ++j, ++sc) {
+                TOK_WAIT(s_full + w, sc & 1u);
                 if (!ok) break;
                 tc_fence_after();
                 float s[128];
@@ -264,26 +344,22 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                     mbar_arrive(s_read + w);
                 }
                 const int j0 = 128 * j;
-                if (CAP) {
-#pragma unroll
-                    for (int k = 0; k < 128; ++k) s[k] = capped(a, s[k]);
-                }
-                if (BIAS) {
-                    const float far = place - (float)j0;
-#pragma unroll
-                    for (int k = 0; k < 128; ++k)
-                        s[k] = fmaf(-slope, fabsf(far - (float)k), CAP ? s[k] : s[k] * a.scale2);
-                }
-                if (j0 + 127 > warp_min) {
+                const bool masked = j0 + 127 > warp_min;
+                if (CAP) cap_scores<128>(a, s);
+                if (BIAS) bias_scores<128>(s, CAP ? 1.0f : a.scale2, slope, place - (float)j0);
+                if (masked) {
 #pragma unroll
                     for (int k = 0; k < 128; ++k)
                         if (j0 + k > lim) s[k] = -INFINITY;
                 }
-                float top = max3(s[0], s[1], s[2]);
+                float top = max3(s[0], s[1], s[2]), top2 = max3(s[3], s[4], s[5]);
 #pragma unroll
-                for (int k = 3; k < 127; k += 2) top = max3(top, s[k], s[k + 1]);
-                top = fmaxf(top, s[127]);
-                if (j > 0) TOK_WAIT(pv_done + w, (j - 1) & 1u);           // frees the probabilities and the output
+                for (int k = 6; k < 126; k += 4) {
+                    top = max3(top, s[k], s[k + 1]);
+                    top2 = max3(top2, s[k + 2], s[k + 3]);
+                }
+                top = fmaxf(max3(top, top2, s[126]), s[127]);
+                if (j > 0) TOK_WAIT(pv_done + w, (sc - 1) & 1u);          // frees the probabilities and the output
                 if (!ok) break;
                 if (j == 0) {
                     m = top;
@@ -291,9 +367,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                     const float grown = fmaxf(m, top);
                     const float f = grown == m ? 1.0f : ex2((m - grown) * c);
                     m = grown;
-                    total *= f;
-                    const float2 s2 = unpack2(sum);
-                    sum = pack2(s2.x * f, s2.y * f);
+                    sum = mul2(sum, pack2(f, f));
                     tc_fence_after();
 #pragma unroll
                     for (int q = 0; q < DP / 32; ++q) {
@@ -308,56 +382,67 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                 }
                 const float base = m == -INFINITY ? 0.0f : -m * c + kLift<T>;
                 const uint64_t c2 = pack2(c, c), b2 = pack2(base, base);
+                auto exps = [&](auto poly) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    uint32_t p[16];
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t p[16];
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const float2 x = unpack2(fma2(pack2(s[32 * q + 2 * k], s[32 * q + 2 * k + 1]), c2, b2));
-                        const float e0 = ex2(x.x), e1 = ex2(x.y);
-                        sum = add2(sum, pack2(e0, e1));
-                        p[k] = Elem<T>::pack(e0, e1);
+                        for (int k = 0; k < 16; ++k) {
+                            const uint64_t y = fma2(pack2(s[32 * q + 2 * k], s[32 * q + 2 * k + 1]), c2, b2);
+                            const uint64_t e = decltype(poly)::value && kPoly(k) ? ex2_poly(y) : ex2_pair(y);
+                            sum = add2(sum, e);
+                            const float2 f = unpack2(e);
+                            p[k] = Elem<T>::pack(f.x, f.y);
+                        }
+                        tmem_st16(tp + 16 * q, p);
                     }
-                    tmem_st16(tp + 16 * q, p);
-                }
+                };
+                // masked entries are exactly zero, which only the hardware's exp2 of -inf gives
+                if (masked) exps(std::false_type{});
+                else exps(std::true_type{});
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(p_full + w);
             }
+            if (!ok) break;
             const float2 s2 = unpack2(sum);
-            total = s2.x + s2.y;
-            if (tiles_k > 0 && ok) TOK_WAIT(pv_done + w, (tiles_k - 1) & 1u);
-            if (ok) {
-                tc_fence_after();
-                const int64_t token = sp.q0 + (int64_t)i;
-                const bool mine = i < sp.lq && token < a.Tq;
-                const float inv = total > 0.0f || total != total ? 1.0f / total : 0.0f;   // empty rows: zero
-                if (mine) lse[(int64_t)head * a.Tq + token] = total == 0.0f ? -INFINITY : (m * c + log2f(total) - kLift<T>) * kLn2;
-                T* row = o + token * o_tok + head * o_head;
+            const float total = s2.x + s2.y;
+            if (tiles_k > 0) TOK_WAIT(pv_done + w, (sc - 1) & 1u);
+            if (!ok) break;
+            tc_fence_after();
+            const int64_t token = x.sp.q0 + (int64_t)i;
+            const bool mine = i < x.sp.lq, none = total == 0.0f;         // rows that see no key give zero
+            const float inv = none ? 0.0f : 1.0f / total;
+            if (mine) lse[(int64_t)x.head * a.Tq + token] = none ? -INFINITY : (m * c + log2f(total) - kLift<T>) * kLn2;
+            T* row = o + token * o_tok + x.head * o_head;
 #pragma unroll
-                for (int q = 0; q < DP / 32; ++q) {
-                    float v[32];
-                    if (tiles_k > 0) {
-                        tmem_ld32(to + 32 * q, reinterpret_cast<uint32_t*>(v));
-                        tmem_wait_ld();
-                    }
-                    if (total == 0.0f) {
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) v[k] = 0.0f;
-                    }
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (mine && 32 * q + 8 * k < a.D)
-                            *reinterpret_cast<uint4*>(row + 32 * q + 8 * k) =
-                                make_uint4(Elem<T>::pack(v[8 * k] * inv, v[8 * k + 1] * inv),
-                                           Elem<T>::pack(v[8 * k + 2] * inv, v[8 * k + 3] * inv),
-                                           Elem<T>::pack(v[8 * k + 4] * inv, v[8 * k + 5] * inv),
-                                           Elem<T>::pack(v[8 * k + 6] * inv, v[8 * k + 7] * inv));
+            for (int q = 0; q < DP / 32; ++q) {
+                float v[32];
+                if (tiles_k > 0) {
+                    tmem_ld32(to + 32 * q, reinterpret_cast<uint32_t*>(v));
+                    tmem_wait_ld();
                 }
-            } else if (lane == 0) {
-                *abort_flag = 1;
-                flag(a.status, PMG_ERR_TIMEOUT);
+                if (q == DP / 32 - 1 && tiles_k > 0) {
+                    tc_fence_before();
+                    mbar_arrive(o_read + w);
+                }
+                if (none) {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) v[k] = 0.0f;
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (mine && 32 * q + 8 * k < a.D)
+                        *reinterpret_cast<uint4*>(row + 32 * q + 8 * k) =
+                            make_uint4(Elem<T>::pack(v[8 * k] * inv, v[8 * k + 1] * inv),
+                                       Elem<T>::pack(v[8 * k + 2] * inv, v[8 * k + 3] * inv),
+                                       Elem<T>::pack(v[8 * k + 4] * inv, v[8 * k + 5] * inv),
+                                       Elem<T>::pack(v[8 * k + 6] * inv, v[8 * k + 7] * inv));
             }
+        }
+        if (!ok && lane == 0) {
+            *abort_flag = 1;
+            flag(a.status, PMG_ERR_TIMEOUT);
         }
     }
     __syncwarp();

@@ -27,6 +27,7 @@ struct Attn {
     float scale2;            // scale log2 e
     float tanh_in;           // 2 scale log2 e / cap: exp2 of (score * tanh_in) = e^(2 s / cap)
     float cap2;              // cap log2 e
+    float cap_in;            // scale / cap
     int32_t* status;
 };
 
@@ -82,11 +83,129 @@ __device__ __forceinline__ bool find_tile(const int32_t* cu, int docs, int rows,
     return false;
 }
 
-// cap tanh(s / cap) in units of log 2 from the raw product: cap2 (1 - 2 / (e^(2 s scale / cap) + 1)).  The hardware's
-// tanh is off by up to 2^-11, which a cap of 50 would turn into 3 % of a probability; this form is off by about
-// 2e-7 cap.
-__device__ __forceinline__ float capped(const Attn& a, float s) {
-    return fmaf(-2.0f * a.cap2, rcp_approx(ex2(s * a.tanh_in) + 1.0f), a.cap2);
+// tanh of half the argument's exponent form: 1 - 2 / (e^(2 s scale / cap) + 1) of a raw product s.  The hardware's tanh is
+// off by up to 2^-11, which a cap of 50 would turn into 3 % of a probability; this form is off by about 2e-7.
+__device__ __forceinline__ float tanh_raw(const Attn& a, float s) {
+    return fmaf(-2.0f, rcp_approx(ex2(s * a.tanh_in) + 1.0f), 1.0f);
+}
+__device__ __forceinline__ float capped(const Attn& a, float s) { return a.cap2 * tanh_raw(a, s); }
+
+// tanh(x) / x in x^2 on |x| <= 1: least largest relative error 5.0e-8 (iteratively reweighted least squares in the
+// Chebyshev basis).
+__device__ constexpr float kTanh[7] = {9.999999502e-01f, -3.333283915e-01f, 1.332520403e-01f, -5.345702773e-02f,
+                                       2.028997689e-02f, -6.203375984e-03f, 1.041021598e-03f};
+
+// Raw products to tanh(scale s / cap).  Scores mostly stay below their cap, where a polynomial on the packed fp32 pipe
+// takes 9 instructions a pair against two trips through the special function unit an element: one warp-wide test.
+template <int N>
+__device__ __forceinline__ void tanh_scores(const Attn& a, float (&s)[N]) {
+    float big = fabsf(s[0]);
+#pragma unroll
+    for (int k = 1; k + 1 < N; k += 2) big = max3(big, fabsf(s[k]), fabsf(s[k + 1]));
+    big = fmaxf(big, fabsf(s[N - 1]));
+    const float in = a.cap_in;
+    if (__all_sync(0xffffffffu, big * in <= 1.0f)) {
+        const uint64_t in2 = pack2(in, in);
+#pragma unroll
+        for (int k = 0; k < N; k += 2) {
+            const uint64_t x = mul2(pack2(s[k], s[k + 1]), in2), u = mul2(x, x);
+            uint64_t p = pack2(kTanh[6], kTanh[6]);
+#pragma unroll
+            for (int i = 5; i >= 0; --i) p = fma2(p, u, pack2(kTanh[i], kTanh[i]));
+            const float2 f = unpack2(mul2(p, x));
+            s[k] = f.x;
+            s[k + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) s[k] = tanh_raw(a, s[k]);
+    }
+}
+template <int N>
+__device__ __forceinline__ void cap_scores(const Attn& a, float (&s)[N]) {
+    tanh_scores<N>(a, s);
+#pragma unroll
+    for (int k = 0; k < N; k += 2) {
+        const float2 f = unpack2(mul2(pack2(s[k], s[k + 1]), pack2(a.cap2, a.cap2)));
+        s[k] = f.x;
+        s[k + 1] = f.y;
+    }
+}
+
+// s[k] c - slope |far - k|.  Where no row of the warp has its own place among the columns, the distance is linear in k.
+template <int N>
+__device__ __forceinline__ void bias_scores(float (&s)[N], float c, float slope, float far) {
+    const bool behind = __all_sync(0xffffffffu, far >= (float)(N - 1)), ahead = __all_sync(0xffffffffu, far <= 0.0f);
+    if (behind || ahead) {
+        const float t = behind ? slope : -slope;              // s c - t far + t k
+        const uint64_t c2 = pack2(c, c), t2 = pack2(t, t), b2 = pack2(-t * far, -t * far);
+#pragma unroll
+        for (int k = 0; k < N; k += 2) {
+            const float2 f = unpack2(fma2(pack2(s[k], s[k + 1]), c2, fma2(t2, pack2((float)k, (float)(k + 1)), b2)));
+            s[k] = f.x;
+            s[k + 1] = f.y;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) s[k] = fmaf(-slope, fabsf(far - (float)k), s[k] * c);
+    }
+}
+
+// 2^x of a pair: the special function unit (16 a cycle and SM), or a polynomial on the fp32 pipe beside it.  2^x = 2^n 2^f,
+// n the nearest integer (by adding 1.5 2^23, which leaves it in the low bits), f in [-1/2, 1/2], 2^f by a polynomial of
+// degree 4 with least largest relative error 2.6e-6, its exponent field raised by n.  x from -125 up to 127.
+__device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
+    const float2 f = unpack2(x);
+    return pack2(ex2(f.x), ex2(f.y));
+}
+__device__ __forceinline__ uint64_t ex2_poly(uint64_t x) {
+    const float2 v = unpack2(x);
+    x = pack2(fmaxf(v.x, -125.0f), fmaxf(v.y, -125.0f));
+    const uint64_t t = add2(x, pack2(12582912.0f, 12582912.0f));
+    const uint64_t f = fma2(add2(t, pack2(-12582912.0f, -12582912.0f)), pack2(-1.0f, -1.0f), x);
+    uint64_t p = pack2(9.570100592e-03f, 9.570100592e-03f);
+    p = fma2(p, f, pack2(5.591786022e-02f, 5.591786022e-02f));
+    p = fma2(p, f, pack2(2.402474486e-01f, 2.402474486e-01f));
+    p = fma2(p, f, pack2(6.931218148e-01f, 6.931218148e-01f));
+    p = fma2(p, f, pack2(9.999992614e-01f, 9.999992614e-01f));
+    const float2 tf = unpack2(t), pf = unpack2(p);
+    return pack2(__int_as_float(__float_as_int(pf.x) + (__float_as_int(tf.x) << 23)),
+                 __int_as_float(__float_as_int(pf.y) + (__float_as_int(tf.y) << 23)));
+}
+// Which of 16 pairs take the polynomial.
+#ifndef TOK_POLY
+#define TOK_POLY 5
+#endif
+__device__ __forceinline__ constexpr bool kPoly(int k) { return (k * TOK_POLY) % 16 < TOK_POLY; }
+
+// Registers move from the loading and issuing warps to the two softmax warpgroups: 2 * 208 + 88 = 3 * 168, what the block
+// of three warpgroups was launched with.
+constexpr int kAttnRegsMany = 208, kAttnRegsFew = 88;
+template <int N>
+__device__ __forceinline__ void reg_alloc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void reg_dealloc() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// Claims a block of this grid that has not started yet (its index becomes this CTA's next work); the 16-byte answer lands
+// in `slot` and completes `bar`.
+__device__ __forceinline__ void claim_block(uint64_t* slot, uint64_t* bar) {
+    mbar_arrive_expect_tx(bar, 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                     smem_u32(slot)),
+                 "r"(smem_u32(bar))
+                 : "memory");
+}
+// The claimed block's x index, -1 where none was left.
+__device__ __forceinline__ int claimed_block(const uint64_t* slot) {
+    uint32_t x, got;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\tld.shared.b128 r, [%2];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\tselp.u32 %1, 1, 0, p;\n\tmov.u32 %0, 0;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, r;\n\t}"
+        : "=r"(x), "=r"(got)
+        : "r"(smem_u32(slot))
+        : "memory");
+    return got ? (int)x : -1;
 }
 
 }  // namespace tok

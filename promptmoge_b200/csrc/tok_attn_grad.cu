@@ -161,7 +161,7 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
     using C = Bwd<DP>;
     const Attn& a = g.a;
     volatile int* abort_flag = b.abort_flag;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const Span sp = span_of(a, doc);
     const int off = sp.lk - sp.lq;
     const int head = KEYS ? 0 : block % a.Hq;                       // query CTAs: their head
@@ -231,28 +231,24 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
             }
             return true;
         };
+        const uint32_t lead = elect_one();
         auto square = [&](int i, int which) {           // scores (0) or dP (1) of tile i
             tc_fence_after();
-            if (lane == 0) {
-                const uint32_t x = smem_u32(smem + which * C::kTile), y = smem_u32(stage(i) + which * C::kTile);
-                for (int s = 0; s < ksteps; ++s) {
-                    const uint32_t at = (s >> 2) * 16384 + (s & 3) * 32;
-                    mma16(tmem + (which ? C::kDP : C::kS), desc16(x + at, 16), desc16(y + at, 16), id_s, s > 0);
+            const uint32_t x = desc_lo(smem_u32(smem + which * C::kTile), 16), y = desc_lo(smem_u32(stage(i) + which * C::kTile), 16);
+#pragma unroll
+            for (int s = 0; s < DP / 16; ++s)
+                if (s < ksteps) {
+                    const uint32_t at = ((s >> 2) * 16384 + (s & 3) * 32) >> 4;
+                    mma16(lead, tmem + (which ? C::kDP : C::kS), x + at, y + at, id_s, s > 0);
                 }
-                mma_commit(which ? b.dp_full : b.s_full);
-            }
-            __syncwarp();
+            mma_commit_if(lead, which ? b.dp_full : b.s_full);
         };
         auto sum = [&](int i, int which) {              // out0 += dS B0, out1 += P B1
             tc_fence_after();
-            if (lane == 0) {
-                const uint32_t x = tmem + (which ? C::kS : C::kDP), y = smem_u32(stage(i) + which * C::kTile);
+            const uint32_t x = tmem + (which ? C::kS : C::kDP), y = desc_lo(smem_u32(stage(i) + which * C::kTile), 16384);
 #pragma unroll
-                for (int s = 0; s < 8; ++s)             // each warpgroup's half lies in its own columns
-                    mma16_ts(tmem + (which ? C::kOut1 : C::kOut0), x + (s >> 2) * 64 + (s & 3) * 8, desc16(y + s * 2048, 16384),
-                             id_o, i > 0 || s > 0);
-            }
-            __syncwarp();
+            for (int s = 0; s < 8; ++s)                 // each warpgroup's half lies in its own columns
+                mma16_ts(lead, tmem + (which ? C::kOut1 : C::kOut0), x + (s >> 2) * 64 + (s & 3) * 8, y + s * 128, id_o, i > 0 || s > 0);
         };
         if (total > 0) {
             ok = wait(b.a_full, 0) && landed(0);
@@ -272,12 +268,12 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
                 ok = wait(b.ds_full, i & 1u);
                 if (!ok) break;
                 sum(i, 0);
-                if (lane == 0) mma_commit(b.b_empty + i % C::kStages);
+                mma_commit_if(lead, b.b_empty + i % C::kStages);
                 if (i + 1 < total) square(i + 1, 1);
             }
+            if (ok) mma_commit_if(lead, b.done);
             if (lane == 0) {
-                if (ok) mma_commit(b.done);
-                else flag(a.status, PMG_ERR_TIMEOUT);
+                if (!ok) flag(a.status, PMG_ERR_TIMEOUT);
                 if (!ok || *abort_flag) {
                     *abort_flag = 1;
                     drain_mma(b.drain);
@@ -442,7 +438,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     uint32_t* slot = reinterpret_cast<uint32_t*>(b.drain + 1);
     b.abort_flag = reinterpret_cast<volatile int*>(slot + 1);
     int* where = reinterpret_cast<int*>(slot + 2);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const bool keys = (int)blockIdx.x < g.key_blocks;
     const int block = keys ? blockIdx.x : blockIdx.x - g.key_blocks;
 
@@ -474,7 +470,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *slot, 0);
     if (where[0] >= 0) {
         if (keys) grad_cta<T, DP, true, CAP, BIAS>(mk, mv, mq, mdo, g, smem, b, tmem, block, where[0], where[1]);
         else grad_cta<T, DP, false, CAP, BIAS>(mq, mdo, mk, mv, g, smem, b, tmem, block, where[0], where[1]);

@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     uint64_t* drain = acc_empty + 2;
     uint32_t* slot = reinterpret_cast<uint32_t*>(drain + 1);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(slot + 1);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::kStages; ++i) {
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *slot, 0);
     pdl_begin();
 
     if (warp == 0) {
@@ -382,35 +382,39 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = idesc16(Elem<T>::kFmt, kBM, BN, AMN, BMN);
-            uint32_t it = 0, k = 0;
-            bool ok = true;
-            for (int u = blockIdx.x; u < sched.units && ok; u += gridDim.x, ++k) {
-                const Unit t = unit_of<BN>(sched, u);
-                const uint32_t buf = k & 1u, d = tmem + buf * BN;
-                if (!mbar_wait(acc_empty + buf, ((k >> 1) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+        constexpr uint32_t idesc = idesc16(Elem<T>::kFmt, kBM, BN, AMN, BMN);
+        const uint32_t lead = elect_one();
+        uint32_t it = 0, k = 0;
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t ph) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, ph, abort_flag)); };
+        for (int u = blockIdx.x; u < sched.units && ok; u += gridDim.x, ++k) {
+            const Unit t = unit_of<BN>(sched, u);
+            const uint32_t buf = k & 1u, d = tmem + buf * BN;
+            ok = wait(acc_empty + buf, ((k >> 1) & 1u) ^ 1u);
+            if (!ok) break;
+            tc_fence_after();
+            for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
+                const int st = it % C::kStages;
+                ok = wait(full + st, (it / C::kStages) & 1u);
+                if (!ok) break;
                 tc_fence_after();
-                for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
-                    const int st = it % C::kStages;
-                    if (!mbar_wait(full + st, (it / C::kStages) & 1u, abort_flag)) { ok = false; break; }
-                    tc_fence_after();
-                    const uint32_t a = smem_u32(smem + st * C::kStage), b = a + C::kA;
+                const uint32_t at = smem_u32(smem + st * C::kStage);
+                const uint32_t a = desc_lo(at, AMN ? 8192 : 16), b = desc_lo(at + C::kA, BMN ? 8192 : 16);
 #pragma unroll
-                    for (int kk = 0; kk < kBK / 16; ++kk)
-                        mma16(d, desc16(AMN ? a + kk * 2048 : a + kk * 32, AMN ? 8192 : 16),
-                              desc16(BMN ? b + kk * 2048 : b + kk * 32, BMN ? 8192 : 16), idesc,
-                              (kb > t.kb0 || kk > 0) ? 1u : 0u);
-                    mma_commit(empty + st);
-                }
-                if (ok) mma_commit(acc_full + buf);
+                for (int kk = 0; kk < kBK / 16; ++kk)
+                    mma16(lead, d, a + kk * (AMN ? 128 : 2), b + kk * (BMN ? 128 : 2), idesc, (kb > t.kb0 || kk > 0) ? 1u : 0u);
+                mma_commit_if(lead, empty + st);
             }
+            if (ok) mma_commit_if(lead, acc_full + buf);
+        }
+        if (lane == 0) {
             if (!ok) flag(status, PMG_ERR_TIMEOUT);
             if (!ok || *abort_flag) {
                 *abort_flag = 1;
                 drain_mma(drain);
             }
         }
+        __syncwarp();
     } else if (warp >= kFirstEpi) {
         const int ew = warp - kFirstEpi, quarter = warp & 3, group = ew >> 2;
         uint8_t* stage = smem + C::kStages * C::kStage + ew * 4096;
