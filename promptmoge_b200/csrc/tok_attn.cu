@@ -8,7 +8,6 @@
 // product (its operand can be no wider); the sums are of the unrounded ones, in fp32.
 #include <algorithm>
 #include <cmath>
-#include <type_traits>
 
 #include "tok_attn.cuh"
 
@@ -59,7 +58,7 @@ struct Fwd {
     static constexpr int kBars = kQ + 2 * kStages * kTile;
     static constexpr int kSmem = kBars + 1024;
     static constexpr uint32_t S(int w) { return 128 * w; }
-    static constexpr uint32_t P(int w) { return kSep ? 256 + 64 * w : 128 * w; }
+    static constexpr uint32_t P(int w) { return kSep ? 256 + 64 * w : 128 * w + 64; }   // written from the end
     static constexpr uint32_t O(int w) { return kSep ? 384 + 64 * w : 256 + 128 * w; }
 };
 
@@ -90,8 +89,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     uint64_t* const v_full = k_empty + C::kStages;
     uint64_t* const v_empty = v_full + C::kStages;
     uint64_t* const s_full = v_empty + C::kStages;
-    uint64_t* const s_read = s_full + 2;
-    uint64_t* const p_full = s_read + 2;
+    uint64_t* const p_full = s_full + 2;
     uint64_t* const pv_done = p_full + 2;
     uint64_t* const o_read = pv_done + 2;
     uint64_t* const item_full = o_read + 2;
@@ -107,7 +105,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             mbar_init(q_full + i, 1);
             mbar_init(q_empty + i, 1);
             mbar_init(s_full + i, 1);
-            mbar_init(s_read + i, 128);
             mbar_init(p_full + i, 128);
             mbar_init(pv_done + i, 1);
             mbar_init(o_read + i, 128);
@@ -264,7 +261,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                         fence_proxy_async();
                         __syncwarp();
                     }
-                    if (!wait(p_full + w, sc[w] + j)) return false;
                     if (j == 0 && !wait(o_read + w, qc[w] ^ 1u)) return false;    // the last item's output is out
                     tc_fence_after();
                     const uint32_t vb = desc_lo(smem_u32(sv + st * C::kTile), 16384);
@@ -278,20 +274,14 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                 for (int w = 0; w < 2 && ok; ++w)
                     if (n[w] > 0) ok = qk(w, 0);
                 for (int j = 0; j < nmax && ok; ++j) {
-                    if (C::kSep) {
-                        // the next scores as soon as these have been read, under the softmax of these
-                        for (int w = 0; w < 2 && ok; ++w)
-                            if (j + 1 < n[w]) {
-                                ok = wait(s_read + w, sc[w] + j);
-                                if (ok) ok = qk(w, j + 1);
-                            }
-                        for (int w = 0; w < 2 && ok; ++w)
-                            if (j < n[w]) ok = pv(w, j);
-                    } else {
-                        for (int w = 0; w < 2 && ok; ++w) {
-                            if (j < n[w]) ok = pv(w, j);
-                            if (ok && j + 1 < n[w]) ok = qk(w, j + 1);
-                        }
+                    // Each half on its own: the next scores and this tile's product follow when its softmax is through,
+                    // while the other half's softmax runs.  Scores first where the probabilities leave them room.
+                    for (int w = 0; w < 2 && ok; ++w) {
+                        if (j >= n[w]) continue;
+                        ok = wait(p_full + w, sc[w] + j);
+                        if (ok && C::kSep && j + 1 < n[w]) ok = qk(w, j + 1);
+                        if (ok) ok = pv(w, j);
+                        if (ok && !C::kSep && j + 1 < n[w]) ok = qk(w, j + 1);
                     }
                 }
                 if (!ok) break;
@@ -316,7 +306,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         const int w = warp >> 2;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + C::S(w), tp = tmem + lanes + C::P(w), to = tmem + lanes + C::O(w);
-        const float c = (CAP || BIAS) ? 1.0f : a.scale2;                  // scores to units of log 2
+        const float c = BIAS ? 1.0f : (CAP ? a.cap2 : a.scale2);          // scores to units of log 2
         uint32_t sc = 0;
         bool ok = true;
         Item x;
@@ -330,35 +320,57 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             const float slope = BIAS ? a.slopes[x.head] * kLog2e : 0.0f;
             const float place = (float)(i + x.sp.lk - x.sp.lq);
             float m = -INFINITY;
-            uint64_t sum = 0;
+            uint64_t sum = 0, sum2 = 0;
             for (int j = 0; j < tiles_k; ++j, ++sc) {
                 TOK_WAIT(s_full + w, sc & 1u);
                 if (!ok) break;
                 tc_fence_after();
-                float s[128];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) tmem_ld32(ts + 32 * q, reinterpret_cast<uint32_t*>(s) + 32 * q);
-                tmem_wait_ld();
-                if (C::kSep) {
-                    tc_fence_before();
-                    mbar_arrive(s_read + w);
-                }
+                // Two passes over the scores, 32 columns at a time, the next on their way: first the maximum, then,
+                // backwards, the probabilities.  Held whole, a row of 128 left the scheduler no registers to overlap
+                // anything with.
                 const int j0 = 128 * j;
                 const bool masked = j0 + 127 > warp_min;
-                if (CAP) cap_scores<128>(a, s);
-                if (BIAS) bias_scores<128>(s, CAP ? 1.0f : a.scale2, slope, place - (float)j0);
-                if (masked) {
+                float s[2][32];
+                bool fast = false;                        // the cap's polynomial serves (tanh_fast)
+                auto fetch = [&](int q) { tmem_ld32(ts + 32 * q, reinterpret_cast<uint32_t*>(s[q & 1])); };
+                auto score = [&](int q) {                 // raw products to what the softmax takes
+                    float (&x)[32] = s[q & 1];
+                    if (CAP) tanh_scores<32>(a, x, BIAS ? tanh_fast(a, largest<32>(x)) : fast);
+                    if (BIAS) bias_scores<32>(x, CAP ? a.cap2 : a.scale2, slope, place - (float)(j0 + 32 * q));
+                    if (masked) {
 #pragma unroll
-                    for (int k = 0; k < 128; ++k)
-                        if (j0 + k > lim) s[k] = -INFINITY;
-                }
-                float top = max3(s[0], s[1], s[2]), top2 = max3(s[3], s[4], s[5]);
+                        for (int k = 0; k < 32; ++k)
+                            if (j0 + 32 * q + k > lim) x[k] = -INFINITY;
+                    }
+                };
+                float top = -INFINITY, top2 = -INFINITY, big = 0.0f;
+                fetch(0);
 #pragma unroll
-                for (int k = 6; k < 126; k += 4) {
-                    top = max3(top, s[k], s[k + 1]);
-                    top2 = max3(top2, s[k + 2], s[k + 3]);
+                for (int q = 0; q < 4; ++q) {
+                    tmem_wait_ld();
+                    if (q < 3) fetch(q + 1);
+                    float (&x)[32] = s[q & 1];
+                    if (CAP && !BIAS) big = fmaxf(big, largest<32>(x));
+                    if (BIAS || (q == 3 && !CAP)) {
+                        score(q);
+                    } else if (masked) {                  // a cap keeps the order: the maximum is capped at the end
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            if (j0 + 32 * q + k > lim) x[k] = -INFINITY;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4) {
+                        top = max3(top, x[k], x[k + 1]);
+                        top2 = max3(top2, x[k + 2], x[k + 3]);
+                    }
                 }
-                top = fmaxf(max3(top, top2, s[126]), s[127]);
+                top = fmaxf(top, top2);
+                fetch(2);
+                if (CAP && !BIAS) {
+                    fast = tanh_fast(a, big);
+                    if (top > -INFINITY) top = tanh_raw(a, top);
+                    score(3);
+                }
                 if (j > 0) TOK_WAIT(pv_done + w, (sc - 1) & 1u);          // frees the probabilities and the output
                 if (!ok) break;
                 if (j == 0) {
@@ -368,44 +380,48 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                     const float f = grown == m ? 1.0f : ex2((m - grown) * c);
                     m = grown;
                     sum = mul2(sum, pack2(f, f));
+                    sum2 = mul2(sum2, pack2(f, f));
                     tc_fence_after();
 #pragma unroll
-                    for (int q = 0; q < DP / 32; ++q) {
-                        float v[32];
-                        tmem_ld32(to + 32 * q, reinterpret_cast<uint32_t*>(v));
-                        tmem_wait_ld();
+                    for (int q = 0; q < DP / 16; ++q) {
+                        uint32_t v[16];
+                        tmem_ld16(to + 16 * q, v);
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) v[k] *= f;
-                        tmem_st32(to + 32 * q, reinterpret_cast<uint32_t*>(v));
+                        for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * f);
+                        tmem_st16(to + 16 * q, v);
                     }
-                    tmem_wait_st();
                 }
                 const float base = m == -INFINITY ? 0.0f : -m * c + kLift<T>;
                 const uint64_t c2 = pack2(c, c), b2 = pack2(base, base);
-                auto exps = [&](auto poly) {
+                auto exps = [&](int q) {
+                    float (&x)[32] = s[q & 1];
+                    uint32_t p[16];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        uint32_t p[16];
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            const uint64_t y = fma2(pack2(s[32 * q + 2 * k], s[32 * q + 2 * k + 1]), c2, b2);
-                            const uint64_t e = decltype(poly)::value && kPoly(k) ? ex2_poly(y) : ex2_pair(y);
-                            sum = add2(sum, e);
-                            const float2 f = unpack2(e);
-                            p[k] = Elem<T>::pack(f.x, f.y);
-                        }
-                        tmem_st16(tp + 16 * q, p);
+                    for (int k = 0; k < 16; ++k) {
+                        const uint64_t y = fma2(pack2(x[2 * k], x[2 * k + 1]), c2, b2);
+                        const uint64_t e = takes_poly(k, CAP ? 0 : 5) ? ex2_poly(y) : ex2_pair(y);
+                        if (k & 1) sum2 = add2(sum2, e);
+                        else sum = add2(sum, e);
+                        const float2 f = unpack2(e);
+                        p[k] = Elem<T>::pack(f.x, f.y);
                     }
+                    tmem_st16(tp + 16 * q, p);
                 };
-                // masked entries are exactly zero, which only the hardware's exp2 of -inf gives
-                if (masked) exps(std::false_type{});
-                else exps(std::true_type{});
+#pragma unroll
+                for (int q = 3; q >= 0; --q) {
+                    if (q < 3) {
+                        tmem_wait_ld();
+                        if (q > 0) fetch(q - 1);
+                        score(q);
+                    }
+                    exps(q);
+                }
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(p_full + w);
             }
             if (!ok) break;
-            const float2 s2 = unpack2(sum);
+            const float2 s2 = unpack2(add2(sum, sum2));
             const float total = s2.x + s2.y;
             if (tiles_k > 0) TOK_WAIT(pv_done + w, (sc - 1) & 1u);
             if (!ok) break;

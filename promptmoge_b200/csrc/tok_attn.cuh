@@ -83,35 +83,42 @@ __device__ __forceinline__ bool find_tile(const int32_t* cu, int docs, int rows,
     return false;
 }
 
-// tanh of half the argument's exponent form: 1 - 2 / (e^(2 s scale / cap) + 1) of a raw product s.  The hardware's tanh is
+// tanh(scale s / cap) of a raw product s as 1 - 2 / (e^(2 s scale / cap) + 1).  The hardware's tanh is
 // off by up to 2^-11, which a cap of 50 would turn into 3 % of a probability; this form is off by about 2e-7.
 __device__ __forceinline__ float tanh_raw(const Attn& a, float s) {
     return fmaf(-2.0f, rcp_approx(ex2(s * a.tanh_in) + 1.0f), 1.0f);
 }
 __device__ __forceinline__ float capped(const Attn& a, float s) { return a.cap2 * tanh_raw(a, s); }
 
-// tanh(x) / x in x^2 on |x| <= 1: least largest relative error 5.0e-8 (iteratively reweighted least squares in the
-// Chebyshev basis).
-__device__ constexpr float kTanh[7] = {9.999999502e-01f, -3.333283915e-01f, 1.332520403e-01f, -5.345702773e-02f,
-                                       2.028997689e-02f, -6.203375984e-03f, 1.041021598e-03f};
+// tanh(x) / x in x^2 on |x| <= 1/2: the polynomial of least largest error in tanh, 1.3e-7 (iteratively reweighted least
+// squares in the Chebyshev basis).
+__device__ constexpr float kTanh[4] = {9.999976762e-01f, -3.332065520e-01f, 1.314514551e-01f, -4.337248023e-02f};
+constexpr float kTanhEnd = 0.5f;
 
-// Raw products to tanh(scale s / cap).  Scores mostly stay below their cap, where a polynomial on the packed fp32 pipe
-// takes 9 instructions a pair against two trips through the special function unit an element: one warp-wide test.
 template <int N>
-__device__ __forceinline__ void tanh_scores(const Attn& a, float (&s)[N]) {
-    float big = fabsf(s[0]);
+__device__ __forceinline__ float largest(const float (&s)[N]) {
+    float a = fabsf(s[0]), b = fabsf(s[1]);
 #pragma unroll
-    for (int k = 1; k + 1 < N; k += 2) big = max3(big, fabsf(s[k]), fabsf(s[k + 1]));
-    big = fmaxf(big, fabsf(s[N - 1]));
-    const float in = a.cap_in;
-    if (__all_sync(0xffffffffu, big * in <= 1.0f)) {
-        const uint64_t in2 = pack2(in, in);
+    for (int k = 2; k < N - 2; k += 4) {
+        a = max3(a, fabsf(s[k]), fabsf(s[k + 1]));
+        b = max3(b, fabsf(s[k + 2]), fabsf(s[k + 3]));
+    }
+    return max3(a, b, fmaxf(fabsf(s[N - 2]), fabsf(s[N - 1])));
+}
+
+// Raw products to tanh(scale s / cap).  Scores mostly stay well below their cap: where `fast` (no |scale s / cap| of the
+// warp's above 1/2) a polynomial on the packed fp32 pipe takes 6 instructions a pair, against two trips through the
+// special function unit an element.
+template <int N>
+__device__ __forceinline__ void tanh_scores(const Attn& a, float (&s)[N], bool fast) {
+    if (fast) {
+        const uint64_t in2 = pack2(a.cap_in, a.cap_in);
 #pragma unroll
         for (int k = 0; k < N; k += 2) {
             const uint64_t x = mul2(pack2(s[k], s[k + 1]), in2), u = mul2(x, x);
-            uint64_t p = pack2(kTanh[6], kTanh[6]);
+            uint64_t p = pack2(kTanh[3], kTanh[3]);
 #pragma unroll
-            for (int i = 5; i >= 0; --i) p = fma2(p, u, pack2(kTanh[i], kTanh[i]));
+            for (int i = 2; i >= 0; --i) p = fma2(p, u, pack2(kTanh[i], kTanh[i]));
             const float2 f = unpack2(mul2(p, x));
             s[k] = f.x;
             s[k + 1] = f.y;
@@ -121,15 +128,8 @@ __device__ __forceinline__ void tanh_scores(const Attn& a, float (&s)[N]) {
         for (int k = 0; k < N; ++k) s[k] = tanh_raw(a, s[k]);
     }
 }
-template <int N>
-__device__ __forceinline__ void cap_scores(const Attn& a, float (&s)[N]) {
-    tanh_scores<N>(a, s);
-#pragma unroll
-    for (int k = 0; k < N; k += 2) {
-        const float2 f = unpack2(mul2(pack2(s[k], s[k + 1]), pack2(a.cap2, a.cap2)));
-        s[k] = f.x;
-        s[k + 1] = f.y;
-    }
+__device__ __forceinline__ bool tanh_fast(const Attn& a, float big) {
+    return __all_sync(0xffffffffu, big * a.cap_in <= kTanhEnd);      // false for NaN
 }
 
 // s[k] c - slope |far - k|.  Where no row of the warp has its own place among the columns, the distance is linear in k.
@@ -152,31 +152,31 @@ __device__ __forceinline__ void bias_scores(float (&s)[N], float c, float slope,
 }
 
 // 2^x of a pair: the special function unit (16 a cycle and SM), or a polynomial on the fp32 pipe beside it.  2^x = 2^n 2^f,
-// n the nearest integer (by adding 1.5 2^23, which leaves it in the low bits), f in [-1/2, 1/2], 2^f by a polynomial of
-// degree 4 with least largest relative error 2.6e-6, its exponent field raised by n.  x from -125 up to 127.
+// n the nearest integer (by adding 1.5 2^23, which leaves it in the low bits), f in [-1/2, 1/2]; 2^f = 1 + f q(f), q of
+// degree 3 with least largest relative error of the whole, 2.9e-6 in fp32 (iteratively reweighted least squares in the
+// Chebyshev basis); its exponent field is raised by n.  x below -127, -inf with it, gives exactly 0 (at -127, f is 0 and
+// the exponent field, 127, is lowered by 127); x up to 127.
 __device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
     const float2 f = unpack2(x);
     return pack2(ex2(f.x), ex2(f.y));
 }
 __device__ __forceinline__ uint64_t ex2_poly(uint64_t x) {
     const float2 v = unpack2(x);
-    x = pack2(fmaxf(v.x, -125.0f), fmaxf(v.y, -125.0f));
+    x = pack2(fmaxf(v.x, -127.0f), fmaxf(v.y, -127.0f));
     const uint64_t t = add2(x, pack2(12582912.0f, 12582912.0f));
     const uint64_t f = fma2(add2(t, pack2(-12582912.0f, -12582912.0f)), pack2(-1.0f, -1.0f), x);
-    uint64_t p = pack2(9.570100592e-03f, 9.570100592e-03f);
-    p = fma2(p, f, pack2(5.591786022e-02f, 5.591786022e-02f));
-    p = fma2(p, f, pack2(2.402474486e-01f, 2.402474486e-01f));
-    p = fma2(p, f, pack2(6.931218148e-01f, 6.931218148e-01f));
-    p = fma2(p, f, pack2(9.999992614e-01f, 9.999992614e-01f));
+    uint64_t p = pack2(9.582852812e-03f, 9.582852812e-03f);
+    p = fma2(p, f, pack2(5.590642500e-02f, 5.590642500e-02f));
+    p = fma2(p, f, pack2(2.402409862e-01f, 2.402409862e-01f));
+    p = fma2(p, f, pack2(6.931241933e-01f, 6.931241933e-01f));
+    p = fma2(p, f, pack2(1.0f, 1.0f));
     const float2 tf = unpack2(t), pf = unpack2(p);
     return pack2(__int_as_float(__float_as_int(pf.x) + (__float_as_int(tf.x) << 23)),
                  __int_as_float(__float_as_int(pf.y) + (__float_as_int(tf.y) << 23)));
 }
-// Which of 16 pairs take the polynomial.
-#ifndef TOK_POLY
-#define TOK_POLY 5
-#endif
-__device__ __forceinline__ constexpr bool kPoly(int k) { return (k * TOK_POLY) % 16 < TOK_POLY; }
+// Which of 16 pairs take the polynomial: with `share` of them the fp32 pipe (2 cycles a packed instruction) and the special
+// function unit (16 a pair) finish together.  A cap leaves the fp32 pipe no room.
+__device__ __forceinline__ constexpr bool takes_poly(int k, int share) { return (k * share) % 16 < share; }
 
 // Registers move from the loading and issuing warps to the two softmax warpgroups: 2 * 208 + 88 = 3 * 168, what the block
 // of three warpgroups was launched with.

@@ -288,7 +288,7 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
         constexpr float kP = Elem<T>::kFmt == 0 ? 15.0f : 0.0f;            // log2 of the factor P carries
         const float lift = ds_lift<T>(g.norms);
         const float pd = Elem<T>::kFmt == 0 ? lift * exp2f(-kP) : 1.0f;
-        const float c = (CAP || BIAS) ? 1.0f : a.scale2;
+        const float c = BIAS ? 1.0f : (CAP ? a.cap2 : a.scale2);
         // columns [lo, hi) of the streamed side take part in this row
         int lo = 0, hi;
         if (KEYS) {
@@ -310,7 +310,6 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
             const int t = t0 + i % per, c0 = 128 * t + 64 * w;             // first column within the document
             const int h = KEYS ? kvh * a.group + i / per : head;
             const float slope = BIAS ? a.slopes[h] * kLog2e : 0.0f;
-            const float far = KEYS ? (float)(c0 + off - row) : (float)(c0 - (row + off));
             const bool masked = c0 < lo_max || c0 + 64 > hi_min;
             const float2* st = reinterpret_cast<const float2*>(smem + C::kStats + (i % C::kStages) * C::kStatRoom) +
                                ((sp.q0 + 128 * t) & 1) + 64 * w;
@@ -323,17 +322,19 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
             tmem_ld32(ts, reinterpret_cast<uint32_t*>(p));
             tmem_ld32(ts + 32, reinterpret_cast<uint32_t*>(p) + 32);
             tmem_wait_ld();
+            if (CAP) {
+                tanh_scores<64>(a, p, tanh_fast(a, largest<64>(p)));
 #pragma unroll
-            for (int k = 0; k < 64; ++k) {
-                float x = p[k];
-                if (CAP) {
-                    u[k] = fmaf(-2.0f, rcp_approx(ex2(x * a.tanh_in) + 1.0f), 1.0f);
-                    x = a.cap2 * u[k];
-                } else if (BIAS) {
-                    x *= a.scale2;
-                }
-                if (BIAS) x = fmaf(-slope, fabsf(far + (float)k), x);
-                p[k] = ex2(fmaf(x, c, kP - (KEYS ? st[k].x : my_lse)));
+                for (int k = 0; k < 64; ++k) u[k] = p[k];
+            }
+            if (BIAS) bias_scores<64>(p, CAP ? a.cap2 : a.scale2, slope, KEYS ? (float)(row - off - c0) : (float)(row + off - c0));
+#pragma unroll
+            for (int k = 0; k < 64; k += 2) {
+                const uint64_t shift = KEYS ? pack2(kP - st[k].x, kP - st[k + 1].x) : pack2(kP - my_lse, kP - my_lse);
+                const uint64_t x = fma2(pack2(p[k], p[k + 1]), pack2(c, c), shift);
+                const float2 e = unpack2(takes_poly(k / 2, CAP ? 0 : 5) ? ex2_poly(x) : ex2_pair(x));
+                p[k] = e.x;
+                p[k + 1] = e.y;
             }
             if (masked) {
 #pragma unroll
