@@ -22,7 +22,6 @@ namespace {
 using namespace tok;
 
 constexpr int kStatBlocks = 256;
-constexpr int kStatPad = 132;                 // columns a tile may read past the last row
 
 struct Grad {
     Attn a;
@@ -111,25 +110,35 @@ __global__ void __launch_bounds__(256)
     }
 }
 
+// Heads up to 64 stream tiles of 64 with one compute warpgroup, two CTAs a SM: one's softmax runs under the other's
+// products, starts and ends.  Wider heads leave tensor memory for one CTA, with tiles of 128 and two warpgroups.
 template <int DP>
 struct Bwd {
-    static constexpr int kTile = 128 * DP * 2;
+    static constexpr int kGroups = DP == 64 ? 1 : 2;          // compute warpgroups, 64 streamed rows each
+    static constexpr int kCtas = DP == 64 ? 2 : 1;
+    static constexpr int kBT = 64 * kGroups;
+    static constexpr int kThreads = 128 * kGroups + 64;       // then the loader and the MMA issuer
     static constexpr int kStages = DP == 64 ? 4 : 2;
-    static constexpr int kStat = 130 * 8;                     // bytes of a tile's stats: from an even column on
-    static constexpr int kStatRoom = 1152;
+    static constexpr int kTile = 128 * DP * 2;                // stationary
+    static constexpr int kStrip = kBT * 128;                  // 64 values of every streamed row
+    static constexpr int kPart = kStrip * (DP / 64);          // a streamed tile
     static constexpr int kStream = 2 * kTile;                 // offset of the ring
-    static constexpr int kStats = kStream + kStages * 2 * kTile;
+    static constexpr int kStats = kStream + kStages * 2 * kPart;
+    static constexpr int kStatRoom = kBT * 8;
     static constexpr int kBars = kStats + kStages * kStatRoom;
-    static constexpr int kSmem = kBars + 512;
-    static constexpr uint32_t kS = 0, kDP = 128, kOut0 = 256, kOut1 = 256 + DP;
+    static constexpr int kSmem = kBars + 256;
+    static constexpr uint32_t kCols = DP == 64 ? 256 : 512;   // tensor memory
+    static constexpr uint32_t kS = 0, kDP = kBT, kOut0 = 2 * kBT, kOut1 = 2 * kBT + DP;
 };
-
-constexpr int kBwdThreads = 320;              // two compute warpgroups (halves of the columns), the loader, the issuer
 
 struct Bars {
     uint64_t *a_full, *b_full, *b_empty, *s_full, *dp_full, *p_full, *ds_full, *done, *drain;
     volatile int* abort_flag;
 };
+
+// log2 of the factor that P carries before it is rounded.
+template <typename T> constexpr float kPLift = 0.0f;
+template <> constexpr float kPLift<__half> = 15.0f;
 
 // The factor that dS carries before it is rounded.
 template <typename T>
@@ -167,65 +176,92 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
     const int head = KEYS ? 0 : block % a.Hq;                       // query CTAs: their head
     const int kvh = KEYS ? block % a.Hk : head / a.group;
     const int r0 = tile * 128;                                      // first stationary row within the document
-    // streamed tiles of 128: queries t0 .. t1 - 1 of each head of the group, or keys
+    // streamed tiles: queries t0 .. t1 - 1 of each head of the group, or keys
     int t0 = 0, t1 = 0;
     if (KEYS) {
         if (r0 < sp.lk) {
-            t1 = (sp.lq + 127) / 128;
-            if (a.causal && r0 >= sp.prefix) t0 = min(t1, max(0, r0 - off) / 128);
+            t1 = (sp.lq + C::kBT - 1) / C::kBT;
+            if (a.causal && r0 >= sp.prefix) t0 = min(t1, max(0, r0 - off) / C::kBT);
         }
     } else {
-        t1 = (key_end(a, sp, r0 + 128) + 127) / 128;
+        t1 = (key_end(a, sp, r0 + 128) + C::kBT - 1) / C::kBT;
     }
     const int per = t1 - t0, total = KEYS ? per * a.group : per;
 
-    if (warp == 8) {
-        if (lane == 0 && total > 0) {
+    if (warp == 4 * C::kGroups) {
+        if (total > 0) {
             bool ok = true;
             const int row = (KEYS ? sp.k0 : sp.q0) + r0, h = KEYS ? kvh : head;
-            mbar_arrive_expect_tx(b.a_full, 2 * C::kTile);
+            if (lane == 0) {
+                mbar_arrive_expect_tx(b.a_full, 2 * C::kTile);
 #pragma unroll
-            for (int c = 0; c < DP / 64; ++c) {
-                tma_tile3d(smem_u32(smem + c * 16384), &ma0, 64 * c, h, row, b.a_full);
-                tma_tile3d(smem_u32(smem + C::kTile + c * 16384), &ma1, 64 * c, h, row, b.a_full);
+                for (int c = 0; c < DP / 64; ++c)
+#pragma unroll
+                    for (int r = 0; r < 128; r += 64) {
+                        tma_tile3d(smem_u32(smem + c * 16384 + r * 128), &ma0, 64 * c, h, row + r, b.a_full);
+                        tma_tile3d(smem_u32(smem + C::kTile + c * 16384 + r * 128), &ma1, 64 * c, h, row + r, b.a_full);
+                    }
             }
+            // each lane's share of a tile's statistics, fetched a tile ahead
+            float2 stat[C::kBT / 32];
+            auto fetch = [&](int i) {
+                const int t = t0 + i % per, bh = kvh * a.group + i / per;
+#pragma unroll
+                for (int e = 0; e < C::kBT / 32; ++e) {
+                    const int64_t at = sp.q0 + (int64_t)C::kBT * t + lane + 32 * e;
+                    stat[e] = at < a.Tq ? g.stat[bh * g.stat_ld + at] : make_float2(0.0f, 0.0f);
+                }
+            };
+            if (KEYS) fetch(0);
             for (int i = 0; i < total; ++i) {
                 const int st = i % C::kStages;
-                if (!mbar_wait(b.b_empty + st, ((i / C::kStages) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
+                ok = __all_sync(0xffffffffu, mbar_wait(b.b_empty + st, ((i / C::kStages) & 1u) ^ 1u, abort_flag));
+                if (!ok) break;
                 const int t = t0 + i % per, bh = KEYS ? kvh * a.group + i / per : kvh;
-                const int brow = (KEYS ? sp.q0 : sp.k0) + 128 * t;
-                uint8_t* to = smem + C::kStream + st * 2 * C::kTile;
-                mbar_arrive_expect_tx(b.b_full + st, 2 * C::kTile + (KEYS ? C::kStat : 0));
+                const int brow = (KEYS ? sp.q0 : sp.k0) + C::kBT * t;
+                if (lane == 0) {
+                    uint8_t* to = smem + C::kStream + st * 2 * C::kPart;
+                    mbar_arrive_expect_tx(b.b_full + st, 2 * C::kPart);
 #pragma unroll
-                for (int c = 0; c < DP / 64; ++c) {
-                    tma_tile3d(smem_u32(to + c * 16384), &mb0, 64 * c, bh, brow, b.b_full + st);
-                    tma_tile3d(smem_u32(to + C::kTile + c * 16384), &mb1, 64 * c, bh, brow, b.b_full + st);
+                    for (int c = 0; c < DP / 64; ++c)
+#pragma unroll
+                        for (int r = 0; r < C::kBT; r += 64) {
+                            tma_tile3d(smem_u32(to + c * C::kStrip + r * 128), &mb0, 64 * c, bh, brow + r, b.b_full + st);
+                            tma_tile3d(smem_u32(to + C::kPart + c * C::kStrip + r * 128), &mb1, 64 * c, bh, brow + r, b.b_full + st);
+                        }
                 }
-                if (KEYS)
-                    bulk_g2s(smem_u32(smem + C::kStats + st * C::kStatRoom), g.stat + bh * g.stat_ld + (brow & ~1), C::kStat,
-                             b.b_full + st);
+                if (KEYS) {
+                    float* to = reinterpret_cast<float*>(smem + C::kStats + st * C::kStatRoom);
+#pragma unroll
+                    for (int e = 0; e < C::kBT / 32; ++e) {
+                        to[lane + 32 * e] = kPLift<T> - stat[e].x;
+                        to[C::kBT + lane + 32 * e] = -stat[e].y;
+                    }
+                    if (i + 1 < total) fetch(i + 1);
+                }
+                mbar_arrive(b.b_full + st);
             }
-            if (!ok) {
+            if (!ok && lane == 0) {
                 *abort_flag = 1;
                 flag(a.status, PMG_ERR_TIMEOUT);
             }
         }
-    } else if (warp == 9) {
+    } else if (warp == 4 * C::kGroups + 1) {
         const int ksteps = (a.D + 15) / 16;
-        const uint32_t id_s = idesc16(Elem<T>::kFmt, 128, 128, false, false);
+        const uint32_t id_s = idesc16(Elem<T>::kFmt, 128, C::kBT, false, false);
         const uint32_t id_o = idesc16(Elem<T>::kFmt, 128, ksteps * 16, false, true);
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t ph) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, ph, abort_flag)); };
-        auto stage = [&](int i) { return smem + C::kStream + (i % C::kStages) * 2 * C::kTile; };
+        auto stage = [&](int i) { return smem + C::kStream + (i % C::kStages) * 2 * C::kPart; };
         // a streamed tile has landed; rows behind the document's last must not reach a sum over rows (0 * NaN)
         auto landed = [&](int i) {
             if (!wait(b.b_full + i % C::kStages, (i / C::kStages) & 1u)) return false;
-            const int valid = (KEYS ? sp.lq : sp.lk) - 128 * (t0 + i % per);
-            if (valid < 128) {
+            const int valid = (KEYS ? sp.lq : sp.lk) - C::kBT * (t0 + i % per);
+            if (valid < C::kBT) {
                 uint8_t* s = stage(i);
                 for (int c = 0; c < (KEYS ? 2 : 1) * (DP / 64); ++c)
-                    for (int x = valid * 128 + lane * 16; x < 16384; x += 512)
-                        *reinterpret_cast<uint4*>(s + c * 16384 + x) = make_uint4(0, 0, 0, 0);
+                    for (int x = valid * 128 + lane * 16; x < C::kStrip; x += 512)
+                        *reinterpret_cast<uint4*>(s + c * C::kStrip + x) = make_uint4(0, 0, 0, 0);
                 fence_proxy_async();
                 __syncwarp();
             }
@@ -234,20 +270,20 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
         const uint32_t lead = elect_one();
         auto square = [&](int i, int which) {           // scores (0) or dP (1) of tile i
             tc_fence_after();
-            const uint32_t x = desc_lo(smem_u32(smem + which * C::kTile), 16), y = desc_lo(smem_u32(stage(i) + which * C::kTile), 16);
+            const uint32_t x = desc_lo(smem_u32(smem + which * C::kTile), 16), y = desc_lo(smem_u32(stage(i) + which * C::kPart), 16);
 #pragma unroll
             for (int s = 0; s < DP / 16; ++s)
                 if (s < ksteps) {
-                    const uint32_t at = ((s >> 2) * 16384 + (s & 3) * 32) >> 4;
-                    mma16(lead, tmem + (which ? C::kDP : C::kS), x + at, y + at, id_s, s > 0);
+                    const uint32_t in = (s & 3) * 2;
+                    mma16(lead, tmem + (which ? C::kDP : C::kS), x + (s >> 2) * 1024 + in, y + (s >> 2) * (C::kStrip / 16) + in, id_s, s > 0);
                 }
             mma_commit_if(lead, which ? b.dp_full : b.s_full);
         };
         auto sum = [&](int i, int which) {              // out0 += dS B0, out1 += P B1
             tc_fence_after();
-            const uint32_t x = tmem + (which ? C::kS : C::kDP), y = desc_lo(smem_u32(stage(i) + which * C::kTile), 16384);
+            const uint32_t x = tmem + (which ? C::kS : C::kDP), y = desc_lo(smem_u32(stage(i) + which * C::kPart), C::kStrip);
 #pragma unroll
-            for (int s = 0; s < 8; ++s)                 // each warpgroup's half lies in its own columns
+            for (int s = 0; s < C::kBT / 16; ++s)       // each warpgroup's half lies in its own columns
                 mma16_ts(lead, tmem + (which ? C::kOut1 : C::kOut0), x + (s >> 2) * 64 + (s & 3) * 8, y + s * 128, id_o, i > 0 || s > 0);
         };
         if (total > 0) {
@@ -285,9 +321,8 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
         const int w = warp >> 2, row = r0 + (warp & 3) * 32 + lane;        // column half; stationary row in the document
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + C::kS + 64 * w, td = tmem + lanes + C::kDP + 64 * w;
-        constexpr float kP = Elem<T>::kFmt == 0 ? 15.0f : 0.0f;            // log2 of the factor P carries
         const float lift = ds_lift<T>(g.norms);
-        const float pd = Elem<T>::kFmt == 0 ? lift * exp2f(-kP) : 1.0f;
+        const float pd = Elem<T>::kFmt == 0 ? lift * exp2f(-kPLift<T>) : 1.0f;
         const float c = BIAS ? 1.0f : (CAP ? a.cap2 : a.scale2);
         // columns [lo, hi) of the streamed side take part in this row
         int lo = 0, hi;
@@ -305,52 +340,66 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
             my_lse = s.x;
             my_delta = s.y;
         }
+        const uint64_t my_shift = pack2(kPLift<T> - my_lse, kPLift<T> - my_lse), my_less = pack2(-my_delta, -my_delta);
         bool ok = true;
         for (int i = 0; i < total; ++i) {
-            const int t = t0 + i % per, c0 = 128 * t + 64 * w;             // first column within the document
+            const int t = t0 + i % per, c0 = C::kBT * t + 64 * w;          // first column within the document
             const int h = KEYS ? kvh * a.group + i / per : head;
             const float slope = BIAS ? a.slopes[h] * kLog2e : 0.0f;
+            const float far = KEYS ? (float)(row - off - c0) : (float)(row + off - c0);
             const bool masked = c0 < lo_max || c0 + 64 > hi_min;
-            const float2* st = reinterpret_cast<const float2*>(smem + C::kStats + (i % C::kStages) * C::kStatRoom) +
-                               ((sp.q0 + 128 * t) & 1) + 64 * w;
+            const float* shift = reinterpret_cast<const float*>(smem + C::kStats + (i % C::kStages) * C::kStatRoom) + 64 * w;
+            const float* less = shift + C::kBT;
+            auto pair = [](const float* at) { return *reinterpret_cast<const ulonglong2*>(at); };   // four columns
             if (KEYS) TOK_WAIT(b.b_full + i % C::kStages, (i / C::kStages) & 1u);
             if (!ok) break;
             TOK_WAIT(b.s_full, i & 1u);
             if (!ok) break;
             tc_fence_after();
-            float p[64], u[CAP ? 64 : 1];
+            float p[64];
             tmem_ld32(ts, reinterpret_cast<uint32_t*>(p));
-            tmem_ld32(ts + 32, reinterpret_cast<uint32_t*>(p) + 32);
             tmem_wait_ld();
-            if (CAP) {
-                tanh_scores<64>(a, p, tanh_fast(a, largest<64>(p)));
+            tmem_ld32(ts + 32, reinterpret_cast<uint32_t*>(p) + 32);
 #pragma unroll
-                for (int k = 0; k < 64; ++k) u[k] = p[k];
-            }
-            if (BIAS) bias_scores<64>(p, CAP ? a.cap2 : a.scale2, slope, KEYS ? (float)(row - off - c0) : (float)(row + off - c0));
+            for (int q = 0; q < 2; ++q) {
+                float (&x)[32] = *reinterpret_cast<float (*)[32]>(p + 32 * q);
+                float u[CAP ? 32 : 1];
+                if (q) tmem_wait_ld();
+                if constexpr (CAP) {
+                    tanh_scores<32>(a, x, tanh_fast(a, largest<32>(x)));
 #pragma unroll
-            for (int k = 0; k < 64; k += 2) {
-                const uint64_t shift = KEYS ? pack2(kP - st[k].x, kP - st[k + 1].x) : pack2(kP - my_lse, kP - my_lse);
-                const uint64_t x = fma2(pack2(p[k], p[k + 1]), pack2(c, c), shift);
-                const float2 e = unpack2(takes_poly(k / 2, CAP ? 0 : 5) ? ex2_poly(x) : ex2_pair(x));
-                p[k] = e.x;
-                p[k + 1] = e.y;
-            }
-            if (masked) {
+                    for (int k = 0; k < 32; ++k) u[k] = fmaf(-x[k], x[k], 1.0f);     // the cap's slope
+                }
+                if (BIAS) bias_scores<32>(x, CAP ? a.cap2 : a.scale2, slope, far - (float)(32 * q));
 #pragma unroll
-                for (int k = 0; k < 64; ++k)
-                    if (c0 + k < lo || c0 + k >= hi) p[k] = 0.0f;
-            }
-            if (KEYS) {
+                for (int k = 0; k < 32; k += 4) {
+                    ulonglong2 z = make_ulonglong2(my_shift, my_shift);
+                    if (KEYS) z = pair(shift + 32 * q + k);
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
+                    for (int e = 0; e < 2; ++e) {
+                        const uint64_t y = fma2(pack2(x[k + 2 * e], x[k + 2 * e + 1]), pack2(c, c), e ? z.y : z.x);
+                        const float2 f = unpack2(takes_poly(k / 2 + e, CAP ? 0 : 5) ? ex2_poly(y) : ex2_pair(y));
+                        x[k + 2 * e] = f.x;
+                        x[k + 2 * e + 1] = f.y;
+                    }
+                }
+                if (masked) {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k)
+                        if (c0 + 32 * q + k < lo || c0 + 32 * q + k >= hi) x[k] = 0.0f;
+                }
+                if (KEYS) {
                     uint32_t r[16];
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) r[k] = Elem<T>::pack(p[32 * q + 2 * k], p[32 * q + 2 * k + 1]);
-                    tmem_st16(ts + 16 * q, r);
+                    for (int k = 0; k < 16; ++k) r[k] = Elem<T>::pack(x[2 * k], x[2 * k + 1]);
+                    tmem_st16(ts + 16 * q, r);            // over scores that have been read
                 }
-                tmem_wait_st();
+                if constexpr (CAP) {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) x[k] *= u[k];
+                }
             }
+            if (KEYS) tmem_wait_st();
             tc_fence_before();
             mbar_arrive(b.p_full);
             TOK_WAIT(b.dp_full, i & 1u);
@@ -363,11 +412,18 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
                 tmem_ld32(td + 32 * q, reinterpret_cast<uint32_t*>(d));
                 tmem_wait_ld();
 #pragma unroll
-                for (int k = 0; k < 32; ++k) {
-                    float x = p[32 * q + k] * (d[k] - (KEYS ? st[32 * q + k].y : my_delta));
-                    if (Elem<T>::kFmt == 0) x *= pd;
-                    if (CAP) x *= fmaf(-u[32 * q + k], u[32 * q + k], 1.0f);
-                    d[k] = x;
+                for (int k = 0; k < 32; k += 4) {
+                    ulonglong2 z = make_ulonglong2(my_less, my_less);
+                    if (KEYS) z = pair(less + 32 * q + k);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int at = k + 2 * e;
+                        uint64_t y = mul2(add2(pack2(d[at], d[at + 1]), e ? z.y : z.x), pack2(p[32 * q + at], p[32 * q + at + 1]));
+                        if (Elem<T>::kFmt == 0) y = mul2(y, pack2(pd, pd));
+                        const float2 f = unpack2(y);
+                        d[at] = f.x;
+                        d[at + 1] = f.y;
+                    }
                 }
                 if (masked) {
 #pragma unroll
@@ -376,7 +432,7 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
                 }
 #pragma unroll
                 for (int k = 0; k < 16; ++k) r[k] = Elem<T>::pack(d[2 * k], d[2 * k + 1]);
-                tmem_st16(td + 16 * q, r);        // behind what this warp has read: columns 32 q .. 32 q + 31
+                tmem_st16(td + 16 * q, r);                // behind what this warp has read
             }
             tmem_wait_st();
             tc_fence_before();
@@ -385,7 +441,7 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
         if (ok && total > 0) TOK_WAIT(b.done, 0);
         if (ok) {
             tc_fence_after();
-            const float f0 = g.scale / lift, f1 = Elem<T>::kFmt == 0 ? exp2f(-kP) : 1.0f;
+            const float f0 = g.scale / lift, f1 = Elem<T>::kFmt == 0 ? exp2f(-kPLift<T>) : 1.0f;
             const int room = KEYS ? sp.room : sp.lq;        // rows behind k_len get zeros
             const int64_t at = (KEYS ? sp.k0 : sp.q0) + (int64_t)row;
             const bool mine = row < room && at < (KEYS ? a.Tk : a.Tq);
@@ -396,8 +452,8 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
                                : static_cast<T*>(g.dq) + at * g.q_tok + head * g.q_head;
                 const float f = which ? f1 : f0;
 #pragma unroll
-                for (int q = 0; q < DP / 64; ++q) {
-                    const int c1 = w * (DP / 2) + 32 * q;
+                for (int q = 0; q < DP / 32 / C::kGroups; ++q) {
+                    const int c1 = w * (DP / C::kGroups) + 32 * q;
                     float v[32];
                     if (total > 0) {
                         tmem_ld32(tmem + lanes + (which ? C::kOut1 : C::kOut0) + c1, reinterpret_cast<uint32_t*>(v));
@@ -421,7 +477,7 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
 }
 
 template <typename T, int DP, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(kBwdThreads, 1)
+__global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas)
     k_attn_grad(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                 const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo, const __grid_constant__ Grad g) {
     using C = Bwd<DP>;
@@ -446,21 +502,21 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     if (threadIdx.x == 0) {
         mbar_init(b.a_full, 1);
         for (int i = 0; i < C::kStages; ++i) {
-            mbar_init(b.b_full + i, 1);
+            mbar_init(b.b_full + i, 33);             // the bytes, and the loader's lanes with the statistics
             mbar_init(b.b_empty + i, 1);
         }
         mbar_init(b.s_full, 1);
         mbar_init(b.dp_full, 1);
-        mbar_init(b.p_full, 256);
-        mbar_init(b.ds_full, 256);
+        mbar_init(b.p_full, 128 * C::kGroups);
+        mbar_init(b.ds_full, 128 * C::kGroups);
         mbar_init(b.done, 1);
         mbar_init(b.drain, 1);
         *b.abort_flag = 0;
         fence_mbar_init();
     }
-    if (warp == 9) tmem_alloc(slot, 512);
+    if (warp == 4 * C::kGroups + 1) tmem_alloc(slot, C::kCols);
     pdl_begin();
-    if (warp == 8) {
+    if (warp == 4 * C::kGroups) {
         int doc = -1, tile = 0;
         const bool found = find_tile(keys ? g.a.cu_k : g.a.cu_q, g.a.docs, 128, block / (keys ? g.a.Hk : g.a.Hq), &doc, &tile);
         if (lane == 0) {
@@ -479,9 +535,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == 4 * C::kGroups + 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, 512);
+        tmem_dealloc(tmem, C::kCols);
     }
 }
 
@@ -527,12 +583,12 @@ int run(Grad g, const Ins& in, cudaStream_t s) {
     if (key_blocks + query_blocks > INT32_MAX) return PMG_ERR_UNSUPPORTED;
     g.key_blocks = (int)key_blocks;
     CUtensorMap mq, mk, mv, mdo;
-    int e = head_map(&mq, in.q.p, in.q.tok, in.q.head, a.Tq, a.Hq, a.D, 128);
-    if (e == PMG_OK) e = head_map(&mdo, in.dout.p, in.dout.tok, in.dout.head, a.Tq, a.Hq, a.D, 128);
-    if (e == PMG_OK) e = head_map(&mk, in.k.p, in.k.tok, in.k.head, a.Tk, a.Hk, a.D, 128);
-    if (e == PMG_OK) e = head_map(&mv, in.v.p, in.v.tok, in.v.head, a.Tk, a.Hk, a.D, 128);
+    int e = head_map(&mq, in.q.p, in.q.tok, in.q.head, a.Tq, a.Hq, a.D, 64);
+    if (e == PMG_OK) e = head_map(&mdo, in.dout.p, in.dout.tok, in.dout.head, a.Tq, a.Hq, a.D, 64);
+    if (e == PMG_OK) e = head_map(&mk, in.k.p, in.k.tok, in.k.head, a.Tk, a.Hk, a.D, 64);
+    if (e == PMG_OK) e = head_map(&mv, in.v.p, in.v.tok, in.v.head, a.Tk, a.Hk, a.D, 64);
     if (e != PMG_OK) return e;
-    k_attn_grad<T, DP, CAP, BIAS><<<(int)(key_blocks + query_blocks), kBwdThreads, C::kSmem, s>>>(mq, mk, mv, mdo, g);
+    k_attn_grad<T, DP, CAP, BIAS><<<(int)(key_blocks + query_blocks), C::kThreads, C::kSmem, s>>>(mq, mk, mv, mdo, g);
     PMG_LAUNCH_CHECK();
     return PMG_OK;
 }
@@ -550,7 +606,7 @@ using namespace pmg;
 
 extern "C" size_t pmg_attention_grad_workspace_bytes(int64_t Tq, int32_t Hq) {
     if (Tq < 0 || Hq < 0) return 0;
-    return 2 * kStatBlocks * sizeof(float) + ((size_t)(Tq + 1) / 2 * 2 * Hq + kStatPad) * sizeof(float2);
+    return 2 * kStatBlocks * sizeof(float) + (size_t)Tq * Hq * sizeof(float2);
 }
 
 extern "C" int pmg_attention_grad(const void* dout, int64_t do_tok, int64_t do_head, const void* o, int64_t o_tok,
@@ -584,7 +640,7 @@ extern "C" int pmg_attention_grad(const void* dout, int64_t do_tok, int64_t do_h
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < pmg_attention_grad_workspace_bytes(Tq, Hq))
         return PMG_ERR_BAD_ARG;
     g.scale = scale;
-    g.stat_ld = (Tq + 1) / 2 * 2;
+    g.stat_ld = Tq;
     g.dq = dq; g.dk = dk; g.dv = dv;
     g.q_tok = dq_tok; g.q_head = dq_head; g.k_tok = dk_tok; g.k_head = dk_head; g.v_tok = dv_tok; g.v_head = dv_head;
     const Ins in{{dout, do_tok, do_head}, {o, o_tok, o_head}, {q, q_tok, q_head}, {k, k_tok, k_head}, {v, v_tok, v_head}, lse,
