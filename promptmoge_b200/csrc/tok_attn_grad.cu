@@ -110,13 +110,14 @@ __global__ void __launch_bounds__(256)
     }
 }
 
-// Heads up to 64 stream tiles of 64 with one compute warpgroup, two CTAs a SM: one's softmax runs under the other's
-// products, starts and ends.  Wider heads leave tensor memory for one CTA, with tiles of 128 and two warpgroups.
+// A compute warpgroup takes 32 streamed columns: rows this short leave registers for two (heads up to 64) or four
+// warpgroups a CTA, and 16 compute warps on every SM.  Heads up to 64 stream tiles of 64, two CTAs a SM: one's softmax runs
+// under the other's products, starts and ends.  Wider heads leave tensor memory for one CTA, with tiles of 128.
 template <int DP>
 struct Bwd {
-    static constexpr int kGroups = DP == 64 ? 1 : 2;          // compute warpgroups, 64 streamed rows each
+    static constexpr int kGroups = DP == 64 ? 2 : 4;          // compute warpgroups, 32 streamed rows each
     static constexpr int kCtas = DP == 64 ? 2 : 1;
-    static constexpr int kBT = 64 * kGroups;
+    static constexpr int kBT = 32 * kGroups;
     static constexpr int kThreads = 128 * kGroups + 64;       // then the loader and the MMA issuer
     static constexpr int kStages = DP == 64 ? 4 : 2;
     static constexpr int kTile = 128 * DP * 2;                // stationary
@@ -204,20 +205,19 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
             }
             // each lane's share of a tile's statistics, fetched a tile ahead
             float2 stat[C::kBT / 32];
-            auto fetch = [&](int i) {
-                const int t = t0 + i % per, bh = kvh * a.group + i / per;
+            auto fetch = [&](int t, int bh) {
 #pragma unroll
                 for (int e = 0; e < C::kBT / 32; ++e) {
                     const int64_t at = sp.q0 + (int64_t)C::kBT * t + lane + 32 * e;
                     stat[e] = at < a.Tq ? g.stat[bh * g.stat_ld + at] : make_float2(0.0f, 0.0f);
                 }
             };
-            if (KEYS) fetch(0);
+            int t = t0, bh = KEYS ? kvh * a.group : kvh;
+            if (KEYS) fetch(t, bh);
             for (int i = 0; i < total; ++i) {
                 const int st = i % C::kStages;
                 ok = __all_sync(0xffffffffu, mbar_wait(b.b_empty + st, ((i / C::kStages) & 1u) ^ 1u, abort_flag));
                 if (!ok) break;
-                const int t = t0 + i % per, bh = KEYS ? kvh * a.group + i / per : kvh;
                 const int brow = (KEYS ? sp.q0 : sp.k0) + C::kBT * t;
                 if (lane == 0) {
                     uint8_t* to = smem + C::kStream + st * 2 * C::kPart;
@@ -237,9 +237,13 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
                         to[lane + 32 * e] = kPLift<T> - stat[e].x;
                         to[C::kBT + lane + 32 * e] = -stat[e].y;
                     }
-                    if (i + 1 < total) fetch(i + 1);
                 }
                 mbar_arrive(b.b_full + st);
+                if (++t == t1) {
+                    t = t0;
+                    ++bh;
+                }
+                if (KEYS && i + 1 < total) fetch(t, bh);
             }
             if (!ok && lane == 0) {
                 *abort_flag = 1;
@@ -254,9 +258,11 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
         auto wait = [&](uint64_t* bar, uint32_t ph) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, ph, abort_flag)); };
         auto stage = [&](int i) { return smem + C::kStream + (i % C::kStages) * 2 * C::kPart; };
         // a streamed tile has landed; rows behind the document's last must not reach a sum over rows (0 * NaN)
+        int lt = t0;                                    // tile of the next call
         auto landed = [&](int i) {
             if (!wait(b.b_full + i % C::kStages, (i / C::kStages) & 1u)) return false;
-            const int valid = (KEYS ? sp.lq : sp.lk) - C::kBT * (t0 + i % per);
+            const int valid = (KEYS ? sp.lq : sp.lk) - C::kBT * lt;
+            if (++lt == t1) lt = t0;
             if (valid < C::kBT) {
                 uint8_t* s = stage(i);
                 for (int c = 0; c < (KEYS ? 2 : 1) * (DP / 64); ++c)
@@ -284,7 +290,7 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
             const uint32_t x = tmem + (which ? C::kS : C::kDP), y = desc_lo(smem_u32(stage(i) + which * C::kPart), C::kStrip);
 #pragma unroll
             for (int s = 0; s < C::kBT / 16; ++s)       // each warpgroup's half lies in its own columns
-                mma16_ts(lead, tmem + (which ? C::kOut1 : C::kOut0), x + (s >> 2) * 64 + (s & 3) * 8, y + s * 128, id_o, i > 0 || s > 0);
+                mma16_ts(lead, tmem + (which ? C::kOut1 : C::kOut0), x + (s >> 1) * 32 + (s & 1) * 8, y + s * 128, id_o, i > 0 || s > 0);
         };
         if (total > 0) {
             ok = wait(b.a_full, 0) && landed(0);
@@ -320,7 +326,7 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
     } else {
         const int w = warp >> 2, row = r0 + (warp & 3) * 32 + lane;        // column half; stationary row in the document
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + lanes + C::kS + 64 * w, td = tmem + lanes + C::kDP + 64 * w;
+        const uint32_t ts = tmem + lanes + C::kS + 32 * w, td = tmem + lanes + C::kDP + 32 * w;
         const float lift = ds_lift<T>(g.norms);
         const float pd = Elem<T>::kFmt == 0 ? lift * exp2f(-kPLift<T>) : 1.0f;
         const float c = BIAS ? 1.0f : (CAP ? a.cap2 : a.scale2);
@@ -342,101 +348,95 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
         }
         const uint64_t my_shift = pack2(kPLift<T> - my_lse, kPLift<T> - my_lse), my_less = pack2(-my_delta, -my_delta);
         bool ok = true;
+        int t = t0, h = KEYS ? kvh * a.group : head;
+        float slope = BIAS ? a.slopes[h] * kLog2e : 0.0f;
         for (int i = 0; i < total; ++i) {
-            const int t = t0 + i % per, c0 = C::kBT * t + 64 * w;          // first column within the document
-            const int h = KEYS ? kvh * a.group + i / per : head;
-            const float slope = BIAS ? a.slopes[h] * kLog2e : 0.0f;
+            const int c0 = C::kBT * t + 32 * w;                            // first column within the document
             const float far = KEYS ? (float)(row - off - c0) : (float)(row + off - c0);
-            const bool masked = c0 < lo_max || c0 + 64 > hi_min;
-            const float* shift = reinterpret_cast<const float*>(smem + C::kStats + (i % C::kStages) * C::kStatRoom) + 64 * w;
+            const bool masked = c0 < lo_max || c0 + 32 > hi_min;
+            const float* shift = reinterpret_cast<const float*>(smem + C::kStats + (i % C::kStages) * C::kStatRoom) + 32 * w;
             const float* less = shift + C::kBT;
-            auto pair = [](const float* at) { return *reinterpret_cast<const ulonglong2*>(at); };   // four columns
+            auto four = [](const float* at) { return *reinterpret_cast<const ulonglong2*>(at); };   // columns
             if (KEYS) TOK_WAIT(b.b_full + i % C::kStages, (i / C::kStages) & 1u);
             if (!ok) break;
             TOK_WAIT(b.s_full, i & 1u);
             if (!ok) break;
             tc_fence_after();
-            float p[64];
+            float p[32], u[CAP ? 32 : 1];
+            uint32_t r[16];
             tmem_ld32(ts, reinterpret_cast<uint32_t*>(p));
             tmem_wait_ld();
-            tmem_ld32(ts + 32, reinterpret_cast<uint32_t*>(p) + 32);
+            if constexpr (CAP) {
+                tanh_scores<32>(a, p, tanh_fast(a, largest<32>(p)));
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                float (&x)[32] = *reinterpret_cast<float (*)[32]>(p + 32 * q);
-                float u[CAP ? 32 : 1];
-                if (q) tmem_wait_ld();
-                if constexpr (CAP) {
-                    tanh_scores<32>(a, x, tanh_fast(a, largest<32>(x)));
+                for (int k = 0; k < 32; ++k) u[k] = fmaf(-p[k], p[k], 1.0f);             // the cap's slope
+            }
+            if (BIAS) bias_scores<32>(p, CAP ? a.cap2 : a.scale2, slope, far);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) u[k] = fmaf(-x[k], x[k], 1.0f);     // the cap's slope
-                }
-                if (BIAS) bias_scores<32>(x, CAP ? a.cap2 : a.scale2, slope, far - (float)(32 * q));
+            for (int k = 0; k < 32; k += 4) {
+                ulonglong2 z = make_ulonglong2(my_shift, my_shift);
+                if (KEYS) z = four(shift + k);
 #pragma unroll
-                for (int k = 0; k < 32; k += 4) {
-                    ulonglong2 z = make_ulonglong2(my_shift, my_shift);
-                    if (KEYS) z = pair(shift + 32 * q + k);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const uint64_t y = fma2(pack2(x[k + 2 * e], x[k + 2 * e + 1]), pack2(c, c), e ? z.y : z.x);
-                        const float2 f = unpack2(takes_poly(k / 2 + e, CAP ? 0 : 5) ? ex2_poly(y) : ex2_pair(y));
-                        x[k + 2 * e] = f.x;
-                        x[k + 2 * e + 1] = f.y;
-                    }
-                }
-                if (masked) {
-#pragma unroll
-                    for (int k = 0; k < 32; ++k)
-                        if (c0 + 32 * q + k < lo || c0 + 32 * q + k >= hi) x[k] = 0.0f;
-                }
-                if (KEYS) {
-                    uint32_t r[16];
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) r[k] = Elem<T>::pack(x[2 * k], x[2 * k + 1]);
-                    tmem_st16(ts + 16 * q, r);            // over scores that have been read
-                }
-                if constexpr (CAP) {
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) x[k] *= u[k];
+                for (int e = 0; e < 2; ++e) {
+                    const uint64_t y = fma2(pack2(p[k + 2 * e], p[k + 2 * e + 1]), pack2(c, c), e ? z.y : z.x);
+                    const float2 f = unpack2(takes_poly(k / 2 + e, CAP ? 0 : 5) ? ex2_poly(y) : ex2_pair(y));
+                    p[k + 2 * e] = f.x;
+                    p[k + 2 * e + 1] = f.y;
                 }
             }
-            if (KEYS) tmem_wait_st();
+            if (masked) {
+#pragma unroll
+                for (int k = 0; k < 32; ++k)
+                    if (c0 + k < lo || c0 + k >= hi) p[k] = 0.0f;
+            }
+            if (KEYS) {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) r[k] = Elem<T>::pack(p[2 * k], p[2 * k + 1]);
+                tmem_st16(ts, r);                         // over scores that this warp has read
+                tmem_wait_st();
+            }
             tc_fence_before();
             mbar_arrive(b.p_full);
+            if constexpr (CAP) {
+#pragma unroll
+                for (int k = 0; k < 32; ++k) p[k] *= u[k];
+            }
             TOK_WAIT(b.dp_full, i & 1u);
             if (!ok) break;
             tc_fence_after();
+            float d[32];
+            tmem_ld32(td, reinterpret_cast<uint32_t*>(d));
+            tmem_wait_ld();
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                float d[32];
-                uint32_t r[16];
-                tmem_ld32(td + 32 * q, reinterpret_cast<uint32_t*>(d));
-                tmem_wait_ld();
+            for (int k = 0; k < 32; k += 4) {
+                ulonglong2 z = make_ulonglong2(my_less, my_less);
+                if (KEYS) z = four(less + k);
 #pragma unroll
-                for (int k = 0; k < 32; k += 4) {
-                    ulonglong2 z = make_ulonglong2(my_less, my_less);
-                    if (KEYS) z = pair(less + 32 * q + k);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int at = k + 2 * e;
-                        uint64_t y = mul2(add2(pack2(d[at], d[at + 1]), e ? z.y : z.x), pack2(p[32 * q + at], p[32 * q + at + 1]));
-                        if (Elem<T>::kFmt == 0) y = mul2(y, pack2(pd, pd));
-                        const float2 f = unpack2(y);
-                        d[at] = f.x;
-                        d[at + 1] = f.y;
-                    }
+                for (int e = 0; e < 2; ++e) {
+                    const int at = k + 2 * e;
+                    uint64_t y = mul2(add2(pack2(d[at], d[at + 1]), e ? z.y : z.x), pack2(p[at], p[at + 1]));
+                    if (Elem<T>::kFmt == 0) y = mul2(y, pack2(pd, pd));
+                    const float2 f = unpack2(y);
+                    d[at] = f.x;
+                    d[at + 1] = f.y;
                 }
-                if (masked) {
-#pragma unroll
-                    for (int k = 0; k < 32; ++k)
-                        if (c0 + 32 * q + k < lo || c0 + 32 * q + k >= hi) d[k] = 0.0f;
-                }
-#pragma unroll
-                for (int k = 0; k < 16; ++k) r[k] = Elem<T>::pack(d[2 * k], d[2 * k + 1]);
-                tmem_st16(td + 16 * q, r);                // behind what this warp has read
             }
+            if (masked) {
+#pragma unroll
+                for (int k = 0; k < 32; ++k)
+                    if (c0 + k < lo || c0 + k >= hi) d[k] = 0.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < 16; ++k) r[k] = Elem<T>::pack(d[2 * k], d[2 * k + 1]);
+            tmem_st16(td, r);
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(b.ds_full);
+            if (++t == t1) {                              // the next head of the group
+                t = t0;
+                ++h;
+                if (BIAS && i + 1 < total) slope = a.slopes[h] * kLog2e;
+            }
         }
         if (ok && total > 0) TOK_WAIT(b.done, 0);
         if (ok) {
@@ -451,9 +451,8 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
                 T* base = KEYS ? static_cast<T*>(which ? g.dv : g.dk) + at * (which ? g.v_tok : g.k_tok) + kvh * (which ? g.v_head : g.k_head)
                                : static_cast<T*>(g.dq) + at * g.q_tok + head * g.q_head;
                 const float f = which ? f1 : f0;
-#pragma unroll
-                for (int q = 0; q < DP / 32 / C::kGroups; ++q) {
-                    const int c1 = w * (DP / C::kGroups) + 32 * q;
+                {
+                    const int c1 = 32 * w;                                  // a group's share of the columns: DP = 32 groups
                     float v[32];
                     if (total > 0) {
                         tmem_ld32(tmem + lanes + (which ? C::kOut1 : C::kOut0) + c1, reinterpret_cast<uint32_t*>(v));
