@@ -10,8 +10,9 @@
 // Bound by HBM: forwards one read and one write of q and k, backwards two reads and one write.  A group of lanes owns a
 // row (D values as 16-byte vectors, one a lane) and walks several heads of one token with that token's angles in
 // registers: the angles are 8 bytes per pair against 2 bytes per value, so loading them per head would cost more
-// first-level cache traffic than the heads themselves.  The partner of a value in the other half of the head is loaded
-// again (a first-level hit) rather than shuffled: one load against one shuffle per two values.
+// first-level cache traffic than the heads themselves.  A block works on queries or on keys, so that the weights stay in
+// registers too.  The partner of a value in the other half of the head is loaded again (a first-level hit) rather than
+// shuffled: one load against one shuffle per two values.
 // Sums and norms are fp32; a value is rounded once, when it is stored.
 #include <algorithm>
 
@@ -37,178 +38,213 @@ struct RopeArgs {
     const float *cos, *sin;
     const int32_t* pos;
     int64_t T;
-    int places, D, half, interleaved, heads, chunks[2];   // heads per item; items per token of each side
+    int places, D, half, interleaved, heads, chunks[2], blocks[2];   // heads per item; items per token, blocks of each side
     float eps;
     int32_t* status;
-    float* part;              // gradients of w: [blocks][2][D]
+    float* part;              // gradients of w: [blocks[0] + blocks[1]][D]
 };
 
-template <typename T, int V> struct Vec;
-template <int V> struct alignas(2 * V) Raw16 { uint16_t v[V]; };
-template <int V> struct alignas(4 * V) Raw32 { float v[V]; };
-template <int V> struct Vec<__half, V> { using type = Raw16<V>; };
-template <int V> struct Vec<__nv_bfloat16, V> { using type = Raw16<V>; };
-template <int V> struct Vec<float, V> { using type = Raw32<V>; };
-
+// A vector of V values of a row (16 or 8 bytes of 16-bit values, 16 bytes of fp32 ones) and its pairs in fp32.
 template <typename T, int V>
-__device__ __forceinline__ void load(const T* p, float (&f)[V]) {
-    typename Vec<T, V>::type r = *reinterpret_cast<const typename Vec<T, V>::type*>(p);
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = r.v[i];
-    } else {
-        const T* t = reinterpret_cast<const T*>(&r);
-#pragma unroll
-        for (int i = 0; i < V; ++i) f[i] = tok::Elem<T>::to(t[i]);
+struct Row {
+    static constexpr int kWords = V * (int)sizeof(T) / 4;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void get(const T* p) {
+        if constexpr (kWords == 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(p);
+            w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+        } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
+            w[0] = v.x; w[1] = v.y;
+        }
     }
-}
-template <typename T, int V>
-__device__ __forceinline__ void store(T* p, const float (&f)[V]) {
-    typename Vec<T, V>::type r;
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) r.v[i] = f[i];
-    } else {
-        T* t = reinterpret_cast<T*>(&r);
-#pragma unroll
-        for (int i = 0; i < V; ++i) t[i] = tok::Elem<T>::from(f[i]);
+    __device__ __forceinline__ float2 pair(int i) const {
+        if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+        else return tok::Elem<T>::unpack(w[i]);
     }
-    *reinterpret_cast<typename Vec<T, V>::type*>(p) = r;
+    __device__ __forceinline__ void set(int i, float2 f) {
+        if constexpr (sizeof(T) == 4) {
+            w[2 * i] = __float_as_uint(f.x);
+            w[2 * i + 1] = __float_as_uint(f.y);
+        } else {
+            w[i] = tok::Elem<T>::pack(f.x, f.y);
+        }
+    }
+    __device__ __forceinline__ void put(T* p) const {
+        if constexpr (kWords == 4) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    }
+};
+
+__device__ __forceinline__ uint64_t two(float2 f) { return tok::pack2(f.x, f.y); }
+__device__ __forceinline__ float2 swapped(float2 f) { return make_float2(f.y, f.x); }
+
+// The position of token t; one outside the table is reported and taken as 0.
+__device__ __forceinline__ int64_t place_of(const RopeArgs& a, int64_t t, bool tell) {
+    const int p = a.pos ? a.pos[t] : (int)t;
+    if (p >= 0 && p < a.places) return p;
+    if (tell) flag(a.status, PMG_ERR_RANGE);
+    return 0;
 }
 
-// G lanes per row; NCH vectors of V values a lane; U heads at once.
-template <typename T, int V, int NCH, int U, bool GRAD>
-__global__ void __launch_bounds__(kThreads) k_qk_norm_rope(const __grid_constant__ RopeArgs a, int G) {
+// G lanes a row, V values a lane, pairs of them in the packed fp32 pipe; U heads at once, the next U on their way.
+// IL: interleaved pairs, which lie within a lane's vector.  The cost of a value is what bounds this after HBM: unpacking
+// by the element and fp32 copies of whole rows took 28 instructions a value and 99 us for 38,400 tokens of 20 heads of 64.
+template <typename T, int V, int U, bool GRAD, bool IL>
+__global__ void __launch_bounds__(kThreads, 3) k_qk_norm_rope(const __grid_constant__ RopeArgs a, int G) {
+    using namespace tok;
+    using R = Row<T, V>;
+    constexpr int NP = V / 2;
     pdl_begin();
     extern __shared__ float sm[];
     const int lane = threadIdx.x & 31, per_warp = 32 / G, gi = lane / G, gl = lane % G;
-    const int64_t per_token = a.chunks[0] + a.chunks[1], items = a.T * per_token;
-    const int64_t warp = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-    const int64_t stride = (int64_t)gridDim.x * (kThreads / 32) * per_warp;
+    const int which = (int)blockIdx.x >= a.blocks[0];
+    const Side& s = a.side[which];
+    const int per_token = a.chunks[which];
+    const int64_t items = a.T * per_token;
+    const int64_t first = (int64_t)(blockIdx.x - (which ? a.blocks[0] : 0)) * (kThreads / 32) + (threadIdx.x >> 5);
+    const int64_t stride = (int64_t)a.blocks[which] * (kThreads / 32) * per_warp;
     const float inv_d = 1.0f / (float)a.D;
-    const int rot = 2 * a.half;
-    float acc[GRAD ? 2 : 1][NCH][V];
+    const bool in = gl * V < a.D;
+    const int at = in ? gl * V : 0;
+    const bool turned = at < 2 * a.half, ahead = !IL && at < a.half;      // ahead: the pair's first values
+    const int other = turned && !IL ? (ahead ? at + a.half : at - a.half) : at;
+    const int ang = IL ? at / 2 : (ahead ? at : at - a.half);
+    uint64_t w2[GRAD ? NP : 1], acc[GRAD ? NP : 1];
     if constexpr (GRAD) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int c = 0; c < NCH; ++c)
-#pragma unroll
-                for (int e = 0; e < V; ++e) acc[s][c][e] = 0.0f;
+        for (int i = 0; i < NP; ++i) {
+            w2[i] = s.w ? pack2(s.w[at + 2 * i], s.w[at + 2 * i + 1]) : pack2(1.0f, 1.0f);
+            acc[i] = 0;
+        }
     }
 
-    for (int64_t base = warp * per_warp; base < items; base += stride) {
+    for (int64_t base = first * per_warp; base < items; base += stride) {
         const bool live = base + gi < items;
         const int64_t item = live ? base + gi : items - 1;
-        const int64_t t = item / per_token;
-        int chunk = (int)(item - t * per_token);
-        const int which = chunk >= a.chunks[0];
-        if (which) chunk -= a.chunks[0];
-        const Side& s = a.side[which];
-        const int h0 = chunk * a.heads, h1 = live ? min(h0 + a.heads, s.H) : h0;
-        int p = a.pos ? a.pos[t] : (int)t;
-        if (p < 0 || p >= a.places) {
-            if (live && gl == 0) flag(a.status, PMG_ERR_RANGE);
-            p = 0;
-        }
-        // own and partner places, angles (sign folded into sn) and weights of this lane's vectors
-        float cs[NCH][V], sn[NCH][V], w[NCH][V], wp[NCH][V];
-        int at[NCH], other[NCH];
-        bool in[NCH];
+        const int64_t t = per_token == 1 ? item : item / per_token;
+        const int h0 = (int)(item - t * per_token) * a.heads;
+        const int n = live && in ? min(a.heads, s.H - h0) : 0;
+        const T* x = reinterpret_cast<const T*>(s.x) + t * s.xt + h0 * s.xh;
+        const T* d = GRAD ? reinterpret_cast<const T*>(s.dy) + t * s.yt + h0 * s.yh : nullptr;
+        T* o = reinterpret_cast<T*>(s.out) + t * s.ot + h0 * s.oh + at;
+        R rx[2][U], rd[2][GRAD ? U : 1], ro[2][IL ? 1 : U];
+        auto fetch = [&](int b, int h) {
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            const int i0 = (gl + c * G) * V;
-            in[c] = i0 < a.D;
-            at[c] = in[c] ? i0 : 0;
-            other[c] = at[c];
-            const bool turned = at[c] < rot;
-            const bool first = at[c] < a.half;
-            if (turned && !a.interleaved) other[c] = first ? at[c] + a.half : at[c] - a.half;
-            if (V == 1 && turned && a.interleaved) other[c] = at[c] ^ 1;
+            for (int u = 0; u < U; ++u) {
+                if (h + u >= n) continue;
+                const T* row = x + (h + u) * s.xh;
+                rx[b][u].get(row + at);
+                if constexpr (GRAD) {
+                    const T* grow = d + (h + u) * s.yh;
+                    rd[b][u].get(grow + at);
+                    if constexpr (!IL) ro[b][u].get(grow + other);
+                } else if constexpr (!IL) {
+                    ro[b][u].get(row + other);
+                }
+            }
+        };
+        fetch(0, 0);
+        // this token's angles; the rotation's sign in sn, and forwards the weights in both
+        uint64_t cs[NP], sn[NP];
+        {
+            float c[V], z[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const int i = at[c] + e;
-                cs[c][e] = 1.0f;
-                sn[c][e] = 0.0f;
-                if (turned) {
-                    const int k = a.interleaved ? i >> 1 : (first ? i : i - a.half);
-                    const bool neg = a.interleaved ? !(i & 1) : first;
-                    cs[c][e] = a.cos[(int64_t)p * a.half + k];
-                    const float v = a.sin[(int64_t)p * a.half + k];
-                    sn[c][e] = neg ? -v : v;
-                }
-                w[c][e] = s.w ? s.w[i] : 1.0f;
+                c[e] = 1.0f;
+                z[e] = 0.0f;
             }
-            if constexpr (!GRAD) {
+            if (turned) {
+                const int64_t p = place_of(a, t, live && gl == 0) * a.half + ang;
+                constexpr int N = IL ? NP : V;
+#pragma unroll
+                for (int e = 0; e < N; e += 2) {
+                    const float2 fc = *reinterpret_cast<const float2*>(a.cos + p + e), fs = *reinterpret_cast<const float2*>(a.sin + p + e);
+                    if constexpr (IL) {
+                        c[2 * e] = c[2 * e + 1] = fc.x;
+                        c[2 * e + 2] = c[2 * e + 3] = fc.y;
+                        z[2 * e] = -fs.x;
+                        z[2 * e + 1] = fs.x;
+                        z[2 * e + 2] = -fs.y;
+                        z[2 * e + 3] = fs.y;
+                    } else {
+                        c[e] = fc.x;
+                        c[e + 1] = fc.y;
+                        z[e] = ahead ? -fs.x : fs.x;
+                        z[e + 1] = ahead ? -fs.y : fs.y;
+                    }
+                }
+            }
+            if (!GRAD && s.w) {
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    const int i = (V > 1 && a.interleaved) ? at[c] + (e ^ 1) : other[c] + e;
-                    wp[c][e] = s.w ? s.w[i] : 1.0f;
+                    c[e] *= s.w[at + e];
+                    z[e] *= s.w[IL ? at + (e ^ 1) : other + e];
                 }
             }
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                cs[i] = pack2(c[2 * i], c[2 * i + 1]);
+                sn[i] = GRAD ? pack2(-z[2 * i], -z[2 * i + 1]) : pack2(z[2 * i], z[2 * i + 1]);
+            }
         }
-        const T* xt = reinterpret_cast<const T*>(s.x) + t * s.xt;
-        const T* yt = GRAD ? reinterpret_cast<const T*>(s.dy) + t * s.yt : nullptr;
-        T* ot = reinterpret_cast<T*>(s.out) + t * s.ot;
-        const bool swap = V > 1 && a.interleaved;
-        for (int hb = 0; hb < a.heads; hb += U) {
-            float x[U][NCH][V], y[U][NCH][V];   // x; its partner (forwards) or g (backwards)
+        auto work = [&](int b, int h) {
+            uint64_t v[U][NP], g[GRAD ? U : 1][NP];
             float sq[U], gx[U];
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int h = h0 + hb + u;
-                const bool on = h < h1;
-                sq[u] = gx[u] = 0.0f;
+                uint64_t q2 = 0, x2 = 0;
 #pragma unroll
-                for (int c = 0; c < NCH; ++c) {
-                    float d[V], dp[V];
-#pragma unroll
-                    for (int e = 0; e < V; ++e) x[u][c][e] = y[u][c][e] = d[e] = dp[e] = 0.0f;
-                    if (on && in[c]) {
-                        load<T, V>(xt + h * s.xh + at[c], x[u][c]);
-                        const T* src = GRAD ? yt + h * s.yh : xt + h * s.xh;
-                        if constexpr (GRAD) load<T, V>(src + at[c], d);
-                        if (!swap) load<T, V>(src + other[c], dp);
-                    }
-                    if (swap) {
-#pragma unroll
-                        for (int e = 0; e < V; ++e) dp[e] = GRAD ? d[e ^ (V > 1)] : x[u][c][e ^ (V > 1)];
-                    }
-#pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        y[u][c][e] = GRAD ? d[e] * cs[c][e] - dp[e] * sn[c][e] : dp[e];
-                        sq[u] += x[u][c][e] * x[u][c][e];
-                        if constexpr (GRAD) gx[u] += y[u][c][e] * w[c][e] * x[u][c][e];
+                for (int i = 0; i < NP; ++i) {
+                    v[u][i] = two(rx[b][u].pair(i));
+                    q2 = fma2(v[u][i], v[u][i], q2);
+                    if constexpr (GRAD) {            // g = R(p)^T dy
+                        const float2 y = rd[b][u].pair(i);
+                        const uint64_t other2 = IL ? two(swapped(y)) : two(ro[b][IL ? 0 : u].pair(i));
+                        g[u][i] = fma2(two(y), cs[i], mul2(other2, sn[i]));
+                        x2 = fma2(mul2(g[u][i], w2[i]), v[u][i], x2);
                     }
                 }
+                const float2 f = unpack2(q2), e = unpack2(x2);
+                sq[u] = h + u < n ? f.x + f.y : 0.0f;
+                gx[u] = h + u < n ? e.x + e.y : 0.0f;
             }
-            for (int o = G >> 1; o > 0; o >>= 1) {
+            for (int k = G >> 1; k > 0; k >>= 1) {
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    sq[u] += __shfl_xor_sync(0xffffffffu, sq[u], o);
-                    if constexpr (GRAD) gx[u] += __shfl_xor_sync(0xffffffffu, gx[u], o);
+                    sq[u] += __shfl_xor_sync(0xffffffffu, sq[u], k);
+                    if constexpr (GRAD) gx[u] += __shfl_xor_sync(0xffffffffu, gx[u], k);
                 }
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int h = h0 + hb + u;
-                const float r = rsqrtf(sq[u] * inv_d + a.eps);
-                const float m = GRAD ? gx[u] * r * r * inv_d : 0.0f;   // n' mean(g w n') = x r m'
+                if (h + u >= n) continue;
+                const float r = rsqrtf(fmaf(sq[u], inv_d, a.eps));
+                const float m = -gx[u] * r * r * inv_d;                  // -n' mean(g w n') = x r m
+                const uint64_t r2 = pack2(r, r), m2 = pack2(m, m);
+                R out;
 #pragma unroll
-                for (int c = 0; c < NCH; ++c) {
-                    float o[V];
-#pragma unroll
-                    for (int e = 0; e < V; ++e) {
-                        if constexpr (GRAD) {
-                            if (which) acc[1][c][e] += y[u][c][e] * (x[u][c][e] * r);
-                            else acc[0][c][e] += y[u][c][e] * (x[u][c][e] * r);
-                            o[e] = r * (y[u][c][e] * w[c][e] - x[u][c][e] * m);
-                        } else {
-                            o[e] = (x[u][c][e] * r * w[c][e]) * cs[c][e] + (y[u][c][e] * r * wp[c][e]) * sn[c][e];
-                        }
+                for (int i = 0; i < NP; ++i) {
+                    uint64_t f;
+                    if constexpr (GRAD) {
+                        acc[i] = fma2(g[u][i], mul2(v[u][i], r2), acc[i]);
+                        f = mul2(fma2(v[u][i], m2, mul2(g[u][i], w2[i])), r2);
+                    } else {
+                        const uint64_t other2 = IL ? two(swapped(unpack2(v[u][i]))) : two(ro[b][IL ? 0 : u].pair(i));
+                        f = mul2(fma2(other2, sn[i], mul2(v[u][i], cs[i])), r2);
                     }
-                    if (h < h1 && in[c]) store<T, V>(ot + h * s.oh + at[c], o);
+                    out.set(i, unpack2(f));
                 }
+                out.put(o + (h + u) * s.oh);
+            }
+        };
+        // every lane of the warp takes the same turns: the sums are shuffled
+        for (int h = 0; h < a.heads; h += 2 * U) {
+            if (h + U < a.heads) fetch(1, h + U);
+            work(0, h);
+            if (h + U < a.heads) {
+                if (h + 2 * U < a.heads) fetch(0, h + 2 * U);
+                work(1, h + U);
             }
         }
     }
@@ -217,78 +253,163 @@ __global__ void __launch_bounds__(kThreads) k_qk_norm_rope(const __grid_constant
         if (a.part == nullptr) return;
         // sums over this block's groups in a fixed order, one row of partials a block
         const int groups = kThreads / G, group = threadIdx.x / G;
-        for (int s = 0; s < 2; ++s) {
-            __syncthreads();
+        if (in) {
 #pragma unroll
-            for (int c = 0; c < NCH; ++c)
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    const int i = (gl + c * G) * V + e;
-                    if (i < a.D) sm[group * a.D + i] = s ? acc[GRAD ? 1 : 0][c][e] : acc[0][c][e];
-                }
-            __syncthreads();
-            for (int i = threadIdx.x; i < a.D; i += kThreads) {
-                float v = 0.0f;
-                for (int g = 0; g < groups; ++g) v += sm[g * a.D + i];
-                a.part[((int64_t)blockIdx.x * 2 + s) * a.D + i] = v;
+            for (int i = 0; i < NP; ++i) {
+                const float2 f = unpack2(acc[i]);
+                sm[group * a.D + at + 2 * i] = f.x;
+                sm[group * a.D + at + 2 * i + 1] = f.y;
             }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < a.D; i += kThreads) {
+            float v = 0.0f;
+            for (int g = 0; g < groups; ++g) v += sm[g * a.D + i];
+            a.part[(int64_t)blockIdx.x * a.D + i] = v;
         }
     }
 }
 
-// Column sums of the partials [blocks][2][D] in block order within each of 32 strands, strands in order.
-__global__ void __launch_bounds__(1024) k_rope_weight_grad(const float* __restrict__ part, int blocks, int D,
-                                                           float* __restrict__ dqw, float* __restrict__ dkw) {
+// Any head size, stride and alignment: a warp a row, a value a lane at a time.
+template <typename T>
+__device__ __forceinline__ float value(const T* p) {
+    if constexpr (sizeof(T) == 4) return *p;
+    else return tok::Elem<T>::to(*p);
+}
+template <typename T, bool GRAD>
+__global__ void __launch_bounds__(kThreads) k_qk_norm_rope_any(const __grid_constant__ RopeArgs a) {
     pdl_begin();
-    __shared__ float sm[32][33];
-    const int col = blockIdx.x * 32 + (threadIdx.x & 31), strand = threadIdx.x >> 5, width = 2 * D;
-    float v = 0.0f;
-    if (col < width)
-        for (int b = strand; b < blocks; b += 32) v += part[(int64_t)b * width + col];
-    sm[strand][threadIdx.x & 31] = v;
-    __syncthreads();
-    if (strand == 0 && col < width) {
-        float total = 0.0f;
-        for (int s = 0; s < 32; ++s) total += sm[s][threadIdx.x];
-        float* to = col < D ? dqw : dkw;
-        if (to) to[col < D ? col : col - D] = total;
+    extern __shared__ float sm[];
+    constexpr int NC = kMaxD / 32;
+    const int lane = threadIdx.x & 31, which = (int)blockIdx.x >= a.blocks[0];
+    const Side& s = a.side[which];
+    const float inv_d = 1.0f / (float)a.D;
+    float acc[NC] = {};
+    const int64_t rows = a.T * s.H, stride = (int64_t)a.blocks[which] * (kThreads / 32);
+    for (int64_t row = (int64_t)(blockIdx.x - (which ? a.blocks[0] : 0)) * (kThreads / 32) + (threadIdx.x >> 5); row < rows; row += stride) {
+        const int64_t t = row / s.H;
+        const int h = (int)(row - t * s.H);
+        const int64_t p = a.half ? place_of(a, t, lane == 0) * a.half : 0;
+        const T* x = reinterpret_cast<const T*>(s.x) + t * s.xt + h * s.xh;
+        const T* d = GRAD ? reinterpret_cast<const T*>(s.dy) + t * s.yt + h * s.yh : nullptr;
+        T* o = reinterpret_cast<T*>(s.out) + t * s.ot + h * s.oh;
+        float v[NC], g[NC], sq = 0.0f, gx = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int i = lane + 32 * c;
+            v[c] = g[c] = 0.0f;
+            if (i >= a.D) continue;
+            v[c] = value(x + i);
+            sq += v[c] * v[c];
+            const bool turned = i < 2 * a.half, ahead = a.interleaved ? !(i & 1) : i < a.half;
+            const int k = a.interleaved ? i / 2 : (ahead ? i : i - a.half);
+            const int other = !turned ? i : (a.interleaved ? i ^ 1 : (ahead ? i + a.half : i - a.half));
+            const float cs = turned ? a.cos[p + k] : 1.0f, sn = turned ? (ahead ? -a.sin[p + k] : a.sin[p + k]) : 0.0f;
+            const float w = s.w ? s.w[i] : 1.0f;
+            if constexpr (GRAD) {
+                g[c] = value(d + i) * cs - value(d + other) * sn;
+                gx += g[c] * w * v[c];
+            } else {                                   // the turned row, without its norm
+                g[c] = v[c] * w * cs + value(x + other) * (s.w ? s.w[other] : 1.0f) * sn;
+            }
+        }
+        sq = warp_sum(sq);
+        gx = warp_sum(gx);
+        const float r = rsqrtf(fmaf(sq, inv_d, a.eps)), m = gx * r * r * inv_d;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int i = lane + 32 * c;
+            if (i >= a.D) continue;
+            float f = g[c] * r;
+            if constexpr (GRAD) {
+                acc[c] += g[c] * (v[c] * r);
+                f = r * (g[c] * (s.w ? s.w[i] : 1.0f) - v[c] * m);
+            }
+            if constexpr (sizeof(T) == 4) o[i] = f;
+            else o[i] = tok::Elem<T>::from(f);
+        }
+    }
+    if constexpr (GRAD) {
+        if (a.part == nullptr) return;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+            if (lane + 32 * c < a.D) sm[(threadIdx.x >> 5) * a.D + lane + 32 * c] = acc[c];
+        __syncthreads();
+        for (int i = threadIdx.x; i < a.D; i += kThreads) {
+            float v = 0.0f;
+            for (int g = 0; g < kThreads / 32; ++g) v += sm[g * a.D + i];
+            a.part[(int64_t)blockIdx.x * a.D + i] = v;
+        }
     }
 }
 
-constexpr int kMaxBlocks = kNumSMs * 4;
+// Column sums of the partials [blocks of queries, then of keys][D]: in block order within each of 32 strands, strands in
+// order.
+__global__ void __launch_bounds__(1024) k_rope_weight_grad(const float* __restrict__ part, int blocks_q, int blocks_k,
+                                                           int D, float* __restrict__ dqw, float* __restrict__ dkw) {
+    pdl_begin();
+    __shared__ float sm[32][33];
+    const int col = blockIdx.x * 32 + (threadIdx.x & 31), strand = threadIdx.x >> 5;
+    const int b0 = blockIdx.y ? blocks_q : 0, b1 = blockIdx.y ? blocks_q + blocks_k : blocks_q;
+    float v = 0.0f;
+    if (col < D)
+#pragma unroll 4
+        for (int b = b0 + strand; b < b1; b += 32) v += part[(int64_t)b * D + col];
+    sm[strand][threadIdx.x & 31] = v;
+    __syncthreads();
+    float* to = blockIdx.y ? dkw : dqw;
+    if (strand == 0 && col < D && to) {
+        float total = 0.0f;
+        for (int s = 0; s < 32; ++s) total += sm[s][threadIdx.x];
+        to[col] = total;
+    }
+}
 
-template <typename T, int V, int NCH, int U, bool GRAD>
-int launch(const RopeArgs& a, int G, int blocks, cudaStream_t s) {
+constexpr int kMaxBlocks = kNumSMs * 6;
+
+// Blocks of each side, in proportion to its rows.
+void share_blocks(RopeArgs& a, const int64_t (&want)[2]) {
+    const int64_t rows = (int64_t)a.side[0].H + a.side[1].H;
+    for (int i = 0; i < 2; ++i)
+        a.blocks[i] = (int)std::min<int64_t>(want[i], std::max<int64_t>(1, (int64_t)kMaxBlocks * a.side[i].H / rows));
+}
+
+template <typename T, int V, bool GRAD>
+int plan(RopeArgs& a, cudaStream_t s) {
+    int G = 1;
+    while (G * V < a.D) G *= 2;
+    // Heads per item: a token's angles are reused over an item's heads, but a small batch needs the items.  All heads
+    // while that leaves 16 warps a SM, else one.
+    const bool wide = a.T * G >= (int64_t)kNumSMs * 512;
+    a.heads = wide ? std::max(a.side[0].H, a.side[1].H) : 1;
+    const int64_t per_block = (int64_t)(kThreads / 32) * (32 / G);
+    int64_t want[2];
+    for (int i = 0; i < 2; ++i) {
+        a.chunks[i] = a.side[i].H ? (a.side[i].H + a.heads - 1) / a.heads : 0;
+        want[i] = (a.T * a.chunks[i] + per_block - 1) / per_block;
+    }
+    share_blocks(a, want);
     const size_t smem = GRAD ? (size_t)(kThreads / G) * a.D * sizeof(float) : 0;
-    k_qk_norm_rope<T, V, NCH, U, GRAD><<<blocks, kThreads, smem, s>>>(a, G);
+    const int blocks = a.blocks[0] + a.blocks[1];
+    constexpr int U = GRAD ? 1 : 2;
+    if (a.interleaved) k_qk_norm_rope<T, V, U, GRAD, true><<<blocks, kThreads, smem, s>>>(a, G);
+    else k_qk_norm_rope<T, V, U, GRAD, false><<<blocks, kThreads, smem, s>>>(a, G);
     PMG_LAUNCH_CHECK();
     return PMG_OK;
 }
 
-template <typename T, int V, int NCH, bool GRAD>
-int plan(RopeArgs& a, float* part, int* blocks_out, cudaStream_t s) {
-    int G = 1;
-    while (G < 32 && G * V < a.D) G *= 2;
-    // Heads per item: all of a token's angles are reused over an item's heads, but a small batch needs the items.
-    // Four at once while that leaves 16 warps a SM; measured figures beside the entry points below.
-    const int64_t groups4 = a.T * ((a.side[0].H + 3) / 4 + (a.side[1].H + 3) / 4);
-    const bool wide = groups4 * G >= (int64_t)kNumSMs * 512;
-    a.heads = wide ? 4 : 1;
-    int64_t items = 0;
-    for (int i = 0; i < 2; ++i) {
-        a.chunks[i] = (a.side[i].H + a.heads - 1) / a.heads;
-        items += a.T * a.chunks[i];
-    }
-    const int64_t per_block = (int64_t)(kThreads / 32) * (32 / G);
-    int64_t blocks = std::max<int64_t>(1, (items + per_block - 1) / per_block);
-    if (GRAD) blocks = std::min<int64_t>(blocks, kMaxBlocks);
-    else blocks = std::min<int64_t>(blocks, (int64_t)1 << 20);
-    *blocks_out = (int)blocks;
-    a.part = part;
-    return wide ? launch<T, V, NCH, (NCH * V > 8 ? 2 : 4), GRAD>(a, G, (int)blocks, s)
-                : launch<T, V, NCH, 1, GRAD>(a, G, (int)blocks, s);
+template <typename T, bool GRAD>
+int plan_any(RopeArgs& a, cudaStream_t s) {
+    int64_t want[2];
+    for (int i = 0; i < 2; ++i) want[i] = (a.T * a.side[i].H + kThreads / 32 - 1) / (kThreads / 32);
+    share_blocks(a, want);
+    const size_t smem = GRAD ? (size_t)(kThreads / 32) * a.D * sizeof(float) : 0;
+    k_qk_norm_rope_any<T, GRAD><<<a.blocks[0] + a.blocks[1], kThreads, smem, s>>>(a);
+    PMG_LAUNCH_CHECK();
+    return PMG_OK;
 }
 
+// Whether every row and every pair's partner can be read as vectors of V values, and the angles as pairs.
 bool aligned(const RopeArgs& a, int V, int size, bool grad) {
     auto ok = [&](const void* p, int64_t t, int64_t h) {
         return ((uintptr_t)p % (V * size)) == 0 && t % V == 0 && h % V == 0;
@@ -297,26 +418,26 @@ bool aligned(const RopeArgs& a, int V, int size, bool grad) {
         if (s.H == 0) continue;
         if (!ok(s.x, s.xt, s.xh) || !ok(s.out, s.ot, s.oh) || (grad && !ok(s.dy, s.yt, s.yh))) return false;
     }
-    return a.D % V == 0 && (a.interleaved ? (2 * a.half) % V == 0 : a.half % V == 0);
+    if (((uintptr_t)a.cos | (uintptr_t)a.sin) & 7) return false;
+    return a.D % V == 0 && a.D <= 32 * V && (a.interleaved ? (2 * a.half) % V == 0 : a.half % V == 0) && a.half % 2 == 0;
 }
 
 template <typename T, bool GRAD>
-int by_width(RopeArgs& a, float* part, int* blocks, cudaStream_t s) {
+int by_width(RopeArgs& a, cudaStream_t s) {
     constexpr int W = 16 / sizeof(T);
-    if (aligned(a, W, sizeof(T), GRAD))
-        return a.D <= 32 * W ? plan<T, W, 1, GRAD>(a, part, blocks, s) : plan<T, W, 2, GRAD>(a, part, blocks, s);
+    if (aligned(a, W, sizeof(T), GRAD)) return plan<T, W, GRAD>(a, s);
     if constexpr (sizeof(T) == 2) {
-        if (aligned(a, 4, 2, GRAD)) return plan<T, 4, 2, GRAD>(a, part, blocks, s);
+        if (aligned(a, 4, 2, GRAD)) return plan<T, 4, GRAD>(a, s);
     }
-    return plan<T, 1, 8, GRAD>(a, part, blocks, s);
+    return plan_any<T, GRAD>(a, s);
 }
 
 template <bool GRAD>
-int by_type(int dtype, RopeArgs& a, float* part, int* blocks, cudaStream_t s) {
+int by_type(int dtype, RopeArgs& a, cudaStream_t s) {
     switch (dtype) {
-        case PMG_BF16: return by_width<__nv_bfloat16, GRAD>(a, part, blocks, s);
-        case PMG_F16: return by_width<__half, GRAD>(a, part, blocks, s);
-        default: return by_width<float, GRAD>(a, part, blocks, s);
+        case PMG_BF16: return by_width<__nv_bfloat16, GRAD>(a, s);
+        case PMG_F16: return by_width<__half, GRAD>(a, s);
+        default: return by_width<float, GRAD>(a, s);
     }
 }
 
@@ -348,12 +469,11 @@ extern "C" int pmg_qk_norm_rope(const void* q, int64_t q_tok, int64_t q_head, co
     a.side[1] = {k, nullptr, k_out, k_weight, k_tok, k_head, 0, 0, ko_tok, ko_head, Hk};
     a.cos = cos; a.sin = sin; a.pos = positions; a.T = T; a.places = rot ? places : INT32_MAX; a.D = D;
     a.half = rot / 2; a.interleaved = interleaved != 0; a.eps = eps; a.status = status;
-    int blocks = 0;
-    return by_type<false>(dtype, a, nullptr, &blocks, as_stream(stream));
+    return by_type<false>(dtype, a, as_stream(stream));
 }
 
 extern "C" size_t pmg_qk_norm_rope_grad_workspace_bytes(int32_t D) {
-    return (size_t)kMaxBlocks * 2 * (D > 0 ? D : 0) * sizeof(float);
+    return (size_t)(kMaxBlocks + 2) * (D > 0 ? D : 0) * sizeof(float);
 }
 
 extern "C" int pmg_qk_norm_rope_grad(const void* dq, int64_t dq_tok, int64_t dq_head, const void* dk, int64_t dk_tok,
@@ -381,12 +501,12 @@ extern "C" int pmg_qk_norm_rope_grad(const void* dq, int64_t dq_tok, int64_t dq_
     a.side[1] = {k, dk, k_grad, k_weight, k_tok, k_head, dk_tok, dk_head, ko_tok, ko_head, Hk};
     a.cos = cos; a.sin = sin; a.pos = positions; a.T = T; a.places = rot ? places : INT32_MAX; a.D = D;
     a.half = rot / 2; a.interleaved = interleaved != 0; a.eps = eps; a.status = status;
-    int blocks = 0;
-    const int rc2 = by_type<true>(dtype, a, weights ? static_cast<float*>(workspace) : nullptr, &blocks, s);
+    a.part = weights ? static_cast<float*>(workspace) : nullptr;
+    const int rc2 = by_type<true>(dtype, a, s);
     if (rc2 != PMG_OK) return rc2;
     if (weights) {
-        k_rope_weight_grad<<<(2 * D + 31) / 32, 1024, 0, s>>>(static_cast<const float*>(workspace), blocks, D,
-                                                              q_weight_grad, k_weight_grad);
+        k_rope_weight_grad<<<dim3((D + 31) / 32, 2), 1024, 0, s>>>(a.part, a.blocks[0], a.blocks[1], D, q_weight_grad,
+                                                                   k_weight_grad);
         PMG_LAUNCH_CHECK();
     }
     return PMG_OK;
