@@ -38,7 +38,7 @@ struct RopeArgs {
     const float *cos, *sin;
     const int32_t* pos;
     int64_t T;
-    int places, D, half, interleaved, heads, chunks[2], blocks[2];   // heads per item; items per token, blocks of each side
+    int places, D, half, interleaved, heads[2], chunks[2], blocks[2];   // heads per item, items per token, blocks of each side
     float eps;
     int32_t* status;
     float* part;              // gradients of w: [blocks[0] + blocks[1]][D]
@@ -91,7 +91,7 @@ __device__ __forceinline__ int64_t place_of(const RopeArgs& a, int64_t t, bool t
 // IL: interleaved pairs, which lie within a lane's vector.  The cost of a value is what bounds this after HBM: unpacking
 // by the element and fp32 copies of whole rows took 28 instructions a value and 99 us for 38,400 tokens of 20 heads of 64.
 template <typename T, int V, int U, bool GRAD, bool IL>
-__global__ void __launch_bounds__(kThreads, 3) k_qk_norm_rope(const __grid_constant__ RopeArgs a, int G) {
+__global__ void __launch_bounds__(kThreads, 2) k_qk_norm_rope(const __grid_constant__ RopeArgs a, int G) {
     using namespace tok;
     using R = Row<T, V>;
     constexpr int NP = V / 2;
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kThreads, 3) k_qk_norm_rope(const __grid_const
     const int lane = threadIdx.x & 31, per_warp = 32 / G, gi = lane / G, gl = lane % G;
     const int which = (int)blockIdx.x >= a.blocks[0];
     const Side& s = a.side[which];
-    const int per_token = a.chunks[which];
+    const int per_token = a.chunks[which], heads = a.heads[which];
     const int64_t items = a.T * per_token;
     const int64_t first = (int64_t)(blockIdx.x - (which ? a.blocks[0] : 0)) * (kThreads / 32) + (threadIdx.x >> 5);
     const int64_t stride = (int64_t)a.blocks[which] * (kThreads / 32) * per_warp;
@@ -110,21 +110,42 @@ __global__ void __launch_bounds__(kThreads, 3) k_qk_norm_rope(const __grid_const
     const bool turned = at < 2 * a.half, ahead = !IL && at < a.half;      // ahead: the pair's first values
     const int other = turned && !IL ? (ahead ? at + a.half : at - a.half) : at;
     const int ang = IL ? at / 2 : (ahead ? at : at - a.half);
-    uint64_t w2[GRAD ? NP : 1], acc[GRAD ? NP : 1];
-    if constexpr (GRAD) {
+    uint64_t w2[NP], p2[GRAD ? 1 : NP], acc[GRAD ? NP : 1];        // the weights here and at the partners
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            w2[i] = s.w ? pack2(s.w[at + 2 * i], s.w[at + 2 * i + 1]) : pack2(1.0f, 1.0f);
-            acc[i] = 0;
+    for (int i = 0; i < NP; ++i) {
+        w2[i] = s.w ? pack2(s.w[at + 2 * i], s.w[at + 2 * i + 1]) : pack2(1.0f, 1.0f);
+        if constexpr (GRAD) acc[i] = 0;
+        else if constexpr (IL) p2[i] = two(swapped(unpack2(w2[i])));
+        else p2[i] = s.w ? pack2(s.w[other + 2 * i], s.w[other + 2 * i + 1]) : pack2(1.0f, 1.0f);
+    }
+
+    // A token's angles are two dependent loads away: its position is fetched two items ahead, its angles one.
+    constexpr int NA = (IL ? NP : V) / 2;
+    float2 fc[NA], fs[NA];
+    auto token = [&](int64_t base) {
+        const int64_t item = min(base + gi, items - 1);
+        return per_token == 1 ? item : item / per_token;
+    };
+    auto angles = [&](int64_t place) {
+        if (!turned) return;
+#pragma unroll
+        for (int e = 0; e < NA; ++e) {
+            fc[e] = *reinterpret_cast<const float2*>(a.cos + place * a.half + ang + 2 * e);
+            fs[e] = *reinterpret_cast<const float2*>(a.sin + place * a.half + ang + 2 * e);
         }
+    };
+    int64_t next_place = 0;
+    if (first * per_warp < items) {
+        angles(place_of(a, token(first * per_warp), gl == 0));
+        next_place = place_of(a, token(first * per_warp + stride), gl == 0);
     }
 
     for (int64_t base = first * per_warp; base < items; base += stride) {
         const bool live = base + gi < items;
         const int64_t item = live ? base + gi : items - 1;
         const int64_t t = per_token == 1 ? item : item / per_token;
-        const int h0 = (int)(item - t * per_token) * a.heads;
-        const int n = live && in ? min(a.heads, s.H - h0) : 0;
+        const int h0 = (int)(item - t * per_token) * heads;
+        const int n = live && in ? min(heads, s.H - h0) : 0;
         const T* x = reinterpret_cast<const T*>(s.x) + t * s.xt + h0 * s.xh;
         const T* d = GRAD ? reinterpret_cast<const T*>(s.dy) + t * s.yt + h0 * s.yh : nullptr;
         T* o = reinterpret_cast<T*>(s.out) + t * s.ot + h0 * s.oh + at;
@@ -145,7 +166,7 @@ __global__ void __launch_bounds__(kThreads, 3) k_qk_norm_rope(const __grid_const
             }
         };
         fetch(0, 0);
-        // this token's angles; the rotation's sign in sn, and forwards the weights in both
+        // this token's turn: the rotation's sign in sn, and forwards the weights in both
         uint64_t cs[NP], sn[NP];
         {
             float c[V], z[V];
@@ -155,38 +176,36 @@ __global__ void __launch_bounds__(kThreads, 3) k_qk_norm_rope(const __grid_const
                 z[e] = 0.0f;
             }
             if (turned) {
-                const int64_t p = place_of(a, t, live && gl == 0) * a.half + ang;
-                constexpr int N = IL ? NP : V;
 #pragma unroll
-                for (int e = 0; e < N; e += 2) {
-                    const float2 fc = *reinterpret_cast<const float2*>(a.cos + p + e), fs = *reinterpret_cast<const float2*>(a.sin + p + e);
+                for (int e = 0; e < NA; ++e) {
                     if constexpr (IL) {
-                        c[2 * e] = c[2 * e + 1] = fc.x;
-                        c[2 * e + 2] = c[2 * e + 3] = fc.y;
-                        z[2 * e] = -fs.x;
-                        z[2 * e + 1] = fs.x;
-                        z[2 * e + 2] = -fs.y;
-                        z[2 * e + 3] = fs.y;
+                        c[4 * e] = c[4 * e + 1] = fc[e].x;
+                        c[4 * e + 2] = c[4 * e + 3] = fc[e].y;
+                        z[4 * e] = -fs[e].x;
+                        z[4 * e + 1] = fs[e].x;
+                        z[4 * e + 2] = -fs[e].y;
+                        z[4 * e + 3] = fs[e].y;
                     } else {
-                        c[e] = fc.x;
-                        c[e + 1] = fc.y;
-                        z[e] = ahead ? -fs.x : fs.x;
-                        z[e + 1] = ahead ? -fs.y : fs.y;
+                        c[2 * e] = fc[e].x;
+                        c[2 * e + 1] = fc[e].y;
+                        z[2 * e] = ahead ? -fs[e].x : fs[e].x;
+                        z[2 * e + 1] = ahead ? -fs[e].y : fs[e].y;
                     }
-                }
-            }
-            if (!GRAD && s.w) {
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    c[e] *= s.w[at + e];
-                    z[e] *= s.w[IL ? at + (e ^ 1) : other + e];
                 }
             }
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
                 cs[i] = pack2(c[2 * i], c[2 * i + 1]);
                 sn[i] = GRAD ? pack2(-z[2 * i], -z[2 * i + 1]) : pack2(z[2 * i], z[2 * i + 1]);
+                if constexpr (!GRAD) {
+                    cs[i] = mul2(cs[i], w2[i]);
+                    sn[i] = mul2(sn[i], p2[i]);
+                }
             }
+        }
+        if (base + stride < items) {
+            angles(next_place);
+            next_place = place_of(a, token(base + 2 * stride), gl == 0);
         }
         auto work = [&](int b, int h) {
             uint64_t v[U][NP], g[GRAD ? U : 1][NP];
@@ -239,11 +258,11 @@ __global__ void __launch_bounds__(kThreads, 3) k_qk_norm_rope(const __grid_const
             }
         };
         // every lane of the warp takes the same turns: the sums are shuffled
-        for (int h = 0; h < a.heads; h += 2 * U) {
-            if (h + U < a.heads) fetch(1, h + U);
+        for (int h = 0; h < heads; h += 2 * U) {
+            if (h + U < heads) fetch(1, h + U);
             work(0, h);
-            if (h + U < a.heads) {
-                if (h + 2 * U < a.heads) fetch(0, h + 2 * U);
+            if (h + U < heads) {
+                if (h + 2 * U < heads) fetch(0, h + 2 * U);
                 work(1, h + U);
             }
         }
@@ -365,7 +384,7 @@ __global__ void __launch_bounds__(1024) k_rope_weight_grad(const float* __restri
     }
 }
 
-constexpr int kMaxBlocks = kNumSMs * 6;
+constexpr int kMaxBlocks = kNumSMs * 8;
 
 // Blocks of each side, in proportion to its rows.
 void share_blocks(RopeArgs& a, const int64_t (&want)[2]) {
@@ -381,17 +400,17 @@ int plan(RopeArgs& a, cudaStream_t s) {
     // Heads per item: a token's angles are reused over an item's heads, but a small batch needs the items.  All heads
     // while that leaves 16 warps a SM, else one.
     const bool wide = a.T * G >= (int64_t)kNumSMs * 512;
-    a.heads = wide ? std::max(a.side[0].H, a.side[1].H) : 1;
     const int64_t per_block = (int64_t)(kThreads / 32) * (32 / G);
     int64_t want[2];
     for (int i = 0; i < 2; ++i) {
-        a.chunks[i] = a.side[i].H ? (a.side[i].H + a.heads - 1) / a.heads : 0;
+        a.heads[i] = wide ? a.side[i].H : 1;
+        a.chunks[i] = wide ? a.side[i].H > 0 : a.side[i].H;
         want[i] = (a.T * a.chunks[i] + per_block - 1) / per_block;
     }
     share_blocks(a, want);
     const size_t smem = GRAD ? (size_t)(kThreads / G) * a.D * sizeof(float) : 0;
     const int blocks = a.blocks[0] + a.blocks[1];
-    constexpr int U = GRAD ? 1 : 2;
+    constexpr int U = 2;
     if (a.interleaved) k_qk_norm_rope<T, V, U, GRAD, true><<<blocks, kThreads, smem, s>>>(a, G);
     else k_qk_norm_rope<T, V, U, GRAD, false><<<blocks, kThreads, smem, s>>>(a, G);
     PMG_LAUNCH_CHECK();
