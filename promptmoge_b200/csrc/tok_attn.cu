@@ -475,24 +475,39 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 // ----------------------------------------------------------------------------------------------------------------- //
 // Bound by one read of the keys and values.  A CTA takes one document, one key head and a stretch of the keys; the up to
 // 16 query rows that share the key head (queries x group) are the 16 rows of mma.sync, so every key is read once for all
-// of them.  A warp walks blocks of keys on its own, straight from global memory into operand registers: the order of a
-// dot product's terms is free, so lanes load 16 bytes of a key each and the queries are loaded in the same order; the
-// values' pairs of keys are joined with byte permutes, their order along the head undone when the output is stored.
-// Warps, then stretches, are joined by their maxima and sums.
+// of them.  One warp keeps a ring of 64-key tiles filled by TMA, 64 to 96 KB of them in flight a CTA and two or three CTAs
+// a SM; four warps take 16 keys of each tile, on their own, through ldmatrix (TMA's 128-byte swizzle is the one that
+// makes it free of bank conflicts).  Loading straight into registers, with the wait for each block's loads in the open,
+// read 1.7 TB/s.  Warps, then stretches, are joined by their maxima and sums.
 
-constexpr int kFewWarps = 8, kFewRows = 16;
+constexpr int kFewWarps = 4, kFewRows = 16, kFewTile = 64, kFewThreads = 32 * (kFewWarps + 1);
+
+template <int DP>
+struct Few {
+    static constexpr int kPart = kFewTile * DP * 2;               // a tile's keys, or values
+    static constexpr int kStages = DP == 64 ? 4 : 3;
+    static constexpr int kBars = kStages * 2 * kPart;
+    static constexpr int kSmem = kBars + 256;
+    static constexpr int kCtas = DP == 64 ? 3 : 2;                // a SM
+};
 
 template <typename T>
-__device__ __forceinline__ void mma_16n8k16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                            uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_16n8k16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if constexpr (Elem<T>::kFmt == 1)
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool TRANS>
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
+    if constexpr (TRANS)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
 
 struct Heads {                    // [T, H, D]: pointer and strides in elements
@@ -502,160 +517,192 @@ struct Heads {                    // [T, H, D]: pointer and strides in elements
 
 // Partial results of a stretch: per row D unnormalised outputs, then maximum and sum (units of log 2).
 template <typename T, int DP, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(32 * kFewWarps)
-    k_attn_few(const Heads hq, const Heads hk, const Heads hv, const __grid_constant__ Attn a, int max_q, int splits,
-               float* __restrict__ part, T* __restrict__ o, int64_t o_tok, int64_t o_head, float* __restrict__ lse) {
-    constexpr int NC = DP / 32, NV = DP / 64, KB = DP == 64 ? 32 : 16;       // chunks of a key, of a value; keys a step
-    pdl_begin();
-    extern __shared__ float sm[];                  // [warps][16][DP], then [warps][16] maxima, [warps][16] sums
-    float* const sm_m = sm + kFewWarps * kFewRows * DP;
-    float* const sm_l = sm_m + kFewWarps * kFewRows;
-    const int split = blockIdx.x, kvh = blockIdx.y, doc = blockIdx.z;
+__global__ void __launch_bounds__(kFewThreads, Few<DP>::kCtas)
+    k_attn_few(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const Heads hq,
+               const __grid_constant__ Attn a, int max_q, int stretch, float* __restrict__ part, T* __restrict__ o,
+               int64_t o_tok, int64_t o_head, float* __restrict__ lse) {
+    using C = Few<DP>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint64_t* const full = reinterpret_cast<uint64_t*>(smem + C::kBars);
+    uint64_t* const empty = full + C::kStages;
+    volatile int* const abort_flag = reinterpret_cast<volatile int*>(empty + C::kStages);
+    const int split = blockIdx.x, splits = gridDim.x, kvh = blockIdx.y, doc = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::kStages; ++i) {
+            mbar_init(full + i, 1);
+            mbar_init(empty + i, kFewWarps);
+        }
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    pdl_begin();
     const Span sp = span_of(a, doc);
-    if (sp.lq > max_q) {
-        if (threadIdx.x == 0) flag(a.status, PMG_ERR_RANGE);
-    }
+    if (sp.lq > max_q && threadIdx.x == 0) flag(a.status, PMG_ERR_RANGE);
     const int rows = min(sp.lq, max_q) * a.group;
-    if (rows == 0) return;
-    const int reach = key_end(a, sp, sp.lq);
-    const int per = ((reach + splits - 1) / splits + KB - 1) / KB * KB;
-    const int kbeg = split * per, kend = min(reach, kbeg + per);
+    const int reach = key_end(a, sp, sp.lq), kbeg = split * stretch;
+    const int kend = split + 1 < splits ? min(reach, kbeg + stretch) : reach;       // the last takes what max_k left out
+    if (rows == 0 || (kbeg >= reach && split > 0)) return;            // the first stretch also stands for no keys at all
+    const int tiles = kend > kbeg ? (kend - kbeg + kFewTile - 1) / kFewTile : 0;
+    __syncthreads();
 
-    // queries: rows g and g + 8, 16 bytes per chunk of 32
-    uint4 qa[NC], qb[NC];
-    int lim[2];
-    float place[2], slope[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int r = g + 8 * h, i = r / a.group, hd = kvh * a.group + r % a.group;
-        const bool on = r < rows;
-        lim[h] = on ? last_key(a, sp, i) : -1;
-        place[h] = (float)(i + sp.lk - sp.lq);
-        slope[h] = BIAS && on ? a.slopes[hd] * kLog2e : 0.0f;
-        const T* p = static_cast<const T*>(hq.p) + (sp.q0 + (int64_t)i) * hq.tok + hd * hq.head;
-#pragma unroll
-        for (int cidx = 0; cidx < NC; ++cidx) {
-            const int d = 32 * cidx + 8 * q;
-            (h ? qb : qa)[cidx] = on && d < a.D && sp.q0 + i < a.Tq ? *reinterpret_cast<const uint4*>(p + d) : make_uint4(0, 0, 0, 0);
-        }
-    }
-    const T* kbase = static_cast<const T*>(hk.p) + (int64_t)sp.k0 * hk.tok + kvh * hk.head;
-    const T* vbase = static_cast<const T*>(hv.p) + (int64_t)sp.k0 * hv.tok + kvh * hv.head;
-    const int klim = min(kend, (int)min((int64_t)INT32_MAX, a.Tk - sp.k0));
-    float acc[8 * NV][4] = {};
+    float acc[DP / 8][4] = {};
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    const float c = (CAP || BIAS) ? 1.0f : a.scale2;
-
-    for (int j0 = kbeg + warp * KB; j0 < kend; j0 += kFewWarps * KB) {
-        uint4 kk[KB / 8][NC], vv[KB / 16][4][NV];
+    const float c = BIAS ? 1.0f : (CAP ? a.cap2 : a.scale2);
+    bool ok = true;
+    if (warp == kFewWarps) {
+        if (lane == 0) {
+            for (int i = 0; i < tiles; ++i) {
+                const int st = i % C::kStages;
+                ok = mbar_wait(empty + st, ((i / C::kStages) & 1u) ^ 1u, abort_flag);
+                if (!ok) break;
+                const uint32_t to = smem_u32(smem + st * 2 * C::kPart);
+                mbar_arrive_expect_tx(full + st, 2 * C::kPart);
 #pragma unroll
-        for (int t = 0; t < KB / 8; ++t)
-#pragma unroll
-            for (int cidx = 0; cidx < NC; ++cidx) {
-                const int key = j0 + 8 * t + g, d = 32 * cidx + 8 * q;
-                kk[t][cidx] = key < klim && d < a.D ? __ldcs(reinterpret_cast<const uint4*>(kbase + (int64_t)key * hk.tok + d)) : make_uint4(0, 0, 0, 0);
-            }
-#pragma unroll
-        for (int t = 0; t < KB / 16; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int v = 0; v < NV; ++v) {
-                    const int key = j0 + 16 * t + 2 * q + (e & 1) + 8 * (e >> 1), d = 64 * v + 8 * g;
-                    vv[t][e][v] = key < klim && d < a.D ? __ldcs(reinterpret_cast<const uint4*>(vbase + (int64_t)key * hv.tok + d)) : make_uint4(0, 0, 0, 0);
+                for (int x = 0; x < DP / 64; ++x) {
+                    tma_tile3d(to + x * 8192, &mk, 64 * x, kvh, sp.k0 + kbeg + kFewTile * i, full + st);
+                    tma_tile3d(to + C::kPart + x * 8192, &mv, 64 * x, kvh, sp.k0 + kbeg + kFewTile * i, full + st);
                 }
-        float s[KB / 8][4];
-#pragma unroll
-        for (int t = 0; t < KB / 8; ++t) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[t][e] = 0.0f;
-#pragma unroll
-            for (int cidx = 0; cidx < NC; ++cidx) {
-                mma_16n8k16<T>(s[t], qa[cidx].x, qb[cidx].x, qa[cidx].y, qb[cidx].y, kk[t][cidx].x, kk[t][cidx].y);
-                mma_16n8k16<T>(s[t], qa[cidx].z, qb[cidx].z, qa[cidx].w, qb[cidx].w, kk[t][cidx].z, kk[t][cidx].w);
             }
         }
-        float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-        for (int t = 0; t < KB / 8; ++t)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int h = e >> 1, key = j0 + 8 * t + 2 * q + (e & 1);
-                float x = s[t][e];
-                if (CAP) x = capped(a, x);
-                if (BIAS) x = fmaf(-slope[h], fabsf(place[h] - (float)key), CAP ? x : x * a.scale2);
-                x = key <= lim[h] && key < kend ? x : -INFINITY;
-                s[t][e] = x;
-                top[h] = fmaxf(top[h], x);
-            }
-        float base[2];
+    } else {
+        // queries: rows g and g + 8 as left operands
+        uint32_t qf[DP / 16][4];
+        int lim[2];
+        float place[2], slope[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-            top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-            const float grown = fmaxf(m[h], top[h]);
-            const float f = grown == m[h] ? 1.0f : ex2((m[h] - grown) * c);
-            m[h] = grown;
-            base[h] = grown == -INFINITY ? 0.0f : -grown * c + kLift<T>;
-            l[h] *= f;
+            const int r = g + 8 * h, i = r / a.group, hd = kvh * a.group + r % a.group;
+            const bool on = r < rows;
+            lim[h] = on ? min(last_key(a, sp, i), kend - 1) : -1;
+            place[h] = (float)(i + sp.lk - sp.lq);
+            slope[h] = BIAS && on ? a.slopes[hd] * kLog2e : 0.0f;
+            const T* p = static_cast<const T*>(hq.p) + (sp.q0 + (int64_t)i) * hq.tok + hd * hq.head;
 #pragma unroll
-            for (int t = 0; t < 8 * NV; ++t) {
-                acc[t][2 * h] *= f;
-                acc[t][2 * h + 1] *= f;
-            }
+            for (int x = 0; x < DP / 16; ++x)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int d = 16 * x + 8 * e + 2 * q;
+                    qf[x][h + 2 * e] = on && d < a.D ? *reinterpret_cast<const uint32_t*>(p + d) : 0u;
+                }
         }
-        uint32_t p[KB / 8][2];
+        // ldmatrix: lane l gives the row of matrix l / 8; K: (keys 0-7, 8-15) x (first, second 8 values), V: the same rows
+        const int kr = warp * 16 + (lane & 7) + ((lane >> 4) << 3), kc = (lane >> 3) & 1;
+        const int vr = warp * 16 + (lane & 7) + (((lane >> 3) & 1) << 3), vc = lane >> 4;
+        for (int i = 0; i < tiles; ++i) {
+            const int st = i % C::kStages, j0 = kbeg + kFewTile * i + 16 * warp;      // this warp's first key
+            ok = __all_sync(0xffffffffu, mbar_wait(full + st, (i / C::kStages) & 1u, abort_flag));
+            if (!ok) break;
+            uint8_t* const kt = smem + st * 2 * C::kPart;
+            uint8_t* const vt = kt + C::kPart;
+            if (j0 < kend) {
+                float s[2][4] = {};
 #pragma unroll
-        for (int t = 0; t < KB / 8; ++t)
+                for (int x = 0; x < DP / 16; ++x) {
+                    uint32_t b[4];
+                    ldmatrix4<false>(b, smem_u32(kt) + (x >> 2) * 8192 + kr * 128 + ((((x & 3) * 2 + kc) ^ (kr & 7)) << 4));
+                    mma_16n8k16<T>(s[0], qf[x], b[0], b[1]);
+                    mma_16n8k16<T>(s[1], qf[x], b[2], b[3]);
+                }
+                if (j0 + 16 > kend) {
+                    // rows behind the last key: whatever lies there must not reach a sum (0 * NaN)
+                    for (int x = lane; x < 16 * (DP / 8); x += 32) {
+                        const int r = x & 15;
+                        if (j0 + r >= kend)
+                            *reinterpret_cast<uint4*>(vt + (x >> 7) * 8192 + (warp * 16 + r) * 128 + ((x >> 4) & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    __syncwarp();
+                }
+                float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float e0 = ex2(fmaf(s[t][2 * h], c, base[h])), e1 = ex2(fmaf(s[t][2 * h + 1], c, base[h]));
-                l[h] += e0 + e1;
-                p[t][h] = Elem<T>::pack(e0, e1);
-            }
+                for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int t = 0; t < KB / 16; ++t)
+                    for (int e = 0; e < 4; ++e) {
+                        const int h = e >> 1, key = j0 + 8 * t + 2 * q + (e & 1);
+                        float x = s[t][e];
+                        if (CAP) x = tanh_raw(a, x);
+                        if (BIAS) x = fmaf(-slope[h], fabsf(place[h] - (float)key), x * (CAP ? a.cap2 : a.scale2));
+                        x = key <= lim[h] ? x : -INFINITY;
+                        s[t][e] = x;
+                        top[h] = fmaxf(top[h], x);
+                    }
+                bool grow = false;
 #pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&vv[t][0][v]);
-                const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&vv[t][1][v]);
-                const uint32_t* w2 = reinterpret_cast<const uint32_t*>(&vv[t][2][v]);
-                const uint32_t* w3 = reinterpret_cast<const uint32_t*>(&vv[t][3][v]);
+                for (int h = 0; h < 2; ++h) {
+                    top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+                    top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+                    grow = grow || (top[h] - m[h]) * c > kGrow;
+                }
+                if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-                for (int d = 0; d < 8; ++d) {       // column g of this product is value 64 v + 8 g + d
-                    const uint32_t sel = (d & 1) ? 0x7632 : 0x5410;
-                    mma_16n8k16<T>(acc[8 * v + d], p[2 * t][0], p[2 * t][1], p[2 * t + 1][0], p[2 * t + 1][1],
-                                   __byte_perm(w0[d >> 1], w1[d >> 1], sel), __byte_perm(w2[d >> 1], w3[d >> 1], sel));
+                    for (int h = 0; h < 2; ++h) {
+                        const float grown = fmaxf(m[h], top[h]);
+                        const float f = grown == m[h] ? 1.0f : ex2((m[h] - grown) * c);
+                        m[h] = grown;
+                        l[h] *= f;
+#pragma unroll
+                        for (int x = 0; x < DP / 8; ++x) {
+                            acc[x][2 * h] *= f;
+                            acc[x][2 * h + 1] *= f;
+                        }
+                    }
+                }
+                uint32_t p[4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float base = m[h] == -INFINITY ? 0.0f : -m[h] * c + kLift<T>;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const float e0 = ex2(fmaf(s[t][2 * h], c, base)), e1 = ex2(fmaf(s[t][2 * h + 1], c, base));
+                        l[h] += e0 + e1;
+                        p[2 * t + h] = Elem<T>::pack(e0, e1);
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < DP / 16; ++x) {
+                    uint32_t b[4];
+                    ldmatrix4<true>(b, smem_u32(vt) + (x >> 2) * 8192 + vr * 128 + ((((x & 3) * 2 + vc) ^ (vr & 7)) << 4));
+                    mma_16n8k16<T>(acc[2 * x], p, b[0], b[1]);
+                    mma_16n8k16<T>(acc[2 * x + 1], p, b[2], b[3]);
                 }
             }
-    }
-    // this warp's rows
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-        const int r = warp * kFewRows + g + 8 * h;
-        if (q == 0) {
-            sm_m[r] = m[h] * c;
-            sm_l[r] = l[h];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty + st);
         }
+    }
+    if (!ok && lane == 0) {
+        *abort_flag = 1;
+        flag(a.status, PMG_ERR_TIMEOUT);
+    }
+    __syncthreads();                                  // every tile has been read: its room takes the warps' rows
+    float* const sm = reinterpret_cast<float*>(smem); // [warps][16][DP], then [warps][16] maxima, [warps][16] sums
+    float* const sm_m = sm + kFewWarps * kFewRows * DP;
+    float* const sm_l = sm_m + kFewWarps * kFewRows;
+    if (warp < kFewWarps) {
 #pragma unroll
-        for (int v = 0; v < NV; ++v)
-#pragma unroll
-            for (int d = 0; d < 8; ++d) {
-                sm[r * DP + 64 * v + 8 * (2 * q) + d] = acc[8 * v + d][2 * h];
-                sm[r * DP + 64 * v + 8 * (2 * q + 1) + d] = acc[8 * v + d][2 * h + 1];
+        for (int h = 0; h < 2; ++h) {
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+            const int r = warp * kFewRows + g + 8 * h;
+            if (q == 0) {
+                sm_m[r] = m[h] * c;
+                sm_l[r] = l[h];
             }
+#pragma unroll
+            for (int x = 0; x < DP / 8; ++x)
+                *reinterpret_cast<float2*>(sm + r * DP + 8 * x + 2 * q) = make_float2(acc[x][2 * h], acc[x][2 * h + 1]);
+        }
     }
     __syncthreads();
     for (int idx = threadIdx.x; idx < rows * (DP / 4); idx += blockDim.x) {
         const int r = idx / (DP / 4), d = (idx % (DP / 4)) * 4;
         float top = -INFINITY;
+#pragma unroll
         for (int w = 0; w < kFewWarps; ++w) top = fmaxf(top, sm_m[w * kFewRows + r]);
         const float ref = top == -INFINITY ? 0.0f : top;
         float total = 0.0f;
         float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll
         for (int w = 0; w < kFewWarps; ++w) {
             const float f = ex2(sm_m[w * kFewRows + r] - ref);
             const float4 x = *reinterpret_cast<const float4*>(sm + (w * kFewRows + r) * DP + d);
@@ -673,7 +720,7 @@ __global__ void __launch_bounds__(32 * kFewWarps)
         }
         const int64_t token = sp.q0 + (int64_t)(r / a.group);
         const int head = kvh * a.group + r % a.group;
-        if (token >= a.Tq || d >= a.D) continue;
+        if (d >= a.D) continue;
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;
         *reinterpret_cast<uint2*>(o + token * o_tok + head * o_head + d) =
             make_uint2(Elem<T>::pack(v.x * inv, v.y * inv), Elem<T>::pack(v.z * inv, v.w * inv));
@@ -683,7 +730,7 @@ __global__ void __launch_bounds__(32 * kFewWarps)
 
 // Joins the stretches of every row, a warp a row.
 template <typename T, int DP>
-__global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ Attn a, int max_q, int splits,
+__global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ Attn a, int max_q, int room, int stretch,
                                                    const float* __restrict__ part, T* __restrict__ o, int64_t o_tok,
                                                    int64_t o_head, float* __restrict__ lse) {
     pdl_begin();
@@ -691,7 +738,8 @@ __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ Attn 
     const Span sp = span_of(a, doc);
     const int q0 = sp.q0;
     if (r >= min(sp.lq, max_q) * a.group) return;
-    const float* from = part + (((int64_t)doc * a.Hk + kvh) * splits * kFewRows + r) * (DP + 4);
+    const int splits = min(room, max(1, (key_end(a, sp, sp.lq) + stretch - 1) / stretch));
+    const float* from = part + (((int64_t)doc * a.Hk + kvh) * room * kFewRows + r) * (DP + 4);
     constexpr int64_t step = kFewRows * (DP + 4);
     float top = -INFINITY;
     for (int s = lane; s < splits; s += 32) top = fmaxf(top, from[s * step + DP]);
@@ -745,19 +793,29 @@ struct Call {
 
 bool few_rows(int max_q, int group) { return (int64_t)max_q * group <= kFewRows; }
 
-// Stretches of the keys: enough CTAs for four on every SM, none shorter than 256 keys.
-int few_splits(int docs, int Hk, int max_k) {
-    const int64_t want = (4 * kNumSMs + (int64_t)docs * Hk - 1) / std::max<int64_t>(1, (int64_t)docs * Hk);
-    return (int)std::max<int64_t>(1, std::min<int64_t>({want, (max_k + 255) / 256, 256}));
+// Keys of a stretch, a multiple of a tile: one round of the CTAs that fit the GPU together for one document, a quarter of
+// that for several, whose lengths differ (CTAs then take turns and even out); at least 256, so that a stretch is longer
+// than its start.
+int few_stretch(int docs, int Hk, int D, int max_k) {
+    const int64_t slots = (int64_t)kNumSMs * (D <= 64 ? Few<64>::kCtas : Few<128>::kCtas) * (docs > 1 ? 4 : 1);
+    const int64_t keys = ((int64_t)docs * Hk * max_k + slots - 1) / slots;
+    return (int)(std::max<int64_t>(keys, 256) + kFewTile - 1) / kFewTile * kFewTile;
+}
+int few_splits(int docs, int Hk, int D, int max_k) {
+    const int stretch = few_stretch(docs, Hk, D, max_k);
+    return std::max(1, (max_k + stretch - 1) / stretch);
 }
 
 template <typename T, int DP, bool CAP, bool BIAS>
 int run(const Attn& a, const Call& c, cudaStream_t s) {
     if (few_rows(c.max_q, a.group)) {
-        const int splits = few_splits(a.docs, a.Hk, c.max_k);
-        constexpr int smem = (kFewWarps * kFewRows * (DP + 2)) * sizeof(float);
-        const int rc = raise_smem<k_attn_few<T, DP, CAP, BIAS>>(smem);
+        const int stretch = few_stretch(a.docs, a.Hk, a.D, c.max_k), splits = few_splits(a.docs, a.Hk, a.D, c.max_k);
+        const int rc = raise_smem<k_attn_few<T, DP, CAP, BIAS>>(Few<DP>::kSmem);
         if (rc != PMG_OK) return rc;
+        CUtensorMap mk, mv;
+        int e = head_map(&mk, c.k.p, c.k.tok, c.k.head, std::max<int64_t>(a.Tk, 1), a.Hk, a.D, kFewTile);
+        if (e == PMG_OK) e = head_map(&mv, c.v.p, c.v.tok, c.v.head, std::max<int64_t>(a.Tk, 1), a.Hk, a.D, kFewTile);
+        if (e != PMG_OK) return e;
         for (int d0 = 0; d0 < a.docs; d0 += 65535) {
             Attn b = a;
             b.docs = std::min(65535, a.docs - d0);
@@ -765,12 +823,12 @@ int run(const Attn& a, const Call& c, cudaStream_t s) {
             b.cu_k += d0;
             if (b.k_len) b.k_len += d0;
             if (b.prefix) b.prefix += d0;
-            k_attn_few<T, DP, CAP, BIAS><<<dim3(splits, a.Hk, b.docs), 32 * kFewWarps, smem, s>>>(
-                c.q, c.k, c.v, b, c.max_q, splits, c.part, static_cast<T*>(c.o), c.o_tok, c.o_head, c.lse);
+            k_attn_few<T, DP, CAP, BIAS><<<dim3(splits, a.Hk, b.docs), kFewThreads, Few<DP>::kSmem, s>>>(
+                mk, mv, c.q, b, c.max_q, stretch, c.part, static_cast<T*>(c.o), c.o_tok, c.o_head, c.lse);
             PMG_LAUNCH_CHECK();
             if (splits > 1) {
                 const int rows = c.max_q * a.group;
-                k_attn_join<T, DP><<<dim3((rows + 3) / 4, a.Hk, b.docs), 128, 0, s>>>(b, c.max_q, splits, c.part,
+                k_attn_join<T, DP><<<dim3((rows + 3) / 4, a.Hk, b.docs), 128, 0, s>>>(b, c.max_q, splits, stretch, c.part,
                                                                                      static_cast<T*>(c.o), c.o_tok, c.o_head, c.lse);
                 PMG_LAUNCH_CHECK();
             }
@@ -806,7 +864,7 @@ using namespace pmg;
 extern "C" size_t pmg_attention_workspace_bytes(int32_t docs, int32_t Hq, int32_t Hk, int32_t D, int32_t max_q,
                                                 int32_t max_k) {
     if (docs < 1 || Hk < 1 || Hq < Hk || max_q < 1 || !few_rows(max_q, Hq / Hk)) return 0;
-    const int splits = few_splits(docs, Hk, max_k);
+    const int splits = few_splits(docs, Hk, D, max_k);
     return splits > 1 ? (size_t)std::min(docs, 65535) * Hk * splits * kFewRows * ((D <= 64 ? 64 : 128) + 4) * sizeof(float) : 0;
 }
 
