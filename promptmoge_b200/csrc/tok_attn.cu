@@ -728,42 +728,59 @@ __global__ void __launch_bounds__(kFewThreads, Few<DP>::kCtas)
     }
 }
 
-// Joins the stretches of every row, a warp a row.
+// Joins the stretches of a row, a block a row: a strand of DP / 4 threads takes every 256 / (DP / 4)-th stretch, the
+// strands are added in order.  (A warp a row walked 74 stretches in 28 us, as long as the keys themselves took.)
 template <typename T, int DP>
-__global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ Attn a, int max_q, int room, int stretch,
+__global__ void __launch_bounds__(256) k_attn_join(const __grid_constant__ Attn a, int max_q, int room, int stretch,
                                                    const float* __restrict__ part, T* __restrict__ o, int64_t o_tok,
                                                    int64_t o_head, float* __restrict__ lse) {
     pdl_begin();
-    const int lane = threadIdx.x & 31, r = blockIdx.x * 4 + (threadIdx.x >> 5), kvh = blockIdx.y, doc = blockIdx.z;
+    constexpr int kWide = DP / 4, kStrands = 256 / kWide;
+    __shared__ float sm_top[8], sm_sum[kStrands];
+    __shared__ float4 sm[kStrands][kWide];
+    const int r = blockIdx.x, kvh = blockIdx.y, doc = blockIdx.z, x = threadIdx.x % kWide, strand = threadIdx.x / kWide;
     const Span sp = span_of(a, doc);
-    const int q0 = sp.q0;
     if (r >= min(sp.lq, max_q) * a.group) return;
     const int splits = min(room, max(1, (key_end(a, sp, sp.lq) + stretch - 1) / stretch));
     const float* from = part + (((int64_t)doc * a.Hk + kvh) * room * kFewRows + r) * (DP + 4);
     constexpr int64_t step = kFewRows * (DP + 4);
     float top = -INFINITY;
-    for (int s = lane; s < splits; s += 32) top = fmaxf(top, from[s * step + DP]);
+    for (int s = threadIdx.x; s < splits; s += 256) top = fmaxf(top, from[s * step + DP]);
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+    if ((threadIdx.x & 31) == 0) sm_top[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 8; ++k) top = fmaxf(top, sm_top[k]);
     const float ref = top == -INFINITY ? 0.0f : top;
-    float v[DP / 32] = {}, total = 0.0f;
-    for (int s = 0; s < splits; ++s) {
+    float total = 0.0f;
+    float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+    for (int s = strand; s < splits; s += kStrands) {
         const float f = ex2(from[s * step + DP] - ref);
+        const float4 y = *reinterpret_cast<const float4*>(from + s * step + 4 * x);
         total += f * from[s * step + DP + 1];
-#pragma unroll
-        for (int k = 0; k < DP / 32; ++k) v[k] += f * from[s * step + lane * (DP / 32) + k];
+        v.x += f * y.x; v.y += f * y.y; v.z += f * y.z; v.w += f * y.w;
     }
-    const int64_t token = q0 + (int64_t)(r / a.group);
-    const int head = kvh * a.group + r % a.group;
-    if (token >= a.Tq) return;
+    sm[strand][x] = v;
+    if (x == 0) sm_sum[strand] = total;
+    __syncthreads();
+    if (strand) return;
+    total = 0.0f;
+    v = make_float4(0, 0, 0, 0);
+#pragma unroll
+    for (int k = 0; k < kStrands; ++k) {
+        const float4 y = sm[k][x];
+        total += sm_sum[k];
+        v.x += y.x; v.y += y.y; v.z += y.z; v.w += y.w;
+    }
+    const int64_t token = sp.q0 + (int64_t)(r / a.group);
+    const int head = kvh * a.group + r % a.group, d = 4 * x;
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-    for (int k = 0; k < DP / 32; k += 2) {
-        const int d = lane * (DP / 32) + k;
-        if (d < a.D)
-            *reinterpret_cast<uint32_t*>(o + token * o_tok + head * o_head + d) = Elem<T>::pack(v[k] * inv, v[k + 1] * inv);
-    }
-    if (lane == 0) lse[(int64_t)head * a.Tq + token] = total == 0.0f ? -INFINITY : (top + log2f(total) - kLift<T>) * kLn2;
+    if (d < a.D)
+        *reinterpret_cast<uint2*>(o + token * o_tok + head * o_head + d) =
+            make_uint2(Elem<T>::pack(v.x * inv, v.y * inv), Elem<T>::pack(v.z * inv, v.w * inv));
+    if (x == 0) lse[(int64_t)head * a.Tq + token] = total == 0.0f ? -INFINITY : (top + log2f(total) - kLift<T>) * kLn2;
 }
 
 // ----------------------------------------------------------------------------------------------------------------- //
@@ -827,10 +844,9 @@ int run(const Attn& a, const Call& c, cudaStream_t s) {
                 mk, mv, c.q, b, c.max_q, stretch, c.part, static_cast<T*>(c.o), c.o_tok, c.o_head, c.lse);
             PMG_LAUNCH_CHECK();
             if (splits > 1) {
-                const int rows = c.max_q * a.group;
-                k_attn_join<T, DP><<<dim3((rows + 3) / 4, a.Hk, b.docs), 128, 0, s>>>(b, c.max_q, splits, stretch, c.part,
-                                                                                     static_cast<T*>(c.o), c.o_tok, c.o_head, c.lse);
-                PMG_LAUNCH_CHECK();
+                const int rc2 = launch_after(k_attn_join<T, DP>, dim3(c.max_q * a.group, a.Hk, b.docs), 256, 0, s, b, c.max_q,
+                                             splits, stretch, (const float*)c.part, static_cast<T*>(c.o), c.o_tok, c.o_head, c.lse);
+                if (rc2 != PMG_OK) return rc2;
             }
         }
         return PMG_OK;

@@ -587,9 +587,8 @@ int run(Grad g, const Ins& in, cudaStream_t s) {
     if (e == PMG_OK) e = head_map(&mk, in.k.p, in.k.tok, in.k.head, a.Tk, a.Hk, a.D, 64);
     if (e == PMG_OK) e = head_map(&mv, in.v.p, in.v.tok, in.v.head, a.Tk, a.Hk, a.D, 64);
     if (e != PMG_OK) return e;
-    k_attn_grad<T, DP, CAP, BIAS><<<(int)(key_blocks + query_blocks), C::kThreads, C::kSmem, s>>>(mq, mk, mv, mdo, g);
-    PMG_LAUNCH_CHECK();
-    return PMG_OK;
+    return launch_after(k_attn_grad<T, DP, CAP, BIAS>, dim3((unsigned)(key_blocks + query_blocks)), C::kThreads, C::kSmem, s, mq,
+                        mk, mv, mdo, g);
 }
 
 template <typename T, int DP>

@@ -180,6 +180,24 @@ __device__ __forceinline__ void drain_mma(uint64_t* bar) {
 
 }  // namespace tok
 
+// Host: launches a kernel that follows another of the same call.  It starts with pdl_begin(), so its launch may be
+// prepared while that one runs; it waits there until that one is complete.
+template <typename... P, typename... A>
+int launch_after(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, A... args) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    PMG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
+    return PMG_OK;
+}
+
 // Host: tensor map of a 16-bit tensor (rank 2 or 3; dims and box innermost first, strides in bytes of dims 1..rank-1),
 // 128-byte swizzle, zero fill out of bounds; box[0] is 64.  Base and strides 16-byte aligned.  PMG_OK or an error.
 int make_tensor_map16(CUtensorMap* map, const void* base, int rank, const uint64_t* dims, const uint64_t* strides,

@@ -714,20 +714,27 @@ __global__ void __launch_bounds__(256) k_col_sum(const float* __restrict__ part,
     }
 }
 
-// Rows copied to 16-byte-aligned rows of `ldd` values, padding zeroed.
-__global__ void __launch_bounds__(256) k_pack_rows(const uint16_t* __restrict__ src, int64_t lds, int64_t rows, int cols,
-                                                   uint16_t* __restrict__ dst, int64_t ldd) {
+// Rows copied to 16-byte-aligned rows of `ldd` values, padding zeroed: one or two matrices of the same width.
+struct Pack {
+    const uint16_t* src[2];
+    uint16_t* dst[2];
+    int64_t lds[2], rows[2], ldd;
+    int cols;
+};
+__global__ void __launch_bounds__(256) k_pack_rows(const __grid_constant__ Pack a) {
     pdl_begin();
-    const int groups = (int)(ldd / 8);
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows * groups; i += gridDim.x * 256ll) {
-        const int64_t r = i / groups;
-        const int c = (int)(i - r * groups) * 8;
-        const uint16_t* p = src + r * lds + c;
+    const int groups = (int)(a.ldd / 8);
+    const int64_t n0 = a.rows[0] * groups, n = n0 + a.rows[1] * groups;
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+        const int m = i >= n0;
+        const int64_t j = m ? i - n0 : i, r = j / groups;
+        const int c = (int)(j - r * groups) * 8;
+        const uint16_t* p = a.src[m] + r * a.lds[m] + c;
         uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-            if (c + e < cols) w[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
-        *reinterpret_cast<uint4*>(dst + r * ldd + c) = make_uint4(w[0], w[1], w[2], w[3]);
+            if (c + e < a.cols) w[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
+        *reinterpret_cast<uint4*>(a.dst[m] + r * a.ldd + c) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 
@@ -796,12 +803,12 @@ int gemm_bn(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, i
     if (rc != PMG_OK) return rc;
     rc = make_tensor_map16(&mb, B, 2, db, sb, bb);
     if (rc != PMG_OK) return rc;
-    k_gemm<T, BN, AMN, BMN><<<std::min(s.units, kNumSMs), kGemmThreads, C::kSmem, st>>>(ma, mb, (int)M, (int)N, s, o, status);
-    PMG_LAUNCH_CHECK();
+    rc = launch_after(k_gemm<T, BN, AMN, BMN>, dim3(std::min(s.units, kNumSMs)), kGemmThreads, C::kSmem, st, ma, mb, (int)M,
+                      (int)N, s, o, status);
+    if (rc != PMG_OK) return rc;
     if (s.full < s.tiles) {
         const int64_t threads = (int64_t)(s.tiles - s.full) * (kBM * BN / 8);
-        k_split_sum<T, BN><<<(int)((threads + 255) / 256), 256, 0, st>>>(s, (int)M, (int)N, o);
-        PMG_LAUNCH_CHECK();
+        return launch_after(k_split_sum<T, BN>, dim3((unsigned)((threads + 255) / 256)), 256, 0, st, s, (int)M, (int)N, o);
     }
     return PMG_OK;
 }
@@ -816,12 +823,31 @@ int gemm(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int6
     }
 }
 
-int pack_rows(const void* src, int64_t ld, int64_t rows, int64_t cols, void* dst, cudaStream_t s) {
-    const int64_t n = rows * (round8(cols) / 8);
-    k_pack_rows<<<(int)std::min<int64_t>((n + 255) / 256, kNumSMs * 16), 256, 0, s>>>(
-        static_cast<const uint16_t*>(src), ld, rows, (int)cols, static_cast<uint16_t*>(dst), round8(cols));
-    PMG_LAUNCH_CHECK();
-    return PMG_OK;
+// Copies of those of two matrices of `cols` columns that TMA cannot read, at `ws`, which moves on; they are replaced.
+struct Matrix {
+    const void* p;
+    int64_t ld, rows;
+};
+int pack(Matrix* x, Matrix* w, int64_t cols, uint8_t*& ws, cudaStream_t s) {
+    Pack a{};
+    a.ldd = round8(cols);
+    a.cols = (int)cols;
+    int n = 0;
+    int64_t groups = 0;
+    for (Matrix* m : {x, w}) {
+        if (!m || tma_ok(m->p, m->ld)) continue;
+        a.src[n] = static_cast<const uint16_t*>(m->p);
+        a.dst[n] = reinterpret_cast<uint16_t*>(ws);
+        a.lds[n] = m->ld;
+        a.rows[n] = m->rows;
+        groups += m->rows * (a.ldd / 8);
+        m->p = ws;
+        m->ld = a.ldd;
+        ws += round256((size_t)m->rows * a.ldd * 2);
+        ++n;
+    }
+    if (n == 0) return PMG_OK;
+    return launch_after(k_pack_rows, dim3((unsigned)std::min<int64_t>((groups + 255) / 256, kNumSMs * 16)), 256, 0, s, a);
 }
 
 template <typename T, int NT>
@@ -851,21 +877,10 @@ int linear(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, in
     if (M <= 8) return rows_nt<T, 1>(x, ldx, w, ldw, (int)M, (int)N, (int)K, o, s);
     if (M <= 16) return rows_nt<T, 2>(x, ldx, w, ldw, (int)M, (int)N, (int)K, o, s);
     if (M <= kFewRows) return rows_nt<T, 4>(x, ldx, w, ldw, (int)M, (int)N, (int)K, o, s);
-    if (!tma_ok(x, ldx)) {
-        const int rc = pack_rows(x, ldx, M, K, ws, s);
-        if (rc != PMG_OK) return rc;
-        x = ws;
-        ldx = round8(K);
-        ws += round256((size_t)M * ldx * 2);
-    }
-    if (!tma_ok(w, ldw)) {
-        const int rc = pack_rows(w, ldw, N, K, ws, s);
-        if (rc != PMG_OK) return rc;
-        w = ws;
-        ldw = round8(K);
-        ws += round256((size_t)N * ldw * 2);
-    }
-    return gemm<T, false, false>(x, ldx, w, ldw, M, N, K, o, reinterpret_cast<float*>(ws), status, s);
+    Matrix mx{x, ldx, M}, mw{w, ldw, N};
+    const int rc = pack(&mx, &mw, K, ws, s);
+    if (rc != PMG_OK) return rc;
+    return gemm<T, false, false>(mx.p, mx.ld, mw.p, mw.ld, M, N, K, o, reinterpret_cast<float*>(ws), status, s);
 }
 
 struct GradPlan {
@@ -911,44 +926,28 @@ int linear_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, const 
         else k_act_grad<T, false><<<grid, 256, 0, s>>>(dyp, lddy, prep, ldp, M, (int)N, act, dst, lddz, (int)round8(N), p.rows_per_block, part);
         PMG_LAUNCH_CHECK();
         if (db) {
-            k_col_sum<T><<<(int)((N + 31) / 32), 256, 0, s>>>(part, (int)p.row_blocks, (int)N, static_cast<T*>(db));
-            PMG_LAUNCH_CHECK();
+            const int rc = launch_after(k_col_sum<T>, dim3((unsigned)((N + 31) / 32)), 256, 0, s, (const float*)part,
+                                        (int)p.row_blocks, (int)N, static_cast<T*>(db));
+            if (rc != PMG_OK) return rc;
         }
     }
+    Matrix mx{x, ldx, M}, mw{w, ldw, N};
+    const int rc = pack(dw ? &mx : nullptr, dx ? &mw : nullptr, K, ws, s);
+    if (rc != PMG_OK) return rc;
     Out o{};
     if (dx) {
-        const void* wp = w;
-        int64_t ld = ldw;
-        uint8_t* left = ws;
-        if (!tma_ok(w, ldw)) {
-            const int rc = pack_rows(w, ldw, N, K, left, s);
-            if (rc != PMG_OK) return rc;
-            wp = left;
-            ld = round8(K);
-            left += round256((size_t)N * ld * 2);
-        }
         o.y = dx;
         o.ldy = lddx;
         o.vec = vec_ok(o);
-        const int rc = gemm<T, false, true>(dz, lddz, wp, ld, M, K, N, o, reinterpret_cast<float*>(left), status, s);
-        if (rc != PMG_OK) return rc;
+        const int rc2 = gemm<T, false, true>(dz, lddz, mw.p, mw.ld, M, K, N, o, reinterpret_cast<float*>(ws), status, s);
+        if (rc2 != PMG_OK) return rc2;
     }
     if (dw) {
-        const void* xp = x;
-        int64_t ld = ldx;
-        uint8_t* left = ws;
-        if (!tma_ok(x, ldx)) {
-            const int rc = pack_rows(x, ldx, M, K, left, s);
-            if (rc != PMG_OK) return rc;
-            xp = left;
-            ld = round8(K);
-            left += round256((size_t)M * ld * 2);
-        }
         o.y = dw;
         o.ldy = lddw;
         o.vec = vec_ok(o);
-        const int rc = gemm<T, true, true>(dz, lddz, xp, ld, N, K, M, o, reinterpret_cast<float*>(left), status, s);
-        if (rc != PMG_OK) return rc;
+        const int rc2 = gemm<T, true, true>(dz, lddz, mx.p, mx.ld, N, K, M, o, reinterpret_cast<float*>(ws), status, s);
+        if (rc2 != PMG_OK) return rc2;
     }
     return PMG_OK;
 }
@@ -996,9 +995,8 @@ extern "C" size_t pmg_linear_grad_workspace_bytes(int64_t M, int64_t N, int64_t 
     const GradPlan p = grad_plan(M, N, act != PMG_ACT_NONE, !pack_dy);
     const size_t dz = p.dz ? round256((size_t)M * round8(N) * 2) : 0;
     const size_t db = bias_grad ? round256((size_t)p.row_blocks * N * sizeof(float)) : 0;
-    const size_t wx = (pack_w ? round256((size_t)N * round8(K) * 2) : 0) + part_bytes(M, K, N);
-    const size_t ww = (pack_x ? round256((size_t)M * round8(K) * 2) : 0) + part_bytes(N, K, M);
-    return dz + db + std::max(wx, ww);
+    const size_t packed = (pack_w ? round256((size_t)N * round8(K) * 2) : 0) + (pack_x ? round256((size_t)M * round8(K) * 2) : 0);
+    return dz + db + packed + std::max(part_bytes(M, K, N), part_bytes(N, K, M));
 }
 
 extern "C" int pmg_linear_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, const void* w, int64_t ldw,

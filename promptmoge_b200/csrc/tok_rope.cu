@@ -372,7 +372,7 @@ __global__ void __launch_bounds__(1024) k_rope_weight_grad(const float* __restri
     const int b0 = blockIdx.y ? blocks_q : 0, b1 = blockIdx.y ? blocks_q + blocks_k : blocks_q;
     float v = 0.0f;
     if (col < D)
-#pragma unroll 4
+#pragma unroll 8
         for (int b = b0 + strand; b < b1; b += 32) v += part[(int64_t)b * D + col];
     sm[strand][threadIdx.x & 31] = v;
     __syncthreads();
@@ -524,9 +524,8 @@ extern "C" int pmg_qk_norm_rope_grad(const void* dq, int64_t dq_tok, int64_t dq_
     const int rc2 = by_type<true>(dtype, a, s);
     if (rc2 != PMG_OK) return rc2;
     if (weights) {
-        k_rope_weight_grad<<<dim3((D + 31) / 32, 2), 1024, 0, s>>>(a.part, a.blocks[0], a.blocks[1], D, q_weight_grad,
-                                                                   k_weight_grad);
-        PMG_LAUNCH_CHECK();
+        return launch_after(k_rope_weight_grad, dim3((D + 31) / 32, 2), 1024, 0, s, (const float*)a.part, a.blocks[0],
+                            a.blocks[1], D, q_weight_grad, k_weight_grad);
     }
     return PMG_OK;
 }

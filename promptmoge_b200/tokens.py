@@ -12,6 +12,8 @@ is kept in a status word per device: `check()` reads it.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -22,31 +24,36 @@ _DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 
 _status_words: dict = {}
+_status_ptrs: dict = {}
 _fn: dict = {}
+_current_device = torch._C._cuda_getDevice
+_current_stream = torch._C._cuda_getCurrentRawStream
 
 
+# Small calls are bound by the host: a call's checks read each attribute of a tensor once, and only a call that fails
+# them runs the functions that say why.
 def _call(name, *args):
     f = _fn.get(name)
     if f is None:
         f = _fn[name] = getattr(_lib.load(), name)
     rc = f(*args)
-    if rc != 0:
+    if rc:
         raise PmgError(name, rc)
 
 
-def _query(name, *args):
-    f = _fn.get(name)
-    if f is None:
-        f = _fn[name] = getattr(_lib.load(), name)
-    return f(*args)
+@functools.lru_cache(maxsize=4096)
+def _query(name, *sizes):
+    """A workspace size, which depends on a call's sizes alone."""
+    return getattr(_lib.load(), name)(*sizes)
 
 
 def _status(index: int) -> int:
-    word = _status_words.get(index)
-    if word is None:
+    ptr = _status_ptrs.get(index)
+    if ptr is None:
         word = _status_words[index] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
         torch.cuda.current_stream(word.device).synchronize()    # zeroed before any other stream's kernel sees it
-    return word.data_ptr()
+        ptr = _status_ptrs[index] = word.data_ptr()
+    return ptr
 
 
 def check(device=None) -> None:
@@ -60,24 +67,6 @@ def check(device=None) -> None:
     if code:
         word.zero_()
         raise PmgError("token operator (" + STATUS.get(code, str(code)) + ")", code)
-
-
-class _On:
-    """Makes a tensor's device current where it is not."""
-    __slots__ = ("index", "before")
-
-    def __init__(self, index):
-        self.index = index
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        return torch._C._cuda_getCurrentRawStream(self.index)
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
 
 
 def _dev(t, name, dim, index=None, dtypes=None):
@@ -103,15 +92,23 @@ def _shape(t, shape, name):
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
-def _ld(t):
-    """Row stride; one that the row count leaves without meaning is taken as the row length."""
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+def _plain(t, dim, index, dtype):
+    """Whether _dev(t, ...) would pass."""
+    return t.dim() == dim and t.dtype is dtype and t.get_device() == index and (t.stride(-1) == 1 or t.shape[-1] <= 1)
 
 
-def _row(t):
-    """(pointer, row stride) and whether the tensor-core path has to copy rows to 16-byte boundaries."""
-    p, ld = t.data_ptr(), _ld(t)
-    return p, ld, int(bool(p & 15 or ld & 7))
+def _matrix(t, name, index, dtype):
+    """(pointer, rows, columns, row stride) of a matrix with rows that do not overlap; a stride that the row count leaves
+    without meaning is taken as the row length."""
+    if t.dim() != 2 or t.dtype is not dtype or t.get_device() != index:
+        _dev(t, name, 2, index, (dtype,))
+    n, k = t.shape
+    ld, one = t.stride()
+    if n <= 1:
+        ld = max(k, 1)
+    if ld < k or (one != 1 and k > 1):
+        _rows_ok(_dev(t, name, 2, index, (dtype,)), name)
+    return t.data_ptr(), n, k, ld
 
 
 def _rows_ok(t, name):
@@ -129,47 +126,56 @@ def linear(x, w, bias=None, activation: str = "none", residual=None, save_pre: b
     type; activation "none", "relu", "silu" or "gelu" (erf).  The output has x's type, or torch.float32 (out_dtype, or
     the residual's type where out_dtype is not given).  out: a tensor to write to (it may be the residual).  With
     save_pre, returns (y, x w^T + bias), the second for linear_grad."""
-    _dev(x, "x", 2, None, _HALF)
-    index = x.get_device()
     dt = x.dtype
-    _dev(w, "w", 2, index, (dt,))
-    M, K = x.shape
-    N = w.shape[0]
-    if w.shape[1] != K:
+    if dt not in _HALF or not x.is_cuda:
+        _dev(x, "x", 2, None, _HALF)
+    index = x.get_device()
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return linear(x, w, bias, activation, residual, save_pre, out_dtype, out)
+    xp, M, K, ldx = _matrix(x, "x", index, dt)
+    wp, N, wk, ldw = _matrix(w, "w", index, dt)
+    if wk != K:
         raise ValueError(f"w must be [N, {K}], got {tuple(w.shape)}")
     if N < 1 or K < 1:
         raise ValueError("w must not be empty")
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
-    _rows_ok(x, "x")
-    _rows_ok(w, "w")
+    bp = None
     if bias is not None:
-        _shape(_dev(bias, "bias", 1, index, (dt,)), (N,), "bias")
+        if not _plain(bias, 1, index, dt) or bias.shape[0] != N:
+            _shape(_dev(bias, "bias", 1, index, (dt,)), (N,), "bias")
+        bp = bias.data_ptr()
+    odt, rp, ldr = out_dtype or dt, None, 0
     if residual is not None:
-        _shape(_rows_ok(_dev(residual, "residual", 2, index, (dt, torch.float32)), "residual"), (M, N), "residual")
-    odt = out_dtype if out_dtype is not None else (residual.dtype if residual is not None else dt)
-    if odt != dt and odt != torch.float32:
+        rdt = residual.dtype
+        if rdt is not dt and rdt is not torch.float32:
+            _dev(residual, "residual", 2, index, (dt, torch.float32))
+        if out_dtype is None:
+            odt = rdt
+        elif rdt is not odt:
+            raise TypeError(f"residual must have the output's type {odt}, got {rdt}")
+        rp, rm, rn, ldr = _matrix(residual, "residual", index, rdt)
+        if rm != M or rn != N:
+            _shape(residual, (M, N), "residual")
+    if odt is not dt and odt is not torch.float32:
         raise TypeError(f"out_dtype must be {dt} or torch.float32, got {odt}")
-    if residual is not None and residual.dtype != odt:
-        raise TypeError(f"residual must have the output's type {odt}, got {residual.dtype}")
     if out is None:
-        y = torch.empty((M, N), dtype=odt, device=x.device)
+        y, ldy = x.new_empty((M, N), dtype=odt), N
+        yp = y.data_ptr()
     else:
-        y = _rows_ok(_dev(out, "out", 2, index, (odt,)), "out")
-        _shape(y, (M, N), "out")
-    pre = torch.empty((M, N), dtype=dt, device=x.device) if save_pre else None
+        y = out
+        yp, om, on, ldy = _matrix(out, "out", index, odt)
+        if om != M or on != N:
+            _shape(out, (M, N), "out")
+    pre = x.new_empty((M, N)) if save_pre else None
     if M:
-        xp, ldx, px = _row(x)
-        wp, ldw, pw = _row(w)
-        need = _query("pmg_linear_workspace_bytes", M, N, K, px, pw)
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-        with _On(index) as stream:
-            _call("pmg_linear", xp, ldx, wp, ldw, _DTYPES[dt], M, N, K, bias.data_ptr() if bias is not None else None,
-                  act, residual.data_ptr() if residual is not None else None,
-                  _ld(residual) if residual is not None else 0, int(odt == torch.float32), y.data_ptr(), _ld(y),
-                  pre.data_ptr() if save_pre else None, N, ws.data_ptr() if need else None, need, _status(index),
-                  stream)
+        need = _query("pmg_linear_workspace_bytes", M, N, K, (xp | 2 * ldx) & 15, (wp | 2 * ldw) & 15) if M > 32 else 0
+        ws = x.new_empty(need, dtype=torch.uint8) if need else None
+        _call("pmg_linear", xp, ldx, wp, ldw, _DTYPES[dt], M, N, K, bp, act, rp, ldr, odt is torch.float32, yp, ldy,
+              pre.data_ptr() if save_pre else None, N, ws.data_ptr() if need else None, need, _status(index),
+              _current_stream(index))
     return (y, pre) if save_pre else y
 
 
@@ -178,85 +184,101 @@ def linear_grad(dy, x, w, pre=None, activation: str = "none", bias_grad: bool = 
     """Gradients (dx, dw, dbias) of linear() for dy [M, N], the gradient of its output, in x's type (dy too); None for
     one that is not asked for.  pre: the second output of linear(..., save_pre=True), needed unless the activation is
     "none".  The residual's gradient is dy itself."""
-    _dev(x, "x", 2, None, _HALF)
-    index, dt = x.get_device(), x.dtype
-    _dev(w, "w", 2, index, (dt,))
-    _dev(dy, "dy", 2, index, (dt,))
-    M, K = x.shape
-    N = w.shape[0]
-    if w.shape[1] != K or N < 1 or K < 1:
+    dt = x.dtype
+    if dt not in _HALF or not x.is_cuda:
+        _dev(x, "x", 2, None, _HALF)
+    index = x.get_device()
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return linear_grad(dy, x, w, pre, activation, bias_grad, input_grad, weight_grad)
+    xp, M, K, ldx = _matrix(x, "x", index, dt)
+    wp, N, wk, ldw = _matrix(w, "w", index, dt)
+    yp, ym, yn, ldy = _matrix(dy, "dy", index, dt)
+    if wk != K or N < 1 or K < 1:
         raise ValueError(f"w must be [N, {K}], got {tuple(w.shape)}")
-    _shape(dy, (M, N), "dy")
+    if ym != M or yn != N:
+        _shape(dy, (M, N), "dy")
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, got {activation!r}")
-    if act and pre is None:
-        raise ValueError("pre (linear(..., save_pre=True)) is needed for an activation's gradient")
-    for t, name in ((x, "x"), (w, "w"), (dy, "dy")):
-        _rows_ok(t, name)
+    pp, ldp = None, 0
     if act:
-        _shape(_rows_ok(_dev(pre, "pre", 2, index, (dt,)), "pre"), (M, N), "pre")
-    dx = torch.empty((M, K), dtype=dt, device=x.device) if input_grad else None
-    dw = torch.empty((N, K), dtype=dt, device=x.device) if weight_grad else None
-    db = torch.empty(N, dtype=dt, device=x.device) if bias_grad else None
-    xp, ldx, px = _row(x)
-    wp, ldw, pw = _row(w)
-    yp, ldy, py = _row(dy)
-    need = _query("pmg_linear_grad_workspace_bytes", M, N, K, act, py, px if weight_grad else 0,
-                  pw if input_grad else 0, int(bias_grad))
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    with _On(index) as stream:
-        _call("pmg_linear_grad", yp, ldy, xp, ldx, wp, ldw, _DTYPES[dt], M, N, K, pre.data_ptr() if act else None,
-              _ld(pre) if act else 0, act, dx.data_ptr() if input_grad else None, K,
-              dw.data_ptr() if weight_grad else None, K, db.data_ptr() if bias_grad else None,
-              ws.data_ptr() if need else None, need, _status(index), stream)
+        if pre is None:
+            raise ValueError("pre (linear(..., save_pre=True)) is needed for an activation's gradient")
+        pp, pm, pn, ldp = _matrix(pre, "pre", index, dt)
+        if pm != M or pn != N:
+            _shape(pre, (M, N), "pre")
+    dx = x.new_empty((M, K)) if input_grad else None
+    dw = x.new_empty((N, K)) if weight_grad else None
+    db = x.new_empty(N) if bias_grad else None
+    need = _query("pmg_linear_grad_workspace_bytes", M, N, K, act, (yp | 2 * ldy) & 15,
+                  (xp | 2 * ldx) & 15 if weight_grad else 0, (wp | 2 * ldw) & 15 if input_grad else 0, int(bias_grad))
+    ws = x.new_empty(need, dtype=torch.uint8) if need else None
+    _call("pmg_linear_grad", yp, ldy, xp, ldx, wp, ldw, _DTYPES[dt], M, N, K, pp, ldp, act,
+          dx.data_ptr() if input_grad else None, K, dw.data_ptr() if weight_grad else None, K,
+          db.data_ptr() if bias_grad else None, ws.data_ptr() if need else None, need, _status(index),
+          _current_stream(index))
     return dx, dw, db
 
 
 # ----------------------------------------------------------------------------------------------------------------- #
 # Norm of queries and keys with the position rotation
 # ----------------------------------------------------------------------------------------------------------------- #
-def _heads(t, name, index, dtypes):
+def _heads(t, name, index, dtype, T, H, D):
     """(pointer, token stride, head stride) of [T, H, D]."""
-    _dev(t, name, 3, index, dtypes)
-    return t.data_ptr(), t.stride(0), t.stride(1)
+    if not _plain(t, 3, index, dtype):
+        _dev(t, name, 3, index, (dtype,))
+    if t.shape != (T, H, D):
+        _shape(t, (T, H, D), name)
+    st, sh, _ = t.stride()
+    return t.data_ptr(), st, sh
 
 
 def _angles(cos, sin, positions, T, D, index):
-    _dev(cos, "cos", 2, index, (torch.float32,))
-    _dev(sin, "sin", 2, index, (torch.float32,))
+    """(cos, sin, pairs, places, positions) as the entry points take them."""
+    if not (_plain(cos, 2, index, torch.float32) and _plain(sin, 2, index, torch.float32)):
+        _dev(cos, "cos", 2, index, (torch.float32,))
+        _dev(sin, "sin", 2, index, (torch.float32,))
     places, half = cos.shape
-    _shape(sin, cos.shape, "sin")
+    if sin.shape != cos.shape:
+        _shape(sin, cos.shape, "sin")
     if 2 * half > D:
         raise ValueError(f"cos and sin rotate {2 * half} values of heads of {D}")
     if not cos.is_contiguous() or not sin.is_contiguous():
         raise ValueError("cos and sin must be contiguous")
-    if positions is not None:
-        _shape(_dev(positions, "positions", 1, index, (torch.int32,)), (T,), "positions")
-    elif T > places and half:
-        raise ValueError(f"{T} tokens without positions need as many rows of cos and sin, got {places}")
     if half and T and places == 0:
         raise ValueError("cos and sin must not be empty")
-    return places, half
+    if positions is not None:
+        if not _plain(positions, 1, index, torch.int32) or positions.shape[0] != T:
+            _shape(_dev(positions, "positions", 1, index, (torch.int32,)), (T,), "positions")
+        return cos.data_ptr(), sin.data_ptr(), half, places, positions.data_ptr()
+    if T > places and half:
+        raise ValueError(f"{T} tokens without positions need as many rows of cos and sin, got {places}")
+    return cos.data_ptr(), sin.data_ptr(), half, places, None
 
 
 def _weight(w, name, D, index):
     if w is None:
         return None
-    _shape(_dev(w, name, 1, index, (torch.float32,)), (D,), name)
+    if not _plain(w, 1, index, torch.float32) or w.shape[0] != D:
+        _shape(_dev(w, name, 1, index, (torch.float32,)), (D,), name)
     return w.data_ptr()
 
 
 def _qk(q, k):
-    _dev(q, "q", 3, None, _HALF_OR_F32)
-    index, dt = q.get_device(), q.dtype
-    _dev(k, "k", 3, index, (dt,))
+    dt = q.dtype
+    if dt not in _DTYPES or not q.is_cuda or q.dim() != 3:
+        _dev(q, "q", 3, None, _HALF_OR_F32)
+    index = q.get_device()
+    if not _plain(k, 3, index, dt):
+        _dev(k, "k", 3, index, (dt,))
     T, Hq, D = q.shape
-    if k.shape[0] != T or k.shape[2] != D:
+    kt, Hk, kd = k.shape
+    if kt != T or kd != D:
         raise ValueError(f"k must be [{T}, heads, {D}], got {tuple(k.shape)}")
     if D < 1 or D > 256:
         raise ValueError(f"heads hold 1 to 256 values, got {D}")
-    return index, dt, T, Hq, k.shape[1], D
+    return index, dt, T, Hq, Hk, D
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps: float = 1e-6, interleaved: bool = False,
@@ -267,19 +289,18 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps: float 
     pairs), or (2i, 2i + 1) when interleaved.  out: a pair of tensors to write to, which may be q and k themselves or
     rows of a cache.  Returns (q, k)."""
     index, dt, T, Hq, Hk, D = _qk(q, k)
-    places, half = _angles(cos, sin, positions, T, D, index)
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, out)
+    cp, sp, half, places, pp = _angles(cos, sin, positions, T, D, index)
     if out is None:
-        qo, ko = (torch.empty(t.shape, dtype=dt, device=q.device) for t in (q, k))
+        qo, ko = q.new_empty((T, Hq, D)), q.new_empty((T, Hk, D))
     else:
         qo, ko = out
-        _shape(_dev(qo, "out[0]", 3, index, (dt,)), q.shape, "out[0]")
-        _shape(_dev(ko, "out[1]", 3, index, (dt,)), k.shape, "out[1]")
-    with _On(index) as stream:
-        _call("pmg_qk_norm_rope", q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
-              _DTYPES[dt], T, Hq, Hk, D, 2 * half, _weight(q_weight, "q_weight", D, index),
-              _weight(k_weight, "k_weight", D, index), cos.data_ptr(), sin.data_ptr(), places,
-              positions.data_ptr() if positions is not None else None, eps, int(interleaved), qo.data_ptr(),
-              qo.stride(0), qo.stride(1), ko.data_ptr(), ko.stride(0), ko.stride(1), _status(index), stream)
+    _call("pmg_qk_norm_rope", *_heads(q, "q", index, dt, T, Hq, D), *_heads(k, "k", index, dt, T, Hk, D), _DTYPES[dt], T,
+          Hq, Hk, D, 2 * half, _weight(q_weight, "q_weight", D, index), _weight(k_weight, "k_weight", D, index), cp, sp,
+          places, pp, eps, bool(interleaved), *_heads(qo, "out[0]", index, dt, T, Hq, D),
+          *_heads(ko, "out[1]", index, dt, T, Hk, D), _status(index), _current_stream(index))
     return qo, ko
 
 
@@ -288,71 +309,71 @@ def qk_norm_rope_grad(dq, dk, q, k, q_weight, k_weight, cos, sin, positions=None
     """Gradients (q, k, q_weight, k_weight) of qk_norm_rope() for the gradients dq, dk of its outputs and its inputs
     q, k; the weights' in fp32, None where there is no weight."""
     index, dt, T, Hq, Hk, D = _qk(q, k)
-    places, half = _angles(cos, sin, positions, T, D, index)
-    _shape(_dev(dq, "dq", 3, index, (dt,)), q.shape, "dq")
-    _shape(_dev(dk, "dk", 3, index, (dt,)), k.shape, "dk")
-    gq, gk = (torch.empty(t.shape, dtype=dt, device=q.device) for t in (q, k))
-    gqw = torch.empty(D, dtype=torch.float32, device=q.device) if q_weight is not None else None
-    gkw = torch.empty(D, dtype=torch.float32, device=q.device) if k_weight is not None else None
-    need = 0
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return qk_norm_rope_grad(dq, dk, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    cp, sp, half, places, pp = _angles(cos, sin, positions, T, D, index)
+    gq, gk = q.new_empty((T, Hq, D)), q.new_empty((T, Hk, D))
+    gqw = q.new_empty(D, dtype=torch.float32) if q_weight is not None else None
+    gkw = q.new_empty(D, dtype=torch.float32) if k_weight is not None else None
+    need, ws = 0, None
     if q_weight is not None or k_weight is not None:
         need = _query("pmg_qk_norm_rope_grad_workspace_bytes", D)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    with _On(index) as stream:
-        _call("pmg_qk_norm_rope_grad", *_heads(dq, "dq", index, (dt,)), *_heads(dk, "dk", index, (dt,)),
-              *_heads(q, "q", index, (dt,)), *_heads(k, "k", index, (dt,)), _DTYPES[dt], T, Hq, Hk, D, 2 * half,
-              _weight(q_weight, "q_weight", D, index), _weight(k_weight, "k_weight", D, index), cos.data_ptr(),
-              sin.data_ptr(), places, positions.data_ptr() if positions is not None else None, eps, int(interleaved),
-              gq.data_ptr(), gq.stride(0), gq.stride(1), gk.data_ptr(), gk.stride(0), gk.stride(1),
-              gqw.data_ptr() if gqw is not None else None, gkw.data_ptr() if gkw is not None else None,
-              ws.data_ptr() if need else None, need, _status(index), stream)
+        ws = q.new_empty(need, dtype=torch.uint8)
+    qs, ks = (T, Hq, D), (T, Hk, D)
+    _call("pmg_qk_norm_rope_grad", *_heads(dq, "dq", index, dt, *qs), *_heads(dk, "dk", index, dt, *ks),
+          *_heads(q, "q", index, dt, *qs), *_heads(k, "k", index, dt, *ks), _DTYPES[dt], T, Hq, Hk, D, 2 * half,
+          _weight(q_weight, "q_weight", D, index), _weight(k_weight, "k_weight", D, index), cp, sp, places, pp, eps,
+          bool(interleaved), gq.data_ptr(), Hq * D, D, gk.data_ptr(), Hk * D, D,
+          gqw.data_ptr() if gqw is not None else None, gkw.data_ptr() if gkw is not None else None,
+          ws.data_ptr() if need else None, need, _status(index), _current_stream(index))
     return gq, gk, gqw, gkw
 
 
 # ----------------------------------------------------------------------------------------------------------------- #
 # Attention over packed documents
 # ----------------------------------------------------------------------------------------------------------------- #
-def _aligned_heads(t, name, shape, index, dt):
+def _aligned_heads(t, name, T, H, D, index, dt):
     """(pointer, token stride, head stride) of [T, H, D] on 16-byte boundaries."""
-    _dev(t, name, 3, index, (dt,))
-    if shape is not None:
-        _shape(t, shape, name)
-    T, H, D = t.shape
-    p, st, sh = t.data_ptr(), t.stride(0), t.stride(1)
-    if T <= 1:
-        st = H * D if sh == D or H <= 1 else (st + 7) // 8 * 8
+    p, st, sh = _heads(t, name, index, dt, T, H, D)
     if H <= 1:
         sh = D
-    if p & 15 or st & 7 or sh & 7:
+    if T <= 1:
+        st = H * D if sh == D else (st + 7) // 8 * 8
+    if (p | 2 * st | 2 * sh) & 15:
         raise ValueError(f"{name}: heads must start on 16-byte boundaries (strides in multiples of 8 values)")
     return p, st, sh
 
 
-def _packing(cu_q, cu_k, k_len, prefix, slopes, Hq, index):
-    docs = cu_q.shape[0] - 1
-    for t, name, n in ((cu_q, "cu_q", docs + 1), (cu_k, "cu_k", docs + 1), (k_len, "k_len", docs),
-                       (prefix, "prefix", docs)):
-        if t is not None:
-            _shape(_dev(t, name, 1, index, (torch.int32,)), (n,), name)
-    if docs < 0:
-        raise ValueError("cu_q must hold the documents' offsets, the total last")
-    if slopes is not None:
-        _shape(_dev(slopes, "slopes", 1, index, (torch.float32,)), (Hq,), "slopes")
-    return docs
+def _words(t, name, n, index, dtype=torch.int32):
+    """The pointer of a vector of n values, or None."""
+    if t is None:
+        return None
+    if not _plain(t, 1, index, dtype) or t.shape[0] != n:
+        _shape(_dev(t, name, 1, index, (dtype,)), (n,), name)
+    return t.data_ptr()
 
 
-def _attention_shapes(q, k, v):
-    _dev(q, "q", 3, None, _HALF)
-    index, dt = q.get_device(), q.dtype
+def _attention_shapes(q, k):
+    dt = q.dtype
+    if dt not in _HALF or not q.is_cuda or q.dim() != 3:
+        _dev(q, "q", 3, None, _HALF)
+    index = q.get_device()
+    if not _plain(k, 3, index, dt):
+        _dev(k, "k", 3, index, (dt,))
     Tq, Hq, D = q.shape
-    _dev(k, "k", 3, index, (dt,))
-    Tk, Hk, _ = k.shape
-    if k.shape[2] != D or Hk < 1 or Hq < 1 or Hq % Hk:
+    Tk, Hk, kd = k.shape
+    if kd != D or Hk < 1 or Hq < 1 or Hq % Hk:
         raise ValueError(f"k must be [keys, heads, {D}] with a number of heads that divides {Hq}, got {tuple(k.shape)}")
-    _shape(v, k.shape, "v")
     if D % 8 or not 8 <= D <= 128:
         raise ValueError(f"heads must hold a multiple of 8 values, 8 to 128, got {D}")
     return index, dt, Tq, Tk, Hq, Hk, D
+
+
+def _documents(cu_q):
+    if cu_q.dim() != 1 or cu_q.shape[0] < 1:
+        raise ValueError("cu_q must hold the documents' offsets, the total last")
+    return cu_q.shape[0] - 1
 
 
 def _score(scale, D, softcap, causal, prefix, max_q, max_k):
@@ -377,23 +398,26 @@ def attention(q, k, v, cu_q, cu_k, max_q: int, max_k: int, scale: float | None =
 
     Returns (o [Tq, Hq, D], lse [Hq, Tq] fp32).  Rows that see no key give 0 and -inf.  max_q * Hq / Hk <= 16 (token by
     token) takes the kernel that reads the keys once for all rows."""
-    index, dt, Tq, Tk, Hq, Hk, D = _attention_shapes(q, k, v)
-    docs = _packing(cu_q, cu_k, k_len, prefix, slopes, Hq, index)
+    index, dt, Tq, Tk, Hq, Hk, D = _attention_shapes(q, k)
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return attention(q, k, v, cu_q, cu_k, max_q, max_k, scale, causal, prefix, softcap, slopes, k_len, out)
+    docs = _documents(cu_q)
     scale = _score(scale, D, softcap, causal, prefix, max_q, max_k)
-    o = torch.empty((Tq, Hq, D), dtype=dt, device=q.device) if out is None else out
-    lse = torch.empty((Hq, Tq), dtype=torch.float32, device=q.device)
-    if not Tq:
-        return o, lse
-    oh = _aligned_heads(o, "out", (Tq, Hq, D), index, dt)
-    need = _query("pmg_attention_workspace_bytes", docs, Hq, Hk, D, max_q, max_k)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    with _On(index) as stream:
-        _call("pmg_attention", *_aligned_heads(q, "q", None, index, dt), *_aligned_heads(k, "k", None, index, dt),
-              *_aligned_heads(v, "v", None, index, dt), _DTYPES[dt], Tq, Tk, Hq, Hk, D, cu_q.data_ptr(),
-              cu_k.data_ptr(), k_len.data_ptr() if k_len is not None else None, docs, max_q, max_k, scale, int(causal),
-              prefix.data_ptr() if prefix is not None else None, softcap,
-              slopes.data_ptr() if slopes is not None else None, *oh, lse.data_ptr(),
-              ws.data_ptr() if need else None, need, _status(index), stream)
+    words = (_words(cu_q, "cu_q", docs + 1, index), _words(cu_k, "cu_k", docs + 1, index),
+             _words(k_len, "k_len", docs, index), _words(prefix, "prefix", docs, index),
+             _words(slopes, "slopes", Hq, index, torch.float32))
+    vh = _aligned_heads(v, "v", Tk, Hk, D, index, dt)
+    qh, kh = _aligned_heads(q, "q", Tq, Hq, D, index, dt), _aligned_heads(k, "k", Tk, Hk, D, index, dt)
+    o = q.new_empty((Tq, Hq, D)) if out is None else out
+    lse = q.new_empty((Hq, Tq), dtype=torch.float32)
+    oh = _aligned_heads(o, "out", Tq, Hq, D, index, dt)
+    if Tq:
+        need = _query("pmg_attention_workspace_bytes", docs, Hq, Hk, D, max_q, max_k) if max_q * Hq <= 16 * Hk else 0
+        ws = q.new_empty(need, dtype=torch.uint8) if need else None
+        _call("pmg_attention", *qh, *kh, *vh, _DTYPES[dt], Tq, Tk, Hq, Hk, D, words[0], words[1], words[2], docs, max_q,
+              max_k, scale, bool(causal), words[3], softcap, words[4], *oh, lse.data_ptr(),
+              ws.data_ptr() if need else None, need, _status(index), _current_stream(index))
     return o, lse
 
 
@@ -401,23 +425,29 @@ def attention_grad(do, o, lse, q, k, v, cu_q, cu_k, max_q: int, max_k: int, scal
                    causal: bool = False, prefix=None, softcap: float = 0.0, slopes=None, k_len=None):
     """Gradients (dq, dk, dv) of attention() for do, the gradient of its output: o and lse are what it returned, the
     rest its arguments.  The slopes are constants of the score and get no gradient.  Key rows behind k_len get zeros."""
-    index, dt, Tq, Tk, Hq, Hk, D = _attention_shapes(q, k, v)
-    docs = _packing(cu_q, cu_k, k_len, prefix, slopes, Hq, index)
+    index, dt, Tq, Tk, Hq, Hk, D = _attention_shapes(q, k)
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return attention_grad(do, o, lse, q, k, v, cu_q, cu_k, max_q, max_k, scale, causal, prefix, softcap, slopes,
+                                  k_len)
+    docs = _documents(cu_q)
     scale = _score(scale, D, softcap, causal, prefix, max_q, max_k)
-    _shape(_dev(lse, "lse", 2, index, (torch.float32,)), (Hq, Tq), "lse")
+    words = (_words(cu_q, "cu_q", docs + 1, index), _words(cu_k, "cu_k", docs + 1, index),
+             _words(k_len, "k_len", docs, index), _words(prefix, "prefix", docs, index),
+             _words(slopes, "slopes", Hq, index, torch.float32))
+    if not _plain(lse, 2, index, torch.float32) or lse.shape != (Hq, Tq):
+        _shape(_dev(lse, "lse", 2, index, (torch.float32,)), (Hq, Tq), "lse")
     if not lse.is_contiguous():
         raise ValueError("lse must be contiguous")
-    doh = _aligned_heads(do, "do", q.shape, index, dt)
-    oh = _aligned_heads(o, "o", q.shape, index, dt)
-    dq, dk, dv = (torch.empty(t.shape, dtype=dt, device=q.device) for t in (q, k, v))
+    qs, ks = (Tq, Hq, D), (Tk, Hk, D)
+    heads = (*_aligned_heads(do, "do", *qs, index, dt), *_aligned_heads(o, "o", *qs, index, dt), lse.data_ptr(),
+             *_aligned_heads(q, "q", *qs, index, dt), *_aligned_heads(k, "k", *ks, index, dt),
+             *_aligned_heads(v, "v", *ks, index, dt))
+    dq, dk, dv = q.new_empty(qs), q.new_empty(ks), q.new_empty(ks)
     need = _query("pmg_attention_grad_workspace_bytes", Tq, Hq)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-    ks = (Hk * D, D)
-    with _On(index) as stream:
-        _call("pmg_attention_grad", *doh, *oh, lse.data_ptr(), *_aligned_heads(q, "q", None, index, dt),
-              *_aligned_heads(k, "k", None, index, dt), *_aligned_heads(v, "v", None, index, dt), _DTYPES[dt], Tq, Tk,
-              Hq, Hk, D, cu_q.data_ptr(), cu_k.data_ptr(), k_len.data_ptr() if k_len is not None else None, docs, scale,
-              int(causal), prefix.data_ptr() if prefix is not None else None, softcap,
-              slopes.data_ptr() if slopes is not None else None, dq.data_ptr(), Hq * D, D, dk.data_ptr(), *ks,
-              dv.data_ptr(), *ks, ws.data_ptr(), need, _status(index), stream)
+    ws = q.new_empty(need, dtype=torch.uint8)
+    st = (Hk * D, D)
+    _call("pmg_attention_grad", *heads, _DTYPES[dt], Tq, Tk, Hq, Hk, D, words[0], words[1], words[2], docs, scale,
+          bool(causal), words[3], softcap, words[4], dq.data_ptr(), Hq * D, D, dk.data_ptr(), *st, dv.data_ptr(), *st,
+          ws.data_ptr(), need, _status(index), _current_stream(index))
     return dq, dk, dv
