@@ -244,7 +244,7 @@ def _angles(cos, sin, positions, T, D, index):
         _shape(sin, cos.shape, "sin")
     if 2 * half > D:
         raise ValueError(f"cos and sin rotate {2 * half} values of heads of {D}")
-    if not cos.is_contiguous() or not sin.is_contiguous():
+    if half and places > 1 and (cos.stride(0) != half or sin.stride(0) != half):
         raise ValueError("cos and sin must be contiguous")
     if half and T and places == 0:
         raise ValueError("cos and sin must not be empty")
@@ -267,9 +267,9 @@ def _weight(w, name, D, index):
 
 def _qk(q, k):
     dt = q.dtype
-    if dt not in _DTYPES or not q.is_cuda or q.dim() != 3:
-        _dev(q, "q", 3, None, _HALF_OR_F32)
     index = q.get_device()
+    if dt not in _DTYPES or index < 0 or q.dim() != 3 or (q.stride(2) != 1 and q.shape[2] > 1):
+        _dev(q, "q", 3, None, _HALF_OR_F32)
     if not _plain(k, 3, index, dt):
         _dev(k, "k", 3, index, (dt,))
     T, Hq, D = q.shape
@@ -293,14 +293,16 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions=None, eps: float 
         with torch.cuda.device(index):
             return qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved, out)
     cp, sp, half, places, pp = _angles(cos, sin, positions, T, D, index)
+    qh, kh = (q.data_ptr(), *q.stride()[:2]), (k.data_ptr(), *k.stride()[:2])
     if out is None:
         qo, ko = q.new_empty((T, Hq, D)), q.new_empty((T, Hk, D))
+        qoh, koh = (qo.data_ptr(), Hq * D, D), (ko.data_ptr(), Hk * D, D)
     else:
         qo, ko = out
-    _call("pmg_qk_norm_rope", *_heads(q, "q", index, dt, T, Hq, D), *_heads(k, "k", index, dt, T, Hk, D), _DTYPES[dt], T,
-          Hq, Hk, D, 2 * half, _weight(q_weight, "q_weight", D, index), _weight(k_weight, "k_weight", D, index), cp, sp,
-          places, pp, eps, bool(interleaved), *_heads(qo, "out[0]", index, dt, T, Hq, D),
-          *_heads(ko, "out[1]", index, dt, T, Hk, D), _status(index), _current_stream(index))
+        qoh, koh = _heads(qo, "out[0]", index, dt, T, Hq, D), _heads(ko, "out[1]", index, dt, T, Hk, D)
+    _call("pmg_qk_norm_rope", *qh, *kh, _DTYPES[dt], T, Hq, Hk, D, 2 * half, _weight(q_weight, "q_weight", D, index),
+          _weight(k_weight, "k_weight", D, index), cp, sp, places, pp, eps, bool(interleaved), *qoh, *koh,
+          _status(index), _current_stream(index))
     return qo, ko
 
 
@@ -356,9 +358,9 @@ def _words(t, name, n, index, dtype=torch.int32):
 
 def _attention_shapes(q, k):
     dt = q.dtype
-    if dt not in _HALF or not q.is_cuda or q.dim() != 3:
-        _dev(q, "q", 3, None, _HALF)
     index = q.get_device()
+    if dt not in _HALF or index < 0 or q.dim() != 3:
+        _dev(q, "q", 3, None, _HALF)
     if not _plain(k, 3, index, dt):
         _dev(k, "k", 3, index, (dt,))
     Tq, Hq, D = q.shape
