@@ -644,6 +644,17 @@ __global__ void __launch_bounds__(256) k_split_sum(const __grid_constant__ Sched
 // ----------------------------------------------------------------------------------------------------------------- //
 constexpr int kStripCols = 256, kStripRows = 8;       // a block's columns; rows at a time
 
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 p = Elem<T>::unpack(w[i]);
+        f[2 * i] = p.x;
+        f[2 * i + 1] = p.y;
+    }
+}
+
 // dz = dy act'(z) rounded to T into dst (null: not wanted) with its row padding zeroed, and this block's column sums of
 // the unrounded dz into part [row blocks][N] (null: not wanted).
 template <typename T, bool VEC>
@@ -656,42 +667,42 @@ __global__ void __launch_bounds__(256) k_act_grad(const T* __restrict__ dy, int6
     const int cg = threadIdx.x & 31, rg = threadIdx.x >> 5, n = blockIdx.x * kStripCols + cg * 8;
     const int64_t r0 = blockIdx.y * rows_per_block, r1 = min(r0 + rows_per_block, M);
     float acc[8] = {};
+    const bool vec = VEC && n + 8 <= N;
+    auto row = [&](const T* p, int64_t ld, int64_t m) {               // 8 values, zero beyond the matrix
+        if (m >= r1) return make_uint4(0, 0, 0, 0);
+        if (vec) return *reinterpret_cast<const uint4*>(p + m * ld + n);
+        uint32_t w[4] = {0, 0, 0, 0};
+        const uint16_t* q = reinterpret_cast<const uint16_t*>(p + m * ld + n);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (n + i < N) w[i >> 1] |= (uint32_t)q[i] << (16 * (i & 1));
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    };
     if (n < padded) {
-#pragma unroll 2
-        for (int64_t m = r0 + rg; m < r1; m += kStripRows) {
-            float g[8], z[8];
-            if (VEC && n + 8 <= N) {
-                const uint4 a = *reinterpret_cast<const uint4*>(dy + m * ldy + n);
-                const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+        constexpr int U = 4;                                          // rows on their way at once
+        for (int64_t m0 = r0 + rg; m0 < r1; m0 += U * kStripRows) {
+            uint4 dr[U], zr[U];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 f = Elem<T>::unpack(w[i]);
-                    g[2 * i] = f.x;
-                    g[2 * i + 1] = f.y;
-                }
-                if (pre) {
-                    const uint4 b = *reinterpret_cast<const uint4*>(pre + m * ldp + n);
-                    const uint32_t v[4] = {b.x, b.y, b.z, b.w};
+            for (int u = 0; u < U; ++u) dr[u] = row(dy, ldy, m0 + u * kStripRows);
+            if (pre) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float2 f = Elem<T>::unpack(v[i]);
-                        z[2 * i] = f.x;
-                        z[2 * i + 1] = f.y;
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    g[i] = n + i < N ? Elem<T>::to(dy[m * ldy + n + i]) : 0.0f;
-                    z[i] = pre && n + i < N ? Elem<T>::to(pre[m * ldp + n + i]) : 0.0f;
-                }
+                for (int u = 0; u < U; ++u) zr[u] = row(pre, ldp, m0 + u * kStripRows);
             }
-            if (pre) times_slope(act, g, z);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] += g[i];
-            if (dst) {
-                *reinterpret_cast<uint4*>(dst + m * ldd + n) = make_uint4(Elem<T>::pack(g[0], g[1]), Elem<T>::pack(g[2], g[3]),
-                                                                          Elem<T>::pack(g[4], g[5]), Elem<T>::pack(g[6], g[7]));
+            for (int u = 0; u < U; ++u) {
+                const int64_t m = m0 + u * kStripRows;
+                float g[8], z[8];
+                unpack8<T>(dr[u], g);
+                if (pre) {
+                    unpack8<T>(zr[u], z);
+                    times_slope(act, g, z);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[i] += g[i];
+                if (dst && m < r1) {
+                    *reinterpret_cast<uint4*>(dst + m * ldd + n) =
+                        make_uint4(Elem<T>::pack(g[0], g[1]), Elem<T>::pack(g[2], g[3]), Elem<T>::pack(g[4], g[5]), Elem<T>::pack(g[6], g[7]));
+                }
             }
         }
     }
