@@ -1,8 +1,8 @@
 // Attention over packed documents, forwards: rows by the tile (k_attn) and few rows over a long cache (k_attn_few).
 //
-// k_attn.  A CTA owns 256 query rows of one document and head, two tiles of 128 that share every key tile of 128.
-// Products run on tcgen05 with the scores, the probabilities (left operand of the second product) and the running
-// output in tensor memory; a warpgroup per tile holds one row a thread, so the softmax needs no shuffle.  The running
+// k_attn.  A CTA owns 256 query rows of one document and head, two tiles of 128 that share every key tile.  Products run on
+// tcgen05 with the scores, the probabilities (left operand of the second product) and the running output in tensor memory;
+// a thread has a row, so the softmax needs no shuffle.  The running
 // maximum is only renewed, and the output only rescaled, when it has grown by more than 2^8: the probabilities then lie
 // within 2^8, and the sums lose nothing to it.  Probabilities are rounded to the operands' 16-bit type for the second
 // product (its operand can be no wider); the sums are of the unrounded ones, in fp32.
@@ -49,20 +49,29 @@ template <typename T> constexpr float kLift = 0.0f;
 template <> constexpr float kLift<__half> = 7.0f;   // fp16 probabilities are kept times 2^7: 2^15 at most, and 7 more
                                                     // binades before they turn subnormal
 
+// A softmax thread has 64 columns of a row: what 96 registers hold, so that 16 softmax warps fit a SM, whose waits hide one
+// another.  Heads up to 64: key tiles of 64, one warpgroup a row tile, two CTAs a SM (tensor memory: 2 (64 + 64) = 256 columns
+// each), four row tiles at different points of their way.  Wider heads leave tensor memory for one CTA: key tiles of 128,
+// two warpgroups a row tile, 2 (128 + 128) = 512 columns.
 template <int DP>
 struct Fwd {
-    static constexpr bool kSep = DP == 64;     // probabilities beside the scores: 2 (128 + 64 + 64) = 512 columns
-    static constexpr int kTile = 128 * DP * 2; // a tile of 128 rows
+    static constexpr int kHalves = DP == 64 ? 1 : 2;
+    static constexpr int kCtas = DP == 64 ? 2 : 1;
+    static constexpr int kBT = 64 * kHalves;                    // keys of a tile
+    static constexpr int kThreads = 256 * kHalves + 64;         // softmax, then the loader and the MMA issuer
+    static constexpr int kLoader = 8 * kHalves, kIssuer = kLoader + 1;
+    static constexpr int kQTile = 128 * DP * 2, kQ = 2 * kQTile;
+    static constexpr int kStrip = kBT * 128, kTile = kStrip * (DP / 64);
     static constexpr int kStages = DP == 64 ? 4 : 2;
-    static constexpr int kQ = 2 * kTile;
     static constexpr int kBars = kQ + 2 * kStages * kTile;
-    static constexpr int kSmem = kBars + 1024;
-    static constexpr uint32_t S(int w) { return 128 * w; }
-    static constexpr uint32_t P(int w) { return kSep ? 256 + 64 * w : 128 * w + 64; }   // written from the end
-    static constexpr uint32_t O(int w) { return kSep ? 384 + 64 * w : 256 + 128 * w; }
+    static constexpr int kTops = kBars + 1024; // what the two warpgroups of a row tile tell each other: [2][2][2][128]
+    static constexpr int kSmem = kTops + (kHalves == 2 ? 4096 : 0);
+    static constexpr uint32_t kCols = DP == 64 ? 256 : 512;
+    static constexpr uint32_t S(int w) { return kBT * w; }
+    static constexpr uint32_t P(int w, int h) { return kBT * w + 64 * h + 32; }   // over its own columns, from the end
+    static constexpr uint32_t O(int w) { return 2 * kBT + DP * w; }
 };
 
-constexpr int kFwdThreads = 384;               // two softmax warpgroups, then the loader, the MMA issuer and two spare warps
 constexpr int kItems = 4;                      // items described ahead
 
 // One item of a CTA's walk: 256 query rows of a document and head.
@@ -72,7 +81,7 @@ struct Item {
 };
 
 template <typename T, int DP, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(kFwdThreads, 1)
+__global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
     k_attn(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
            const __grid_constant__ CUtensorMap mv, const __grid_constant__ Attn a, T* __restrict__ o, int64_t o_tok,
            int64_t o_head, float* __restrict__ lse) {
@@ -92,7 +101,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     uint64_t* const p_full = s_full + 2;
     uint64_t* const pv_done = p_full + 2;
     uint64_t* const o_read = pv_done + 2;
-    uint64_t* const item_full = o_read + 2;
+    uint64_t* const told = o_read + 2;
+    uint64_t* const item_full = told + 2;
     uint64_t* const item_empty = item_full + kItems;
     uint64_t* const drain = item_empty + kItems;
     Item* const items = reinterpret_cast<Item*>(drain + 1);
@@ -105,9 +115,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
             mbar_init(q_full + i, 1);
             mbar_init(q_empty + i, 1);
             mbar_init(s_full + i, 1);
-            mbar_init(p_full + i, 128);
+            mbar_init(p_full + i, 128 * C::kHalves);
             mbar_init(pv_done + i, 1);
-            mbar_init(o_read + i, 128);
+            mbar_init(o_read + i, 128 * C::kHalves);
+            mbar_init(told + i, 256);
         }
         for (int i = 0; i < C::kStages; ++i) {
             mbar_init(k_full + i, 1);
@@ -117,14 +128,14 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         }
         for (int i = 0; i < kItems; ++i) {
             mbar_init(item_full + i, 1);
-            mbar_init(item_empty + i, 9);            // eight softmax warps and the issuer
+            mbar_init(item_empty + i, 8 * C::kHalves + 1);           // the softmax warps and the issuer
         }
         mbar_init(next_bar, 1);
         mbar_init(drain, 1);
         *abort_flag = 0;
         fence_mbar_init();
     }
-    if (warp == 9) tmem_alloc(slot, 512);
+    if (warp == C::kIssuer) tmem_alloc(slot, C::kCols);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -141,9 +152,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         return true;
     };
 
-    if (warp >= 8) {
-        reg_dealloc<kAttnRegsFew>();
-        if (warp == 8) {
+    if (warp >= C::kLoader) {
+        if (warp == C::kLoader) {
             // ------------------------------------------------------------------------------------------------ loads
             bool ok = true;
             uint32_t it = 0, kt = 0, qc[2] = {0, 0};
@@ -160,8 +170,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                     // later rows of a causal document reach further: they start first
                     x.r0 = 256 * (a.causal ? (x.sp.lq + 255) / 256 - 1 - tile : tile);
                     if (x.r0 < 0) x.r0 = 1 << 30;                     // offsets that had to be cut: no such rows
-                    x.n0 = x.r0 < x.sp.lq ? (key_end(a, x.sp, x.r0 + 128) + 127) / 128 : 0;
-                    x.n1 = x.r0 + 128 < x.sp.lq ? (key_end(a, x.sp, x.r0 + 256) + 127) / 128 : 0;
+                    x.n0 = x.r0 < x.sp.lq ? (key_end(a, x.sp, x.r0 + 128) + C::kBT - 1) / C::kBT : 0;
+                    x.n1 = x.r0 + 128 < x.sp.lq ? (key_end(a, x.sp, x.r0 + 256) + C::kBT - 1) / C::kBT : 0;
                     const int at = it % kItems;
                     ok = __all_sync(0xffffffffu, mbar_wait(item_empty + at, ((it / kItems) & 1u) ^ 1u, abort_flag));
                     if (!ok) break;
@@ -173,10 +183,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                             if ((w ? x.n1 : x.n0) == 0) continue;
                             ok = mbar_wait(q_empty + w, (qc[w] & 1u) ^ 1u, abort_flag);
                             if (!ok) break;
-                            mbar_arrive_expect_tx(q_full + w, C::kTile);
+                            mbar_arrive_expect_tx(q_full + w, C::kQTile);
 #pragma unroll
                             for (int c = 0; c < DP / 64; ++c)
-                                tma_tile3d(smem_u32(smem + w * C::kTile + c * 16384), &mq, 64 * c, x.head, x.sp.q0 + x.r0 + 128 * w, q_full + w);
+                                tma_tile3d(smem_u32(smem + w * C::kQTile + c * 16384), &mq, 64 * c, x.head, x.sp.q0 + x.r0 + 128 * w, q_full + w);
                             ++qc[w];
                         }
                         for (int j = 0; j < nmax && ok; ++j, ++kt) {
@@ -187,13 +197,13 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                             mbar_arrive_expect_tx(k_full + st, C::kTile);
 #pragma unroll
                             for (int c = 0; c < DP / 64; ++c)
-                                tma_tile3d(smem_u32(sk + st * C::kTile + c * 16384), &mk, 64 * c, kvh, x.sp.k0 + 128 * j, k_full + st);
+                                tma_tile3d(smem_u32(sk + st * C::kTile + c * C::kStrip), &mk, 64 * c, kvh, x.sp.k0 + C::kBT * j, k_full + st);
                             ok = mbar_wait(v_empty + st, ph, abort_flag);
                             if (!ok) break;
                             mbar_arrive_expect_tx(v_full + st, C::kTile);
 #pragma unroll
                             for (int c = 0; c < DP / 64; ++c)
-                                tma_tile3d(smem_u32(sv + st * C::kTile + c * 16384), &mv, 64 * c, kvh, x.sp.k0 + 128 * j, v_full + st);
+                                tma_tile3d(smem_u32(sv + st * C::kTile + c * C::kStrip), &mv, 64 * c, kvh, x.sp.k0 + C::kBT * j, v_full + st);
                         }
                     }
                     ++it;
@@ -218,10 +228,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                 *abort_flag = 1;
                 flag(a.status, PMG_ERR_TIMEOUT);
             }
-        } else if (warp == 9) {
+        } else {
             // ------------------------------------------------------------------------------------------------ MMAs
             const int ksteps = (a.D + 15) / 16;
-            const uint32_t id_qk = idesc16(Elem<T>::kFmt, 128, 128, false, false);
+            const uint32_t id_qk = idesc16(Elem<T>::kFmt, 128, C::kBT, false, false);
             const uint32_t id_pv = idesc16(Elem<T>::kFmt, 128, ksteps * 16, false, true);
             const uint32_t lead = elect_one();
             bool ok = true;
@@ -237,12 +247,12 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                     if (j == 0 && !wait(q_full + w, qc[w])) return false;
                     if (!wait(k_full + st, t / C::kStages)) return false;
                     tc_fence_after();
-                    const uint32_t qa = desc_lo(smem_u32(smem + w * C::kTile), 16), kb = desc_lo(smem_u32(sk + st * C::kTile), 16);
+                    const uint32_t qa = desc_lo(smem_u32(smem + w * C::kQTile), 16), kb = desc_lo(smem_u32(sk + st * C::kTile), 16);
 #pragma unroll
                     for (int s = 0; s < DP / 16; ++s)
                         if (s < ksteps) {
-                            const uint32_t at = ((s >> 2) * 16384 + (s & 3) * 32) >> 4;
-                            mma16(lead, tmem + C::S(w), qa + at, kb + at, id_qk, s > 0);
+                            const uint32_t in = (s & 3) * 2;
+                            mma16(lead, tmem + C::S(w), qa + (s >> 2) * 1024 + in, kb + (s >> 2) * (C::kStrip / 16) + in, id_qk, s > 0);
                         }
                     mma_commit_if(lead, s_full + w);
                     if (w == 1 || j >= n[1]) mma_commit_if(lead, k_empty + st);     // the tile's last reader
@@ -252,21 +262,21 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                 auto pv = [&](int w, int j) -> bool {
                     const uint32_t t = kt + j, st = t % C::kStages;
                     if (!wait(v_full + st, t / C::kStages)) return false;
-                    const int valid = x.sp.lk - 128 * j;
-                    if (valid < 128 && (w == 0 || n[0] <= j)) {
+                    const int valid = x.sp.lk - C::kBT * j;
+                    if (valid < C::kBT && (w == 0 || n[0] <= j)) {
                         // rows behind the document's last key: whatever lies there must not reach a sum (0 * NaN)
                         for (int c = 0; c < DP / 64; ++c)
-                            for (int b = valid * 128 + lane * 16; b < 16384; b += 512)
-                                *reinterpret_cast<uint4*>(sv + st * C::kTile + c * 16384 + b) = make_uint4(0, 0, 0, 0);
+                            for (int b = valid * 128 + lane * 16; b < C::kStrip; b += 512)
+                                *reinterpret_cast<uint4*>(sv + st * C::kTile + c * C::kStrip + b) = make_uint4(0, 0, 0, 0);
                         fence_proxy_async();
                         __syncwarp();
                     }
                     if (j == 0 && !wait(o_read + w, qc[w] ^ 1u)) return false;    // the last item's output is out
                     tc_fence_after();
-                    const uint32_t vb = desc_lo(smem_u32(sv + st * C::kTile), 16384);
+                    const uint32_t vb = desc_lo(smem_u32(sv + st * C::kTile), C::kStrip);
 #pragma unroll
-                    for (int s = 0; s < 8; ++s)
-                        mma16_ts(lead, tmem + C::O(w), tmem + C::P(w) + 8 * s, vb + s * 128, id_pv, j > 0 || s > 0);
+                    for (int s = 0; s < C::kBT / 16; ++s)
+                        mma16_ts(lead, tmem + C::O(w), tmem + C::P(w, s >> 2) + 8 * (s & 3), vb + s * 128, id_pv, j > 0 || s > 0);
                     mma_commit_if(lead, pv_done + w);
                     if (w == 1 || j >= n[1]) mma_commit_if(lead, v_empty + st);
                     return true;
@@ -274,14 +284,13 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                 for (int w = 0; w < 2 && ok; ++w)
                     if (n[w] > 0) ok = qk(w, 0);
                 for (int j = 0; j < nmax && ok; ++j) {
-                    // Each half on its own: the next scores and this tile's product follow when its softmax is through,
-                    // while the other half's softmax runs.  Scores first where the probabilities leave them room.
+                    // Each row tile on its own: its product and its next scores (over its probabilities) follow when its
+                    // softmax is through, while the other's runs.
                     for (int w = 0; w < 2 && ok; ++w) {
                         if (j >= n[w]) continue;
                         ok = wait(p_full + w, sc[w] + j);
-                        if (ok && C::kSep && j + 1 < n[w]) ok = qk(w, j + 1);
                         if (ok) ok = pv(w, j);
-                        if (ok && !C::kSep && j + 1 < n[w]) ok = qk(w, j + 1);
+                        if (ok && j + 1 < n[w]) ok = qk(w, j + 1);
                     }
                 }
                 if (!ok) break;
@@ -302,13 +311,26 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         }
     } else {
         // ------------------------------------------------------------------------------------------------- softmax
-        reg_alloc<kAttnRegsMany>();
-        const int w = warp >> 2;
+        // Where two warpgroups share a row tile they tell each other their maxima (and at the end their sums) through shared
+        // memory, take the same maximum, and rescale and store half the output each.
+        const int w = (warp >> 2) / C::kHalves, h = (warp >> 2) % C::kHalves;
+        constexpr int kOut = DP / C::kHalves;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t ts = tmem + lanes + C::S(w), tp = tmem + lanes + C::P(w), to = tmem + lanes + C::O(w);
+        const uint32_t ts = tmem + lanes + C::S(w) + 64 * h, tp = tmem + lanes + C::P(w, h), to = tmem + lanes + C::O(w) + h * kOut;
+        float* const tops = reinterpret_cast<float*>(smem + C::kTops) + w * 256 + (warp & 3) * 32 + lane;
         const float c = BIAS ? 1.0f : (CAP ? a.cap2 : a.scale2);          // scores to units of log 2
-        uint32_t sc = 0;
+        uint32_t sc = 0, xc = 0;                                          // tiles; exchanges
         bool ok = true;
+        auto tell = [&](float v) {
+            tops[(xc & 1) * 512 + h * 128] = v;
+            mbar_arrive(told + w);
+        };
+        auto hear = [&](float& v) {                                       // false: gave up
+            if (!__all_sync(0xffffffffu, mbar_wait(told + w, xc & 1u, abort_flag))) return false;
+            v = tops[(xc & 1) * 512 + (h ^ 1) * 128];
+            ++xc;
+            return true;
+        };
         Item x;
         for (uint32_t it = 0;; ++it) {
             ok = next_item(it, x);
@@ -325,54 +347,54 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                 TOK_WAIT(s_full + w, sc & 1u);
                 if (!ok) break;
                 tc_fence_after();
-                // Two passes over the scores, 32 columns at a time, the next on their way: first the maximum, then,
-                // backwards, the probabilities.  Held whole, a row of 128 left the scheduler no registers to overlap
-                // anything with.
-                const int j0 = 128 * j;
-                const bool masked = j0 + 127 > warp_min;
-                float s[2][32];
+                const int j0 = C::kBT * j + 64 * h;
+                // 32 columns at a time: the first are read again for their probabilities, which costs less than the
+                // registers to keep them.
+                float s[32];
                 bool fast = false;                        // the cap's polynomial serves (tanh_fast)
-                auto fetch = [&](int q) { tmem_ld32(ts + 32 * q, reinterpret_cast<uint32_t*>(s[q & 1])); };
-                auto score = [&](int q) {                 // raw products to what the softmax takes
-                    float (&x)[32] = s[q & 1];
-                    if (CAP) tanh_scores<32>(a, x, BIAS ? tanh_fast(a, largest<32>(x)) : fast);
-                    if (BIAS) bias_scores<32>(x, CAP ? a.cap2 : a.scale2, slope, place - (float)(j0 + 32 * q));
+                const bool masked = j0 + 63 > warp_min;
+                auto fetch = [&](int q) {
+                    tmem_ld32(ts + 32 * q, reinterpret_cast<uint32_t*>(s));
+                    tmem_wait_ld();
+                };
+                auto mask = [&](int q) {
                     if (masked) {
 #pragma unroll
                         for (int k = 0; k < 32; ++k)
-                            if (j0 + 32 * q + k > lim) x[k] = -INFINITY;
+                            if (j0 + 32 * q + k > lim) s[k] = -INFINITY;
                     }
                 };
+                auto score = [&](int q) {                 // raw products to what the softmax takes
+                    if (CAP) tanh_scores<32>(a, s, BIAS ? tanh_fast(a, largest<32>(s)) : fast);
+                    if (BIAS) bias_scores<32>(s, CAP ? a.cap2 : a.scale2, slope, place - (float)(j0 + 32 * q));
+                    mask(q);
+                };
                 float top = -INFINITY, top2 = -INFINITY, big = 0.0f;
-                fetch(0);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    tmem_wait_ld();
-                    if (q < 3) fetch(q + 1);
-                    float (&x)[32] = s[q & 1];
-                    if (CAP && !BIAS) big = fmaxf(big, largest<32>(x));
-                    if (BIAS || (q == 3 && !CAP)) {
-                        score(q);
-                    } else if (masked) {                  // a cap keeps the order: the maximum is capped at the end
-#pragma unroll
-                        for (int k = 0; k < 32; ++k)
-                            if (j0 + 32 * q + k > lim) x[k] = -INFINITY;
-                    }
+                for (int q = 0; q < 2; ++q) {
+                    fetch(q);
+                    if (CAP && !BIAS) big = fmaxf(big, largest<32>(s));
+                    if (BIAS) score(q);
+                    else mask(q);                         // a cap keeps the order: the maximum is capped afterwards
 #pragma unroll
                     for (int k = 0; k < 32; k += 4) {
-                        top = max3(top, x[k], x[k + 1]);
-                        top2 = max3(top2, x[k + 2], x[k + 3]);
+                        top = max3(top, s[k], s[k + 1]);
+                        top2 = max3(top2, s[k + 2], s[k + 3]);
                     }
                 }
                 top = fmaxf(top, top2);
-                fetch(2);
+                if (C::kHalves == 2) tell(top);
                 if (CAP && !BIAS) {
                     fast = tanh_fast(a, big);
-                    if (top > -INFINITY) top = tanh_raw(a, top);
-                    score(3);
+                    score(1);
                 }
-                if (j > 0) TOK_WAIT(pv_done + w, (sc - 1) & 1u);          // frees the probabilities and the output
-                if (!ok) break;
+                if (C::kHalves == 2) {
+                    float other = 0.0f;
+                    ok = hear(other);
+                    if (!ok) break;
+                    top = fmaxf(top, other);
+                }
+                if (CAP && !BIAS && top > -INFINITY) top = tanh_raw(a, top);
                 if (j == 0) {
                     m = top;
                 } else if (__any_sync(0xffffffffu, (top - m) * c > kGrow)) {
@@ -383,7 +405,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                     sum2 = mul2(sum2, pack2(f, f));
                     tc_fence_after();
 #pragma unroll
-                    for (int q = 0; q < DP / 16; ++q) {
+                    for (int q = 0; q < kOut / 16; ++q) {
                         uint32_t v[16];
                         tmem_ld16(to + 16 * q, v);
 #pragma unroll
@@ -394,11 +416,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                 const float base = m == -INFINITY ? 0.0f : -m * c + kLift<T>;
                 const uint64_t c2 = pack2(c, c), b2 = pack2(base, base);
                 auto exps = [&](int q) {
-                    float (&x)[32] = s[q & 1];
                     uint32_t p[16];
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        const uint64_t y = fma2(pack2(x[2 * k], x[2 * k + 1]), c2, b2);
+                        const uint64_t y = fma2(pack2(s[2 * k], s[2 * k + 1]), c2, b2);
                         const uint64_t e = takes_poly(k, CAP ? 0 : 5) ? ex2_poly(y) : ex2_pair(y);
                         if (k & 1) sum2 = add2(sum2, e);
                         else sum = add2(sum, e);
@@ -407,38 +428,39 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                     }
                     tmem_st16(tp + 16 * q, p);
                 };
-#pragma unroll
-                for (int q = 3; q >= 0; --q) {
-                    if (q < 3) {
-                        tmem_wait_ld();
-                        if (q > 0) fetch(q - 1);
-                        score(q);
-                    }
-                    exps(q);
-                }
+                exps(1);
+                fetch(0);
+                score(0);
+                exps(0);
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(p_full + w);
             }
             if (!ok) break;
             const float2 s2 = unpack2(add2(sum, sum2));
-            const float total = s2.x + s2.y;
+            float total = s2.x + s2.y, rest = 0.0f;
+            if (C::kHalves == 2) {
+                tell(total);
+                ok = hear(rest);
+                if (!ok) break;
+                total = h ? rest + total : total + rest;
+            }
             if (tiles_k > 0) TOK_WAIT(pv_done + w, (sc - 1) & 1u);
             if (!ok) break;
             tc_fence_after();
             const int64_t token = x.sp.q0 + (int64_t)i;
             const bool mine = i < x.sp.lq, none = total == 0.0f;         // rows that see no key give zero
             const float inv = none ? 0.0f : 1.0f / total;
-            if (mine) lse[(int64_t)x.head * a.Tq + token] = none ? -INFINITY : (m * c + log2f(total) - kLift<T>) * kLn2;
-            T* row = o + token * o_tok + x.head * o_head;
+            if (mine && h == 0) lse[(int64_t)x.head * a.Tq + token] = none ? -INFINITY : (m * c + log2f(total) - kLift<T>) * kLn2;
+            T* row = o + token * o_tok + x.head * o_head + h * kOut;
 #pragma unroll
-            for (int q = 0; q < DP / 32; ++q) {
+            for (int q = 0; q < kOut / 32; ++q) {
                 float v[32];
                 if (tiles_k > 0) {
                     tmem_ld32(to + 32 * q, reinterpret_cast<uint32_t*>(v));
                     tmem_wait_ld();
                 }
-                if (q == DP / 32 - 1 && tiles_k > 0) {
+                if (q == kOut / 32 - 1 && tiles_k > 0) {
                     tc_fence_before();
                     mbar_arrive(o_read + w);
                 }
@@ -448,7 +470,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
                 }
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    if (mine && 32 * q + 8 * k < a.D)
+                    if (mine && h * kOut + 32 * q + 8 * k < a.D)
                         *reinterpret_cast<uint4*>(row + 32 * q + 8 * k) =
                             make_uint4(Elem<T>::pack(v[8 * k] * inv, v[8 * k + 1] * inv),
                                        Elem<T>::pack(v[8 * k + 2] * inv, v[8 * k + 3] * inv),
@@ -464,9 +486,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == C::kIssuer) {
         tc_fence_after();
-        tmem_dealloc(tmem, 512);
+        tmem_dealloc(tmem, C::kCols);
     }
 }
 
@@ -856,12 +878,12 @@ int run(const Attn& a, const Call& c, cudaStream_t s) {
     if (rc != PMG_OK) return rc;
     CUtensorMap mq, mk, mv;
     int e = head_map(&mq, c.q.p, c.q.tok, c.q.head, a.Tq, a.Hq, a.D, 128);
-    if (e == PMG_OK) e = head_map(&mk, c.k.p, c.k.tok, c.k.head, std::max<int64_t>(a.Tk, 1), a.Hk, a.D, 128);
-    if (e == PMG_OK) e = head_map(&mv, c.v.p, c.v.tok, c.v.head, std::max<int64_t>(a.Tk, 1), a.Hk, a.D, 128);
+    if (e == PMG_OK) e = head_map(&mk, c.k.p, c.k.tok, c.k.head, std::max<int64_t>(a.Tk, 1), a.Hk, a.D, C::kBT);
+    if (e == PMG_OK) e = head_map(&mv, c.v.p, c.v.tok, c.v.head, std::max<int64_t>(a.Tk, 1), a.Hk, a.D, C::kBT);
     if (e != PMG_OK) return e;
     const int64_t blocks = (a.Tq / 256 + a.docs) * a.Hq;
     if (blocks > INT32_MAX) return PMG_ERR_UNSUPPORTED;
-    k_attn<T, DP, CAP, BIAS><<<(int)blocks, kFwdThreads, C::kSmem, s>>>(mq, mk, mv, a, static_cast<T*>(c.o), c.o_tok, c.o_head, c.lse);
+    k_attn<T, DP, CAP, BIAS><<<(int)blocks, C::kThreads, C::kSmem, s>>>(mq, mk, mv, a, static_cast<T*>(c.o), c.o_tok, c.o_head, c.lse);
     PMG_LAUNCH_CHECK();
     return PMG_OK;
 }

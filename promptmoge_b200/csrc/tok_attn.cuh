@@ -178,14 +178,6 @@ __device__ __forceinline__ uint64_t ex2_poly(uint64_t x) {
 // function unit (16 a pair) finish together.  A cap leaves the fp32 pipe no room.
 __device__ __forceinline__ constexpr bool takes_poly(int k, int share) { return (k * share) % 16 < share; }
 
-// Registers move from the loading and issuing warps to the two softmax warpgroups: 2 * 208 + 88 = 3 * 168, what the block
-// of three warpgroups was launched with.
-constexpr int kAttnRegsMany = 208, kAttnRegsFew = 88;
-template <int N>
-__device__ __forceinline__ void reg_alloc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void reg_dealloc() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-
 // Claims a block of this grid that has not started yet (its index becomes this CTA's next work); the 16-byte answer lands
 // in `slot` and completes `bar`.
 __device__ __forceinline__ void claim_block(uint64_t* slot, uint64_t* bar) {
