@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
     // Every warp but the loader reads the items in order through this.
     auto next_item = [&](uint32_t it, Item& x) -> bool {
         const int at = it % kItems;
-        if (!__all_sync(0xffffffffu, mbar_wait(item_full + at, (it / kItems) & 1u, abort_flag))) return false;
+        if (!__all_sync(0xffffffffu, wait_bar(item_full + at, (it / kItems) & 1u, abort_flag))) return false;
         x = items[at];
         __syncwarp();
         if (lane == 0) mbar_arrive(item_empty + at);
@@ -163,7 +163,8 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
                 Item x;
                 x.doc = -1;
                 int tile = 0;
-                const bool found = find_tile(a.cu_q, a.docs, 256, block / a.Hq, &x.doc, &tile);
+                const bool found = a.causal ? find_level(a.cu_q, a.docs, 256, block / a.Hq, &x.doc, &tile)
+                                            : find_tile(a.cu_q, a.docs, 256, block / a.Hq, &x.doc, &tile);
                 if (found) {
                     x.sp = span_of(a, x.doc);
                     x.head = block % a.Hq;
@@ -173,7 +174,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
                     x.n0 = x.r0 < x.sp.lq ? (key_end(a, x.sp, x.r0 + 128) + C::kBT - 1) / C::kBT : 0;
                     x.n1 = x.r0 + 128 < x.sp.lq ? (key_end(a, x.sp, x.r0 + 256) + C::kBT - 1) / C::kBT : 0;
                     const int at = it % kItems;
-                    ok = __all_sync(0xffffffffu, mbar_wait(item_empty + at, ((it / kItems) & 1u) ^ 1u, abort_flag));
+                    ok = __all_sync(0xffffffffu, wait_bar(item_empty + at, ((it / kItems) & 1u) ^ 1u, abort_flag));
                     if (!ok) break;
                     if (lane == 0) {
                         items[at] = x;
@@ -181,7 +182,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
                         const int kvh = x.head / a.group, nmax = max(x.n0, x.n1);
                         for (int w = 0; w < 2 && ok; ++w) {
                             if ((w ? x.n1 : x.n0) == 0) continue;
-                            ok = mbar_wait(q_empty + w, (qc[w] & 1u) ^ 1u, abort_flag);
+                            ok = wait_bar(q_empty + w, (qc[w] & 1u) ^ 1u, abort_flag);
                             if (!ok) break;
                             mbar_arrive_expect_tx(q_full + w, C::kQTile);
 #pragma unroll
@@ -192,13 +193,13 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
                         for (int j = 0; j < nmax && ok; ++j, ++kt) {
                             const int st = kt % C::kStages;
                             const uint32_t ph = ((kt / C::kStages) & 1u) ^ 1u;
-                            ok = mbar_wait(k_empty + st, ph, abort_flag);
+                            ok = wait_bar(k_empty + st, ph, abort_flag);
                             if (!ok) break;
                             mbar_arrive_expect_tx(k_full + st, C::kTile);
 #pragma unroll
                             for (int c = 0; c < DP / 64; ++c)
                                 tma_tile3d(smem_u32(sk + st * C::kTile + c * C::kStrip), &mk, 64 * c, kvh, x.sp.k0 + C::kBT * j, k_full + st);
-                            ok = mbar_wait(v_empty + st, ph, abort_flag);
+                            ok = wait_bar(v_empty + st, ph, abort_flag);
                             if (!ok) break;
                             mbar_arrive_expect_tx(v_full + st, C::kTile);
 #pragma unroll
@@ -210,7 +211,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
                     ok = __shfl_sync(0xffffffffu, (int)ok, 0);
                     if (!ok) break;
                 }
-                ok = __all_sync(0xffffffffu, mbar_wait(next_bar, claim & 1u, abort_flag));
+                ok = __all_sync(0xffffffffu, wait_bar(next_bar, claim & 1u, abort_flag));
                 if (!ok) break;
                 block = claimed_block(next_slot);
                 __syncwarp();
@@ -218,7 +219,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
             }
             if (ok) {
                 const int at = it % kItems;
-                ok = __all_sync(0xffffffffu, mbar_wait(item_empty + at, ((it / kItems) & 1u) ^ 1u, abort_flag));
+                ok = __all_sync(0xffffffffu, wait_bar(item_empty + at, ((it / kItems) & 1u) ^ 1u, abort_flag));
                 if (ok && lane == 0) {
                     items[at].doc = -1;
                     mbar_arrive(item_full + at);
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
             const uint32_t lead = elect_one();
             bool ok = true;
             uint32_t kt = 0, qc[2] = {0, 0}, sc[2] = {0, 0};    // key tiles; items and tiles of each half so far
-            auto wait = [&](uint64_t* bar, uint32_t ph) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, ph & 1u, abort_flag)); };
+            auto wait = [&](uint64_t* bar, uint32_t ph) { return (bool)__all_sync(0xffffffffu, wait_bar(bar, ph & 1u, abort_flag)); };
             Item x;
             for (uint32_t it = 0;; ++it) {
                 ok = next_item(it, x);
@@ -326,7 +327,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
             mbar_arrive(told + w);
         };
         auto hear = [&](float& v) {                                       // false: gave up
-            if (!__all_sync(0xffffffffu, mbar_wait(told + w, xc & 1u, abort_flag))) return false;
+            if (!__all_sync(0xffffffffu, wait_bar(told + w, xc & 1u, abort_flag))) return false;
             v = tops[(xc & 1) * 512 + (h ^ 1) * 128];
             ++xc;
             return true;
@@ -420,7 +421,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
                         const uint64_t y = fma2(pack2(s[2 * k], s[2 * k + 1]), c2, b2);
-                        const uint64_t e = takes_poly(k, CAP ? 0 : 5) ? ex2_poly(y) : ex2_pair(y);
+                        const uint64_t e = takes_poly(k, CAP ? 0 : 4) ? ex2_poly(y) : ex2_pair(y);
                         if (k & 1) sum2 = add2(sum2, e);
                         else sum = add2(sum, e);
                         const float2 f = unpack2(e);

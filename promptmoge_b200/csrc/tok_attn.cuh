@@ -13,7 +13,7 @@
 // A whole warp's bounded wait; clears `ok` where any lane gave up.
 #define TOK_WAIT(bar, parity)                                                                        \
     do {                                                                                             \
-        if (!__all_sync(0xffffffffu, mbar_wait((bar), (parity), abort_flag))) { ok = false; break; } \
+        if (!__all_sync(0xffffffffu, wait_bar((bar), (parity), abort_flag))) { ok = false; break; } \
     } while (0)
 
 namespace pmg {
@@ -81,6 +81,30 @@ __device__ __forceinline__ bool find_tile(const int32_t* cu, int docs, int rows,
         t -= total;
     }
     return false;
+}
+
+// The same tiles level by level: the first tile of every document, then the second of those that have one, and so on.  A
+// causal document's tiles shrink from one end to the other; taken in this order from that end, what a GPU starts last is
+// small, whatever document it belongs to.
+__device__ __forceinline__ bool find_level(const int32_t* cu, int docs, int rows, int t, int* doc, int* level) {
+    const int lane = threadIdx.x & 31;
+    for (int e = 0;; ++e) {
+        int found = 0;
+        for (int d0 = 0; d0 < docs; d0 += 32) {
+            const int d = d0 + lane;
+            const int n = d < docs ? max(0, cu[d + 1] - cu[d]) : 0;
+            const uint32_t has = __ballot_sync(0xffffffffu, (n + rows - 1) / rows > e);
+            const int count = __popc(has);
+            if (t < count) {
+                *doc = d0 + __fns(has, 0, t + 1);
+                *level = e;
+                return true;
+            }
+            t -= count;
+            found += count;
+        }
+        if (found == 0) return false;
+    }
 }
 
 // tanh(scale s / cap) of a raw product s as 1 - 2 / (e^(2 s scale / cap) + 1).  The hardware's tanh is

@@ -216,7 +216,7 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
             if (KEYS) fetch(t, bh);
             for (int i = 0; i < total; ++i) {
                 const int st = i % C::kStages;
-                ok = __all_sync(0xffffffffu, mbar_wait(b.b_empty + st, ((i / C::kStages) & 1u) ^ 1u, abort_flag));
+                ok = __all_sync(0xffffffffu, wait_bar(b.b_empty + st, ((i / C::kStages) & 1u) ^ 1u, abort_flag));
                 if (!ok) break;
                 const int brow = (KEYS ? sp.q0 : sp.k0) + C::kBT * t;
                 if (lane == 0) {
@@ -255,7 +255,7 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
         const uint32_t id_s = idesc16(Elem<T>::kFmt, 128, C::kBT, false, false);
         const uint32_t id_o = idesc16(Elem<T>::kFmt, 128, ksteps * 16, false, true);
         bool ok = true;
-        auto wait = [&](uint64_t* bar, uint32_t ph) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, ph, abort_flag)); };
+        auto wait = [&](uint64_t* bar, uint32_t ph) { return (bool)__all_sync(0xffffffffu, wait_bar(bar, ph, abort_flag)); };
         auto stage = [&](int i) { return smem + C::kStream + (i % C::kStages) * 2 * C::kPart; };
         // a streamed tile has landed; rows behind the document's last must not reach a sum over rows (0 * NaN)
         int lt = t0;                                    // tile of the next call
@@ -517,7 +517,15 @@ __global__ void __launch_bounds__(Bwd<DP>::kThreads, Bwd<DP>::kCtas)
     pdl_begin();
     if (warp == 4 * C::kGroups) {
         int doc = -1, tile = 0;
-        const bool found = find_tile(keys ? g.a.cu_k : g.a.cu_q, g.a.docs, 128, block / (keys ? g.a.Hk : g.a.Hq), &doc, &tile);
+        const int32_t* cu = keys ? g.a.cu_k : g.a.cu_q;
+        const int t = block / (keys ? g.a.Hk : g.a.Hq);
+        bool found;
+        if (g.a.causal) {                // the first keys are seen by most queries, the last queries see most keys
+            found = find_level(cu, g.a.docs, 128, t, &doc, &tile);
+            if (found && !keys) tile = (max(0, cu[doc + 1] - cu[doc]) + 127) / 128 - 1 - tile;
+        } else {
+            found = find_tile(cu, g.a.docs, 128, t, &doc, &tile);
+        }
         if (lane == 0) {
             where[0] = found ? doc : -1;
             where[1] = tile;
