@@ -49,6 +49,9 @@ template <typename T> constexpr float kLift = 0.0f;
 template <> constexpr float kLift<__half> = 7.0f;   // fp16 probabilities are kept times 2^7: 2^15 at most, and 7 more
                                                     // binades before they turn subnormal
 
+template <typename T> constexpr float kUnlift = 1.0f;
+template <> constexpr float kUnlift<__half> = 0.0078125f;
+
 // A softmax thread has 64 columns of a row: what 96 registers hold, so that 16 softmax warps fit a SM, whose waits hide one
 // another.  Heads up to 64: key tiles of 64, one warpgroup a row tile, two CTAs a SM (tensor memory: 2 (64 + 64) = 256 columns
 // each), four row tiles at different points of their way.  Wider heads leave tensor memory for one CTA: key tiles of 128,
@@ -452,7 +455,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
             const int64_t token = x.sp.q0 + (int64_t)i;
             const bool mine = i < x.sp.lq, none = total == 0.0f;         // rows that see no key give zero
             const float inv = none ? 0.0f : 1.0f / total;
-            if (mine && h == 0) lse[(int64_t)x.head * a.Tq + token] = none ? -INFINITY : (m * c + log2f(total) - kLift<T>) * kLn2;
+            if (mine && h == 0) lse[(int64_t)x.head * a.Tq + token] = none ? -INFINITY : (m * c + log2f(total * kUnlift<T>)) * kLn2;
             T* row = o + token * o_tok + x.head * o_head + h * kOut;
 #pragma unroll
             for (int q = 0; q < kOut / 32; ++q) {
@@ -619,13 +622,13 @@ __global__ void __launch_bounds__(kFewThreads, Few<DP>::kCtas)
             uint8_t* const kt = smem + st * 2 * C::kPart;
             uint8_t* const vt = kt + C::kPart;
             if (j0 < kend) {
-                float s[2][4] = {};
+                float s[8] = {};                         // row tile x 8 keys, as the instruction leaves them: 4 t + e
 #pragma unroll
                 for (int x = 0; x < DP / 16; ++x) {
                     uint32_t b[4];
                     ldmatrix4<false>(b, smem_u32(kt) + (x >> 2) * 8192 + kr * 128 + ((((x & 3) * 2 + kc) ^ (kr & 7)) << 4));
-                    mma_16n8k16<T>(s[0], qf[x], b[0], b[1]);
-                    mma_16n8k16<T>(s[1], qf[x], b[2], b[3]);
+                    mma_16n8k16<T>(*reinterpret_cast<float (*)[4]>(s), qf[x], b[0], b[1]);
+                    mma_16n8k16<T>(*reinterpret_cast<float (*)[4]>(s + 4), qf[x], b[2], b[3]);
                 }
                 if (j0 + 16 > kend) {
                     // rows behind the last key: whatever lies there must not reach a sum (0 * NaN)
@@ -636,17 +639,17 @@ __global__ void __launch_bounds__(kFewThreads, Few<DP>::kCtas)
                     }
                     __syncwarp();
                 }
+                if (CAP) tanh_scores<8>(a, s, tanh_fast(a, largest<8>(s)));
                 float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int h = e >> 1, key = j0 + 8 * t + 2 * q + (e & 1);
-                        float x = s[t][e];
-                        if (CAP) x = tanh_raw(a, x);
+                        float x = s[4 * t + e];
                         if (BIAS) x = fmaf(-slope[h], fabsf(place[h] - (float)key), x * (CAP ? a.cap2 : a.scale2));
                         x = key <= lim[h] ? x : -INFINITY;
-                        s[t][e] = x;
+                        s[4 * t + e] = x;
                         top[h] = fmaxf(top[h], x);
                     }
                 bool grow = false;
@@ -676,7 +679,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<DP>::kCtas)
                     const float base = m[h] == -INFINITY ? 0.0f : -m[h] * c + kLift<T>;
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
-                        const float e0 = ex2(fmaf(s[t][2 * h], c, base)), e1 = ex2(fmaf(s[t][2 * h + 1], c, base));
+                        const float e0 = ex2(fmaf(s[4 * t + 2 * h], c, base)), e1 = ex2(fmaf(s[4 * t + 2 * h + 1], c, base));
                         l[h] += e0 + e1;
                         p[2 * t + h] = Elem<T>::pack(e0, e1);
                     }
@@ -747,7 +750,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<DP>::kCtas)
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;
         *reinterpret_cast<uint2*>(o + token * o_tok + head * o_head + d) =
             make_uint2(Elem<T>::pack(v.x * inv, v.y * inv), Elem<T>::pack(v.z * inv, v.w * inv));
-        if (d == 0) lse[(int64_t)head * a.Tq + token] = total == 0.0f ? -INFINITY : (top + log2f(total) - kLift<T>) * kLn2;
+        if (d == 0) lse[(int64_t)head * a.Tq + token] = total == 0.0f ? -INFINITY : (top + log2f(total * kUnlift<T>)) * kLn2;
     }
 }
 
@@ -803,7 +806,7 @@ __global__ void __launch_bounds__(256) k_attn_join(const __grid_constant__ Attn 
     if (d < a.D)
         *reinterpret_cast<uint2*>(o + token * o_tok + head * o_head + d) =
             make_uint2(Elem<T>::pack(v.x * inv, v.y * inv), Elem<T>::pack(v.z * inv, v.w * inv));
-    if (x == 0) lse[(int64_t)head * a.Tq + token] = total == 0.0f ? -INFINITY : (top + log2f(total) - kLift<T>) * kLn2;
+    if (x == 0) lse[(int64_t)head * a.Tq + token] = total == 0.0f ? -INFINITY : (top + log2f(total * kUnlift<T>)) * kLn2;
 }
 
 // ----------------------------------------------------------------------------------------------------------------- //
