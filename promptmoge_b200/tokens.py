@@ -226,32 +226,30 @@ def linear_grad(dy, x, w, pre=None, activation: str = "none", bias_grad: bool = 
 # ----------------------------------------------------------------------------------------------------------------- #
 def _heads(t, name, index, dtype, T, H, D):
     """(pointer, token stride, head stride) of [T, H, D]."""
-    if not _plain(t, 3, index, dtype):
-        _dev(t, name, 3, index, (dtype,))
-    if t.shape != (T, H, D):
-        _shape(t, (T, H, D), name)
-    st, sh, _ = t.stride()
-    return t.data_ptr(), st, sh
+    if t.dtype is dtype and t.get_device() == index and t.shape == (T, H, D):
+        st, sh, one = t.stride()
+        if one == 1 or D <= 1:
+            return t.data_ptr(), st, sh
+    _shape(_dev(t, name, 3, index, (dtype,)), (T, H, D), name)
+    return t.data_ptr(), *t.stride()[:2]
 
 
 def _angles(cos, sin, positions, T, D, index):
     """(cos, sin, pairs, places, positions) as the entry points take them."""
-    if not (_plain(cos, 2, index, torch.float32) and _plain(sin, 2, index, torch.float32)):
-        _dev(cos, "cos", 2, index, (torch.float32,))
-        _dev(sin, "sin", 2, index, (torch.float32,))
+    for t, name in ((cos, "cos"), (sin, "sin")):
+        if t.dtype is not torch.float32 or t.get_device() != index or t.dim() != 2:
+            _dev(t, name, 2, index, (torch.float32,))
     places, half = cos.shape
-    if sin.shape != cos.shape:
+    if sin.shape != (places, half):
         _shape(sin, cos.shape, "sin")
     if 2 * half > D:
         raise ValueError(f"cos and sin rotate {2 * half} values of heads of {D}")
-    if half and places > 1 and (cos.stride(0) != half or sin.stride(0) != half):
+    if not (cos.is_contiguous() and sin.is_contiguous()):
         raise ValueError("cos and sin must be contiguous")
     if half and T and places == 0:
         raise ValueError("cos and sin must not be empty")
     if positions is not None:
-        if not _plain(positions, 1, index, torch.int32) or positions.shape[0] != T:
-            _shape(_dev(positions, "positions", 1, index, (torch.int32,)), (T,), "positions")
-        return cos.data_ptr(), sin.data_ptr(), half, places, positions.data_ptr()
+        return cos.data_ptr(), sin.data_ptr(), half, places, _words(positions, "positions", T, index)
     if T > places and half:
         raise ValueError(f"{T} tokens without positions need as many rows of cos and sin, got {places}")
     return cos.data_ptr(), sin.data_ptr(), half, places, None
@@ -260,9 +258,7 @@ def _angles(cos, sin, positions, T, D, index):
 def _weight(w, name, D, index):
     if w is None:
         return None
-    if not _plain(w, 1, index, torch.float32) or w.shape[0] != D:
-        _shape(_dev(w, name, 1, index, (torch.float32,)), (D,), name)
-    return w.data_ptr()
+    return _words(w, name, D, index, torch.float32)
 
 
 def _qk(q, k):
@@ -348,12 +344,17 @@ def _aligned_heads(t, name, T, H, D, index, dt):
 
 
 def _words(t, name, n, index, dtype=torch.int32):
-    """The pointer of a vector of n values, or None."""
-    if t is None:
-        return None
-    if not _plain(t, 1, index, dtype) or t.shape[0] != n:
+    """The pointer of a vector of n values."""
+    if t.dtype is not dtype or t.get_device() != index or t.shape != (n,) or (n > 1 and t.stride(0) != 1):
         _shape(_dev(t, name, 1, index, (dtype,)), (n,), name)
     return t.data_ptr()
+
+
+def _mask_words(cu_q, cu_k, k_len, prefix, slopes, docs, Hq, index):
+    return (_words(cu_q, "cu_q", docs + 1, index), _words(cu_k, "cu_k", docs + 1, index),
+            None if k_len is None else _words(k_len, "k_len", docs, index),
+            None if prefix is None else _words(prefix, "prefix", docs, index),
+            None if slopes is None else _words(slopes, "slopes", Hq, index, torch.float32))
 
 
 def _attention_shapes(q, k):
@@ -361,7 +362,7 @@ def _attention_shapes(q, k):
     index = q.get_device()
     if dt not in _HALF or index < 0 or q.dim() != 3:
         _dev(q, "q", 3, None, _HALF)
-    if not _plain(k, 3, index, dt):
+    if k.dtype is not dt or k.dim() != 3:
         _dev(k, "k", 3, index, (dt,))
     Tq, Hq, D = q.shape
     Tk, Hk, kd = k.shape
@@ -406,14 +407,15 @@ def attention(q, k, v, cu_q, cu_k, max_q: int, max_k: int, scale: float | None =
             return attention(q, k, v, cu_q, cu_k, max_q, max_k, scale, causal, prefix, softcap, slopes, k_len, out)
     docs = _documents(cu_q)
     scale = _score(scale, D, softcap, causal, prefix, max_q, max_k)
-    words = (_words(cu_q, "cu_q", docs + 1, index), _words(cu_k, "cu_k", docs + 1, index),
-             _words(k_len, "k_len", docs, index), _words(prefix, "prefix", docs, index),
-             _words(slopes, "slopes", Hq, index, torch.float32))
-    vh = _aligned_heads(v, "v", Tk, Hk, D, index, dt)
+    words = _mask_words(cu_q, cu_k, k_len, prefix, slopes, docs, Hq, index)
     qh, kh = _aligned_heads(q, "q", Tq, Hq, D, index, dt), _aligned_heads(k, "k", Tk, Hk, D, index, dt)
-    o = q.new_empty((Tq, Hq, D)) if out is None else out
+    vh = _aligned_heads(v, "v", Tk, Hk, D, index, dt)
+    if out is None:
+        o = q.new_empty((Tq, Hq, D))
+        oh = (o.data_ptr(), Hq * D, D)
+    else:
+        o, oh = out, _aligned_heads(out, "out", Tq, Hq, D, index, dt)
     lse = q.new_empty((Hq, Tq), dtype=torch.float32)
-    oh = _aligned_heads(o, "out", Tq, Hq, D, index, dt)
     if Tq:
         need = _query("pmg_attention_workspace_bytes", docs, Hq, Hk, D, max_q, max_k) if max_q * Hq <= 16 * Hk else 0
         ws = q.new_empty(need, dtype=torch.uint8) if need else None
@@ -434,9 +436,7 @@ def attention_grad(do, o, lse, q, k, v, cu_q, cu_k, max_q: int, max_k: int, scal
                                   k_len)
     docs = _documents(cu_q)
     scale = _score(scale, D, softcap, causal, prefix, max_q, max_k)
-    words = (_words(cu_q, "cu_q", docs + 1, index), _words(cu_k, "cu_k", docs + 1, index),
-             _words(k_len, "k_len", docs, index), _words(prefix, "prefix", docs, index),
-             _words(slopes, "slopes", Hq, index, torch.float32))
+    words = _mask_words(cu_q, cu_k, k_len, prefix, slopes, docs, Hq, index)
     if not _plain(lse, 2, index, torch.float32) or lse.shape != (Hq, Tq):
         _shape(_dev(lse, "lse", 2, index, (torch.float32,)), (Hq, Tq), "lse")
     if not lse.is_contiguous():
