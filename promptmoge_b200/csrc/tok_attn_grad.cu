@@ -21,7 +21,7 @@ namespace {
 
 using namespace tok;
 
-constexpr int kStatBlocks = 256;
+constexpr int kStatBlocks = kNumSMs * 4;
 
 struct Grad {
     Attn a;
@@ -46,30 +46,41 @@ __global__ void __launch_bounds__(256)
     const bool in = 8 * gl < D;
     float big_do = 0.0f, big_v = 0.0f;
     const int64_t rows = Tq * Hq;
-    for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < rows; r0 += (int64_t)gridDim.x * kRows) {
-        const int64_t r = r0 + threadIdx.x / G, t = r / Hq;
-        const int h = (int)(r - t * Hq);
-        float dot = 0.0f, sq = 0.0f;
-        if (r < rows && in) {
-            const uint4 x = *reinterpret_cast<const uint4*>(dout + t * do_tok + h * do_head + 8 * gl);
-            const uint4 y = *reinterpret_cast<const uint4*>(o + t * o_tok + h * o_head + 8 * gl);
-            const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+    constexpr int U = 4;                                  // rows on their way at once
+    for (int64_t r0 = (int64_t)blockIdx.x * kRows * U; r0 < rows; r0 += (int64_t)gridDim.x * kRows * U) {
+        uint4 xs[U], ys[U];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 a = Elem<T>::unpack(xs[i]), b = Elem<T>::unpack(ys[i]);
-                dot += a.x * b.x + a.y * b.y;
-                sq += a.x * a.x + a.y * a.y;
+        for (int u = 0; u < U; ++u) {
+            const int64_t r = r0 + u * kRows + threadIdx.x / G, t = r / Hq;
+            const int h = (int)(r - t * Hq);
+            xs[u] = ys[u] = make_uint4(0, 0, 0, 0);
+            if (r < rows && in) {
+                xs[u] = *reinterpret_cast<const uint4*>(dout + t * do_tok + h * do_head + 8 * gl);
+                ys[u] = *reinterpret_cast<const uint4*>(o + t * o_tok + h * o_head + 8 * gl);
             }
         }
 #pragma unroll
-        for (int x = G / 2; x > 0; x >>= 1) {
-            dot += __shfl_xor_sync(0xffffffffu, dot, x);
-            sq += __shfl_xor_sync(0xffffffffu, sq, x);
-        }
-        if (sq < INFINITY) big_do = fmaxf(big_do, sq);
-        if (r < rows && gl == 0) {
-            const float l = lse[(int64_t)h * Tq + t];
-            stat[h * stat_ld + t] = make_float2(l == -INFINITY ? INFINITY : l * kLog2e, dot);
+        for (int u = 0; u < U; ++u) {
+            const int64_t r = r0 + u * kRows + threadIdx.x / G, t = r / Hq;
+            const int h = (int)(r - t * Hq);
+            const uint32_t xw[4] = {xs[u].x, xs[u].y, xs[u].z, xs[u].w}, yw[4] = {ys[u].x, ys[u].y, ys[u].z, ys[u].w};
+            float dot = 0.0f, sq = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 a = Elem<T>::unpack(xw[i]), b = Elem<T>::unpack(yw[i]);
+                dot += a.x * b.x + a.y * b.y;
+                sq += a.x * a.x + a.y * a.y;
+            }
+#pragma unroll
+            for (int x = G / 2; x > 0; x >>= 1) {
+                dot += __shfl_xor_sync(0xffffffffu, dot, x);
+                sq += __shfl_xor_sync(0xffffffffu, sq, x);
+            }
+            if (sq < INFINITY) big_do = fmaxf(big_do, sq);
+            if (r < rows && gl == 0) {
+                const float l = lse[(int64_t)h * Tq + t];
+                stat[h * stat_ld + t] = make_float2(l == -INFINITY ? INFINITY : l * kLog2e, dot);
+            }
         }
     }
     if constexpr (Elem<T>::kFmt == 0) {

@@ -770,15 +770,11 @@ bool tma_ok(const void* p, int64_t ld) { return !(reinterpret_cast<uintptr_t>(p)
 
 constexpr int kFewRows = 32;
 
-// Tile width: the widest that still gives every SM a tile, and the narrowest otherwise.
-int tile_n(int64_t M, int64_t N) {
-    const int64_t tm = (M + kBM - 1) / kBM;
-    for (int bn : {256, 128})
-        if (N > bn / 2 && tm * ((N + bn - 1) / bn) >= kNumSMs) return bn;
-    return N > 64 && tm * ((N + 63) / 64) > kNumSMs ? 128 : 64;
-}
-
-Sched schedule(int64_t M, int64_t N, int64_t K, int bn) {
+// How a product is cut.  In cycles of one SM, measured: a K block takes 512 with tiles of 128 x 256 (the products' own time)
+// and 390 with narrower ones (the loads'); the epilogue of the last tile about 25 a column; a last wave cut along K costs its
+// second kernel, about 7000.  With tiles of 256 the gradient of a 4096 x 1024 weight over 9600 rows takes one wave of 128 tiles
+// (58 us), with 128 two of 256 tiles (92 us); 1200 x 1024 x 1024 takes 6.8 us with 80 tiles of 128, 9 us with 40 of 256.
+Sched schedule(int64_t M, int64_t N, int64_t K, int bn, int64_t* cost) {
     Sched s{};
     s.tiles_n = (int)((N + bn - 1) / bn);
     s.tiles = (int)((M + kBM - 1) / kBM) * s.tiles_n;
@@ -786,27 +782,50 @@ Sched schedule(int64_t M, int64_t N, int64_t K, int bn) {
     s.full = s.tiles;
     s.splits = 1;
     s.kper = s.kblocks;
-    const int rest = s.tiles % kNumSMs;
-    // cut the last wave along K when at least two splits of four blocks each find an SM
-    int splits = rest ? std::min({kNumSMs / rest, s.kblocks / 4, 16}) : 1;
+    const int64_t block = bn == 256 ? 512 : 390, epilogue = 25 * bn;
+    const int waves = s.tiles / kNumSMs, rest = s.tiles % kNumSMs;
+    *cost = (waves + (rest > 0)) * s.kblocks * block + epilogue;
+    // at least two splits of four blocks each
+    const int splits = rest ? std::min({kNumSMs / rest, s.kblocks / 4, 16}) : 1;
     if (splits >= 2) {
-        s.full = s.tiles - rest;
-        s.kper = (s.kblocks + splits - 1) / splits;
-        s.splits = (s.kblocks + s.kper - 1) / s.kper;
+        const int kper = (s.kblocks + splits - 1) / splits;
+        const int64_t cut = (waves * s.kblocks + kper) * block + epilogue + 7000;
+        if (cut < *cost) {
+            *cost = cut;
+            s.full = s.tiles - rest;
+            s.kper = kper;
+            s.splits = (s.kblocks + kper - 1) / kper;
+        }
     }
     s.units = s.full + (s.tiles - s.full) * s.splits;
     return s;
 }
 
+// Tile width and schedule of least cost.
+int choose(int64_t M, int64_t N, int64_t K, Sched* s) {
+    int best = 0;
+    int64_t least = 0;
+    for (int bn : {256, 128, 64}) {
+        int64_t cost;
+        const Sched t = schedule(M, N, K, bn, &cost);
+        if (best == 0 || cost < least) {
+            best = bn;
+            least = cost;
+            *s = t;
+        }
+    }
+    return best;
+}
+
 size_t part_bytes(int64_t M, int64_t N, int64_t K) {
-    const int bn = tile_n(M, N);
-    const Sched s = schedule(M, N, K, bn);
+    Sched s;
+    const int bn = choose(M, N, K, &s);
     return (size_t)(s.units - s.full) * kBM * bn * sizeof(float);
 }
 
 template <typename T, int BN, bool AMN, bool BMN>
 int gemm_bn(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N, int64_t K, const Out& o,
-            float* part, int32_t* status, cudaStream_t st) {
+            Sched s, int32_t* status, cudaStream_t st) {
     using C = Cfg<BN>;
     static bool attr_set[64] = {};
     int dev = 0;
@@ -816,8 +835,6 @@ int gemm_bn(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, i
         PMG_CUDA_TRY(cudaFuncSetAttribute(k_gemm<T, BN, AMN, BMN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
         attr_set[dev] = true;
     }
-    Sched s = schedule(M, N, K, BN);
-    s.part = part;
     CUtensorMap ma, mb;
     const uint64_t da[2] = {(uint64_t)(AMN ? M : K), (uint64_t)(AMN ? K : M)}, sa[1] = {(uint64_t)lda * 2};
     const uint64_t db[2] = {(uint64_t)(BMN ? N : K), (uint64_t)(BMN ? K : N)}, sb[1] = {(uint64_t)ldb * 2};
@@ -839,10 +856,13 @@ int gemm_bn(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, i
 template <typename T, bool AMN, bool BMN>
 int gemm(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N, int64_t K, const Out& o,
          float* part, int32_t* status, cudaStream_t st) {
-    switch (tile_n(M, N)) {
-        case 256: return gemm_bn<T, 256, AMN, BMN>(A, lda, B, ldb, M, N, K, o, part, status, st);
-        case 128: return gemm_bn<T, 128, AMN, BMN>(A, lda, B, ldb, M, N, K, o, part, status, st);
-        default: return gemm_bn<T, 64, AMN, BMN>(A, lda, B, ldb, M, N, K, o, part, status, st);
+    Sched c;
+    const int bn = choose(M, N, K, &c);
+    c.part = part;
+    switch (bn) {
+        case 256: return gemm_bn<T, 256, AMN, BMN>(A, lda, B, ldb, M, N, K, o, c, status, st);
+        case 128: return gemm_bn<T, 128, AMN, BMN>(A, lda, B, ldb, M, N, K, o, c, status, st);
+        default: return gemm_bn<T, 64, AMN, BMN>(A, lda, B, ldb, M, N, K, o, c, status, st);
     }
 }
 
