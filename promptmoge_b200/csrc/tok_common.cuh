@@ -129,6 +129,57 @@ __device__ __forceinline__ void mma_commit_if(uint32_t lead, uint64_t* bar) {
         : "memory");
 }
 
+// A pair of CTAs on one tile (cta_group::2): each holds its rows of A, half the rows of B and its rows of the result.  The
+// even CTA issues; loads of either signal its barrier, and what it commits arrives in both.
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address of `bar` in the even CTA.
+__device__ __forceinline__ uint32_t even_bar(uint64_t* bar) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(bar)));
+    return r;
+}
+__device__ __forceinline__ void arrive_even(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(even_bar(bar)) : "memory");
+}
+__device__ __forceinline__ void tma_tile2d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+        "[%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void mma16_pair(uint32_t lead, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(kDescHi), "r"(lead)
+        : "memory");
+}
+__device__ __forceinline__ void commit_pair_if(uint32_t lead, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n\t}" ::"r"(
+            smem_u32(bar)),
+        "r"(lead), "h"((uint16_t)3)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_alloc_pair(uint32_t* slot, uint32_t ncols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(ncols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+
 // 32 columns of this thread's tensor-memory lane; no wait (tmem_wait_ld before the values are used).
 __device__ __forceinline__ void tmem_ld32(uint32_t t, uint32_t* r) {
     asm volatile(
@@ -177,8 +228,10 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatil
 }
 
 // Waits (bounded) until every MMA this thread issued has retired, so that tensor memory may be freed after an abort.
+template <bool PAIR = false>
 __device__ __forceinline__ void drain_mma(uint64_t* bar) {
-    mma_commit(bar);
+    if constexpr (PAIR) commit_pair_if(1, bar);
+    else mma_commit(bar);
     const uint64_t t0 = global_ns();
     while (!mbar_try_wait_sleep(bar, 0, 4000) && global_ns() - t0 < kWaitNs) {
     }
@@ -188,9 +241,13 @@ __device__ __forceinline__ void drain_mma(uint64_t* bar) {
 
 // Host: launches a kernel that follows another of the same call.  It starts with pdl_begin(), so its launch may be
 // prepared while that one runs; it waits there until that one is complete.
-template <typename... P, typename... A>
+// CLUSTER: CTAs of a cluster.
+template <int CLUSTER = 1, typename... P, typename... A>
 int launch_after(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, A... args) {
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = CLUSTER;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
@@ -199,7 +256,7 @@ int launch_after(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cuda
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = CLUSTER > 1 ? 2 : 1;
     PMG_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, P(args)...));
     return PMG_OK;
 }

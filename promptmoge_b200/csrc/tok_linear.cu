@@ -7,7 +7,7 @@
 //   k_rows    up to 32 rows: bound by one read of W.  A block owns 16 output columns, its warps split K; mma.sync with W
 //             as the 16-row operand, every lane's 16-byte load feeding two instructions (a dot product does not mind the
 //             order of K, so no shuffle or shared-memory transpose is needed).
-//   k_gemm    everything larger: tcgen05 with 128 x BN tiles, TMA ring, accumulators double-buffered in tensor memory so
+//   k_gemm    everything larger: tcgen05 with tiles of 128 x 64, 128 x 128 or, by pairs of CTAs, 256 x 256, TMA ring, accumulators double-buffered in tensor memory so
 //             that the epilogue of one tile runs under the next tile's products.
 //   k_split_sum   the last wave of tiles, when it would leave most SMs idle, is cut along K into fp32 partials that this
 //             kernel adds in split order (no atomics: results do not depend on timing) and takes through the epilogue.
@@ -297,7 +297,11 @@ constexpr int kGemmThreads = 32 * (kFirstEpi + kEpiWarps);
 
 template <int BN>
 struct Cfg {
-    static constexpr int kA = kBM * kBK * 2, kB = BN * kBK * 2, kStage = kA + kB;
+    // 256 columns: two CTAs on a tile of 256 rows, half the columns' operand in each.  A SM then loads 32 KB for what takes
+    // 48 KB alone; under the power limit, which long runs meet, that is worth more than where the loads keep up.
+    static constexpr bool kPair = BN == 256;
+    static constexpr int kRows = kPair ? 2 * kBM : kBM, kOwnN = kPair ? BN / 2 : BN;
+    static constexpr int kA = kBM * kBK * 2, kB = kOwnN * kBK * 2, kStage = kA + kB;
     static constexpr int kStages = 196608 / kStage > 8 ? 8 : 196608 / kStage;
     static constexpr int kStaging = kEpiWarps * 4096;          // 32 rows of 128 bytes a warp
     static constexpr int kBias = kEpiWarps * 64 * 4;
@@ -308,7 +312,7 @@ struct Cfg {
 // What a CTA walks: units 0 .. full-1 are whole tiles, the rest (tile, split) pairs of the remaining tiles.
 struct Sched {
     int tiles_n, tiles, full, splits, units, kblocks, kper;
-    float* part;            // [units - full][128][BN]
+    float* part;            // [units - full][rows of a tile][BN]
 };
 
 struct Unit {
@@ -328,7 +332,7 @@ __device__ __forceinline__ Unit unit_of(const Sched& s, int u) {
         r.kb0 = (r.slot % s.splits) * s.kper;
         r.kb1 = min(r.kb0 + s.kper, s.kblocks);
     }
-    r.m0 = (tile / s.tiles_n) * kBM;
+    r.m0 = (tile / s.tiles_n) * Cfg<BN>::kRows;
     r.n0 = (tile % s.tiles_n) * BN;
     return r;
 }
@@ -355,41 +359,53 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(acc_full + i, 1);
-            mbar_init(acc_empty + i, 32 * kEpiWarps);
+            mbar_init(acc_empty + i, (C::kPair ? 2 : 1) * kEpiWarps);
         }
         mbar_init(drain, 1);
         *abort_flag = 0;
         fence_mbar_init();
     }
-    if (warp == 1) tmem_alloc(slot, 2 * BN);
+    if (warp == 1) {
+        if constexpr (C::kPair) tmem_alloc_pair(slot, 2 * BN);
+        else tmem_alloc(slot, 2 * BN);
+    }
     tc_fence_before();
     __syncthreads();
+    if constexpr (C::kPair) cluster_sync();             // the other CTA's barriers are ready too
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *slot, 0);
+    const int rank = C::kPair ? (int)cluster_rank() : 0;
+    const int first = C::kPair ? blockIdx.x >> 1 : blockIdx.x, step = C::kPair ? gridDim.x >> 1 : gridDim.x;
     pdl_begin();
 
     if (warp == 0) {
         if (lane == 0) {
             uint32_t it = 0;
             bool ok = true;
-            for (int u = blockIdx.x; u < sched.units && ok; u += gridDim.x) {
+            for (int u = first; u < sched.units && ok; u += step) {
                 const Unit t = unit_of<BN>(sched, u);
+                const int m0 = t.m0 + rank * kBM, n0 = t.n0 + rank * C::kOwnN;
                 for (int kb = t.kb0; kb < t.kb1; ++kb, ++it) {
                     const int st = it % C::kStages;
                     if (!mbar_wait(empty + st, ((it / C::kStages) & 1u) ^ 1u, abort_flag)) { ok = false; break; }
-                    mbar_arrive_expect_tx(full + st, C::kStage);
+                    if (rank == 0) mbar_arrive_expect_tx(full + st, (C::kPair ? 2 : 1) * C::kStage);
                     const uint32_t a = smem_u32(smem + st * C::kStage), b = a + C::kA;
+                    const uint32_t bar = C::kPair ? even_bar(full + st) : 0;
+                    auto load = [&](uint32_t to, const CUtensorMap* map, int x, int y) {
+                        if constexpr (C::kPair) tma_tile2d_pair(to, map, x, y, bar);
+                        else tma_tile2d(to, map, x, y, full + st);
+                    };
                     if constexpr (AMN) {
 #pragma unroll
-                        for (int i = 0; i < kBM / 64; ++i) tma_tile2d(a + i * 8192, &ma, t.m0 + 64 * i, kb * kBK, full + st);
+                        for (int i = 0; i < kBM / 64; ++i) load(a + i * 8192, &ma, m0 + 64 * i, kb * kBK);
                     } else {
-                        tma_tile2d(a, &ma, kb * kBK, t.m0, full + st);
+                        load(a, &ma, kb * kBK, m0);
                     }
                     if constexpr (BMN) {
 #pragma unroll
-                        for (int i = 0; i < BN / 64; ++i) tma_tile2d(b + i * 8192, &mb, t.n0 + 64 * i, kb * kBK, full + st);
+                        for (int i = 0; i < C::kOwnN / 64; ++i) load(b + i * 8192, &mb, n0 + 64 * i, kb * kBK);
                     } else {
-                        tma_tile2d(b, &mb, kb * kBK, t.n0, full + st);
+                        load(b, &mb, kb * kBK, n0);
                     }
                 }
             }
@@ -398,13 +414,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 flag(status, PMG_ERR_TIMEOUT);
             }
         }
-    } else if (warp == 1) {
-        constexpr uint32_t idesc = idesc16(Elem<T>::kFmt, kBM, BN, AMN, BMN);
+    } else if (warp == 1 && rank == 0) {
+        constexpr uint32_t idesc = idesc16(Elem<T>::kFmt, C::kRows, BN, AMN, BMN);
         const uint32_t lead = elect_one();
         uint32_t it = 0, k = 0;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t ph) { return (bool)__all_sync(0xffffffffu, mbar_wait(bar, ph, abort_flag)); };
-        for (int u = blockIdx.x; u < sched.units && ok; u += gridDim.x, ++k) {
+        for (int u = first; u < sched.units && ok; u += step, ++k) {
             const Unit t = unit_of<BN>(sched, u);
             const uint32_t buf = k & 1u, d = tmem + buf * BN;
             ok = wait(acc_empty + buf, ((k >> 1) & 1u) ^ 1u);
@@ -418,17 +434,23 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 const uint32_t at = smem_u32(smem + st * C::kStage);
                 const uint32_t a = desc_lo(at, AMN ? 8192 : 16), b = desc_lo(at + C::kA, BMN ? 8192 : 16);
 #pragma unroll
-                for (int kk = 0; kk < kBK / 16; ++kk)
-                    mma16(lead, d, a + kk * (AMN ? 128 : 2), b + kk * (BMN ? 128 : 2), idesc, (kb > t.kb0 || kk > 0) ? 1u : 0u);
-                mma_commit_if(lead, empty + st);
+                for (int kk = 0; kk < kBK / 16; ++kk) {
+                    const uint32_t da = a + kk * (AMN ? 128 : 2), db = b + kk * (BMN ? 128 : 2), acc = (kb > t.kb0 || kk > 0) ? 1u : 0u;
+                    if constexpr (C::kPair) mma16_pair(lead, d, da, db, idesc, acc);
+                    else mma16(lead, d, da, db, idesc, acc);
+                }
+                if constexpr (C::kPair) commit_pair_if(lead, empty + st);
+                else mma_commit_if(lead, empty + st);
             }
-            if (ok) mma_commit_if(lead, acc_full + buf);
+            if (!ok) break;
+            if constexpr (C::kPair) commit_pair_if(lead, acc_full + buf);
+            else mma_commit_if(lead, acc_full + buf);
         }
         if (lane == 0) {
             if (!ok) flag(status, PMG_ERR_TIMEOUT);
             if (!ok || *abort_flag) {
                 *abort_flag = 1;
-                drain_mma(drain);
+                drain_mma<C::kPair>(drain);
             }
         }
         __syncwarp();
@@ -439,15 +461,29 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         const int srow = lane >> 3, sch = lane & 7;           // coalesced side: 4 rows x 8 chunks of 16 bytes
         uint32_t k = 0;
         bool ok = true;
-        for (int u = blockIdx.x; u < sched.units; u += gridDim.x, ++k) {
+        for (int u = first; u < sched.units; u += step, ++k) {
             const Unit t = unit_of<BN>(sched, u);
             const uint32_t buf = k & 1u;
-            const int mw = t.m0 + quarter * 32;               // this warp's first row
+            const int mw = t.m0 + rank * kBM + quarter * 32;  // this warp's first row
             const bool whole = t.slot < 0;
             const bool wide = !whole || o.f32;                // 32 columns of 4 bytes, else 64 of 2, per 128-byte row
             const int cols = wide ? 32 : 64, n_end = min(N - t.n0, BN);
             bool waited = false;
-            for (int c0 = group * cols; c0 < BN; c0 += 2 * cols) {
+            // this warp's columns of the bias, ahead of the accumulators
+            constexpr int kBiasRegs = BN / 64;
+            float bias_r[kBiasRegs];
+            if (whole && o.bias) {
+#pragma unroll
+                for (int i = 0; i < kBiasRegs; ++i) {
+                    // column `lane` of the i-th 32 columns this group takes
+                    const int c = (wide ? 64 * i + 32 * group : 128 * (i >> 1) + 64 * group + 32 * (i & 1)) + lane;
+                    bias_r[i] = c < n_end ? Elem<T>::to(static_cast<const T*>(o.bias)[t.n0 + c]) : 0.0f;
+                }
+            }
+#pragma unroll 1
+            for (int ch = 0; ch < BN / 64; ++ch) {
+                const int c0 = group * cols + 2 * cols * ch;
+                if (c0 >= BN) break;
                 const int n = t.n0 + c0;
                 uint4 res[8];
                 const bool add = whole && o.resid && c0 < n_end;
@@ -477,11 +513,18 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 }
                 if (whole && o.bias) {
                     __syncwarp();
+                    float b0 = 0.0f, b1 = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int nn = n + lane + 32 * i;
-                        bias_s[lane + 32 * i] = (lane + 32 * i < cols && nn < N) ? Elem<T>::to(static_cast<const T*>(o.bias)[nn]) : 0.0f;
+                    for (int i = 0; i < kBiasRegs; ++i) {
+                        if (i == (wide ? ch : 2 * ch)) b0 = bias_r[i];
+                        if (i == 2 * ch + 1) b1 = bias_r[i];
                     }
+                    if (BN == 64 && !wide) {                           // 64 columns: one group has them all
+                        const int c = 32 + lane;
+                        b1 = c < n_end ? Elem<T>::to(static_cast<const T*>(o.bias)[t.n0 + c]) : 0.0f;
+                    }
+                    bias_s[lane] = b0;
+                    if (!wide) bias_s[lane + 32] = b1;
                 }
                 if (!waited) {
                     waited = true;
@@ -550,7 +593,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 const int rows = min(32, M - mw), left = N - n;
                 if (!whole) {
                     put32(v);
-                    flush(sched.part + ((int64_t)t.slot * kBM + quarter * 32) * BN + c0, BN, 4, rows, cols, true);
+                    flush(sched.part + ((int64_t)t.slot * C::kRows + rank * kBM + quarter * 32) * BN + c0, BN, 4, rows, cols, true);
                     continue;
                 }
                 if (o.pre) {
@@ -603,7 +646,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                 if (!ok) break;
             }
             tc_fence_before();
-            mbar_arrive(acc_empty + buf);
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (C::kPair) arrive_even(acc_empty + buf);
+                else mbar_arrive(acc_empty + buf);
+            }
         }
         if (!ok && lane == 0) {
             *abort_flag = 1;
@@ -613,9 +660,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    if constexpr (C::kPair) cluster_sync();             // neither leaves while the other may still signal or read it
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, 2 * BN);
+        if constexpr (C::kPair) tmem_dealloc_pair(tmem, 2 * BN);
+        else tmem_dealloc(tmem, 2 * BN);
     }
 }
 
@@ -623,20 +672,20 @@ template <typename T, int BN>
 __global__ void __launch_bounds__(256) k_split_sum(const __grid_constant__ Sched s, const int M, const int N,
                                                    const __grid_constant__ Out o) {
     pdl_begin();
-    const int per_tile = kBM * BN / 8;
+    constexpr int kRows = Cfg<BN>::kRows, per_tile = kRows * BN / 8;
     const int i = blockIdx.x * 256 + threadIdx.x;
     const int rest = i / per_tile, tile = s.full + rest, e = (i % per_tile) * 8;
     if (tile >= s.tiles) return;
     const int r = e / BN, c = e % BN;
-    const int m = (tile / s.tiles_n) * kBM + r, n = (tile % s.tiles_n) * BN + c;
+    const int m = (tile / s.tiles_n) * kRows + r, n = (tile % s.tiles_n) * BN + c;
     if (m >= M || n >= N) return;
     float z[8] = {};
-    const float* p = s.part + ((int64_t)rest * s.splits * kBM + r) * BN + c;
+    const float* p = s.part + ((int64_t)rest * s.splits * kRows + r) * BN + c;
     for (int k = 0; k < s.splits; ++k) {
         const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
         z[0] += a.x; z[1] += a.y; z[2] += a.z; z[3] += a.w;
         z[4] += b.x; z[5] += b.y; z[6] += b.z; z[7] += b.w;
-        p += kBM * BN;
+        p += kRows * BN;
     }
     finish8<T>(o, m, n, N, z);
 }
@@ -779,16 +828,17 @@ constexpr int kFewRows = 32;
 Sched schedule(int64_t M, int64_t N, int64_t K, int bn, int64_t* cost) {
     Sched s{};
     s.tiles_n = (int)((N + bn - 1) / bn);
-    s.tiles = (int)((M + kBM - 1) / kBM) * s.tiles_n;
+    const int rows = bn == 256 ? 2 * kBM : kBM, slots = bn == 256 ? kNumSMs / 2 : kNumSMs;      // two CTAs a tile, or one
+    s.tiles = (int)((M + rows - 1) / rows) * s.tiles_n;
     s.kblocks = (int)((K + kBK - 1) / kBK);
     s.full = s.tiles;
     s.splits = 1;
     s.kper = s.kblocks;
     const int64_t block = bn == 256 ? 512 : 390, epilogue = 25 * bn;
-    const int waves = s.tiles / kNumSMs, rest = s.tiles % kNumSMs;
+    const int waves = s.tiles / slots, rest = s.tiles % slots;
     *cost = (waves + (rest > 0)) * s.kblocks * block + epilogue;
     // at least two splits of four blocks each
-    const int splits = rest ? std::min({kNumSMs / rest, s.kblocks / 4, 16}) : 1;
+    const int splits = rest ? std::min({slots / rest, s.kblocks / 4, 16}) : 1;
     if (splits >= 2) {
         const int kper = (s.kblocks + splits - 1) / splits;
         const int64_t cut = (waves * s.kblocks + kper) * block + epilogue + 7000;
@@ -822,7 +872,7 @@ int choose(int64_t M, int64_t N, int64_t K, Sched* s) {
 size_t part_bytes(int64_t M, int64_t N, int64_t K) {
     Sched s;
     const int bn = choose(M, N, K, &s);
-    return (size_t)(s.units - s.full) * kBM * bn * sizeof(float);
+    return (size_t)(s.units - s.full) * (bn == 256 ? 2 * kBM : kBM) * bn * sizeof(float);
 }
 
 template <typename T, int BN, bool AMN, bool BMN>
@@ -840,16 +890,17 @@ int gemm_bn(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, i
     CUtensorMap ma, mb;
     const uint64_t da[2] = {(uint64_t)(AMN ? M : K), (uint64_t)(AMN ? K : M)}, sa[1] = {(uint64_t)lda * 2};
     const uint64_t db[2] = {(uint64_t)(BMN ? N : K), (uint64_t)(BMN ? K : N)}, sb[1] = {(uint64_t)ldb * 2};
-    const uint32_t ba[2] = {64, (uint32_t)(AMN ? kBK : kBM)}, bb[2] = {64, (uint32_t)(BMN ? kBK : BN)};
+    const uint32_t ba[2] = {64, (uint32_t)(AMN ? kBK : kBM)}, bb[2] = {64, (uint32_t)(BMN ? kBK : C::kOwnN)};
     int rc = make_tensor_map16(&ma, A, 2, da, sa, ba);
     if (rc != PMG_OK) return rc;
     rc = make_tensor_map16(&mb, B, 2, db, sb, bb);
     if (rc != PMG_OK) return rc;
-    rc = launch_after(k_gemm<T, BN, AMN, BMN>, dim3(std::min(s.units, kNumSMs)), kGemmThreads, C::kSmem, st, ma, mb, (int)M,
-                      (int)N, s, o, status);
+    constexpr int kCtas = C::kPair ? 2 : 1;
+    rc = launch_after<kCtas>(k_gemm<T, BN, AMN, BMN>, dim3(std::min(s.units, kNumSMs / kCtas) * kCtas), kGemmThreads, C::kSmem, st,
+                             ma, mb, (int)M, (int)N, s, o, status);
     if (rc != PMG_OK) return rc;
     if (s.full < s.tiles) {
-        const int64_t threads = (int64_t)(s.tiles - s.full) * (kBM * BN / 8);
+        const int64_t threads = (int64_t)(s.tiles - s.full) * (C::kRows * BN / 8);
         return launch_after(k_split_sum<T, BN>, dim3((unsigned)((threads + 255) / 256)), 256, 0, st, s, (int)M, (int)N, o);
     }
     return PMG_OK;
