@@ -319,6 +319,16 @@ struct Unit {
     int m0, n0, kb0, kb1, slot;      // slot < 0: a whole tile
 };
 
+// Tiles are taken in bands of eight rows of tiles, down each band's columns: what runs at one time then spans about as
+// many rows as columns, and reads the least of either operand.
+constexpr int kBand = 8;
+__device__ __forceinline__ void place_of_tile(const Sched& s, int tile, int* m, int* n) {
+    const int rows = s.tiles / s.tiles_n, band = tile / (kBand * s.tiles_n), first = band * kBand, high = min(kBand, rows - first);
+    const int in = tile - first * s.tiles_n;
+    *m = first + in % high;
+    *n = in / high;
+}
+
 template <int BN>
 __device__ __forceinline__ Unit unit_of(const Sched& s, int u) {
     Unit r;
@@ -332,8 +342,9 @@ __device__ __forceinline__ Unit unit_of(const Sched& s, int u) {
         r.kb0 = (r.slot % s.splits) * s.kper;
         r.kb1 = min(r.kb0 + s.kper, s.kblocks);
     }
-    r.m0 = (tile / s.tiles_n) * Cfg<BN>::kRows;
-    r.n0 = (tile % s.tiles_n) * BN;
+    place_of_tile(s, tile, &r.m0, &r.n0);
+    r.m0 *= Cfg<BN>::kRows;
+    r.n0 *= BN;
     return r;
 }
 
@@ -677,7 +688,9 @@ __global__ void __launch_bounds__(256) k_split_sum(const __grid_constant__ Sched
     const int rest = i / per_tile, tile = s.full + rest, e = (i % per_tile) * 8;
     if (tile >= s.tiles) return;
     const int r = e / BN, c = e % BN;
-    const int m = (tile / s.tiles_n) * kRows + r, n = (tile % s.tiles_n) * BN + c;
+    int tm, tn;
+    place_of_tile(s, tile, &tm, &tn);
+    const int m = tm * kRows + r, n = tn * BN + c;
     if (m >= M || n >= N) return;
     float z[8] = {};
     const float* p = s.part + ((int64_t)rest * s.splits * kRows + r) * BN + c;
