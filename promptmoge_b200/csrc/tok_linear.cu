@@ -7,12 +7,14 @@
 //   k_rows    up to 32 rows: bound by one read of W.  A block owns 16 output columns, its warps split K; mma.sync with W
 //             as the 16-row operand, every lane's 16-byte load feeding two instructions (a dot product does not mind the
 //             order of K, so no shuffle or shared-memory transpose is needed).
-//   k_gemm    everything larger: tcgen05 with tiles of 128 x 64, 128 x 128 or, by pairs of CTAs, 256 x 256, TMA ring, accumulators double-buffered in tensor memory so
-//             that the epilogue of one tile runs under the next tile's products.
+//   k_gemm    everything larger: tcgen05 with tiles of 128 x 64, 128 x 128 or, by pairs of CTAs, 256 x 256, TMA ring,
+//             accumulators double-buffered in tensor memory so that the epilogue of one tile runs under the next one's
+//             products; sixteen warps take it, straight from registers to memory.
 //   k_split_sum   the last wave of tiles, when it would leave most SMs idle, is cut along K into fp32 partials that this
 //             kernel adds in split order (no atomics: results do not depend on timing) and takes through the epilogue.
-// Measured: 38,400 x 1024 x 4096 with gelu 258 us (1250 TFLOP/s, tensor core 75 % active; cuBLAS's sustained rate here is
-// 1357), its gradients over 9600 rows 177 us, 1200 x 1024 x 1024 9 us, one row 1024 -> 4096 3.4 us (2.5 TB/s).
+// Measured: 38,400 x 1024 x 4096 with gelu 249 us (1295 TFLOP/s) alone and 288 in long runs, where the power limit holds the
+// clock at 1.3 GHz (without the activation 263; cuBLAS 274); its gradients over 9600 rows 167 us, 1200 x 1024 x 1024 9 us, one
+// row 1024 -> 4096 3.4 us (2.5 TB/s).  With eight warps that staged their rows in shared memory: 278 and 321 us.
 // dz is rounded to the operands' 16-bit type before its two products (tensor cores take no other), db is summed from the
 // unrounded fp32 values.
 #include <algorithm>
@@ -28,19 +30,12 @@ using namespace tok;
 // Activations
 // ----------------------------------------------------------------------------------------------------------------- //
 
-// Phi(x) - 1/2 = x p(t), t = 2 x^2 / 25 - 1 on |x| <= 5: the degree-11 polynomial of least largest |x (p - exact)| by
-// iteratively reweighted least squares in the Chebyshev basis, constant term raised so that Phi saturates to exactly 0
-// and 1 at the ends.  |error| <= 2.1e-6 evaluated in fp32, 9.3e-6 of x Phi(x); erff in its place costs the epilogue
-// about three times as many instructions, and no output type here resolves more than 2^-11.
-__device__ constexpr float kPhi[12] = {1.41363868e-01f, -7.02976871e-02f, 5.15348489e-02f, -4.04097587e-02f,
-                                       3.12585325e-02f, -2.34790368e-02f, 1.72561175e-02f, -1.06230432e-02f,
-                                       4.62778831e-03f, -3.28729113e-03f, 3.42820314e-03f, -1.37248793e-03f};
-
-__device__ __forceinline__ float fma_sat(float a, float b, float c) {
-    float r;
-    asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
+// Phi(-a) = 2^q(a) for a >= 0: q is smooth, so a short polynomial holds it.  Degree 5, of least largest
+// max(a, 1) |2^q(a) - Phi(-a)| on [0, 7] (linear programming on a grid); |error| of Phi and of a Phi <= 7e-7 evaluated in
+// fp32, and no output type here resolves more than 2^-11.  q falls on to -399 at 16, so that Phi(-16) is 0.  Then
+// gelu(x) = max(x, 0) - |x| Phi(-|x|).  A product whose tiles keep the tensor cores busy runs at the power limit, where each
+// operation per output counts as energy: 9 of them in place of the 17 of a polynomial in x^2 for Phi itself.
+__device__ constexpr float kTail[6] = {-1.00000191f, -1.151052f, -0.459414065f, -0.0523432381f, 0.00728237722f, -0.000500259455f};
 
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
@@ -48,20 +43,22 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-__device__ __forceinline__ float2 phi_pair(float a, float b) {
-    const float ca = fminf(fmaxf(a, -5.0f), 5.0f), cb = fminf(fmaxf(b, -5.0f), 5.0f);
-    const uint64_t c = pack2(ca, cb);
-    const uint64_t t = fma2(mul2(c, c), pack2(0.08f, 0.08f), pack2(-1.0f, -1.0f));
-    uint64_t p = pack2(kPhi[11], kPhi[11]);
+// Phi(-|x|) for two values, and the bounded |x| that it was taken at
+__device__ __forceinline__ float2 tail_pair(float a, float b, float& xa, float& xb) {
+    xa = fminf(fabsf(a), 16.0f);
+    xb = fminf(fabsf(b), 16.0f);
+    const uint64_t x = pack2(xa, xb);
+    uint64_t p = pack2(kTail[5], kTail[5]);
 #pragma unroll
-    for (int i = 10; i >= 0; --i) p = fma2(p, t, pack2(kPhi[i], kPhi[i]));
-    const float2 f = unpack2(p);
-    return make_float2(fma_sat(ca, f.x, 0.5f), fma_sat(cb, f.y, 0.5f));
+    for (int i = 4; i >= 0; --i) p = fma2(p, x, pack2(kTail[i], kTail[i]));
+    const float2 q = unpack2(p);
+    return make_float2(ex2(q.x), ex2(q.y));
 }
 __device__ __forceinline__ void gelu_pair(float& a, float& b) {
-    const float2 f = phi_pair(a, b);
-    a *= f.x;
-    b *= f.y;
+    float xa, xb;
+    const float2 f = tail_pair(a, b, xa, xb);
+    a = fmaf(-xa, f.x, max_nan(a, 0.0f));
+    b = fmaf(-xb, f.y, max_nan(b, 0.0f));
 }
 
 // N values, the choice made once for all of them.
@@ -85,9 +82,11 @@ __device__ __forceinline__ void times_slope(int act, float (&g)[8], const float 
     if (act == PMG_ACT_GELU) {
 #pragma unroll
         for (int i = 0; i < 8; i += 2) {
-            const float2 p = phi_pair(z[i], z[i + 1]);
-            g[i] *= fmaf(z[i] * 0.39894228f, ex2(z[i] * z[i] * (-0.5f * kLog2e)), p.x);
-            g[i + 1] *= fmaf(z[i + 1] * 0.39894228f, ex2(z[i + 1] * z[i + 1] * (-0.5f * kLog2e)), p.y);
+            float xa, xb;
+            const float2 f = tail_pair(z[i], z[i + 1], xa, xb);
+            const float pa = z[i] < 0.0f ? f.x : 1.0f - f.x, pb = z[i + 1] < 0.0f ? f.y : 1.0f - f.y;
+            g[i] *= fmaf(z[i] * 0.39894228f, ex2(z[i] * z[i] * (-0.5f * kLog2e)), pa);
+            g[i + 1] *= fmaf(z[i + 1] * 0.39894228f, ex2(z[i + 1] * z[i + 1] * (-0.5f * kLog2e)), pb);
         }
     } else if (act == PMG_ACT_SILU) {
 #pragma unroll
@@ -112,7 +111,7 @@ struct Out {
     int64_t ldr, ldy, ldp;
     int act;
     int f32;                 // y and the residual are fp32, else the operands' type
-    int vec;                 // rows of y, resid and pre start on 16-byte boundaries
+    int vec;                 // rows of y, resid and pre start on boundaries of 16 bytes (1), 32 (2) or less (0)
 };
 
 // 8 values z[0..7] of row m from column n on: bias, activation, residual, stores.  Used where rows are not staged.
@@ -292,7 +291,7 @@ __global__ void __launch_bounds__(512) k_rows(const uint16_t* __restrict__ x, in
 // Tiles
 // ----------------------------------------------------------------------------------------------------------------- //
 constexpr int kBM = 128, kBK = 64;
-constexpr int kEpiWarps = 8, kFirstEpi = 4;
+constexpr int kEpiWarps = 16, kFirstEpi = 4;
 constexpr int kGemmThreads = 32 * (kFirstEpi + kEpiWarps);
 
 template <int BN>
@@ -303,15 +302,15 @@ struct Cfg {
     static constexpr int kRows = kPair ? 2 * kBM : kBM, kOwnN = kPair ? BN / 2 : BN;
     static constexpr int kA = kBM * kBK * 2, kB = kOwnN * kBK * 2, kStage = kA + kB;
     static constexpr int kStages = 196608 / kStage > 8 ? 8 : 196608 / kStage;
-    static constexpr int kStaging = kEpiWarps * 4096;          // 32 rows of 128 bytes a warp
-    static constexpr int kBias = kEpiWarps * 64 * 4;
-    static constexpr int kBars = kStages * kStage + kStaging + kBias;
+    static constexpr int kBias = 4 * BN * 2;                   // a quarter of the columns a warp, in the operands' type
+    static constexpr int kBars = kStages * kStage + kBias;
     static constexpr int kSmem = kBars + 256;
 };
 
 // What a CTA walks: units 0 .. full-1 are whole tiles, the rest (tile, split) pairs of the remaining tiles.
 struct Sched {
-    int tiles_n, tiles, full, splits, units, kblocks, kper;
+    int tiles_m, tiles_n, tiles, full, splits, units, kblocks, kper;
+    float inv_band;         // 1 / (tiles of a band)
     float* part;            // [units - full][rows of a tile][BN]
 };
 
@@ -323,10 +322,19 @@ struct Unit {
 // many rows as columns, and reads the least of either operand.
 constexpr int kBand = 8;
 __device__ __forceinline__ void place_of_tile(const Sched& s, int tile, int* m, int* n) {
-    const int rows = s.tiles / s.tiles_n, band = tile / (kBand * s.tiles_n), first = band * kBand, high = min(kBand, rows - first);
-    const int in = tile - first * s.tiles_n;
-    *m = first + in % high;
-    *n = in / high;
+    const int size = kBand * s.tiles_n;
+    // tile / size: an estimate that is put right, shorter than the division that every warp would wait for at every tile
+    int band = (int)((float)tile * s.inv_band), in = tile - band * size;
+    while (in < 0) { --band; in += size; }
+    while (in >= size) { ++band; in -= size; }
+    const int first = band * kBand, high = s.tiles_m - first;
+    if (high >= kBand) {
+        *m = first + in % kBand;
+        *n = in / kBand;
+    } else {
+        *m = first + in % high;
+        *n = in / high;
+    }
 }
 
 template <int BN>
@@ -346,6 +354,67 @@ __device__ __forceinline__ Unit unit_of(const Sched& s, int u) {
     r.m0 *= Cfg<BN>::kRows;
     r.n0 *= BN;
     return r;
+}
+
+// W words of a row in registers to and from memory, E elements of 2 or 4 bytes of which the first `left` count.  vec: 2 where
+// the address is a multiple of 32 bytes (one instruction a sector), 1 of 16, 0 of an element.
+template <int W, typename E>
+__device__ __forceinline__ void store_row(const uint32_t* w, E* p, int left, int vec) {
+    constexpr int per = 4 / sizeof(E);
+    if (left >= W * per && vec) {
+        if (vec == 2) {
+#pragma unroll
+            for (int i = 0; i < W; i += 8)
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p + i * per), "r"(w[i]), "r"(w[i + 1]),
+                             "r"(w[i + 2]), "r"(w[i + 3]), "r"(w[i + 4]), "r"(w[i + 5]), "r"(w[i + 6]), "r"(w[i + 7])
+                             : "memory");
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; i += 4)
+                *reinterpret_cast<uint4*>(p + i * per) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        if constexpr (per == 1) {
+            if (i < left) reinterpret_cast<uint32_t*>(p)[i] = w[i];
+        } else {
+            if (2 * i < left) p[2 * i] = (E)w[i];
+            if (2 * i + 1 < left) p[2 * i + 1] = (E)(w[i] >> 16);
+        }
+    }
+}
+template <int W, typename E>
+__device__ __forceinline__ void load_row(uint32_t* w, const E* p, int left, int vec) {
+    constexpr int per = 4 / sizeof(E);
+    if (left >= W * per && vec) {
+        if (vec == 2) {
+#pragma unroll
+            for (int i = 0; i < W; i += 8)
+                asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                             : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]), "=r"(w[i + 5]),
+                               "=r"(w[i + 6]), "=r"(w[i + 7])
+                             : "l"(p + i * per)
+                             : "memory");
+        } else {
+#pragma unroll
+            for (int i = 0; i < W; i += 4) {
+                const uint4 q = *reinterpret_cast<const uint4*>(p + i * per);
+                w[i] = q.x; w[i + 1] = q.y; w[i + 2] = q.z; w[i + 3] = q.w;
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+        if constexpr (per == 1) {
+            w[i] = i < left ? reinterpret_cast<const uint32_t*>(p)[i] : 0u;
+        } else {
+            w[i] = 2 * i < left ? (uint32_t)p[2 * i] : 0u;
+            if (2 * i + 1 < left) w[i] |= (uint32_t)p[2 * i + 1] << 16;
+        }
+    }
 }
 
 template <typename T, int BN, bool AMN, bool BMN>
@@ -466,76 +535,50 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
         __syncwarp();
     } else if (warp >= kFirstEpi) {
+        // Warp w of the sixteen takes the quarter of the rows that it can read (w mod 4) and a quarter of the columns, a
+        // lane a row.  Rows go from registers to memory in sectors of 32 bytes, not by way of shared memory, whose
+        // bandwidth the products and their loads fill (64 + 64 of 128 bytes a cycle).
+        constexpr int kOwn = BN / 4, kChunk = kOwn < 32 ? kOwn : 32;
         const int ew = warp - kFirstEpi, quarter = warp & 3, group = ew >> 2;
-        uint8_t* stage = smem + C::kStages * C::kStage + ew * 4096;
-        float* bias_s = reinterpret_cast<float*>(smem + C::kStages * C::kStage + C::kStaging) + ew * 64;
-        const int srow = lane >> 3, sch = lane & 7;           // coalesced side: 4 rows x 8 chunks of 16 bytes
+        T* bias_s = reinterpret_cast<T*>(smem + C::kStages * C::kStage) + ew * kOwn;
         uint32_t k = 0;
         bool ok = true;
-        for (int u = first; u < sched.units; u += step, ++k) {
-            const Unit t = unit_of<BN>(sched, u);
-            const uint32_t buf = k & 1u;
-            const int mw = t.m0 + rank * kBM + quarter * 32;  // this warp's first row
-            const bool whole = t.slot < 0;
-            const bool wide = !whole || o.f32;                // 32 columns of 4 bytes, else 64 of 2, per 128-byte row
-            const int cols = wide ? 32 : 64, n_end = min(N - t.n0, BN);
-            bool waited = false;
-            // this warp's columns of the bias, ahead of the accumulators
-            constexpr int kBiasRegs = BN / 64;
-            float bias_r[kBiasRegs];
-            if (whole && o.bias) {
+        // A tile's bias comes while the tile before is worked on.
+        constexpr int kBiasRegs = (kOwn + 31) / 32;
+        T bias_r[kBiasRegs];
+        auto ask_bias = [&](const Unit& t) {
+            if (!o.bias || t.slot >= 0) return;
 #pragma unroll
-                for (int i = 0; i < kBiasRegs; ++i) {
-                    // column `lane` of the i-th 32 columns this group takes
-                    const int c = (wide ? 64 * i + 32 * group : 128 * (i >> 1) + 64 * group + 32 * (i & 1)) + lane;
-                    bias_r[i] = c < n_end ? Elem<T>::to(static_cast<const T*>(o.bias)[t.n0 + c]) : 0.0f;
-                }
+            for (int i = 0; i < kBiasRegs; ++i) {
+                const int c = 32 * i + lane, n = t.n0 + group * kOwn + c;
+                bias_r[i] = c < kOwn && n < N ? static_cast<const T*>(o.bias)[n] : Elem<T>::from(0.0f);
             }
+        };
+        Unit t = unit_of<BN>(sched, min(first, sched.units - 1)), next;
+        ask_bias(t);
+        for (int u = first; u < sched.units; u += step, ++k, t = next) {
+            next = unit_of<BN>(sched, min(u + step, sched.units - 1));
+            const uint32_t buf = k & 1u;
+            const int in = quarter * 32 + lane, m = t.m0 + rank * kBM + in;
+            const bool whole = t.slot < 0, row = m < M;
+            const int own = min(kOwn, N - t.n0 - group * kOwn);            // columns of this warp within the matrix
+            if (whole && o.bias) {
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < kBiasRegs; ++i)
+                    if (32 * i + lane < kOwn) bias_s[32 * i + lane] = bias_r[i];
+                __syncwarp();
+            }
+            ask_bias(next);
+            bool waited = false;
 #pragma unroll 1
-            for (int ch = 0; ch < BN / 64; ++ch) {
-                const int c0 = group * cols + 2 * cols * ch;
-                if (c0 >= BN) break;
-                const int n = t.n0 + c0;
-                uint4 res[8];
-                const bool add = whole && o.resid && c0 < n_end;
-                if (add) {                                    // residual rows, coalesced, ahead of the accumulators
-                    const int esz = o.f32 ? 4 : 2, per = 16 / esz;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int m = mw + 4 * i + srow, nn = n + sch * per;
-                        res[i] = make_uint4(0, 0, 0, 0);
-                        if (m < M && nn < N) {
-                            const uint8_t* p = static_cast<const uint8_t*>(o.resid) + ((int64_t)m * o.ldr + nn) * esz;
-                            if (o.vec && nn + per <= N) {
-                                res[i] = *reinterpret_cast<const uint4*>(p);
-                            } else {
-                                uint32_t* w = reinterpret_cast<uint32_t*>(&res[i]);
-                                if (esz == 4) {
-                                    for (int e = 0; e < 4; ++e)
-                                        if (nn + e < N) w[e] = reinterpret_cast<const uint32_t*>(p)[e];
-                                } else {
-                                    for (int e = 0; e < 8; ++e)
-                                        if (nn + e < N)
-                                            w[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[e] << (16 * (e & 1));
-                                }
-                            }
-                        }
-                    }
-                }
-                if (whole && o.bias) {
-                    __syncwarp();
-                    float b0 = 0.0f, b1 = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < kBiasRegs; ++i) {
-                        if (i == (wide ? ch : 2 * ch)) b0 = bias_r[i];
-                        if (i == 2 * ch + 1) b1 = bias_r[i];
-                    }
-                    if (BN == 64 && !wide) {                           // 64 columns: one group has them all
-                        const int c = 32 + lane;
-                        b1 = c < n_end ? Elem<T>::to(static_cast<const T*>(o.bias)[t.n0 + c]) : 0.0f;
-                    }
-                    bias_s[lane] = b0;
-                    if (!wide) bias_s[lane + 32] = b1;
+            for (int c0 = 0; c0 < own || !waited; c0 += kChunk) {
+                const int c = group * kOwn + c0, n = t.n0 + c, left = N - n;
+                const bool add = whole && o.resid && row;
+                uint32_t res[kChunk];                         // ahead of the accumulators
+                if (add) {
+                    if (o.f32) load_row<kChunk>(res, static_cast<const float*>(o.resid) + (int64_t)m * o.ldr + n, left, o.vec);
+                    else load_row<kChunk / 2>(res, static_cast<const uint16_t*>(o.resid) + (int64_t)m * o.ldr + n, left, o.vec);
                 }
                 if (!waited) {
                     waited = true;
@@ -543,125 +586,67 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                     if (!ok) break;
                     tc_fence_after();
                 }
-                if (c0 >= n_end) continue;                    // columns beyond the matrix
-                const uint32_t src = tmem + ((uint32_t)(quarter * 32) << 16) + buf * BN + c0;
-                float v[64];
-                tmem_ld32(src, reinterpret_cast<uint32_t*>(v));
-                if (!wide) tmem_ld32(src + 32, reinterpret_cast<uint32_t*>(v) + 32);
+                const uint32_t src = tmem + ((uint32_t)(quarter * 32) << 16) + buf * BN + c;
+                float v[kChunk];
+                if constexpr (kChunk == 32) tmem_ld32(src, reinterpret_cast<uint32_t*>(v));
+                else tmem_ld16(src, *reinterpret_cast<uint32_t (*)[16]>(v));
                 tmem_wait_ld();
-                if (whole && o.bias) {
+                if (c0 + kChunk >= own) {                     // all that this warp wants is in registers
+                    tc_fence_before();
                     __syncwarp();
-#pragma unroll
-                    for (int i = 0; i < 64; i += 4) {
-                        if (i < 32 || !wide) {
-                            const float4 b4 = *reinterpret_cast<const float4*>(bias_s + i);
-                            v[i] += b4.x; v[i + 1] += b4.y; v[i + 2] += b4.z; v[i + 3] += b4.w;
-                        }
+                    if (lane == 0) {
+                        if constexpr (C::kPair) arrive_even(acc_empty + buf);
+                        else mbar_arrive(acc_empty + buf);
                     }
                 }
-                // staged rows: 16-byte chunk c of row r sits at chunk c ^ (r & 7)
-                uint8_t* mine = stage + lane * 128;
-                const int sw = lane & 7;
-                auto flush = [&](void* base, int64_t ld, int esz, int row_limit, int col_limit, bool vec) {
-                    __syncwarp();
-                    const int per = 16 / esz;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int r = 4 * i + srow, nn = sch * per;
-                        const uint4 q = *reinterpret_cast<const uint4*>(stage + r * 128 + ((sch ^ (r & 7)) * 16));
-                        if (r < row_limit && nn < col_limit) {
-                            uint8_t* p = static_cast<uint8_t*>(base) + (r * ld + nn) * esz;
-                            if (vec && nn + per <= col_limit) {
-                                *reinterpret_cast<uint4*>(p) = q;
-                            } else {
-                                const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-                                if (esz == 4) {
-                                    for (int e = 0; e < 4; ++e)
-                                        if (nn + e < col_limit) reinterpret_cast<uint32_t*>(p)[e] = w[e];
-                                } else {
-                                    for (int e = 0; e < 8; ++e)
-                                        if (nn + e < col_limit)
-                                            reinterpret_cast<uint16_t*>(p)[e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-                                }
-                            }
-                        }
-                    }
-                    __syncwarp();
-                };
-                auto put16 = [&](const float* f, int half) {   // 32 values as 16-bit, chunks 4 half .. 4 half + 3
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        *reinterpret_cast<uint4*>(mine + (((4 * half + c) ^ sw) * 16)) =
-                            make_uint4(Elem<T>::pack(f[8 * c], f[8 * c + 1]), Elem<T>::pack(f[8 * c + 2], f[8 * c + 3]),
-                                       Elem<T>::pack(f[8 * c + 4], f[8 * c + 5]), Elem<T>::pack(f[8 * c + 6], f[8 * c + 7]));
-                };
-                auto put32 = [&](const float* f) {
-#pragma unroll
-                    for (int c = 0; c < 8; ++c)
-                        *reinterpret_cast<float4*>(mine + ((c ^ sw) * 16)) =
-                            make_float4(f[4 * c], f[4 * c + 1], f[4 * c + 2], f[4 * c + 3]);
-                };
-                const int rows = min(32, M - mw), left = N - n;
                 if (!whole) {
-                    put32(v);
-                    flush(sched.part + ((int64_t)t.slot * C::kRows + rank * kBM + quarter * 32) * BN + c0, BN, 4, rows, cols, true);
+                    float* p = sched.part + ((int64_t)t.slot * C::kRows + rank * kBM + in) * BN + c;
+                    store_row<kChunk>(reinterpret_cast<uint32_t*>(v), p, row ? left : 0,
+                                      reinterpret_cast<uintptr_t>(sched.part) & 31 ? 1 : 2);
                     continue;
                 }
+                if (o.bias) {
+#pragma unroll
+                    for (int i = 0; i < kChunk; i += 8) {
+                        const uint4 q = *reinterpret_cast<const uint4*>(bias_s + c0 + i);
+                        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 f = Elem<T>::unpack(w[e]);
+                            v[i + 2 * e] += f.x;
+                            v[i + 2 * e + 1] += f.y;
+                        }
+                    }
+                }
+                uint32_t h[kChunk / 2];
                 if (o.pre) {
-                    put16(v, 0);
-                    if (!wide) put16(v + 32, 1);
-                    flush(static_cast<T*>(o.pre) + (int64_t)mw * o.ldp + n, o.ldp, 2, rows, min(left, cols), o.vec);
+#pragma unroll
+                    for (int i = 0; i < kChunk; i += 2) h[i / 2] = Elem<T>::pack(v[i], v[i + 1]);
+                    store_row<kChunk / 2>(h, static_cast<uint16_t*>(o.pre) + (int64_t)m * o.ldp + n, row ? left : 0, o.vec);
                 }
-                activate<32>(o.act, v);
-                if (!wide) activate<32>(o.act, v + 32);
-                if (add) {
-                    __syncwarp();
+                activate<kChunk>(o.act, v);
+                if (o.f32) {
+                    if (add) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int r = 4 * i + srow;
-                        *reinterpret_cast<uint4*>(stage + r * 128 + ((sch ^ (r & 7)) * 16)) = res[i];
+                        for (int i = 0; i < kChunk; ++i) v[i] += __uint_as_float(res[i]);
                     }
-                    __syncwarp();
-                    if (wide) {
-#pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            const float4 f = *reinterpret_cast<const float4*>(mine + ((c ^ sw) * 16));
-                            v[4 * c] += f.x; v[4 * c + 1] += f.y; v[4 * c + 2] += f.z; v[4 * c + 3] += f.w;
-                        }
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < 8; ++c) {
-                            const uint4 q = *reinterpret_cast<const uint4*>(mine + ((c ^ sw) * 16));
-                            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const float2 f = Elem<T>::unpack(w[e]);
-                                v[8 * c + 2 * e] += f.x;
-                                v[8 * c + 2 * e + 1] += f.y;
-                            }
-                        }
-                    }
-                }
-                if (wide) {
-                    put32(v);
-                    flush(static_cast<float*>(o.y) + (int64_t)mw * o.ldy + n, o.ldy, 4, rows, min(left, cols), o.vec);
+                    store_row<kChunk>(reinterpret_cast<uint32_t*>(v), static_cast<float*>(o.y) + (int64_t)m * o.ldy + n,
+                                      row ? left : 0, o.vec);
                 } else {
-                    put16(v, 0);
-                    put16(v + 32, 1);
-                    flush(static_cast<T*>(o.y) + (int64_t)mw * o.ldy + n, o.ldy, 2, rows, min(left, cols), o.vec);
+                    if (add) {
+#pragma unroll
+                        for (int i = 0; i < kChunk; i += 2) {
+                            const float2 f = Elem<T>::unpack(res[i / 2]);
+                            v[i] += f.x;
+                            v[i + 1] += f.y;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < kChunk; i += 2) h[i / 2] = Elem<T>::pack(v[i], v[i + 1]);
+                    store_row<kChunk / 2>(h, static_cast<uint16_t*>(o.y) + (int64_t)m * o.ldy + n, row ? left : 0, o.vec);
                 }
             }
             if (!ok) break;
-            if (!waited) {                                    // a group with no columns of its own (BN = 64 in 2 bytes)
-                ok = __all_sync(0xffffffffu, mbar_wait(acc_full + buf, (k >> 1) & 1u, abort_flag));
-                if (!ok) break;
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                if constexpr (C::kPair) arrive_even(acc_empty + buf);
-                else mbar_arrive(acc_empty + buf);
-            }
         }
         if (!ok && lane == 0) {
             *abort_flag = 1;
@@ -842,7 +827,9 @@ Sched schedule(int64_t M, int64_t N, int64_t K, int bn, int64_t* cost) {
     Sched s{};
     s.tiles_n = (int)((N + bn - 1) / bn);
     const int rows = bn == 256 ? 2 * kBM : kBM, slots = bn == 256 ? kNumSMs / 2 : kNumSMs;      // two CTAs a tile, or one
-    s.tiles = (int)((M + rows - 1) / rows) * s.tiles_n;
+    s.tiles_m = (int)((M + rows - 1) / rows);
+    s.tiles = s.tiles_m * s.tiles_n;
+    s.inv_band = 1.0f / (float)(kBand * s.tiles_n);
     s.kblocks = (int)((K + kBK - 1) / kBK);
     s.full = s.tiles;
     s.splits = 1;
@@ -973,10 +960,16 @@ int rows_nt(const void* x, int64_t ldx, const void* w, int64_t ldw, int M, int N
     return PMG_OK;
 }
 
-bool vec_ok(const Out& o) {
-    const int per = o.f32 ? 4 : 8;
-    auto ok = [](const void* p, int64_t ld, int per_) { return !p || (!(reinterpret_cast<uintptr_t>(p) & 15) && ld % per_ == 0); };
-    return ok(o.y, o.ldy, per) && ok(o.resid, o.ldr, per) && ok(o.pre, o.ldp, 8);
+// What store_row may use: 2, 1 or 0 by the least aligned of the row starts.
+int vec_ok(const Out& o) {
+    uintptr_t bits = 0;
+    auto see = [&](const void* p, int64_t ld, int esz) {
+        if (p) bits |= reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * esz);
+    };
+    see(o.y, o.ldy, o.f32 ? 4 : 2);
+    see(o.resid, o.ldr, o.f32 ? 4 : 2);
+    see(o.pre, o.ldp, 2);
+    return bits & 15 ? 0 : bits & 31 ? 1 : 2;
 }
 
 template <typename T>
