@@ -3,7 +3,7 @@
 The refiner reads one token feature map per frame (`RefinerEngine.set_frame`: [B, channels, h, w] fp16).  `TokenBlock`
 is the layer that makes or adapts such tokens: every frame is a document of h * w tokens that attend to each other with
 rotated positions; it trains (`torch.autograd`, through the operators' own gradients) and, with `causal`, serves streams
-token by token over a cache (`prefill`, `step`).
+token by token over a cache (`step`, which also takes prompts).
 
     block = TokenBlock(1024, heads=16, key_heads=4).cuda()
     feature = mix_frames(block, encoder_feature)          # [B, 1024, 30, 40] fp16, as set_frame takes it
