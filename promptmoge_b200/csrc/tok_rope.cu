@@ -51,13 +51,18 @@ template <typename T, int V>
 struct Row {
     static constexpr int kWords = V * (int)sizeof(T) / 4;
     uint32_t w[kWords];
-    __device__ __forceinline__ void get(const T* p) {
-        if constexpr (kWords == 4) {
+    // from one place, or its halves from two
+    template <bool WHOLE>
+    __device__ __forceinline__ void get(const T* p, const T* q) {
+        if constexpr (WHOLE && kWords == 4) {
             const uint4 v = *reinterpret_cast<const uint4*>(p);
             w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+        } else if constexpr (kWords == 4) {
+            const uint2 u = *reinterpret_cast<const uint2*>(p), v = *reinterpret_cast<const uint2*>(q);
+            w[0] = u.x; w[1] = u.y; w[2] = v.x; w[3] = v.y;
         } else {
-            const uint2 v = *reinterpret_cast<const uint2*>(p);
-            w[0] = v.x; w[1] = v.y;
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
+            w[1] = *reinterpret_cast<const uint32_t*>(q);
         }
     }
     __device__ __forceinline__ float2 pair(int i) const {
@@ -72,9 +77,17 @@ struct Row {
             w[i] = tok::Elem<T>::pack(f.x, f.y);
         }
     }
-    __device__ __forceinline__ void put(T* p) const {
-        if constexpr (kWords == 4) *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-        else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    template <bool WHOLE>
+    __device__ __forceinline__ void put(T* p, T* q) const {
+        if constexpr (WHOLE && kWords == 4) {
+            *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else if constexpr (kWords == 4) {
+            *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+            *reinterpret_cast<uint2*>(q) = make_uint2(w[2], w[3]);
+        } else {
+            *reinterpret_cast<uint32_t*>(p) = w[0];
+            *reinterpret_cast<uint32_t*>(q) = w[1];
+        }
     }
 };
 
@@ -97,6 +110,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_qk_norm_rope(const __grid_const
     using namespace tok;
     using R = Row<T, V>;
     constexpr int NP = V / 2;
+    auto partner = [](int i) { return IL ? i : (i + NP / 2) % NP; };        // the packed pair with a pair's other sides
     pdl_begin();
     extern __shared__ float sm[];
     const int lane = threadIdx.x & 31, per_warp = 32 / G, gi = lane / G, gl = lane % G;
@@ -108,22 +122,23 @@ __global__ void __launch_bounds__(kThreads, 2) k_qk_norm_rope(const __grid_const
     const int64_t stride = (int64_t)a.blocks[which] * (kThreads / 32) * per_warp;
     const float inv_d = 1.0f / (float)a.D;
     const bool in = gl * V < a.D;
-    const int at = in ? gl * V : 0;
-    const bool turned = at < 2 * a.half, ahead = !IL && at < a.half;      // ahead: the pair's first values
-    const int other = turned && !IL ? (ahead ? at + a.half : at - a.half) : at;
-    const int from = lane - gl + other / V;             // the lane that holds the partners
-    const int ang = IL ? at / 2 : (ahead ? at : at - a.half);
-    uint64_t w2[NP], p2[GRAD ? 1 : NP], acc[GRAD ? NP : 1];        // the weights here and at the partners
+    // A lane's values: V / 2 from `at` on and V / 2 from `bt` on.  They are one run, except where the pairs are (i, i +
+    // rot/2): there a turned lane holds both sides of its pairs, and nothing has to be exchanged.
+    constexpr int HV = V / 2;
+    const bool turned = IL ? gl * V < 2 * a.half : gl * HV < a.half;
+    const int ang = gl * HV;
+    const int at = !in ? 0 : IL || !turned ? gl * V : gl * HV;
+    const int bt = !in ? 0 : IL || !turned ? at + HV : at + a.half;
+    uint64_t w2[NP], acc[GRAD ? NP : 1];                // the weights
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
-        w2[i] = s.w ? pack2(s.w[at + 2 * i], s.w[at + 2 * i + 1]) : pack2(1.0f, 1.0f);
+        const int c = i < NP / 2 ? at + 2 * i : bt + 2 * i - HV;
+        w2[i] = s.w ? pack2(s.w[c], s.w[c + 1]) : pack2(1.0f, 1.0f);
         if constexpr (GRAD) acc[i] = 0;
-        else if constexpr (IL) p2[i] = two(swapped(unpack2(w2[i])));
-        else p2[i] = s.w ? pack2(s.w[other + 2 * i], s.w[other + 2 * i + 1]) : pack2(1.0f, 1.0f);
     }
 
     // A token's angles are two dependent loads away: its position is fetched two items ahead, its angles one.
-    constexpr int NA = (IL ? NP : V) / 2;
+    constexpr int NA = V / 4;
     float2 fc[NA], fs[NA];
     auto token = [&](int64_t base) {
         const int64_t item = min(base + gi, items - 1);
@@ -151,14 +166,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_qk_norm_rope(const __grid_const
         const int n = live && in ? min(heads, s.H - h0) : 0;
         const T* x = reinterpret_cast<const T*>(s.x) + t * s.xt + h0 * s.xh;
         const T* d = GRAD ? reinterpret_cast<const T*>(s.dy) + t * s.yt + h0 * s.yh : nullptr;
-        T* o = reinterpret_cast<T*>(s.out) + t * s.ot + h0 * s.oh + at;
+        T* o = reinterpret_cast<T*>(s.out) + t * s.ot + h0 * s.oh;
         R rx[2][U], rd[2][GRAD ? U : 1];
         auto fetch = [&](int b, int h) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (h + u >= n) continue;
-                rx[b][u].get(x + (h + u) * s.xh + at);
-                if constexpr (GRAD) rd[b][u].get(d + (h + u) * s.yh + at);
+                rx[b][u].template get<IL>(x + (h + u) * s.xh + at, x + (h + u) * s.xh + bt);
+                if constexpr (GRAD) rd[b][u].template get<IL>(d + (h + u) * s.yh + at, d + (h + u) * s.yh + bt);
             }
         };
 #pragma unroll
@@ -189,10 +204,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_qk_norm_rope(const __grid_const
                         z[4 * e + 2] = -fs[e].y;
                         z[4 * e + 3] = fs[e].y;
                     } else {
-                        c[2 * e] = fc[e].x;
-                        c[2 * e + 1] = fc[e].y;
-                        z[2 * e] = ahead ? -fs[e].x : fs[e].x;
-                        z[2 * e + 1] = ahead ? -fs[e].y : fs[e].y;
+                        c[2 * e] = c[HV + 2 * e] = fc[e].x;
+                        c[2 * e + 1] = c[HV + 2 * e + 1] = fc[e].y;
+                        z[2 * e] = -fs[e].x;
+                        z[2 * e + 1] = -fs[e].y;
+                        z[HV + 2 * e] = fs[e].x;
+                        z[HV + 2 * e + 1] = fs[e].y;
                     }
                 }
             }
@@ -202,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_qk_norm_rope(const __grid_const
                 sn[i] = GRAD ? pack2(-z[2 * i], -z[2 * i + 1]) : pack2(z[2 * i], z[2 * i + 1]);
                 if constexpr (!GRAD) {
                     cs[i] = mul2(cs[i], w2[i]);
-                    sn[i] = mul2(sn[i], p2[i]);
+                    sn[i] = mul2(sn[i], IL ? two(swapped(unpack2(w2[i]))) : w2[partner(i)]);
                 }
             }
         }
@@ -213,14 +230,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_qk_norm_rope(const __grid_const
         auto work = [&](int b, int h) {
             uint64_t v[U][NP], g[GRAD ? U : 1][NP];
             float sq[U], gx[U];
-            R ro[IL ? 1 : U];                            // the partners of x, or of its gradient
-            if constexpr (!IL) {
-#pragma unroll
-                for (int u = 0; u < U; ++u)
-#pragma unroll
-                    for (int k = 0; k < R::kWords; ++k)
-                        ro[u].w[k] = __shfl_sync(0xffffffffu, GRAD ? rd[b][GRAD ? u : 0].w[k] : rx[b][u].w[k], from);
-            }
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 uint64_t q2 = 0, x2 = 0;
@@ -230,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_qk_norm_rope(const __grid_const
                     q2 = fma2(v[u][i], v[u][i], q2);
                     if constexpr (GRAD) {            // g = R(p)^T dy
                         const float2 y = rd[b][u].pair(i);
-                        const uint64_t other2 = IL ? two(swapped(y)) : two(ro[IL ? 0 : u].pair(i));
+                        const uint64_t other2 = two(IL ? swapped(y) : rd[b][u].pair(partner(i)));
                         g[u][i] = fma2(two(y), cs[i], mul2(other2, sn[i]));
                         x2 = fma2(mul2(g[u][i], w2[i]), v[u][i], x2);
                     }
@@ -260,12 +269,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_qk_norm_rope(const __grid_const
                         acc[i] = fma2(g[u][i], mul2(v[u][i], r2), acc[i]);
                         f = mul2(fma2(v[u][i], m2, mul2(g[u][i], w2[i])), r2);
                     } else {
-                        const uint64_t other2 = IL ? two(swapped(unpack2(v[u][i]))) : two(ro[IL ? 0 : u].pair(i));
+                        const uint64_t other2 = IL ? two(swapped(unpack2(v[u][i]))) : v[u][partner(i)];
                         f = mul2(fma2(other2, sn[i], mul2(v[u][i], cs[i])), r2);
                     }
                     out.set(i, unpack2(f));
                 }
-                out.put(o + (h + u) * s.oh);
+                out.template put<IL>(o + (h + u) * s.oh + at, o + (h + u) * s.oh + bt);
             }
         };
         // every lane of the warp takes the same turns: the sums are shuffled
@@ -287,8 +296,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_qk_norm_rope(const __grid_const
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
                 const float2 f = unpack2(acc[i]);
-                sm[group * a.D + at + 2 * i] = f.x;
-                sm[group * a.D + at + 2 * i + 1] = f.y;
+                const int c = i < NP / 2 ? at + 2 * i : bt + 2 * i - HV;
+                sm[group * a.D + c] = f.x;
+                sm[group * a.D + c + 1] = f.y;
             }
         }
         __syncthreads();
@@ -443,17 +453,18 @@ int plan_any(RopeArgs& a, cudaStream_t s) {
     return PMG_OK;
 }
 
-// Whether every row and every pair's partner can be read as vectors of V values, and the angles as pairs.
+// Whether a lane's V values can be read as one vector (interleaved) or two, and the angles as pairs.
 bool aligned(const RopeArgs& a, int V, int size, bool grad) {
+    const int unit = a.interleaved ? V : V / 2;
     auto ok = [&](const void* p, int64_t t, int64_t h) {
-        return ((uintptr_t)p % (V * size)) == 0 && t % V == 0 && h % V == 0;
+        return ((uintptr_t)p % (unit * size)) == 0 && t % unit == 0 && h % unit == 0;
     };
     for (const Side& s : a.side) {
         if (s.H == 0) continue;
         if (!ok(s.x, s.xt, s.xh) || !ok(s.out, s.ot, s.oh) || (grad && !ok(s.dy, s.yt, s.yh))) return false;
     }
     if (((uintptr_t)a.cos | (uintptr_t)a.sin) & 7) return false;
-    return a.D % V == 0 && a.D <= 32 * V && (a.interleaved ? (2 * a.half) % V == 0 : a.half % V == 0) && a.half % 2 == 0;
+    return a.D % V == 0 && a.D <= 32 * V && (2 * a.half) % V == 0 && a.half % 2 == 0;
 }
 
 template <typename T, bool GRAD>
