@@ -8,13 +8,13 @@
 //   dw = sum over tokens and heads of g n',   dx = r (g w - n' mean(g w n')).
 //
 // Bound by HBM: forwards one read and one write of q and k, backwards two reads and one write.  A group of lanes owns a
-// row (D values as 16-byte vectors, one a lane) and walks several heads of one token with that token's angles in
-// registers: the angles are 8 bytes per pair against 2 bytes per value, so loading them per head would cost more
-// first-level cache traffic than the heads themselves.  A block works on queries or on keys, so that the weights stay in
-// registers too.  The partner of a value in the other half of the head comes by shuffle, so that registers hold four heads'
-// rows (backwards two) while the next are on their way.
-// Measured: 38,400 tokens, 16 + 4 heads of 64, bf16: 54 us (3.6 TB/s of 6.5), backwards 19,201 tokens, 16 + 4 heads of 128,
-// fp16: 81 us (3.6 TB/s); torch's own sum of as much memory as the first reads runs at 4.0 TB/s.
+// row (D values, 16 bytes a lane) and walks all heads of one token with that token's angles in registers: the angles are 8
+// bytes per pair against 2 bytes per value, so loading them per head would cost more first-level cache traffic than the
+// heads themselves (four heads an item: 72 us and more for the first size below).  A block works on queries or on keys, so
+// that the weights stay in registers too.  Where pairs are (i, i + rot/2) a lane holds V/2 values on either side: the
+// exchange that one run of V values a lane needs took 54 us.  Two heads are worked on while the next two are on their way.
+// Measured: 38,400 tokens, 16 + 4 heads of 64, bf16: 43 us (4.6 TB/s of 6.5; 4.9 with four times the tokens; copying as much
+// takes 31), backwards 19,201 tokens, 16 + 4 heads of 128, fp16: 78 us (3.8 TB/s).
 // Sums and norms are fp32; a value is rounded once, when it is stored.
 #include <algorithm>
 
@@ -23,7 +23,7 @@
 namespace pmg {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256;                         // a block's, backwards and for the general form
 constexpr int kMaxD = 256;
 
 struct Side {                 // queries or keys
@@ -103,10 +103,12 @@ __device__ __forceinline__ int64_t place_of(const RopeArgs& a, int64_t t, bool t
 }
 
 // G lanes a row, V values a lane, pairs of them in the packed fp32 pipe; U heads at once, the next U on their way.
-// IL: interleaved pairs, which lie within a lane's vector.  The cost of a value is what bounds this after HBM: unpacking
-// by the element and fp32 copies of whole rows took 28 instructions a value and 99 us for 38,400 tokens of 20 heads of 64.
+// IL: interleaved pairs, which lie within a lane's vector.  What bounds this after HBM is the chain of a row, so warps count:
+// forwards 28 a SM in blocks of four (72 registers) 43 us, 16 of them with four heads in flight 47, 32 of 64 registers, which
+// spill, 45; backwards 16 a SM in blocks of eight (128 registers) 78 us, 8 of them 106, 24 with one head in flight 90.
+template <bool GRAD> constexpr int kBlock = GRAD ? kThreads : 128;
 template <typename T, int V, int U, bool GRAD, bool IL>
-__global__ void __launch_bounds__(kThreads, 2) k_qk_norm_rope(const __grid_constant__ RopeArgs a, int G) {
+__global__ void __launch_bounds__(kBlock<GRAD>, GRAD ? 2 : 7) k_qk_norm_rope(const __grid_constant__ RopeArgs a, int G) {
     using namespace tok;
     using R = Row<T, V>;
     constexpr int NP = V / 2;
@@ -118,8 +120,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_qk_norm_rope(const __grid_const
     const Side& s = a.side[which];
     const int per_token = a.chunks[which], heads = a.heads[which];
     const int64_t items = a.T * per_token;
-    const int64_t first = (int64_t)(blockIdx.x - (which ? a.blocks[0] : 0)) * (kThreads / 32) + (threadIdx.x >> 5);
-    const int64_t stride = (int64_t)a.blocks[which] * (kThreads / 32) * per_warp;
+    const int64_t first = (int64_t)(blockIdx.x - (which ? a.blocks[0] : 0)) * (kBlock<GRAD> / 32) + (threadIdx.x >> 5);
+    const int64_t stride = (int64_t)a.blocks[which] * (kBlock<GRAD> / 32) * per_warp;
     const float inv_d = 1.0f / (float)a.D;
     const bool in = gl * V < a.D;
     // A lane's values: V / 2 from `at` on and V / 2 from `bt` on.  They are one run, except where the pairs are (i, i +
@@ -129,6 +131,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_qk_norm_rope(const __grid_const
     const int ang = gl * HV;
     const int at = !in ? 0 : IL || !turned ? gl * V : gl * HV;
     const int bt = !in ? 0 : IL || !turned ? at + HV : at + a.half;
+    const int ab = bt - at;
     uint64_t w2[NP], acc[GRAD ? NP : 1];                // the weights
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
@@ -158,31 +161,28 @@ __global__ void __launch_bounds__(kThreads, 2) k_qk_norm_rope(const __grid_const
         next_place = place_of(a, token(first * per_warp + stride), gl == 0);
     }
 
+    R rx[2][U] = {}, rd[2][GRAD ? U : 1] = {};          // rows that are not read keep what they held, and count as 0
     for (int64_t base = first * per_warp; base < items; base += stride) {
         const bool live = base + gi < items;
         const int64_t item = live ? base + gi : items - 1;
         const int64_t t = per_token == 1 ? item : item / per_token;
         const int h0 = (int)(item - t * per_token) * heads;
         const int n = live && in ? min(heads, s.H - h0) : 0;
-        const T* x = reinterpret_cast<const T*>(s.x) + t * s.xt + h0 * s.xh;
-        const T* d = GRAD ? reinterpret_cast<const T*>(s.dy) + t * s.yt + h0 * s.yh : nullptr;
-        T* o = reinterpret_cast<T*>(s.out) + t * s.ot + h0 * s.oh;
-        R rx[2][U], rd[2][GRAD ? U : 1];
+        // where the next head is read and written
+        const T* x = reinterpret_cast<const T*>(s.x) + t * s.xt + h0 * s.xh + at;
+        const T* d = GRAD ? reinterpret_cast<const T*>(s.dy) + t * s.yt + h0 * s.yh + at : nullptr;
+        T* o = reinterpret_cast<T*>(s.out) + t * s.ot + h0 * s.oh + at;
         auto fetch = [&](int b, int h) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                if (h + u >= n) continue;
-                rx[b][u].template get<IL>(x + (h + u) * s.xh + at, x + (h + u) * s.xh + bt);
-                if constexpr (GRAD) rd[b][u].template get<IL>(d + (h + u) * s.yh + at, d + (h + u) * s.yh + bt);
+                if (h + u < n) {
+                    rx[b][u].template get<IL>(x, x + ab);
+                    if constexpr (GRAD) rd[b][u].template get<IL>(d, d + ab);
+                }
+                x += s.xh;
+                if constexpr (GRAD) d += s.yh;
             }
         };
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                rx[b][u] = R{};
-                if constexpr (GRAD) rd[b][u] = R{};
-            }
         fetch(0, 0);
         // this token's turn: the rotation's sign in sn, and forwards the weights in both
         uint64_t cs[NP], sn[NP];
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_qk_norm_rope(const __grid_const
                 }
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
+            for (int u = 0; u < U; ++u, o += s.oh) {
                 if (h + u >= n) continue;
                 const float r = rsqrtf(fmaf(sq[u], inv_d, a.eps));
                 const float m = -gx[u] * r * r * inv_d;                  // -n' mean(g w n') = x r m
@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_qk_norm_rope(const __grid_const
                     }
                     out.set(i, unpack2(f));
                 }
-                out.template put<IL>(o + (h + u) * s.oh + at, o + (h + u) * s.oh + bt);
+                out.template put<IL>(o, o + ab);
             }
         };
         // every lane of the warp takes the same turns: the sums are shuffled
@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_qk_norm_rope(const __grid_const
     if constexpr (GRAD) {
         if (a.part == nullptr) return;
         // sums over this block's groups in a fixed order, one row of partials a block
-        const int groups = kThreads / G, group = threadIdx.x / G;
+        const int groups = kBlock<GRAD> / G, group = threadIdx.x / G;
         if (in) {
 #pragma unroll
             for (int i = 0; i < NP; ++i) {
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_qk_norm_rope(const __grid_const
             }
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < a.D; i += kThreads) {
+        for (int i = threadIdx.x; i < a.D; i += kBlock<GRAD>) {
             float v = 0.0f;
             for (int g = 0; g < groups; ++g) v += sm[g * a.D + i];
             a.part[(int64_t)blockIdx.x * a.D + i] = v;
@@ -425,7 +425,7 @@ int plan(RopeArgs& a, cudaStream_t s) {
     // Heads per item: a token's angles are reused over an item's heads, but a small batch needs the items.  All heads
     // while that leaves 16 warps a SM, else one.
     const bool wide = a.T * G >= (int64_t)kNumSMs * 512;
-    const int64_t per_block = (int64_t)(kThreads / 32) * (32 / G);
+    const int64_t per_block = (int64_t)(kBlock<GRAD> / 32) * (32 / G);
     int64_t want[2];
     for (int i = 0; i < 2; ++i) {
         a.heads[i] = wide ? a.side[i].H : 1;
@@ -433,11 +433,11 @@ int plan(RopeArgs& a, cudaStream_t s) {
         want[i] = (a.T * a.chunks[i] + per_block - 1) / per_block;
     }
     share_blocks(a, want, GRAD);
-    const size_t smem = GRAD ? (size_t)(kThreads / G) * a.D * sizeof(float) : 0;
+    const size_t smem = GRAD ? (size_t)(kBlock<GRAD> / G) * a.D * sizeof(float) : 0;
     const int blocks = a.blocks[0] + a.blocks[1];
-    constexpr int U = GRAD ? 2 : 4;
-    if (a.interleaved) k_qk_norm_rope<T, V, U, GRAD, true><<<blocks, kThreads, smem, s>>>(a, G);
-    else k_qk_norm_rope<T, V, U, GRAD, false><<<blocks, kThreads, smem, s>>>(a, G);
+    constexpr int U = 2;
+    if (a.interleaved) k_qk_norm_rope<T, V, U, GRAD, true><<<blocks, kBlock<GRAD>, smem, s>>>(a, G);
+    else k_qk_norm_rope<T, V, U, GRAD, false><<<blocks, kBlock<GRAD>, smem, s>>>(a, G);
     PMG_LAUNCH_CHECK();
     return PMG_OK;
 }
