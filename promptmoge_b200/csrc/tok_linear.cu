@@ -13,7 +13,7 @@
 //   k_split_sum   the last wave of tiles, when it would leave most SMs idle, is cut along K into fp32 partials that this
 //             kernel adds in split order (no atomics: results do not depend on timing) and takes through the epilogue.
 // Measured: 38,400 x 1024 x 4096 with gelu 249 us (1295 TFLOP/s) alone and 288 in long runs, where the power limit holds the
-// clock at 1.3 GHz (without the activation 263; cuBLAS 274); its gradients over 9600 rows 167 us, 1200 x 1024 x 1024 9 us, one
+// clock at 1.3 GHz (without the activation 263; cuBLAS 274); its gradients over 9600 rows 162 us, 1200 x 1024 x 1024 9 us, one
 // row 1024 -> 4096 3.4 us (2.5 TB/s).  With eight warps that staged their rows in shared memory: 278 and 321 us.
 // dz is rounded to the operands' 16-bit type before its two products (tensor cores take no other), db is summed from the
 // unrounded fp32 values.
@@ -77,7 +77,7 @@ __device__ __forceinline__ void activate(int act, float* v) {
 }
 
 // dz = dy act'(z) for 8 values.  gelu' = Phi(z) + z phi(z): Phi by the polynomial, phi by one exp2; with erff and expf this
-// pass took 75 us for 9600 x 4096, four fifths of it arithmetic; now 55 (4.3 TB/s).
+// pass took 75 us for 9600 x 4096, four fifths of it arithmetic; now 48 (4.9 TB/s).
 __device__ __forceinline__ void times_slope(int act, float (&g)[8], const float (&z)[8]) {
     if (act == PMG_ACT_GELU) {
 #pragma unroll
@@ -707,7 +707,7 @@ __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
 // dz = dy act'(z) rounded to T into dst (null: not wanted) with its row padding zeroed, and this block's column sums of
 // the unrounded dz into part [row blocks][N] (null: not wanted).
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) k_act_grad(const T* __restrict__ dy, int64_t ldy, const T* __restrict__ pre,
+__global__ void __launch_bounds__(256, 4) k_act_grad(const T* __restrict__ dy, int64_t ldy, const T* __restrict__ pre,
                                                   int64_t ldp, int64_t M, int N, int act, T* __restrict__ dst,
                                                   int64_t ldd, int padded, int64_t rows_per_block,
                                                   float* __restrict__ part) {
@@ -728,7 +728,7 @@ __global__ void __launch_bounds__(256) k_act_grad(const T* __restrict__ dy, int6
         return make_uint4(w[0], w[1], w[2], w[3]);
     };
     if (n < padded) {
-        constexpr int U = 4;                                          // rows on their way at once
+        constexpr int U = 2;        // rows on their way at once; 4 of them leave half the warps, and took 4 us longer
         for (int64_t m0 = r0 + rg; m0 < r1; m0 += U * kStripRows) {
             uint4 dr[U], zr[U];
 #pragma unroll
@@ -993,7 +993,7 @@ struct GradPlan {
 GradPlan grad_plan(int64_t M, int64_t N, bool act, bool dy_ok) {
     GradPlan p;
     const int64_t strips = (N + kStripCols - 1) / kStripCols;
-    const int64_t want = std::max<int64_t>(1, kNumSMs * 8 / strips);
+    const int64_t want = std::max<int64_t>(1, kNumSMs * 4 / strips);      // blocks for one wave, four a SM
     p.rows_per_block = std::max<int64_t>(kStripRows * 2, (M + want - 1) / want);
     p.row_blocks = std::max<int64_t>(1, (M + p.rows_per_block - 1) / p.rows_per_block);
     p.dz = act || !dy_ok;
