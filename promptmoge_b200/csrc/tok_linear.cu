@@ -13,7 +13,7 @@
 //   k_split_sum   the last wave of tiles, when it would leave most SMs idle, is cut along K into fp32 partials that this
 //             kernel adds in split order (no atomics: results do not depend on timing) and takes through the epilogue.
 // Measured: 38,400 x 1024 x 4096 with gelu 249 us (1295 TFLOP/s) alone and 288 in long runs, where the power limit holds the
-// clock at 1.3 GHz (without the activation 263; cuBLAS 274); its gradients over 9600 rows 162 us, 1200 x 1024 x 1024 9 us, one
+// clock at 1.3 GHz (without the activation 263; cuBLAS 274); its gradients over 9600 rows 162 us, 1200 x 1024 x 1024 8 us, one
 // row 1024 -> 4096 3.4 us (2.5 TB/s).  With eight warps that staged their rows in shared memory: 278 and 321 us.
 // dz is rounded to the operands' 16-bit type before its two products (tensor cores take no other), db is summed from the
 // unrounded fp32 values.
@@ -33,7 +33,7 @@ using namespace tok;
 // Phi(-a) = 2^q(a) for a >= 0: q is smooth, so a short polynomial holds it.  Degree 5, of least largest
 // max(a, 1) |2^q(a) - Phi(-a)| on [0, 7] (linear programming on a grid); |error| of Phi and of a Phi <= 7e-7 evaluated in
 // fp32, and no output type here resolves more than 2^-11.  q falls on to -399 at 16, so that Phi(-16) is 0.  Then
-// gelu(x) = max(x, 0) - |x| Phi(-|x|).  A product whose tiles keep the tensor cores busy runs at the power limit, where each
+// gelu(x) = max(x, 0) - |x| Phi(-|x|), with its limit 0 at -inf.  A product whose tiles keep the tensor cores busy runs at the power limit, where each
 // operation per output counts as energy: 9 of them in place of the 17 of a polynomial in x^2 for Phi itself.
 __device__ constexpr float kTail[6] = {-1.00000191f, -1.151052f, -0.459414065f, -0.0523432381f, 0.00728237722f, -0.000500259455f};
 
@@ -819,10 +819,11 @@ bool tma_ok(const void* p, int64_t ld) { return !(reinterpret_cast<uintptr_t>(p)
 
 constexpr int kFewRows = 32;
 
-// How a product is cut.  In cycles of one SM, measured: a K block takes 512 with tiles of 128 x 256 (the products' own time)
-// and 390 with narrower ones (the loads'); the epilogue of the last tile about 25 a column; a last wave cut along K costs its
-// second kernel, about 7000.  With tiles of 256 the gradient of a 4096 x 1024 weight over 9600 rows takes one wave of 128 tiles
-// (58 us), with 128 two of 256 tiles (92 us); 1200 x 1024 x 1024 takes 6.8 us with 80 tiles of 128, 9 us with 40 of 256.
+// How a product is cut.  In cycles of one SM, measured: a K block takes 512 with tiles of 256 x 256 by two CTAs (the
+// products' own time) and 390 with narrower ones (the loads'); the epilogue of the last tile about 25 a column; a last wave
+// cut along K costs its second kernel, about 7000.  The gradient of a 4096 x 1024 weight over 9600 rows takes 57 us with
+// tiles of 256 (64 on 74 pairs), 76 with 128; 1200 x 1024 x 1024 takes 8.3 us with 80 tiles of 128, 12 with 20 of 256;
+// 600 x 1024 x 1024 takes 7.3 us with tiles of 64 columns, 8.0 with 128.
 Sched schedule(int64_t M, int64_t N, int64_t K, int bn, int64_t* cost) {
     Sched s{};
     s.tiles_n = (int)((N + bn - 1) / bn);

@@ -217,3 +217,37 @@ def test_linear_refusals():
         tokens.linear(x[:1].expand(4, 16), w)
     with pytest.raises(ValueError):
         tokens.linear_grad(r, x, w, activation="gelu")
+
+
+@pytest.mark.parametrize("M", [2, 20, 300])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["relu", "silu", "gelu"])
+def test_activation_over_its_whole_range(M, dtype, act):
+    """Pre-activations from far below to far above 0 (the bias alone, the product being 0), with +inf and NaN."""
+    from promptmoge_b200 import tokens
+    z = torch.cat([torch.linspace(-9, 9, 301), torch.tensor([-6e4, -300.0, -40.0, -17.0, -16.0, -15.9, 16.0, 300.0, 6e4])])
+    z = z.to(dtype).cuda()
+    x, w = torch.zeros(M, 24, dtype=dtype, device="cuda"), torch.zeros(len(z), 24, dtype=dtype, device="cuda")
+    want = ACT[act](z.double())
+    y = tokens.linear(x, w, z, activation=act)
+    assert ((y.double() - want).abs() <= U[dtype] * want.abs() + 2.0 ** -22 * want.abs() + 1.5e-5).all()
+    z = torch.tensor([float("inf"), float("nan"), 1.0] * 20, dtype=dtype, device="cuda")
+    y = tokens.linear(x, torch.zeros(60, 24, dtype=dtype, device="cuda"), z, activation=act)
+    assert (y[:, 0::3] == float("inf")).all() and torch.isnan(y[:, 1::3]).all() and torch.isfinite(y[:, 2::3]).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(40, 48, 64), (200, 130, 96), (2400, 1536, 1024)])
+@pytest.mark.parametrize("off,ld", [(0, 1600), (16, 1616), (8, 1608), (1, 1601)])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+def test_output_and_residual_rows_on_any_boundary(M, N, K, off, ld, out):
+    """Rows of 32-byte, 16-byte and element alignment, residual and output in one larger tensor, nothing else touched."""
+    from promptmoge_b200 import tokens
+    x, w, b, r = _inputs(M, N, K, torch.bfloat16)
+    big = torch.full((M, ld), 5.0, dtype=out, device="cuda")
+    place = big[:, off:off + N]
+    place.copy_(r)
+    want = x.double() @ w.double().t() + b.double() + r.double()
+    tokens.linear(x, w, b, residual=place, out=place)
+    tol = U[out] * want.abs() + _slack(x, w, K) + 2.0 ** -22 * (want.abs() + r.double().abs()) + 1e-6
+    assert ((place.double() - want).abs() <= tol).all()
+    assert (big[:, :off] == 5).all() and (big[:, off + N:] == 5).all()
