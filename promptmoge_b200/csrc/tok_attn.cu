@@ -407,10 +407,10 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
                 if (CAP && !BIAS && top > -INFINITY) top = tanh_raw(a, top);
                 if (j == 0) {
                     m = top;
-                } else if (__any_sync(0xffffffffu, (top - m) * c > kGrow)) {
-                    const float grown = fmaxf(m, top);
-                    const float f = grown == m ? 1.0f : ex2((m - grown) * c);
-                    m = grown;
+                } else if (const bool grew = (top - m) * c > kGrow; __any_sync(0xffffffffu, grew)) {
+                    // only the rows that grew, so that no row's bits follow from what its neighbours see
+                    const float f = grew ? ex2((m - top) * c) : 1.0f;
+                    if (grew) m = top;
                     sum = mul2(sum, pack2(f, f));
                     sum2 = mul2(sum2, pack2(f, f));
                     tc_fence_after();
@@ -659,19 +659,18 @@ __global__ void __launch_bounds__(kFewThreads, Few<DP>::kCtas)
                         s[4 * t + e] = x;
                         top[h] = fmaxf(top[h], x);
                     }
-                bool grow = false;
+                bool grew[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
                     top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-                    grow = grow || (top[h] - m[h]) * c > kGrow;
+                    grew[h] = (top[h] - m[h]) * c > kGrow;
                 }
-                if (__any_sync(0xffffffffu, grow)) {
+                if (__any_sync(0xffffffffu, grew[0] || grew[1])) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const float grown = fmaxf(m[h], top[h]);
-                        const float f = grown == m[h] ? 1.0f : ex2((m[h] - grown) * c);
-                        m[h] = grown;
+                        const float f = grew[h] ? ex2((m[h] - top[h]) * c) : 1.0f;
+                        if (grew[h]) m[h] = top[h];
                         l[h] *= f;
 #pragma unroll
                         for (int x = 0; x < DP / 8; ++x) {
