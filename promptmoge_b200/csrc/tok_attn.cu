@@ -407,10 +407,11 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
                 if (CAP && !BIAS && top > -INFINITY) top = tanh_raw(a, top);
                 if (j == 0) {
                     m = top;
-                } else if (const bool grew = (top - m) * c > kGrow; __any_sync(0xffffffffu, grew)) {
+                } else if (__any_sync(0xffffffffu, (top - m) * c > kGrow)) {
                     // only the rows that grew, so that no row's bits follow from what its neighbours see
-                    const float f = grew ? ex2((m - top) * c) : 1.0f;
-                    if (grew) m = top;
+                    if (!((top - m) * c > kGrow)) top = m;
+                    const float f = top == m ? 1.0f : ex2((m - top) * c);
+                    m = top;
                     sum = mul2(sum, pack2(f, f));
                     sum2 = mul2(sum2, pack2(f, f));
                     tc_fence_after();
