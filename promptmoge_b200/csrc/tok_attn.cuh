@@ -177,15 +177,16 @@ __device__ __forceinline__ void bias_scores(float (&s)[N], float c, float slope,
 // 2^x of a pair: the special function unit (16 a cycle and SM), or a polynomial on the fp32 pipe beside it.  2^x = 2^n 2^f,
 // n the nearest integer (by adding 1.5 2^23, which leaves it in the low bits), f in [-1/2, 1/2]; 2^f = 1 + f q(f), q of
 // degree 3 with least largest relative error of the whole, 2.9e-6 in fp32 (iteratively reweighted least squares in the
-// Chebyshev basis); its exponent field is raised by n.  x below -127, -inf with it, gives exactly 0 (at -127, f is 0 and
-// the exponent field, 127, is lowered by 127); x up to 127.
+// Chebyshev basis); the factor 2^n is put together from its exponent field and multiplied, which keeps a NaN (adding n to
+// the exponent field of 2^f does not).  x below -126.5, -inf with it, gives exactly 0 (n is -127 there, and the field 0);
+// x up to 127; +inf and NaN give NaN.
 __device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
     const float2 f = unpack2(x);
     return pack2(ex2(f.x), ex2(f.y));
 }
 __device__ __forceinline__ uint64_t ex2_poly(uint64_t x) {
     const float2 v = unpack2(x);
-    x = pack2(fmaxf(v.x, -127.0f), fmaxf(v.y, -127.0f));
+    x = pack2(max_nan(v.x, -127.0f), max_nan(v.y, -127.0f));
     const uint64_t t = add2(x, pack2(12582912.0f, 12582912.0f));
     const uint64_t f = fma2(add2(t, pack2(-12582912.0f, -12582912.0f)), pack2(-1.0f, -1.0f), x);
     uint64_t p = pack2(9.582852812e-03f, 9.582852812e-03f);
@@ -193,9 +194,8 @@ __device__ __forceinline__ uint64_t ex2_poly(uint64_t x) {
     p = fma2(p, f, pack2(2.402409862e-01f, 2.402409862e-01f));
     p = fma2(p, f, pack2(6.931241933e-01f, 6.931241933e-01f));
     p = fma2(p, f, pack2(1.0f, 1.0f));
-    const float2 tf = unpack2(t), pf = unpack2(p);
-    return pack2(__int_as_float(__float_as_int(pf.x) + (__float_as_int(tf.x) << 23)),
-                 __int_as_float(__float_as_int(pf.y) + (__float_as_int(tf.y) << 23)));
+    const float2 tf = unpack2(t);
+    return mul2(p, pack2(__int_as_float((__float_as_int(tf.x) << 23) + 0x3f800000), __int_as_float((__float_as_int(tf.y) << 23) + 0x3f800000)));
 }
 // Which of 16 pairs take the polynomial: with `share` of them the fp32 pipe (2 cycles a packed instruction) and the special
 // function unit (16 a pair) finish together.  A cap leaves the fp32 pipe no room.

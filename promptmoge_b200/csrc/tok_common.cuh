@@ -80,6 +80,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
+// The larger; NaN where either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 
 // kind::f16 instruction descriptor: D = fp32, A and B of one 16-bit format, operands K-major or MN-major.
 __host__ __device__ constexpr uint32_t idesc16(int fmt, int M, int N, bool a_mn, bool b_mn) {

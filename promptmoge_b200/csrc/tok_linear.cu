@@ -37,12 +37,6 @@ using namespace tok;
 // operation per output counts as energy: 9 of them in place of the 17 of a polynomial in x^2 for Phi itself.
 __device__ constexpr float kTail[6] = {-1.00000191f, -1.151052f, -0.459414065f, -0.0523432381f, 0.00728237722f, -0.000500259455f};
 
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-
 // Phi(-|x|) for two values, and the bounded |x| that it was taken at
 __device__ __forceinline__ float2 tail_pair(float a, float b, float& xa, float& xb) {
     xa = fminf(fabsf(a), 16.0f);
