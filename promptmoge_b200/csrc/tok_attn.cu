@@ -404,7 +404,8 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
                     if (!ok) break;
                     top = fmaxf(top, other);
                 }
-                if (CAP && !BIAS && top > -INFINITY) top = tanh_raw(a, top);
+                // where the row sees a key of this tile: a raw product of -inf stands for -cap, not for no key
+                if (CAP && !BIAS && C::kBT * j <= lim) top = tanh_raw(a, top);
                 if (j == 0) {
                     m = top;
                 } else if (__any_sync(0xffffffffu, (top - m) * c > kGrow)) {

@@ -56,3 +56,24 @@ def test_a_row_that_is_not_finite_shows_in_the_gradients(d, dtype, mask):
         assert torch.equal(dv[~seen], clean[2][~seen]) and torch.equal(dk[~seen], clean[1][~seen])
         rest = torch.arange(lq, device="cuda") != i
         assert torch.equal(dq[rest], clean[0][rest]) and torch.equal(dq[:, 0], clean[0][:, 0])
+
+
+@pytest.mark.parametrize("lq,hq,hk", [(100, 2, 1), (4, 4, 1)])
+@pytest.mark.parametrize("d,dtype", [(64, torch.bfloat16), (128, torch.float16)])
+@pytest.mark.parametrize("infinite", [64, 128, 200])
+@pytest.mark.parametrize("slopes", [False, True])
+def test_capped_scores_of_minus_infinity_count_as_the_cap(lq, hq, hk, d, dtype, infinite, slopes):
+    """tanh takes -inf to -cap, a score like any other, also where a row's first keys have nothing else.  Tolerances as in
+    the forward test, with the scores' size bounded by the cap (and the distances)."""
+    from promptmoge_b200 import tokens
+    lk, cap = 200, 1.0
+    q, k, v, cq, ck, sl = make([lq], [lk], hq, hk, d, dtype, slopes=True)
+    q[:, :, 0] = 1
+    k[:infinite] = 0
+    k[:infinite, :, 0] = -float("inf")
+    kw = dict(softcap=cap, slopes=sl / 64 if slopes else None)
+    o, lse = tokens.attention(q, k, v, cq, ck, lq, lk, **kw)
+    want, want_lse, mass = reference(q, k, v, cq, ck, d ** -0.5, **kw)
+    e = 2.0 ** -18 * (1 + cap + (float(sl.max()) / 64 * lk if slopes else 0))
+    assert ((lse.double() - want_lse).abs() <= e).all()
+    assert ((o.double() - want).abs() <= U[dtype] * want.abs() + (U[dtype] + e) * mass + 1e-7).all()
