@@ -348,7 +348,8 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
             const int tiles_k = w ? x.n1 : x.n0;
             const int i = x.r0 + 128 * w + (warp & 3) * 32 + lane;        // this thread's row in the document
             const int lim = last_key(a, x.sp, i);
-            const int warp_min = __reduce_min_sync(0xffffffffu, i < x.sp.lq ? lim : INT32_MAX);
+            // With a cap, rows behind the document count as masked: neither they nor hidden keys choose tanh's form.
+            const int warp_min = __reduce_min_sync(0xffffffffu, CAP || i < x.sp.lq ? lim : INT32_MAX);
             const float slope = BIAS ? a.slopes[x.head] * kLog2e : 0.0f;
             const float place = (float)(i + x.sp.lk - x.sp.lq);
             float m = -INFINITY;
@@ -375,7 +376,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
                     }
                 };
                 auto score = [&](int q) {                 // raw products to what the softmax takes
-                    if (CAP) tanh_scores<32>(a, s, BIAS ? tanh_fast(a, largest<32>(s)) : fast);
+                    if (CAP) tanh_scores<32>(a, s, BIAS ? !masked && tanh_fast(a, largest<32>(s)) : fast);
                     if (BIAS) bias_scores<32>(s, CAP ? a.cap2 : a.scale2, slope, place - (float)(j0 + 32 * q));
                     mask(q);
                 };
@@ -395,7 +396,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
                 top = fmaxf(top, top2);
                 if (C::kHalves == 2) tell(top);
                 if (CAP && !BIAS) {
-                    fast = tanh_fast(a, big);
+                    fast = !masked && tanh_fast(a, big);
                     score(1);
                 }
                 if (C::kHalves == 2) {
@@ -603,13 +604,14 @@ __global__ void __launch_bounds__(kFewThreads, Few<DP>::kCtas)
     } else {
         // queries: rows g and g + 8 as left operands
         uint32_t qf[DP / 16][4];
-        int lim[2];
+        int lim[2], whole = INT32_MAX;                   // whole: the last key that every row sees
         float place[2], slope[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const int r = g + 8 * h, i = r / a.group, hd = kvh * a.group + r % a.group;
             const bool on = r < rows;
             lim[h] = on ? min(last_key(a, sp, i), kend - 1) : -1;
+            if (on) whole = min(whole, lim[h]);
             place[h] = (float)(i + sp.lk - sp.lq);
             slope[h] = BIAS && on ? a.slopes[hd] * kLog2e : 0.0f;
             const T* p = static_cast<const T*>(hq.p) + (sp.q0 + (int64_t)i) * hq.tok + hd * hq.head;
@@ -621,6 +623,7 @@ __global__ void __launch_bounds__(kFewThreads, Few<DP>::kCtas)
                     qf[x][h + 2 * e] = on && d < a.D ? *reinterpret_cast<const uint32_t*>(p + d) : 0u;
                 }
         }
+        whole = __reduce_min_sync(0xffffffffu, whole);
         // ldmatrix: lane l gives the row of matrix l / 8; K: (keys 0-7, 8-15) x (first, second 8 values), V: the same rows
         const int kr = warp * 16 + (lane & 7) + ((lane >> 4) << 3), kc = (lane >> 3) & 1;
         const int vr = warp * 16 + (lane & 7) + (((lane >> 3) & 1) << 3), vc = lane >> 4;
@@ -648,7 +651,8 @@ __global__ void __launch_bounds__(kFewThreads, Few<DP>::kCtas)
                     }
                     __syncwarp();
                 }
-                if (CAP) tanh_scores<8>(a, s, tanh_fast(a, largest<8>(s)));
+                // as by the tile: keys hidden from a row have no part in the choice of tanh's form
+                if (CAP) tanh_scores<8>(a, s, j0 + 15 <= whole && tanh_fast(a, largest<8>(s)));
                 float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                 for (int t = 0; t < 2; ++t)

@@ -382,7 +382,8 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
             tmem_ld32(ts, reinterpret_cast<uint32_t*>(p));
             tmem_wait_ld();
             if constexpr (CAP) {
-                tanh_scores<32>(a, p, tanh_fast(a, largest<32>(p)));
+                // rows and columns that take no part do not choose tanh's form
+                tanh_scores<32>(a, p, !masked && tanh_fast(a, live ? largest<32>(p) : 0.0f));
 #pragma unroll
                 for (int k = 0; k < 32; ++k) u[k] = fmaf(-p[k], p[k], 1.0f);             // the cap's slope
             }

@@ -23,3 +23,44 @@ def test_rows_do_not_follow_from_keys_that_others_see(lq, lk, hq, hk, d, dtype):
         o, lse = tokens.attention(q, k, v, cq, ck, lq, lk, causal=True)
         got.append((o[:first - lk + lq], lse[:, :first - lk + lq]))
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.parametrize("lq", [[100, 3, 40], [4, 3, 2]])                 # by the tile; few rows
+@pytest.mark.parametrize("d,dtype", [(64, torch.bfloat16), (128, torch.float16)])
+@pytest.mark.parametrize("slopes", [False, True])
+@pytest.mark.parametrize("causal", [False, True])
+def test_capped_scores_ignore_what_lies_outside(lq, d, dtype, slopes, causal):
+    """Which form of tanh a row takes must not follow from keys behind a length, or from the neighbours' rows."""
+    from promptmoge_b200 import tokens
+    lk, room = [90, 40, 70], [110, 41, 200]
+    q, k, v, cq, ck, sl = make(lq, lk, 4, 1, d, dtype, slopes=True, room=room)
+    q *= 0.25                                              # scores well below half the cap
+    do = torch.randn_like(q)
+    used = torch.tensor(lk, dtype=torch.int32, device="cuda")
+    kw = dict(causal=causal, softcap=20.0, slopes=sl if slopes else None, k_len=used)
+    mine = slice(lq[0], lq[0] + lq[1])                     # the second document; the others change with the spare rows
+    got = []
+    for fill in (0.0, 200.0, float("nan")):
+        for n, r, c in zip(lk, room, ck.tolist()):
+            k[c + n:c + r] = fill
+        if fill:
+            q[:lq[0]] = 200.0
+            q[lq[0] + lq[1]:] = -200.0
+            k[room[0] + room[1]:] = fill
+        o, lse = tokens.attention(q, k, v, cq, ck, max(lq), max(room), **kw)
+        dq, dk, dv = tokens.attention_grad(do, o, lse, q, k, v, cq, ck, max(lq), max(room), **kw)
+        keys = slice(room[0], room[0] + lk[1])
+        got.append([t.clone() for t in (o[mine], lse[:, mine], dq[mine], dk[keys], dv[keys])])
+    for other in got[1:]:
+        for name, a, b in zip(("o", "lse", "dq", "dk", "dv"), got[0], other):
+            assert torch.equal(a, b), name
+    # keys that the causal mask hides from the first rows, huge against zero
+    if causal:
+        q, k, v, cq, ck, _ = make([160], [160], 2, 1, d, dtype)
+        q *= 0.25
+        firsts = []
+        for fill in (0.0, 200.0):
+            k[100:] = fill
+            o, lse = tokens.attention(q, k, v, cq, ck, 160, 160, causal=True, softcap=20.0)
+            firsts.append((o[:96], lse[:, :96]))
+        assert all(torch.equal(a, b) for a, b in zip(*firsts))
