@@ -10,8 +10,8 @@
 // is transposed or sent through shared memory.  Scores are computed twice for it (7 products a tile instead of 5), and
 // in return no gradient is summed by atomics: results do not depend on timing, and no fp32 copy of dQ is kept.
 // P and dS are rounded to the operands' 16-bit type (tensor cores take no other); fp16 values are kept times a power of
-// two, 2^15 for P (which is at most 1) and for dS the one that |dS| <= 2 max|dO| max|V| allows, so that small gradients
-// do not turn subnormal.
+// two, 2^15 for P (which is at most 1) and for dS the one that |dS| <= 2 max|dO| max|V| over its document allows, so that
+// small gradients do not turn subnormal.
 //
 // Bound by the chain of a step, as forwards (tensor core 37 % active, issue slots 59 %).  Measured: 8 frames of up to 1200
 // tokens, 16 heads of 64 over 4 key heads, distance bias: 176 us; 8192 tokens, 16 heads of 64: 770 TFLOP/s of the 5
@@ -25,102 +25,137 @@ namespace {
 
 using namespace tok;
 
-constexpr int kStatBlocks = kNumSMs * 4;
+// The factor that fp16 dS carries follows from a document's largest |dO| and |V|, of its own rows alone, so that neither
+// another document nor what lies behind a length reaches it.  Blocks of the statistics take `rows` tokens of one document, and
+// leave the largest square of them for the document's CTAs to go through: those of dO at the block's first query, those of
+// V at eight places for every query of the document (where its keys are more than that, a block takes several turns).
+struct Stat {
+    int q_rows, k_rows;      // tokens of a block
+    int64_t q_blocks;        // blocks of queries, before those of keys
+    float2* stat;            // [Hq][Tq] lse log2 e (infinite for empty rows), delta
+    float* norms;            // [Tq] of dO, [8 Tq] of V
+};
+
+__host__ __device__ __forceinline__ int stat_rows(int heads) { return heads >= 16 ? 8 : 128 / heads; }
+
+__device__ __forceinline__ int64_t stat_places(const Span& s, int k_rows) {
+    return min((int64_t)(s.lk + k_rows - 1) / k_rows, 8 * (int64_t)s.lq);
+}
 
 struct Grad {
     Attn a;
     float scale;
-    const float2* stat;      // [Hq][stat_ld] lse log2 e (infinite for empty rows), delta
-    const float* norms;      // fp16: [2][kStatBlocks] largest |dO|^2 and |V|^2 of each block's rows
-    int64_t stat_ld;
+    Stat st;
     void *dq, *dk, *dv;
     int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;      // of dq, dk, dv
     int key_blocks;
 };
 
+struct Heads {
+    const void* p;
+    int64_t tok, head;
+};
+
+// The document of block t where documents have a block for every `rows` tokens begun, and one more at most; and which of its
+// blocks that is.
+__device__ __forceinline__ int stat_block(const int32_t* cu, int docs, int rows, int64_t t, int64_t* which) {
+    int lo = 0, hi = docs;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if ((int64_t)(cu[mid] / rows) + mid <= t) lo = mid;
+        else hi = mid;
+    }
+    *which = t - ((int64_t)(cu[lo] / rows) + lo);
+    return lo;
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(256)
-    k_attn_stat(const T* __restrict__ dout, int64_t do_tok, int64_t do_head, const T* __restrict__ o, int64_t o_tok,
-                int64_t o_head, const float* __restrict__ lse, const T* __restrict__ v, int64_t v_tok, int64_t v_head,
-                int64_t Tq, int64_t Tk, int Hq, int Hk, int D, float2* __restrict__ stat, int64_t stat_ld,
-                float* __restrict__ norms) {
+    k_attn_stat(const Heads dout, const Heads o, const float* __restrict__ lse, const Heads v, const __grid_constant__ Attn a,
+                const __grid_constant__ Stat st) {
     pdl_begin();
     constexpr int G = DP / 8, kRows = 256 / G;            // lanes a row
-    const int gl = threadIdx.x % G;
-    const bool in = 8 * gl < D;
-    float big_do = 0.0f, big_v = 0.0f;
-    const int64_t rows = Tq * Hq;
-    constexpr int U = 4;                                  // rows on their way at once
-    for (int64_t r0 = (int64_t)blockIdx.x * kRows * U; r0 < rows; r0 += (int64_t)gridDim.x * kRows * U) {
-        uint4 xs[U], ys[U];
+    const int gl = threadIdx.x % G, own = threadIdx.x / G;
+    const bool in = 8 * gl < a.D;
+    const bool keys = blockIdx.x >= st.q_blocks;
+    const int rows = keys ? st.k_rows : st.q_rows;
+    int64_t which = blockIdx.x;
+    Span sp{0, (int)a.Tq};                                // bf16 has no use for documents here
+    if constexpr (Elem<T>::kFmt == 0)
+        sp = span_of(a, stat_block(keys ? a.cu_k : a.cu_q, a.docs, rows, keys ? blockIdx.x - st.q_blocks : blockIdx.x, &which));
+    const int64_t places = keys ? stat_places(sp, rows) : (sp.lq + rows - 1) / rows;
+    if (which < 0 || which >= places) return;
+    float big = 0.0f;
+    if (!keys) {
+        constexpr int U = 4;                              // rows on their way at once
+        const int t0 = (int)which * rows, n = min(rows, sp.lq - t0) * a.Hq;
+        for (int r0 = 0; r0 < n; r0 += kRows * U) {
+            uint4 xs[U], ys[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t r = r0 + u * kRows + threadIdx.x / G, t = r / Hq;
-            const int h = (int)(r - t * Hq);
-            xs[u] = ys[u] = make_uint4(0, 0, 0, 0);
-            if (r < rows && in) {
-                xs[u] = *reinterpret_cast<const uint4*>(dout + t * do_tok + h * do_head + 8 * gl);
-                ys[u] = *reinterpret_cast<const uint4*>(o + t * o_tok + h * o_head + 8 * gl);
+            for (int u = 0; u < U; ++u) {
+                const int r = r0 + u * kRows + own, h = r % a.Hq;
+                const int64_t t = sp.q0 + t0 + r / a.Hq;
+                xs[u] = ys[u] = make_uint4(0, 0, 0, 0);
+                if (r < n && in) {
+                    xs[u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(dout.p) + t * dout.tok + h * dout.head + 8 * gl);
+                    ys[u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(o.p) + t * o.tok + h * o.head + 8 * gl);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int r = r0 + u * kRows + own, h = r % a.Hq;
+                const int64_t t = sp.q0 + t0 + r / a.Hq;
+                const uint32_t xw[4] = {xs[u].x, xs[u].y, xs[u].z, xs[u].w}, yw[4] = {ys[u].x, ys[u].y, ys[u].z, ys[u].w};
+                float dot = 0.0f, sq = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 x = Elem<T>::unpack(xw[i]), y = Elem<T>::unpack(yw[i]);
+                    dot += x.x * y.x + x.y * y.y;
+                    sq += x.x * x.x + x.y * x.y;
+                }
+#pragma unroll
+                for (int x = G / 2; x > 0; x >>= 1) {
+                    dot += __shfl_xor_sync(0xffffffffu, dot, x);
+                    if constexpr (Elem<T>::kFmt == 0) sq += __shfl_xor_sync(0xffffffffu, sq, x);
+                }
+                if (sq < INFINITY) big = fmaxf(big, sq);
+                if (r < n && gl == 0) {
+                    const float l = lse[(int64_t)h * a.Tq + t];
+                    st.stat[h * a.Tq + t] = make_float2(l == -INFINITY ? INFINITY : l * kLog2e, dot);
+                }
             }
         }
+    } else {
+        for (int64_t t0 = which * rows; t0 < sp.lk; t0 += places * rows) {
+            const int n = (int)min((int64_t)rows, sp.lk - t0) * a.Hk;
+            for (int r = own; r - own < n; r += kRows) {
+                float sq = 0.0f;
+                if (r < n && in) {
+                    const int64_t t = sp.k0 + t0 + r / a.Hk;
+                    const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const T*>(v.p) + t * v.tok + r % a.Hk * v.head + 8 * gl);
+                    const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t r = r0 + u * kRows + threadIdx.x / G, t = r / Hq;
-            const int h = (int)(r - t * Hq);
-            const uint32_t xw[4] = {xs[u].x, xs[u].y, xs[u].z, xs[u].w}, yw[4] = {ys[u].x, ys[u].y, ys[u].z, ys[u].w};
-            float dot = 0.0f, sq = 0.0f;
+                    for (int i = 0; i < 4; ++i) {
+                        const float2 y = Elem<T>::unpack(xw[i]);
+                        sq += y.x * y.x + y.y * y.y;
+                    }
+                }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 a = Elem<T>::unpack(xw[i]), b = Elem<T>::unpack(yw[i]);
-                dot += a.x * b.x + a.y * b.y;
-                sq += a.x * a.x + a.y * a.y;
-            }
-#pragma unroll
-            for (int x = G / 2; x > 0; x >>= 1) {
-                dot += __shfl_xor_sync(0xffffffffu, dot, x);
-                sq += __shfl_xor_sync(0xffffffffu, sq, x);
-            }
-            if (sq < INFINITY) big_do = fmaxf(big_do, sq);
-            if (r < rows && gl == 0) {
-                const float l = lse[(int64_t)h * Tq + t];
-                stat[h * stat_ld + t] = make_float2(l == -INFINITY ? INFINITY : l * kLog2e, dot);
+                for (int x = G / 2; x > 0; x >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, x);
+                if (sq < INFINITY) big = fmaxf(big, sq);
             }
         }
     }
     if constexpr (Elem<T>::kFmt == 0) {
-        const int64_t vrows = Tk * Hk;
-        for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < vrows; r0 += (int64_t)gridDim.x * kRows) {
-            const int64_t r = r0 + threadIdx.x / G, t = r / Hk;
-            const int h = (int)(r - t * Hk);
-            float sq = 0.0f;
-            if (r < vrows && in) {
-                const uint4 x = *reinterpret_cast<const uint4*>(v + t * v_tok + h * v_head + 8 * gl);
-                const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+        __shared__ float sm[8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 a = Elem<T>::unpack(xs[i]);
-                    sq += a.x * a.x + a.y * a.y;
-                }
-            }
-#pragma unroll
-            for (int x = G / 2; x > 0; x >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, x);
-            if (sq < INFINITY) big_v = fmaxf(big_v, sq);
-        }
-        __shared__ float sm[2][8];
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) {
-            big_do = fmaxf(big_do, __shfl_xor_sync(0xffffffffu, big_do, x));
-            big_v = fmaxf(big_v, __shfl_xor_sync(0xffffffffu, big_v, x));
-        }
-        if ((threadIdx.x & 31) == 0) {
-            sm[0][threadIdx.x >> 5] = big_do;
-            sm[1][threadIdx.x >> 5] = big_v;
-        }
+        for (int x = 16; x > 0; x >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
+        if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = big;
         __syncthreads();
-        if (threadIdx.x < 2) {
-            float m = 0.0f;
-            for (int i = 0; i < 8; ++i) m = fmaxf(m, sm[threadIdx.x][i]);
-            norms[threadIdx.x * kStatBlocks + blockIdx.x] = m;
+        if (threadIdx.x == 0) {
+#pragma unroll
+            for (int i = 1; i < 8; ++i) big = fmaxf(big, sm[i]);
+            st.norms[keys ? a.Tq + 8 * (int64_t)sp.q0 + which : sp.q0 + which] = big;
         }
     }
 }
@@ -156,18 +191,18 @@ struct Bars {
 template <typename T> constexpr float kPLift = 0.0f;
 template <> constexpr float kPLift<__half> = 15.0f;
 
-// The factor that dS carries before it is rounded.
+// The factor that a document's dS carries before it is rounded.
 template <typename T>
-__device__ __forceinline__ float ds_lift(const float* norms) {
+__device__ __forceinline__ float ds_lift(const Stat& st, const Span& sp, int64_t Tq) {
     if constexpr (Elem<T>::kFmt == 1) {
         return 1.0f;
     } else {
         const int lane = threadIdx.x & 31;
+        const float *of_do = st.norms + sp.q0, *of_v = st.norms + Tq + 8 * (int64_t)sp.q0;
+        const int64_t n_do = (sp.lq + st.q_rows - 1) / st.q_rows, n_v = stat_places(sp, st.k_rows);
         float a = 0.0f, b = 0.0f;
-        for (int i = lane; i < kStatBlocks; i += 32) {
-            a = fmaxf(a, norms[i]);
-            b = fmaxf(b, norms[kStatBlocks + i]);
-        }
+        for (int64_t i = lane; i < n_do; i += 32) a = fmaxf(a, of_do[i]);
+        for (int64_t i = lane; i < n_v; i += 32) b = fmaxf(b, of_v[i]);
 #pragma unroll
         for (int x = 16; x > 0; x >>= 1) {
             a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, x));
@@ -224,7 +259,7 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
 #pragma unroll
                 for (int e = 0; e < C::kBT / 32; ++e) {
                     const int64_t at = sp.q0 + (int64_t)C::kBT * t + lane + 32 * e;
-                    stat[e] = at < a.Tq ? g.stat[bh * g.stat_ld + at] : make_float2(0.0f, 0.0f);
+                    stat[e] = at < a.Tq ? g.st.stat[bh * a.Tq + at] : make_float2(0.0f, 0.0f);
                 }
             };
             int t = t0, bh = KEYS ? kvh * a.group : kvh;
@@ -342,7 +377,7 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
         const int w = warp >> 2, row = r0 + (warp & 3) * 32 + lane;        // column half; stationary row in the document
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + C::kS + 32 * w, td = tmem + lanes + C::kDP + 32 * w;
-        const float lift = ds_lift<T>(g.norms);
+        const float lift = ds_lift<T>(g.st, sp, a.Tq);
         const float pd = Elem<T>::kFmt == 0 ? lift * exp2f(-kPLift<T>) : 1.0f;
         const float c = BIAS ? 1.0f : (CAP ? a.cap2 : a.scale2);
         // columns [lo, hi) of the streamed side take part in this row
@@ -357,7 +392,7 @@ __device__ __forceinline__ void grad_cta(const CUtensorMap& ma0, const CUtensorM
         const int lo_max = __reduce_max_sync(0xffffffffu, live ? lo : 0), hi_min = __reduce_min_sync(0xffffffffu, live ? hi : INT32_MAX);
         float my_lse = INFINITY, my_delta = 0.0f;
         if (!KEYS && live && sp.q0 + (int64_t)row < a.Tq) {
-            const float2 s = g.stat[head * g.stat_ld + sp.q0 + row];
+            const float2 s = g.st.stat[head * a.Tq + sp.q0 + row];
             my_lse = s.x;
             my_delta = s.y;
         }
@@ -577,11 +612,6 @@ int raise_smem(int bytes) {
     return PMG_OK;
 }
 
-struct Heads {
-    const void* p;
-    int64_t tok, head;
-};
-
 struct Ins {
     Heads dout, o, q, k, v;
     const float* lse;
@@ -594,14 +624,16 @@ int run(Grad g, const Ins& in, cudaStream_t s) {
     const Attn& a = g.a;
     const int rc = raise_smem<k_attn_grad<T, DP, CAP, BIAS>>(C::kSmem);
     if (rc != PMG_OK) return rc;
-    float2* stat = reinterpret_cast<float2*>(in.ws + 2 * kStatBlocks);
-    k_attn_stat<T, DP><<<kStatBlocks, 256, 0, s>>>(static_cast<const T*>(in.dout.p), in.dout.tok, in.dout.head,
-                                                   static_cast<const T*>(in.o.p), in.o.tok, in.o.head, in.lse,
-                                                   static_cast<const T*>(in.v.p), in.v.tok, in.v.head, a.Tq, a.Tk, a.Hq, a.Hk,
-                                                   a.D, stat, g.stat_ld, in.ws);
+    g.st.q_rows = stat_rows(a.Hq);
+    g.st.k_rows = stat_rows(a.Hk);
+    const bool by_document = Elem<T>::kFmt == 0;
+    g.st.q_blocks = by_document ? a.Tq / g.st.q_rows + a.docs : (a.Tq + g.st.q_rows - 1) / g.st.q_rows;
+    g.st.stat = reinterpret_cast<float2*>(in.ws);
+    g.st.norms = in.ws + 2 * a.Tq * a.Hq;
+    const int64_t stat_blocks = g.st.q_blocks + (by_document ? a.Tk / g.st.k_rows + a.docs : 0);
+    if (stat_blocks > INT32_MAX) return PMG_ERR_UNSUPPORTED;
+    k_attn_stat<T, DP><<<(unsigned)stat_blocks, 256, 0, s>>>(in.dout, in.o, in.lse, in.v, a, g.st);
     PMG_LAUNCH_CHECK();
-    g.stat = stat;
-    g.norms = in.ws;
     const int64_t key_blocks = (a.Tk / 128 + a.docs) * a.Hk, query_blocks = (a.Tq / 128 + a.docs) * a.Hq;
     if (key_blocks + query_blocks > INT32_MAX) return PMG_ERR_UNSUPPORTED;
     g.key_blocks = (int)key_blocks;
@@ -628,7 +660,7 @@ using namespace pmg;
 
 extern "C" size_t pmg_attention_grad_workspace_bytes(int64_t Tq, int32_t Hq) {
     if (Tq < 0 || Hq < 0) return 0;
-    return 2 * kStatBlocks * sizeof(float) + (size_t)Tq * Hq * sizeof(float2);
+    return (size_t)Tq * (Hq * sizeof(float2) + 9 * sizeof(float));
 }
 
 extern "C" int pmg_attention_grad(const void* dout, int64_t do_tok, int64_t do_head, const void* o, int64_t o_tok,
@@ -662,7 +694,6 @@ extern "C" int pmg_attention_grad(const void* dout, int64_t do_tok, int64_t do_h
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) || workspace_bytes < pmg_attention_grad_workspace_bytes(Tq, Hq))
         return PMG_ERR_BAD_ARG;
     g.scale = scale;
-    g.stat_ld = Tq;
     g.dq = dq; g.dk = dk; g.dv = dv;
     g.q_tok = dq_tok; g.q_head = dq_head; g.k_tok = dk_tok; g.k_head = dk_head; g.v_tok = dv_tok; g.v_head = dv_head;
     const Ins in{{dout, do_tok, do_head}, {o, o_tok, o_head}, {q, q_tok, q_head}, {k, k_tok, k_head}, {v, v_tok, v_head}, lse,

@@ -64,3 +64,50 @@ def test_capped_scores_ignore_what_lies_outside(lq, d, dtype, slopes, causal):
             o, lse = tokens.attention(q, k, v, cq, ck, 160, 160, causal=True, softcap=20.0)
             firsts.append((o[:96], lse[:, :96]))
         assert all(torch.equal(a, b) for a, b in zip(*firsts))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,hk", [(2, 2), (16, 1)])
+def test_fp16_gradients_ignore_what_lies_outside(d, hq, hk):
+    """Finite leftovers behind a cache's length, and rows behind the last document."""
+    from promptmoge_b200 import tokens
+    lq, lk, room = [200, 33, 0, 1], [700, 0, 30, 129], [720, 40, 64, 300]
+    q, k, v, cq, ck, _ = make(lq + [16], lk, hq, hk, d, torch.float16, room=room)
+    do = torch.randn_like(q) * 0.01
+    cq, used = offsets(lq), torch.tensor(lk, dtype=torch.int32, device="cuda")
+    got, own = [], sum(lq)
+    for fill in (0.0, 6e4, -6e4):
+        for n, r, c in zip(lk, room, ck.tolist()):
+            k[c + n:c + r] = fill
+            v[c + n:c + r] = fill
+        for t in (q, do):
+            t[own:] = fill
+        out = torch.full_like(q, fill)
+        o, lse = tokens.attention(q, k, v, cq, ck, 200, 720, causal=True, k_len=used, out=out)
+        lse[:, own:] = 0
+        dq, dk, dv = tokens.attention_grad(do, o, lse, q, k, v, cq, ck, 200, 720, causal=True, k_len=used)
+        got.append([o[:own], lse[:, :own], dq[:own], dk, dv])
+    tokens.check()
+    for other in got[1:]:
+        for name, a, b in zip(("o", "lse", "dq", "dk", "dv"), got[0], other):
+            assert torch.equal(a, b), name
+
+
+@pytest.mark.parametrize("d,hq,hk", [(64, 2, 1), (128, 4, 4)])
+def test_fp16_gradients_of_a_document_are_its_own(d, hq, hk):
+    """Large gradients and values in one document leave the bits of the others'."""
+    from promptmoge_b200 import tokens
+    lens = [130, 5, 300, 77]
+    q, k, v, cq, ck, _ = make(lens, lens, hq, hk, d, torch.float16)
+    do = torch.randn_like(q) * 2.0 ** -8
+    keep = torch.ones(sum(lens), dtype=torch.bool, device="cuda")
+    keep[135:435] = False
+
+    def grads():
+        o, lse = tokens.attention(q, k, v, cq, ck, 300, 300)
+        return tokens.attention_grad(do, o, lse, q, k, v, cq, ck, 300, 300)
+    want = grads()
+    do[135:435] *= 2.0 ** 16
+    v[135:435] *= 2.0 ** 10
+    for a, b in zip(grads(), want):
+        assert torch.equal(a[keep], b[keep])
