@@ -92,8 +92,8 @@ struct Item {
 template <typename T, int DP, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
     k_attn(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
-           const __grid_constant__ CUtensorMap mv, const __grid_constant__ Attn a, T* __restrict__ o, int64_t o_tok,
-           int64_t o_head, float* __restrict__ lse) {
+           const __grid_constant__ CUtensorMap mv, const __grid_constant__ Attn a, const int max_q, T* __restrict__ o,
+           int64_t o_tok, int64_t o_head, float* __restrict__ lse) {
     using C = Fwd<DP>;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* const sk = smem + C::kQ;
@@ -220,6 +220,8 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
                     ok = __shfl_sync(0xffffffffu, (int)ok, 0);
                     if (!ok) break;
                 }
+                // there are as many blocks as documents, and more: each answers for one, which may have no tile at all
+                if (block < a.docs) report_span(a, block, max_q);
                 ok = __all_sync(0xffffffffu, wait_bar(next_bar, claim & 1u, abort_flag));
                 if (!ok) break;
                 block = claimed_block(next_slot);
@@ -573,8 +575,9 @@ __global__ void __launch_bounds__(kFewThreads, Few<DP>::kCtas)
         fence_mbar_init();
     }
     pdl_begin();
-    const Span sp = span_of(a, doc);
-    if (sp.lq > max_q && threadIdx.x == 0) flag(a.status, PMG_ERR_RANGE);
+    bool bad;
+    const Span sp = cut_span(a, doc, &bad);
+    if ((bad || sp.lq > max_q) && threadIdx.x == 0) flag(a.status, PMG_ERR_RANGE);
     const int rows = min(sp.lq, max_q) * a.group;
     const int reach = key_end(a, sp, sp.lq), kbeg = split * stretch;
     const int kend = split + 1 < splits ? min(reach, kbeg + stretch) : reach;       // the last takes what max_k left out
@@ -899,7 +902,7 @@ int run(const Attn& a, const Call& c, cudaStream_t s) {
     if (e != PMG_OK) return e;
     const int64_t blocks = (a.Tq / 256 + a.docs) * a.Hq;
     if (blocks > INT32_MAX) return PMG_ERR_UNSUPPORTED;
-    k_attn<T, DP, CAP, BIAS><<<(int)blocks, C::kThreads, C::kSmem, s>>>(mq, mk, mv, a, static_cast<T*>(c.o), c.o_tok, c.o_head, c.lse);
+    k_attn<T, DP, CAP, BIAS><<<(int)blocks, C::kThreads, C::kSmem, s>>>(mq, mk, mv, a, c.max_q, static_cast<T*>(c.o), c.o_tok, c.o_head, c.lse);
     PMG_LAUNCH_CHECK();
     return PMG_OK;
 }

@@ -36,19 +36,29 @@ struct Span {
     int room;                        // key rows that belong to the document
 };
 
-// A document's span, cut to the tensors: offsets that leave them, run backwards, or lengths over the room are reported.
-__device__ __forceinline__ Span span_of(const Attn& a, int d) {
+// A document's span, cut to the tensors: offsets that leave them, run backwards, or lengths over the room.
+__device__ __forceinline__ Span cut_span(const Attn& a, int d, bool* bad) {
     Span s;
     s.q0 = min(max(a.cu_q[d], 0), (int)a.Tq);
     s.lq = min(max(a.cu_q[d + 1], s.q0), (int)a.Tq) - s.q0;
     s.k0 = min(max(a.cu_k[d], 0), (int)a.Tk);
     s.room = min(max(a.cu_k[d + 1], s.k0), (int)a.Tk) - s.k0;
     s.lk = a.k_len ? max(0, min(a.k_len[d], s.room)) : s.room;
-    if (threadIdx.x == 0 && (s.q0 != a.cu_q[d] || s.q0 + s.lq != a.cu_q[d + 1] || s.k0 != a.cu_k[d] ||
-                             s.k0 + s.room != a.cu_k[d + 1] || (a.k_len && s.lk != a.k_len[d])))
-        flag(a.status, PMG_ERR_RANGE);
+    *bad = s.q0 != a.cu_q[d] || s.q0 + s.lq != a.cu_q[d + 1] || s.k0 != a.cu_k[d] || s.k0 + s.room != a.cu_k[d + 1] ||
+           (a.k_len && s.lk != a.k_len[d]);
     s.prefix = a.prefix ? min(max(a.prefix[d], 0), s.lk) : 0;
     return s;
+}
+__device__ __forceinline__ Span span_of(const Attn& a, int d) {
+    bool bad;
+    return cut_span(a, d, &bad);
+}
+
+// Reports a document whose span had to be cut, or that has more than max_q queries.
+__device__ __forceinline__ void report_span(const Attn& a, int d, int max_q) {
+    bool bad;
+    const Span s = cut_span(a, d, &bad);
+    if (bad || s.lq > max_q) flag(a.status, PMG_ERR_RANGE);
 }
 
 // The last key that row i (place p = i + lk - lq) sees; negative: none.

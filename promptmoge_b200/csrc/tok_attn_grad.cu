@@ -79,6 +79,8 @@ __global__ void __launch_bounds__(256)
     const bool in = 8 * gl < a.D;
     const bool keys = blockIdx.x >= st.q_blocks;
     const int rows = keys ? st.k_rows : st.q_rows;
+    if (blockIdx.x == 0)                                  // also those without a tile that some block works on
+        for (int d = threadIdx.x; d < a.docs; d += 256) report_span(a, d, INT32_MAX);
     int64_t which = blockIdx.x;
     Span sp{0, (int)a.Tq};                                // bf16 has no use for documents here
     if constexpr (Elem<T>::kFmt == 0)
