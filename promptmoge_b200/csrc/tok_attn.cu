@@ -935,7 +935,7 @@ extern "C" int pmg_attention(const void* q, int64_t q_tok, int64_t q_head, const
     Attn a;
     const int rc = fill_attn(&a, dtype, cu_q, cu_k, k_len, docs, Tq, Tk, Hq, Hk, D, scale, causal, prefix, softcap, slopes, status);
     if (rc != PMG_OK) return rc;
-    if (docs == 0 || Tq == 0 || max_q == 0) return PMG_OK;
+    if (docs == 0 || Tq == 0) return PMG_OK;
     if (Tk == 0) {                    // nothing is read of the keys: any valid place serves their tensor maps
         k = v = q;
         k_tok = v_tok = q_tok;
@@ -944,6 +944,7 @@ extern "C" int pmg_attention(const void* q, int64_t q_tok, int64_t q_head, const
     if (!q || !k || !v || !o || !lse || max_q < 0 || max_k < 0) return PMG_ERR_BAD_ARG;
     auto ok = [](const void* p, int64_t t, int64_t h) { return !(reinterpret_cast<uintptr_t>(p) & 15) && !(t & 7) && !(h & 7); };
     if (!ok(q, q_tok, q_head) || !ok(k, k_tok, k_head) || !ok(v, v_tok, v_head) || !ok(o, o_tok, o_head)) return PMG_ERR_BAD_ARG;
+    if (max_q == 0) max_k = 0;        // one short launch a document, which reports those that do have queries
     const size_t need = pmg_attention_workspace_bytes(docs, Hq, Hk, D, max_q, max_k);
     if (workspace_bytes < need || (need && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15)))) return PMG_ERR_BAD_ARG;
     Call c{{q, q_tok, q_head}, {k, k_tok, k_head}, {v, v_tok, v_head}, o, o_tok, o_head, lse, max_q, max_k, static_cast<float*>(workspace)};

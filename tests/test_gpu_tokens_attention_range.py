@@ -56,3 +56,13 @@ def test_a_document_longer_than_max_q_is_reported_by_the_tile(causal):
     tokens.attention(q, k, v, cq, ck, 30, 40, causal=causal)
     tokens.check()
     reports(lambda: tokens.attention(q, k, v, cq, ck, 29, 40, causal=causal))
+
+
+@pytest.mark.parametrize("lk", [40, 9000])
+def test_queries_although_max_q_is_zero(lk):
+    from promptmoge_b200 import tokens
+    q, k, v, cq, ck, _ = make([3], [lk], 2, 1, 64, torch.float16)
+    reports(lambda: tokens.attention(q, k, v, cq, ck, 0, lk))
+    none = words(0, 0)
+    tokens.attention(q, k, v, none, ck, 0, lk)             # documents without queries: nothing to report
+    tokens.check()
