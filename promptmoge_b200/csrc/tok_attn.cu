@@ -19,13 +19,15 @@
 
 namespace pmg {
 
+constexpr int64_t kMostTokens = INT32_MAX - 512;   // of a tensor: a tile's rows behind the last still have an int32 place
+
 int fill_attn(tok::Attn* a, int dtype, const int32_t* cu_q, const int32_t* cu_k, const int32_t* k_len, int docs, int64_t Tq,
               int64_t Tk, int Hq, int Hk, int D, float scale, int causal, const int32_t* prefix, float softcap,
               const float* slopes, int32_t* status) {
     if (dtype != PMG_F16 && dtype != PMG_BF16) return PMG_ERR_UNSUPPORTED;
     if (docs < 0 || Tq < 0 || Tk < 0 || Hq < 1 || Hk < 1 || Hq % Hk || D < 8 || !cu_q || !cu_k) return PMG_ERR_BAD_ARG;
     if (!(scale > 0.0f) || !std::isfinite(scale) || !(softcap >= 0.0f) || !std::isfinite(softcap)) return PMG_ERR_BAD_ARG;
-    if (D % 8 || D > 128 || Tq > INT32_MAX - 512 || Tk > INT32_MAX - 512 || Hq > 65535) return PMG_ERR_UNSUPPORTED;
+    if (D % 8 || D > 128 || Tq > kMostTokens || Tk > kMostTokens || Hq > 65535) return PMG_ERR_UNSUPPORTED;
     *a = tok::Attn{};
     a->cu_q = cu_q; a->cu_k = cu_k; a->k_len = k_len; a->prefix = causal ? prefix : nullptr; a->slopes = slopes;
     a->Tq = Tq; a->Tk = Tk; a->docs = docs; a->Hq = Hq; a->Hk = Hk; a->group = Hq / Hk; a->D = D; a->causal = causal != 0;
@@ -853,15 +855,16 @@ bool few_rows(int max_q, int group) { return (int64_t)max_q * group <= kFewRows;
 
 // Keys of a stretch, a multiple of a tile: one round of the CTAs that fit the GPU together for one document, a quarter of
 // that for several, whose lengths differ (CTAs then take turns and even out); at least 256, so that a stretch is longer
-// than its start.
+// than its start, and no more than all of them.  No document holds more keys than a tensor may; a larger bound counts as that.
 int few_stretch(int docs, int Hk, int D, int max_k) {
+    const int64_t most = std::min<int64_t>(max_k, kMostTokens);
     const int64_t slots = (int64_t)kNumSMs * (D <= 64 ? Few<64>::kCtas : Few<128>::kCtas) * (docs > 1 ? 4 : 1);
-    const int64_t keys = ((int64_t)docs * Hk * max_k + slots - 1) / slots;
-    return (int)(std::max<int64_t>(keys, 256) + kFewTile - 1) / kFewTile * kFewTile;
+    const int64_t pairs = (int64_t)docs * Hk, keys = pairs >= slots ? most : (pairs * most + slots - 1) / slots;
+    return (int)((std::max<int64_t>(keys, 256) + kFewTile - 1) / kFewTile * kFewTile);
 }
 int few_splits(int docs, int Hk, int D, int max_k) {
-    const int stretch = few_stretch(docs, Hk, D, max_k);
-    return std::max(1, (max_k + stretch - 1) / stretch);
+    const int64_t most = std::min<int64_t>(max_k, kMostTokens), stretch = few_stretch(docs, Hk, D, max_k);
+    return (int)std::max<int64_t>(1, (most + stretch - 1) / stretch);
 }
 
 template <typename T, int DP, bool CAP, bool BIAS>

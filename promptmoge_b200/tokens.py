@@ -84,6 +84,7 @@ def _dev(t, name, dim, index=None, dtypes=None):
 
 
 _HALF = (torch.float16, torch.bfloat16)
+_INT32_MAX = 2 ** 31 - 1
 _HALF_OR_F32 = (torch.float16, torch.bfloat16, torch.float32)
 
 
@@ -383,8 +384,8 @@ def _score(scale, D, softcap, causal, prefix, max_q, max_k):
     scale = D ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < float("inf") or not 0.0 <= softcap < float("inf"):
         raise ValueError("scale must be positive and softcap not negative, both finite")
-    if max_q < 0 or max_k < 0:
-        raise ValueError("max_q and max_k must not be negative")
+    if not (0 <= max_q <= _INT32_MAX and 0 <= max_k <= _INT32_MAX):
+        raise ValueError("max_q and max_k must be 0 to 2^31 - 1")
     if prefix is not None and not causal:
         raise ValueError("prefix needs causal (without it every key is seen)")
     return scale

@@ -66,3 +66,18 @@ def test_queries_although_max_q_is_zero(lk):
     none = words(0, 0)
     tokens.attention(q, k, v, none, ck, 0, lk)             # documents without queries: nothing to report
     tokens.check()
+
+
+def test_any_upper_bound_of_the_keys():
+    """max_k only chooses how the keys are shared out: the largest int32 serves every document."""
+    from promptmoge_b200 import tokens
+    for docs, hk in ((1, 1), (3, 2), (444, 8)):
+        lk = [(37 * i) % 90 + 1 for i in range(docs)]
+        q, k, v, cq, ck, _ = make([1] * docs, lk, hk, hk, 64, torch.float16)
+        want = tokens.attention(q, k, v, cq, ck, 1, max(lk))
+        got = tokens.attention(q, k, v, cq, ck, 1, 2 ** 31 - 1)
+        tokens.check()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for most in (dict(max_k=2 ** 31), dict(max_q=2 ** 32 + 1, max_k=90)):
+        with pytest.raises(ValueError):
+            tokens.attention(q, k, v, cq, ck, **(dict(max_q=1) | most))
