@@ -2,8 +2,8 @@
 
 The refiner reads one token feature map per frame (`RefinerEngine.set_frame`: [B, channels, h, w] fp16).  `TokenBlock`
 is the layer that makes or adapts such tokens: every frame is a document of h * w tokens that attend to each other with
-rotated positions; it trains (`torch.autograd`, through the operators' own gradients) and, with `causal`, serves streams
-token by token over a cache (`step`, which also takes prompts).
+rotated positions; it trains (`torch.autograd`, through the operators' own gradients; a second derivative raises) and,
+with `causal`, serves streams token by token over a cache (`step`, which also takes prompts).
 
     block = TokenBlock(1024, heads=16, key_heads=4).cuda()
     feature = mix_frames(block, encoder_feature)          # [B, 1024, 30, 40] fp16, as set_frame takes it
@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import torch
 from torch import nn
+from torch.autograd.function import once_differentiable
 
 from . import tokens
 
@@ -55,6 +56,7 @@ class _Linear(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, w, pre = ctx.saved_tensors
         need = ctx.needs_input_grad
@@ -70,6 +72,7 @@ class _NormRope(torch.autograd.Function):
         return tokens.qk_norm_rope(q, k, qw, kw, cos, sin, positions)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq, dk):
         q, k, qw, kw, cos, sin, positions = ctx.saved_tensors
         g = tokens.qk_norm_rope_grad(dq.contiguous(), dk.contiguous(), q, k, qw, kw, cos, sin, positions)
@@ -85,6 +88,7 @@ class _Attention(torch.autograd.Function):
         return o
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, do):
         q, k, v, o, lse, offsets = ctx.saved_tensors
         g = tokens.attention_grad(do.contiguous(), o, lse, q, k, v, offsets, offsets, ctx.longest, ctx.longest,
