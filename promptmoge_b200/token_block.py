@@ -97,7 +97,12 @@ class _Attention(torch.autograd.Function):
 
 
 class TokenCache:
-    """Keys and values of `streams` streams with room for `room` tokens each."""
+    """Keys and values of `streams` streams with room for `room` tokens each.
+
+    `lengths` (int32, on the device) says how many each holds and may be set, to 0 for a new stream.  `TokenBlock.step`
+    raises before it writes where a stream has no room left.  It knows the lengths from its own steps and reads them anew
+    when they were set; what a replayed graph adds it does not see: a token without room then stays within its stream, on
+    the last row, and the status word tells (`tokens.check`)."""
 
     def __init__(self, block: "TokenBlock", streams: int, room: int, device="cuda"):
         shape = (streams * room, block.key_heads, block.head)
@@ -105,13 +110,35 @@ class TokenCache:
         self.streams, self.room = streams, room
         self.offsets = torch.arange(streams + 1, dtype=torch.int32, device=device) * room
         self.lengths = torch.zeros(streams, dtype=torch.int32, device=device)
+        self._held, self._mark = [0] * streams, self._version()
+
+    def _version(self):
+        return self.lengths, self.lengths._version
+
+    def after(self, packing: Packing) -> list:
+        """The streams' lengths with the packing's tokens; ValueError where they have no room for them."""
+        known = self._mark is not None and self._mark[0] is self.lengths and self._mark[1] == self.lengths._version
+        if not known and not torch.cuda.is_current_stream_capturing():
+            self._held, self._mark = self.lengths.tolist(), self._version()
+        lengths = [held + new for held, new in zip(self._held, packing.lengths)]
+        for stream, n in enumerate(lengths):
+            if n > self.room:
+                raise ValueError(f"stream {stream} holds {self._held[stream]} of {self.room} tokens: "
+                                 f"{packing.lengths[stream]} more do not fit")
+        return lengths
 
     def rows(self, packing_offsets, total: int):
         """Cache rows of the next tokens of every stream, and their positions."""
         at = torch.arange(total, device=self.lengths.device, dtype=torch.int32)
         stream = torch.searchsorted(packing_offsets, at, right=True) - 1
         place = at - packing_offsets[stream] + self.lengths[stream]
-        return stream * self.room + place, place
+        return stream * self.room + place.clamp(max=self.room - 1), place
+
+    def grow(self, packing: Packing, lengths: list) -> None:
+        """Counts the packing's tokens in; lengths: what after() gave."""
+        self.lengths += packing.offsets.diff()
+        self._held = lengths
+        self._mark = None if torch.cuda.is_current_stream_capturing() else self._version()
 
 
 class TokenBlock(nn.Module):
@@ -164,17 +191,18 @@ class TokenBlock(nn.Module):
     @torch.no_grad()
     def step(self, x, packing: Packing, cache: TokenCache, cos, sin):
         """The next tokens of every stream (packing: how many of each; one at a time, or a prompt), their keys and
-        values appended to the cache.  The caller keeps within the cache's room."""
+        values appended to the cache; ValueError where a stream has no room for them."""
         if not self.causal:
             raise ValueError("serving token by token needs a causal block")
         if len(packing.lengths) != cache.streams:
             raise ValueError(f"the cache holds {cache.streams} streams, got {len(packing.lengths)}")
+        lengths = cache.after(packing)
         x = x.contiguous()
         rows, place = cache.rows(packing.offsets, packing.total)
         q, k, v = self._project(x)
         q, k = tokens.qk_norm_rope(q, k, self.q_norm, self.k_norm, cos, sin, place)
         cache.k[rows], cache.v[rows] = k, v
-        cache.lengths += packing.offsets.diff()
+        cache.grow(packing, lengths)
         o, _ = tokens.attention(q, cache.k, cache.v, packing.offsets, cache.offsets, packing.longest, cache.room,
                                 k_len=cache.lengths, **self._options())
         return self._finish(x, o)
