@@ -167,6 +167,11 @@ class TokenBlock(nn.Module):
         self.q_norm, self.k_norm = nn.Parameter(torch.ones(self.head)), nn.Parameter(torch.ones(self.head))
         self.register_buffer("slopes", slopes)
 
+    def _rows(self, x, packing: Packing):
+        if x.shape != (packing.total, self.width):
+            raise ValueError(f"x must be [{packing.total}, {self.width}] for this packing, got {tuple(x.shape)}")
+        return x.contiguous()
+
     def _project(self, x):
         h = _Linear.apply(self.norm1(x).to(self.dtype), self.qkv_w, self.qkv_b, "none", None)
         a, b = self.heads * self.head, (self.heads + self.key_heads) * self.head
@@ -183,7 +188,7 @@ class TokenBlock(nn.Module):
 
     def forward(self, x, packing: Packing, cos, sin, positions, prefix=None):
         """x [T, width] fp32 -> the same; positions [T] int32 into the angle table; prefix [documents] int32."""
-        x = x.contiguous()
+        x = self._rows(x, packing)
         q, k, v = self._project(x)
         q, k = _NormRope.apply(q, k, self.q_norm, self.k_norm, cos, sin, positions)
         return self._finish(x, _Attention.apply(q, k, v, packing.offsets, packing.longest, self._options(prefix)))
@@ -197,7 +202,7 @@ class TokenBlock(nn.Module):
         if len(packing.lengths) != cache.streams:
             raise ValueError(f"the cache holds {cache.streams} streams, got {len(packing.lengths)}")
         lengths = cache.after(packing)
-        x = x.contiguous()
+        x = self._rows(x, packing)
         rows, place = cache.rows(packing.offsets, packing.total)
         q, k, v = self._project(x)
         q, k = tokens.qk_norm_rope(q, k, self.q_norm, self.k_norm, cos, sin, place)

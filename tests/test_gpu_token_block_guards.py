@@ -88,3 +88,18 @@ def test_a_replayed_step_keeps_within_its_stream():
     with pytest.raises(ValueError, match="do not fit"):
         cache.lengths.clamp_(max=8)
         block.step(x, one, cache, cos, sin)
+
+
+def test_tokens_and_packing_have_to_agree():
+    """Tokens of no document have no result: they are refused, not left as memory came."""
+    from promptmoge_b200.token_block import Packing, TokenCache
+    block = _block(causal=True)
+    cos, sin, place = _frame()
+    x = torch.randn(20, 128, device="cuda")
+    for lengths in ([19], [10, 11], [], [20, 1]):
+        with pytest.raises(ValueError, match="for this packing"):
+            block(x, Packing(lengths), cos, sin, place)
+    with pytest.raises(ValueError, match="for this packing"):
+        block.step(x, Packing([19]), TokenCache(block, 1, 32), cos, sin)
+    with pytest.raises(ValueError, match="for this packing"):
+        block(x[:, :64], Packing([20]), cos, sin, place)
