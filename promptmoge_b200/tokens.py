@@ -13,6 +13,7 @@ is kept in a status word per device: `check()` reads it.
 from __future__ import annotations
 
 import functools
+import threading
 
 import torch
 
@@ -25,6 +26,7 @@ ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 
 _status_words: dict = {}
 _status_ptrs: dict = {}
+_status_lock = threading.Lock()
 _fn: dict = {}
 _current_device = torch._C._cuda_getDevice
 _current_stream = torch._C._cuda_getCurrentRawStream
@@ -50,9 +52,13 @@ def _query(name, *sizes):
 def _status(index: int) -> int:
     ptr = _status_ptrs.get(index)
     if ptr is None:
-        word = _status_words[index] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
-        torch.cuda.current_stream(word.device).synchronize()    # zeroed before any other stream's kernel sees it
-        ptr = _status_ptrs[index] = word.data_ptr()
+        with _status_lock:                  # one word for all threads that come here first
+            ptr = _status_ptrs.get(index)
+            if ptr is None:
+                word = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
+                torch.cuda.current_stream(word.device).synchronize()    # zeroed before any other stream's kernel sees it
+                _status_words[index] = word
+                ptr = _status_ptrs[index] = word.data_ptr()
     return ptr
 
 

@@ -13,3 +13,45 @@ def test_workspace_sizes_for_any_upper_bound_of_the_keys():
             "        assert 0 <= n < 1 << 30, (docs, hk, d, most, n)\n")
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, (r.returncode, r.stderr[-2000:])
+
+
+def test_one_status_word_for_all_threads(monkeypatch):
+    """Threads on their first call: all get the word that check() reads."""
+    import threading
+    import time
+
+    import torch
+
+    from promptmoge_b200 import tokens
+    made = []
+
+    class Word:
+        device = None
+
+        def data_ptr(self):
+            return id(self)
+
+    def zeros(*_, **__):
+        time.sleep(0.02)
+        made.append(Word())
+        return made[-1]
+
+    class Stream:
+        def synchronize(self):
+            time.sleep(0.02)
+
+    monkeypatch.setattr(tokens, "_status_words", {})
+    monkeypatch.setattr(tokens, "_status_ptrs", {})
+    monkeypatch.setattr(torch, "zeros", zeros)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda *_: Stream())
+    got, gate = [], threading.Barrier(8)
+
+    def first():
+        gate.wait()
+        got.append(tokens._status(0))
+    threads = [threading.Thread(target=first) for _ in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(made) == 1 and set(got) == {tokens._status_words[0].data_ptr()}
