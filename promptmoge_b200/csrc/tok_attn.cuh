@@ -192,10 +192,6 @@ __device__ __forceinline__ void bias_scores(float (&s)[N], float c, float slope,
 // Chebyshev basis); the factor 2^n is put together from its exponent field and multiplied, which keeps a NaN (adding n to
 // the exponent field of 2^f does not).  x below -126.5, -inf with it, gives exactly 0 (n is -127 there, and the field 0);
 // x up to 127; +inf and NaN give NaN.
-__device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
-    const float2 f = unpack2(x);
-    return pack2(ex2(f.x), ex2(f.y));
-}
 __device__ __forceinline__ uint64_t ex2_poly(uint64_t x) {
     const float2 v = unpack2(x);
     x = pack2(max_nan(v.x, -127.0f), max_nan(v.y, -127.0f));

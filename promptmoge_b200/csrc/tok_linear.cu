@@ -30,37 +30,78 @@ using namespace tok;
 // Activations
 // ----------------------------------------------------------------------------------------------------------------- //
 
-// Phi(-a) = 2^q(a) for a >= 0: q is smooth, so a short polynomial holds it.  Degree 5, of least largest
-// max(a, 1) |2^q(a) - Phi(-a)| on [0, 7] (linear programming on a grid); |error| of Phi and of a Phi <= 7e-7 evaluated in
-// fp32, and no output type here resolves more than 2^-11.  q falls on to -399 at 16, so that Phi(-16) is 0.  Then
-// gelu(x) = max(x, 0) - |x| Phi(-|x|), with its limit 0 at -inf.  A product whose tiles keep the tensor cores busy runs at the power limit, where each
-// operation per output counts as energy: 9 of them in place of the 17 of a polynomial in x^2 for Phi itself.
-__device__ constexpr float kTail[6] = {-1.00000191f, -1.151052f, -0.459414065f, -0.0523432381f, 0.00728237722f, -0.000500259455f};
+// gelu(x) = x Phi(x) = max(x, 0) - a Phi(-a), a = |x|, with its limit 0 at -inf: what is approximated is the tail Phi(-a), and
+// its relative error is that of a negative result.  Behind a = 13 Phi(-a) is under 2^-126 and comes out as 0.
+//
+// For 16-bit results Phi(-a) = 2^q(a): q is smooth, so a short polynomial holds it (least largest weighted error, by linear
+// programming on a grid).  fp16, which turns to 0 at 5.8: degree 6, relative error of Phi 4.2e-5 (2^-14; the type rounds to
+// 2^-11).  bf16: degree 8, 2.4e-4 up to 13 (2^-12; the type rounds to 2^-8).  Both evaluated in fp32.  A product whose tiles
+// keep the tensor cores busy runs at the power limit, where each operation per output counts as energy: 10 or 11 of them,
+// in place of the 20 of the finer form.
+template <typename T> struct Tail;
+template <> struct Tail<__half> {
+    static constexpr int kDegree = 6;
+    static __device__ __forceinline__ constexpr float at(int i) {
+        constexpr float c[] = {-1.000057179e+00f, -1.150326502e+00f, -4.609019817e-01f, -5.148804179e-02f, 7.304450847e-03f,
+                               -6.289135209e-04f, 2.407393613e-05f};
+        return c[i];
+    }
+};
+template <> struct Tail<__nv_bfloat16> {
+    static constexpr int kDegree = 8;
+    static __device__ __forceinline__ constexpr float at(int i) {
+        constexpr float c[] = {-1.000191180e+00f, -1.150026044e+00f, -4.608018950e-01f, -5.209471939e-02f, 7.814329701e-03f,
+                               -8.084457054e-04f, 5.337338495e-05f, -2.002034972e-06f, 3.226851094e-08f};
+        return c[i];
+    }
+};
 
-// Phi(-|x|) for two values, and the bounded |x| that it was taken at
-__device__ __forceinline__ float2 tail_pair(float a, float b, float& xa, float& xb) {
-    xa = fminf(fabsf(a), 16.0f);
-    xb = fminf(fabsf(b), 16.0f);
-    const uint64_t x = pack2(xa, xb);
-    uint64_t p = pack2(kTail[5], kTail[5]);
-#pragma unroll
-    for (int i = 4; i >= 0; --i) p = fma2(p, x, pack2(kTail[i], kTail[i]));
-    const float2 q = unpack2(p);
-    return make_float2(ex2(q.x), ex2(q.y));
-}
+// For fp32 results, and for the slope: Phi(-a) = 2^(-a^2 / 2 log2 e) t P(t), t = 1 / (1 + 0.3 a) (least squares, repeated with
+// weights times the error).  P of degree 7 with least largest relative error, 1.2e-7, 5e-7 in fp32.  The slope's, of degree
+// 5, has least largest error relative to t P(t) + a / sqrt(2 pi), the size of what it is added to: 6e-7.
+__device__ constexpr float kMills[8] = {1.196245409e-01f, 1.208263142e-01f, 9.946506889e-02f, 1.300325943e-01f,
+                                        -5.645003673e-02f, 2.093463112e-01f, -1.589336760e-01f, 3.608882384e-02f};
+__device__ constexpr float kSlope[6] = {1.200557486e-01f, 1.135166463e-01f, 1.463589779e-01f, -2.274043795e-02f,
+                                        2.222955805e-01f, -7.948681410e-02f};
+constexpr float kHalfLog2e = 0.72134752f, kHalfLog2eRest = (float)(0.72134752044448170368 - (double)kHalfLog2e);
+template <typename T, bool FINE>
 __device__ __forceinline__ void gelu_pair(float& a, float& b) {
-    float xa, xb;
-    const float2 f = tail_pair(a, b, xa, xb);
+    const float xa = fminf(fabsf(a), 14.0f), xb = fminf(fabsf(b), 14.0f);
+    const uint64_t x = pack2(xa, xb);
+    float2 f;                                            // Phi(-|x|)
+    if constexpr (FINE) {
+        const uint64_t t = pack2(rcp_approx(fmaf(xa, 0.3f, 1.0f)), rcp_approx(fmaf(xb, 0.3f, 1.0f)));
+        uint64_t p = pack2(kMills[7], kMills[7]);
+#pragma unroll
+        for (int i = 6; i >= 0; --i) p = fma2(p, t, pack2(kMills[i], kMills[i]));
+        const uint64_t k = pack2(-kHalfLog2e, -kHalfLog2e), minus = pack2(-1.0f, -1.0f);
+        const uint64_t sq = mul2(x, x), y = mul2(sq, k);
+        // what rounding the exponent loses (up to 2^-17 of the result): k sq - y, k (x^2 - sq), and the rest of k
+        uint64_t r = fma2(sq, k, mul2(y, minus));
+        r = fma2(fma2(x, x, mul2(sq, minus)), k, r);
+        r = fma2(sq, pack2(-kHalfLog2eRest, -kHalfLog2eRest), r);
+        const uint64_t e = ex2_pair(y);
+        f = unpack2(mul2(mul2(p, t), fma2(mul2(e, pack2(kLn2, kLn2)), r, e)));
+    } else {
+        constexpr int N = Tail<T>::kDegree;
+        uint64_t p = pack2(Tail<T>::at(N), Tail<T>::at(N));
+#pragma unroll
+        for (int i = N - 1; i >= 0; --i) p = fma2(p, x, pack2(Tail<T>::at(i), Tail<T>::at(i)));
+        f = unpack2(ex2_pair(p));
+    }
     a = fmaf(-xa, f.x, max_nan(a, 0.0f));
     b = fmaf(-xb, f.y, max_nan(b, 0.0f));
 }
 
-// N values, the choice made once for all of them.
-template <int N>
-__device__ __forceinline__ void activate(int act, float* v) {
-    if (act == PMG_ACT_GELU) {
+// N values, the choice made once for all of them; fine: for an fp32 result.
+template <typename T, int N>
+__device__ __forceinline__ void activate(int act, bool fine, float* v) {
+    if (act == PMG_ACT_GELU && fine) {
 #pragma unroll
-        for (int i = 0; i < N; i += 2) gelu_pair(v[i], v[i + 1]);
+        for (int i = 0; i < N; i += 2) gelu_pair<T, true>(v[i], v[i + 1]);
+    } else if (act == PMG_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) gelu_pair<T, false>(v[i], v[i + 1]);
     } else if (act == PMG_ACT_SILU) {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] *= rcp_approx(1.0f + ex2(-v[i] * kLog2e));
@@ -70,17 +111,18 @@ __device__ __forceinline__ void activate(int act, float* v) {
     }
 }
 
-// dz = dy act'(z) for 8 values.  gelu' = Phi(z) + z phi(z): Phi by the polynomial, phi by one exp2; with erff and expf this
-// pass took 75 us for 9600 x 4096, four fifths of it arithmetic; now 48 (4.9 TB/s).
+// dz = dy act'(z) for 8 values.  gelu' = Phi(z) + z phi(z) is G(a) = 2^(-a^2 / 2 log2 e) (t P(t) - a / sqrt(2 pi)) for z = -a and
+// 1 - G(a) for z = a.  With erff and expf this pass took 75 us for 9600 x 4096, four fifths of it arithmetic; now 48 (4.9 TB/s).
 __device__ __forceinline__ void times_slope(int act, float (&g)[8], const float (&z)[8]) {
     if (act == PMG_ACT_GELU) {
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-            float xa, xb;
-            const float2 f = tail_pair(z[i], z[i + 1], xa, xb);
-            const float pa = z[i] < 0.0f ? f.x : 1.0f - f.x, pb = z[i + 1] < 0.0f ? f.y : 1.0f - f.y;
-            g[i] *= fmaf(z[i] * 0.39894228f, ex2(z[i] * z[i] * (-0.5f * kLog2e)), pa);
-            g[i + 1] *= fmaf(z[i + 1] * 0.39894228f, ex2(z[i + 1] * z[i + 1] * (-0.5f * kLog2e)), pb);
+        for (int i = 0; i < 8; ++i) {                    // one by one: constants of packed operations take registers
+            const float x = fabsf(z[i]), t = rcp_approx(fmaf(x, 0.3f, 1.0f));
+            float p = kSlope[5];
+#pragma unroll
+            for (int k = 4; k >= 0; --k) p = fmaf(p, t, kSlope[k]);
+            const float f = fmaf(p, t, x * -0.39894228f) * ex2(x * x * -kHalfLog2e);
+            g[i] *= z[i] < 0.0f ? f : 1.0f - f;
         }
     } else if (act == PMG_ACT_SILU) {
 #pragma unroll
@@ -129,7 +171,7 @@ __device__ __forceinline__ void finish8(const Out& o, int64_t m, int n, int N, f
                 if (i < cnt) p[i] = Elem<T>::from(z[i]);
         }
     }
-    activate<8>(o.act, z);
+    activate<T, 8>(o.act, o.f32, z);
     if (o.f32) {
         if (o.resid) {
             const float* r = static_cast<const float*>(o.resid) + m * o.ldr + n;
@@ -265,7 +307,7 @@ __global__ void __launch_bounds__(512) k_rows(const uint16_t* __restrict__ x, in
             p[0] = Elem<T>::from(z[0]);
             if (two) p[1] = Elem<T>::from(z[1]);
         }
-        activate<2>(o.act, z);
+        activate<T, 2>(o.act, o.f32, z);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             if (e && !two) break;
@@ -618,7 +660,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                     for (int i = 0; i < kChunk; i += 2) h[i / 2] = Elem<T>::pack(v[i], v[i + 1]);
                     store_row<kChunk / 2>(h, static_cast<uint16_t*>(o.pre) + (int64_t)m * o.ldp + n, row ? left : 0, o.vec);
                 }
-                activate<kChunk>(o.act, v);
+                activate<T, kChunk>(o.act, o.f32, v);
                 if (o.f32) {
                     if (add) {
 #pragma unroll
