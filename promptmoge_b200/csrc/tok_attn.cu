@@ -593,7 +593,8 @@ __global__ void __launch_bounds__(kFewThreads, Few<DP>::kCtas)
     bool ok = true;
     if (warp == kFewWarps) {
         if (lane == 0) {
-            for (int i = 0; i < tiles; ++i) {
+            int i = 0;
+            for (; i < tiles; ++i) {
                 const int st = i % C::kStages;
                 ok = mbar_wait(empty + st, ((i / C::kStages) & 1u) ^ 1u, abort_flag);
                 if (!ok) break;
@@ -605,6 +606,11 @@ __global__ void __launch_bounds__(kFewThreads, Few<DP>::kCtas)
                     tma_tile3d(to + C::kPart + x * 8192, &mv, 64 * x, kvh, sp.k0 + kbeg + kFewTile * i, full + st);
                 }
             }
+            // all has landed before the ring's room takes the warps' rows, or the block leaves, also after an abort
+            const uint64_t t0 = global_ns();
+            for (int n = max(i - C::kStages, 0); n < i; ++n)
+                while (!mbar_try_wait_sleep(full + n % C::kStages, (n / C::kStages) & 1u, 4000) && global_ns() - t0 < kWaitNs) {
+                }
         }
     } else {
         // queries: rows g and g + 8 as left operands

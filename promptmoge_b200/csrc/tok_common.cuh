@@ -237,13 +237,20 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatil
     }
 }
 
-// Waits (bounded) until every MMA this thread issued has retired, so that tensor memory may be freed after an abort.
+// After an abort: waits (bounded) until every MMA this thread issued has retired, so that tensor memory may be freed, and as
+// long again as copies into shared memory take many times over: the block must not leave while one may still land, in what is
+// another block's by then.  Loaders stop at their next wait, a few microseconds after the abort at most; where the issuer
+// came to its end instead it has waited for all that they sent.
+constexpr uint64_t kLandNs = 1000000;
 template <bool PAIR = false>
 __device__ __forceinline__ void drain_mma(uint64_t* bar) {
     if constexpr (PAIR) commit_pair_if(1, bar);
     else mma_commit(bar);
     const uint64_t t0 = global_ns();
     while (!mbar_try_wait_sleep(bar, 0, 4000) && global_ns() - t0 < kWaitNs) {
+    }
+    const uint64_t t1 = global_ns();
+    while (global_ns() - t1 < kLandNs) {
     }
 }
 
