@@ -512,7 +512,7 @@ extern "C" int pmg_qk_norm_rope(const void* q, int64_t q_tok, int64_t q_head, co
     RopeArgs a{};
     a.side[0] = {q, nullptr, q_out, q_weight, q_tok, q_head, 0, 0, qo_tok, qo_head, Hq};
     a.side[1] = {k, nullptr, k_out, k_weight, k_tok, k_head, 0, 0, ko_tok, ko_head, Hk};
-    a.cos = cos; a.sin = sin; a.pos = positions; a.T = T; a.places = rot ? places : INT32_MAX; a.D = D;
+    a.cos = cos; a.sin = sin; a.pos = rot ? positions : nullptr; a.T = T; a.places = rot ? places : INT32_MAX; a.D = D;
     a.half = rot / 2; a.interleaved = interleaved != 0; a.eps = eps; a.status = status;
     return by_type<false>(dtype, a, as_stream(stream));
 }
@@ -544,7 +544,7 @@ extern "C" int pmg_qk_norm_rope_grad(const void* dq, int64_t dq_tok, int64_t dq_
     RopeArgs a{};
     a.side[0] = {q, dq, q_grad, q_weight, q_tok, q_head, dq_tok, dq_head, qo_tok, qo_head, Hq};
     a.side[1] = {k, dk, k_grad, k_weight, k_tok, k_head, dk_tok, dk_head, ko_tok, ko_head, Hk};
-    a.cos = cos; a.sin = sin; a.pos = positions; a.T = T; a.places = rot ? places : INT32_MAX; a.D = D;
+    a.cos = cos; a.sin = sin; a.pos = rot ? positions : nullptr; a.T = T; a.places = rot ? places : INT32_MAX; a.D = D;
     a.half = rot / 2; a.interleaved = interleaved != 0; a.eps = eps; a.status = status;
     a.part = weights ? static_cast<float*>(workspace) : nullptr;
     const int rc2 = by_type<true>(dtype, a, s);
