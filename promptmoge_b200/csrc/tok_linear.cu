@@ -64,31 +64,29 @@ __device__ constexpr float kMills[8] = {1.196245409e-01f, 1.208263142e-01f, 9.94
 __device__ constexpr float kSlope[6] = {1.200557486e-01f, 1.135166463e-01f, 1.463589779e-01f, -2.274043795e-02f,
                                         2.222955805e-01f, -7.948681410e-02f};
 constexpr float kHalfLog2e = 0.72134752f, kHalfLog2eRest = (float)(0.72134752044448170368 - (double)kHalfLog2e);
-template <typename T, bool FINE>
+// One value at a time: constants of packed operations take registers, which the epilogue does not have.
+__device__ __forceinline__ float gelu_fine(float a) {
+    const float x = fminf(fabsf(a), 14.0f), t = rcp_approx(fmaf(x, 0.3f, 1.0f));
+    float p = kMills[7];
+#pragma unroll
+    for (int i = 6; i >= 0; --i) p = fmaf(p, t, kMills[i]);
+    const float sq = x * x, y = sq * -kHalfLog2e;
+    // what rounding the exponent loses (up to 2^-17 of the result): k sq - y, k (x^2 - sq), and the rest of k
+    float r = fmaf(sq, -kHalfLog2e, -y);
+    r = fmaf(fmaf(x, x, -sq), -kHalfLog2e, r);
+    r = fmaf(sq, -kHalfLog2eRest, r);
+    const float e = ex2(y);
+    return fmaf(-x, p * t * fmaf(e * kLn2, r, e), max_nan(a, 0.0f));
+}
+template <typename T>
 __device__ __forceinline__ void gelu_pair(float& a, float& b) {
     const float xa = fminf(fabsf(a), 14.0f), xb = fminf(fabsf(b), 14.0f);
     const uint64_t x = pack2(xa, xb);
-    float2 f;                                            // Phi(-|x|)
-    if constexpr (FINE) {
-        const uint64_t t = pack2(rcp_approx(fmaf(xa, 0.3f, 1.0f)), rcp_approx(fmaf(xb, 0.3f, 1.0f)));
-        uint64_t p = pack2(kMills[7], kMills[7]);
+    constexpr int N = Tail<T>::kDegree;
+    uint64_t p = pack2(Tail<T>::at(N), Tail<T>::at(N));
 #pragma unroll
-        for (int i = 6; i >= 0; --i) p = fma2(p, t, pack2(kMills[i], kMills[i]));
-        const uint64_t k = pack2(-kHalfLog2e, -kHalfLog2e), minus = pack2(-1.0f, -1.0f);
-        const uint64_t sq = mul2(x, x), y = mul2(sq, k);
-        // what rounding the exponent loses (up to 2^-17 of the result): k sq - y, k (x^2 - sq), and the rest of k
-        uint64_t r = fma2(sq, k, mul2(y, minus));
-        r = fma2(fma2(x, x, mul2(sq, minus)), k, r);
-        r = fma2(sq, pack2(-kHalfLog2eRest, -kHalfLog2eRest), r);
-        const uint64_t e = ex2_pair(y);
-        f = unpack2(mul2(mul2(p, t), fma2(mul2(e, pack2(kLn2, kLn2)), r, e)));
-    } else {
-        constexpr int N = Tail<T>::kDegree;
-        uint64_t p = pack2(Tail<T>::at(N), Tail<T>::at(N));
-#pragma unroll
-        for (int i = N - 1; i >= 0; --i) p = fma2(p, x, pack2(Tail<T>::at(i), Tail<T>::at(i)));
-        f = unpack2(ex2_pair(p));
-    }
+    for (int i = N - 1; i >= 0; --i) p = fma2(p, x, pack2(Tail<T>::at(i), Tail<T>::at(i)));
+    const float2 f = unpack2(ex2_pair(p));               // Phi(-|x|)
     a = fmaf(-xa, f.x, max_nan(a, 0.0f));
     b = fmaf(-xb, f.y, max_nan(b, 0.0f));
 }
@@ -98,10 +96,10 @@ template <typename T, int N>
 __device__ __forceinline__ void activate(int act, bool fine, float* v) {
     if (act == PMG_ACT_GELU && fine) {
 #pragma unroll
-        for (int i = 0; i < N; i += 2) gelu_pair<T, true>(v[i], v[i + 1]);
+        for (int i = 0; i < N; ++i) v[i] = gelu_fine(v[i]);
     } else if (act == PMG_ACT_GELU) {
 #pragma unroll
-        for (int i = 0; i < N; i += 2) gelu_pair<T, false>(v[i], v[i + 1]);
+        for (int i = 0; i < N; i += 2) gelu_pair<T>(v[i], v[i + 1]);
     } else if (act == PMG_ACT_SILU) {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] *= rcp_approx(1.0f + ex2(-v[i] * kLog2e));
