@@ -77,3 +77,20 @@ def test_capped_scores_of_minus_infinity_count_as_the_cap(lq, hq, hk, d, dtype, 
     e = 2.0 ** -18 * (1 + cap + (float(sl.max()) / 64 * lk if slopes else 0))
     assert ((lse.double() - want_lse).abs() <= e).all()
     assert ((o.double() - want).abs() <= U[dtype] * want.abs() + (U[dtype] + e) * mass + 1e-7).all()
+
+
+@pytest.mark.parametrize("d,dtype", [(64, torch.float16), (128, torch.bfloat16)])
+def test_a_score_that_is_not_finite_shows_across_stretches(d, dtype):
+    """Few rows over a long cache: the stretch with the key is joined with those without."""
+    from promptmoge_b200 import tokens
+    q, k, v, cq, ck, _ = make([2], [9000], 4, 2, d, dtype)
+    q[:, :, 0] = 1
+    for j in (0, 700, 4500, 8999):
+        for bad in (float("nan"), float("inf")):
+            x = k.clone()
+            x[j, 0] = 0
+            x[j, 0, 0] = bad
+            o, lse = tokens.attention(q, x, v, cq, ck, 2, 9000)
+            clean, clean_lse = tokens.attention(q, k, v, cq, ck, 2, 9000)
+            assert torch.isnan(o[:, :2]).all() and not (torch.isfinite(lse[:2]) | torch.isneginf(lse[:2])).any(), (j, bad)
+            assert torch.equal(o[:, 2:], clean[:, 2:]) and torch.equal(lse[2:], clean_lse[2:])
