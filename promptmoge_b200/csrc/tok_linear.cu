@@ -451,7 +451,9 @@ __device__ __forceinline__ void load_row(uint32_t* w, const E* p, int left, int 
     }
 }
 
-template <typename T, int BN, bool AMN, bool BMN>
+// FINE: GELU for an fp32 result, and no other activation; its code beside the others slows all of them (without an activation
+// 38,400 x 1024 x 4096 takes 270 us in long runs, and 285 with it).
+template <typename T, int BN, bool AMN, bool BMN, bool FINE>
 __global__ void __launch_bounds__(kGemmThreads, 1)
     k_gemm(const __grid_constant__ CUtensorMap ma, const __grid_constant__ CUtensorMap mb, const int M, const int N,
            const __grid_constant__ Sched sched, const __grid_constant__ Out o, int32_t* status) {
@@ -658,7 +660,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
                     for (int i = 0; i < kChunk; i += 2) h[i / 2] = Elem<T>::pack(v[i], v[i + 1]);
                     store_row<kChunk / 2>(h, static_cast<uint16_t*>(o.pre) + (int64_t)m * o.ldp + n, row ? left : 0, o.vec);
                 }
-                activate<T, kChunk>(o.act, o.f32, v);
+                if constexpr (FINE) {
+#pragma unroll
+                    for (int i = 0; i < kChunk; ++i) v[i] = gelu_fine(v[i]);
+                } else {
+                    activate<T, kChunk>(o.act, false, v);
+                }
                 if (o.f32) {
                     if (add) {
 #pragma unroll
@@ -910,7 +917,7 @@ size_t part_bytes(int64_t M, int64_t N, int64_t K) {
     return (size_t)(s.units - s.full) * (bn == 256 ? 2 * kBM : kBM) * bn * sizeof(float);
 }
 
-template <typename T, int BN, bool AMN, bool BMN>
+template <typename T, int BN, bool AMN, bool BMN, bool FINE>
 int gemm_bn(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N, int64_t K, const Out& o,
             Sched s, int32_t* status, cudaStream_t st) {
     using C = Cfg<BN>;
@@ -919,7 +926,7 @@ int gemm_bn(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, i
     PMG_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64) return PMG_ERR_UNSUPPORTED;
     if (!attr_set[dev]) {
-        PMG_CUDA_TRY(cudaFuncSetAttribute(k_gemm<T, BN, AMN, BMN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+        PMG_CUDA_TRY(cudaFuncSetAttribute(k_gemm<T, BN, AMN, BMN, FINE>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
         attr_set[dev] = true;
     }
     CUtensorMap ma, mb;
@@ -931,7 +938,7 @@ int gemm_bn(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, i
     rc = make_tensor_map16(&mb, B, 2, db, sb, bb);
     if (rc != PMG_OK) return rc;
     constexpr int kCtas = C::kPair ? 2 : 1;
-    rc = launch_after<kCtas>(k_gemm<T, BN, AMN, BMN>, dim3(std::min(s.units, kNumSMs / kCtas) * kCtas), kGemmThreads, C::kSmem, st,
+    rc = launch_after<kCtas>(k_gemm<T, BN, AMN, BMN, FINE>, dim3(std::min(s.units, kNumSMs / kCtas) * kCtas), kGemmThreads, C::kSmem, st,
                              ma, mb, (int)M, (int)N, s, o, status);
     if (rc != PMG_OK) return rc;
     if (s.full < s.tiles) {
@@ -941,16 +948,16 @@ int gemm_bn(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, i
     return PMG_OK;
 }
 
-template <typename T, bool AMN, bool BMN>
+template <typename T, bool AMN, bool BMN, bool FINE = false>
 int gemm(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N, int64_t K, const Out& o,
          float* part, int32_t* status, cudaStream_t st) {
     Sched c;
     const int bn = choose(M, N, K, &c);
     c.part = part;
     switch (bn) {
-        case 256: return gemm_bn<T, 256, AMN, BMN>(A, lda, B, ldb, M, N, K, o, c, status, st);
-        case 128: return gemm_bn<T, 128, AMN, BMN>(A, lda, B, ldb, M, N, K, o, c, status, st);
-        default: return gemm_bn<T, 64, AMN, BMN>(A, lda, B, ldb, M, N, K, o, c, status, st);
+        case 256: return gemm_bn<T, 256, AMN, BMN, FINE>(A, lda, B, ldb, M, N, K, o, c, status, st);
+        case 128: return gemm_bn<T, 128, AMN, BMN, FINE>(A, lda, B, ldb, M, N, K, o, c, status, st);
+        default: return gemm_bn<T, 64, AMN, BMN, FINE>(A, lda, B, ldb, M, N, K, o, c, status, st);
     }
 }
 
@@ -1017,7 +1024,8 @@ int linear(const void* x, int64_t ldx, const void* w, int64_t ldw, int64_t M, in
     Matrix mx{x, ldx, M}, mw{w, ldw, N};
     const int rc = pack(&mx, &mw, K, ws, s);
     if (rc != PMG_OK) return rc;
-    return gemm<T, false, false>(mx.p, mx.ld, mw.p, mw.ld, M, N, K, o, reinterpret_cast<float*>(ws), status, s);
+    const auto product = o.act == PMG_ACT_GELU && o.f32 ? gemm<T, false, false, true> : gemm<T, false, false>;
+    return product(mx.p, mx.ld, mw.p, mw.ld, M, N, K, o, reinterpret_cast<float*>(ws), status, s);
 }
 
 struct GradPlan {
