@@ -518,8 +518,8 @@ int pmg_linear_grad(const void* dy, int64_t lddy, const void* x, int64_t ldx, co
 /* Queries q [T,Hq,D] and keys k [T,Hk,D] (F32, F16 or BF16; strides of token and head, values of a head contiguous),
  * each head scaled to unit root mean square (eps inside the root), times its weight [D] fp32 (NULL: ones), then the
  * first `rot` values rotated by the angles of the token's position: cos, sin [places][rot/2] fp32, positions [T] int32
- * (NULL: 0, 1, 2, ...).  Pairs are (i, i + rot/2), or (2i, 2i + 1) when interleaved.  A position outside
- * [0, places) sets PMG_ERR_RANGE in `status` and is taken as 0.  Outputs may be the inputs (in place) or rows of a
+ * (NULL: 0, 1, 2, ...; not read where rot is 0).  Pairs are (i, i + rot/2), or (2i, 2i + 1) when interleaved.  A
+ * position outside [0, places) sets PMG_ERR_RANGE in `status` and is taken as 0.  Outputs may be the inputs (in place) or rows of a
  * cache.  D <= 256, rot even. */
 int pmg_qk_norm_rope(const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok, int64_t k_head,
                      int32_t dtype, int64_t T, int32_t Hq, int32_t Hk, int32_t D, int32_t rot, const float* q_weight,
@@ -545,13 +545,14 @@ int pmg_qk_norm_rope_grad(const void* dq, int64_t dq_tok, int64_t dq_head, const
  * h * Hq/Hk .. sharing key head h).  Document d holds queries cu_q[d] .. cu_q[d+1] and keys cu_k[d] .. cu_k[d+1] (device
  * int32 [docs+1], from 0 to Tq and Tk without decreasing; rows of no document are not written), of the latter only the
  * first k_len[d] where k_len is given (a cache with spare room).  Offsets and lengths that leave the tensors or each
- * other are cut to them and set PMG_ERR_RANGE in `status`.  max_q, max_k: upper bounds of a document's queries and keys, which choose the kernel; a document
- * with more queries sets PMG_ERR_RANGE.
+ * other are cut to them and set PMG_ERR_RANGE in `status`.  max_q, max_k: upper bounds of a document's queries and keys,
+ * which choose the kernel and how it shares out the keys (any up to INT32_MAX); a document with more than max_q queries
+ * sets PMG_ERR_RANGE.
  * Query i of a document stands at place p = i + Lk - Lq among its Lk keys and attends to key j if j <= p or
  * j < prefix[d] (causal; prefix may be NULL), or to all of them.  Scores: s = scale q.k; softcap > 0: s = softcap
  * tanh(s / softcap); slopes [Hq] fp32: s -= slope |p - j|.  o = softmax(s) v; lse [Hq,Tq] fp32 = log sum exp(s).
- * A row that sees no key gives o = 0 and lse = -inf.  Memory outside a document's keys never reaches its rows,
- * whatever it holds.  Results do not depend on timing. */
+ * A row that sees no key gives o = 0 and lse = -inf; one that sees a score of NaN or +inf gives NaN.  Memory outside a
+ * document's keys never reaches its rows, whatever it holds.  Results do not depend on timing. */
 size_t pmg_attention_workspace_bytes(int32_t docs, int32_t Hq, int32_t Hk, int32_t D, int32_t max_q, int32_t max_k);
 int pmg_attention(const void* q, int64_t q_tok, int64_t q_head, const void* k, int64_t k_tok, int64_t k_head,
                   const void* v, int64_t v_tok, int64_t v_head, int32_t dtype, int64_t Tq, int64_t Tk, int32_t Hq,

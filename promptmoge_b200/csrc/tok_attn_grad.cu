@@ -14,8 +14,8 @@
 // small gradients do not turn subnormal.
 //
 // Bound by the chain of a step, as forwards (tensor core 37 % active, issue slots 59 %).  Measured: 8 frames of up to 1200
-// tokens, 16 heads of 64 over 4 key heads, distance bias: 176 us; 8192 tokens, 16 heads of 64: 770 TFLOP/s of the 5
-// products that the gradient needs, heads of 128: 890.
+// tokens, 16 heads of 64 over 4 key heads, distance bias: 175 us; 8192 tokens, 16 heads of 64: 715 (warm) to 750
+// TFLOP/s of the 5 products that the gradient needs, heads of 128: 815 to 870.
 #include <algorithm>
 
 #include "tok_attn.cuh"

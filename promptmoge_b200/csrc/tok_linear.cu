@@ -12,9 +12,10 @@
 //             products; sixteen warps take it, straight from registers to memory.
 //   k_split_sum   the last wave of tiles, when it would leave most SMs idle, is cut along K into fp32 partials that this
 //             kernel adds in split order (no atomics: results do not depend on timing) and takes through the epilogue.
-// Measured: 38,400 x 1024 x 4096 with gelu 249 us (1295 TFLOP/s) alone and 288 in long runs, where the power limit holds the
-// clock at 1.3 GHz (without the activation 263; cuBLAS 274); its gradients over 9600 rows 162 us, 1200 x 1024 x 1024 8 us, one
-// row 1024 -> 4096 3.4 us (2.5 TB/s).  With eight warps that staged their rows in shared memory: 278 and 321 us.
+// Measured: 38,400 x 1024 x 4096 with gelu 252 us (1280 TFLOP/s) alone and 295 to 310 in long runs, where the power limit holds
+// the clock at 1.1 to 1.3 GHz (without the activation 271 to 283; cuBLAS 279); its gradients over 9600 rows 164 us, 1200 x 1024
+// x 1024 10 us, one row 1024 -> 4096 3.5 us (2.4 TB/s).  With eight warps that staged their rows in shared memory the first took
+// 278 us, and 321 in long runs.
 // dz is rounded to the operands' 16-bit type before its two products (tensor cores take no other), db is summed from the
 // unrounded fp32 values.
 #include <algorithm>
@@ -110,7 +111,7 @@ __device__ __forceinline__ void activate(int act, bool fine, float* v) {
 }
 
 // dz = dy act'(z) for 8 values.  gelu' = Phi(z) + z phi(z) is G(a) = 2^(-a^2 / 2 log2 e) (t P(t) - a / sqrt(2 pi)) for z = -a and
-// 1 - G(a) for z = a.  With erff and expf this pass took 75 us for 9600 x 4096, four fifths of it arithmetic; now 48 (4.9 TB/s).
+// 1 - G(a) for z = a.  With erff and expf this pass took 75 us for 9600 x 4096, four fifths of it arithmetic; now 50 (4.7 TB/s).
 __device__ __forceinline__ void times_slope(int act, float (&g)[8], const float (&z)[8]) {
     if (act == PMG_ACT_GELU) {
 #pragma unroll

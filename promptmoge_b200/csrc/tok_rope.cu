@@ -13,8 +13,8 @@
 // heads themselves (four heads an item: 72 us and more for the first size below).  A block works on queries or on keys, so
 // that the weights stay in registers too.  Where pairs are (i, i + rot/2) a lane holds V/2 values on either side: the
 // exchange that one run of V values a lane needs took 54 us.  Two heads are worked on while the next two are on their way.
-// Measured: 38,400 tokens, 16 + 4 heads of 64, bf16: 43 us (4.6 TB/s of 6.5; 4.9 with four times the tokens; copying as much
-// takes 31), backwards 19,201 tokens, 16 + 4 heads of 128, fp16: 78 us (3.8 TB/s).
+// Measured: 38,400 tokens, 16 + 4 heads of 64, bf16: 44 us (4.5 TB/s of 6.5; copying as much takes 31), in fp32 75 to 79 us
+// (5.0 to 5.2 TB/s), backwards 124; backwards 19,201 tokens, 16 + 4 heads of 128, fp16: 78 us (3.8 TB/s).
 // Sums and norms are fp32; a value is rounded once, when it is stored.
 #include <algorithm>
 

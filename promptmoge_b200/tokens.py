@@ -7,8 +7,11 @@
 Tokens of several frames (or streams) are packed one after another along the first axis.  Tensors are CUDA tensors of
 one device, floating point, with contiguous innermost axis and otherwise any strides; kernels run on that device's
 current stream, allocate outputs and scratch from torch's allocator and never synchronise.  Sums, norms and softmax
-statistics are fp32.  What a kernel finds wrong with the data (a position outside the angle table, a wait that ran out)
-is kept in a status word per device: `check()` reads it.
+statistics are fp32.  What a kernel finds wrong with the data (a position outside the angle table, a document longer than
+max_q, a wait that ran out) is kept in a status word per device: `check()` reads it.
+
+Results carry no autograd graph, whatever their inputs require: the *_grad functions are the backward passes, and
+`token_block.TokenBlock` puts both into one.
 """
 from __future__ import annotations
 
@@ -406,8 +409,9 @@ def attention(q, k, v, cu_q, cu_k, max_q: int, max_k: int, scale: float | None =
     prefix[d] (int32) where prefix is given.  Scores: scale (default D ** -0.5) times q.k, through softcap *
     tanh(. / softcap) if softcap is not 0, less slopes[h] (fp32) * |p - j| if slopes are given.
 
-    Returns (o [Tq, Hq, D], lse [Hq, Tq] fp32).  Rows that see no key give 0 and -inf.  max_q * Hq / Hk <= 16 (token by
-    token) takes the kernel that reads the keys once for all rows."""
+    Returns (o [Tq, Hq, D], lse [Hq, Tq] fp32).  Rows that see no key give 0 and -inf; rows of no document (in front of
+    cu_q[0] and from the last offset on) are not written.  max_q * Hq / Hk <= 16 (token by token) takes the kernel that
+    reads the keys once for all rows."""
     index, dt, Tq, Tk, Hq, Hk, D = _attention_shapes(q, k)
     if _current_device() != index:
         with torch.cuda.device(index):
