@@ -28,18 +28,20 @@ using namespace tok;
 // The factor that fp16 dS carries follows from a document's largest |dO| and |V|, of its own rows alone, so that neither
 // another document nor what lies behind a length reaches it.  Blocks of the statistics take `rows` tokens of one document, and
 // leave the largest square of them for the document's CTAs to go through: those of dO at the block's first query, those of
-// V at eight places for every query of the document (where its keys are more than that, a block takes several turns).
+// V at kPlaces places for every query of the document (where its keys are more than that, a block takes several turns: one
+// query over 65,501 keys, 1131 us; with 8 places 2337).
+constexpr int kPlaces = 64;
 struct Stat {
     int q_rows, k_rows;      // tokens of a block
     int64_t q_blocks;        // blocks of queries, before those of keys
     float2* stat;            // [Hq][Tq] lse log2 e (infinite for empty rows), delta
-    float* norms;            // [Tq] of dO, [8 Tq] of V
+    float* norms;            // [Tq] of dO, [kPlaces Tq] of V
 };
 
 __host__ __device__ __forceinline__ int stat_rows(int heads) { return heads >= 16 ? 8 : 128 / heads; }
 
 __device__ __forceinline__ int64_t stat_places(const Span& s, int k_rows) {
-    return min((int64_t)(s.lk + k_rows - 1) / k_rows, 8 * (int64_t)s.lq);
+    return min((int64_t)(s.lk + k_rows - 1) / k_rows, kPlaces * (int64_t)s.lq);
 }
 
 struct Grad {
@@ -88,8 +90,8 @@ __global__ void __launch_bounds__(256)
     const int64_t places = keys ? stat_places(sp, rows) : (sp.lq + rows - 1) / rows;
     if (which < 0 || which >= places) return;
     float big = 0.0f;
+    constexpr int U = 4;                                  // rows on their way at once
     if (!keys) {
-        constexpr int U = 4;                              // rows on their way at once
         const int t0 = (int)which * rows, n = min(rows, sp.lq - t0) * a.Hq;
         for (int r0 = 0; r0 < n; r0 += kRows * U) {
             uint4 xs[U], ys[U];
@@ -130,21 +132,28 @@ __global__ void __launch_bounds__(256)
     } else {
         for (int64_t t0 = which * rows; t0 < sp.lk; t0 += places * rows) {
             const int n = (int)min((int64_t)rows, sp.lk - t0) * a.Hk;
-            for (int r = own; r - own < n; r += kRows) {
-                float sq = 0.0f;
-                if (r < n && in) {
+            for (int r0 = 0; r0 < n; r0 += kRows * U) {
+                uint4 xs[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int r = r0 + u * kRows + own;
                     const int64_t t = sp.k0 + t0 + r / a.Hk;
-                    const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const T*>(v.p) + t * v.tok + r % a.Hk * v.head + 8 * gl);
-                    const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
+                    xs[u] = make_uint4(0, 0, 0, 0);
+                    if (r < n && in) xs[u] = *reinterpret_cast<const uint4*>(static_cast<const T*>(v.p) + t * v.tok + r % a.Hk * v.head + 8 * gl);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const uint32_t xw[4] = {xs[u].x, xs[u].y, xs[u].z, xs[u].w};
+                    float sq = 0.0f;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float2 y = Elem<T>::unpack(xw[i]);
                         sq += y.x * y.x + y.y * y.y;
                     }
-                }
 #pragma unroll
-                for (int x = G / 2; x > 0; x >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, x);
-                if (sq < INFINITY) big = fmaxf(big, sq);
+                    for (int x = G / 2; x > 0; x >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, x);
+                    if (sq < INFINITY) big = fmaxf(big, sq);
+                }
             }
         }
     }
@@ -157,7 +166,7 @@ __global__ void __launch_bounds__(256)
         if (threadIdx.x == 0) {
 #pragma unroll
             for (int i = 1; i < 8; ++i) big = fmaxf(big, sm[i]);
-            st.norms[keys ? a.Tq + 8 * (int64_t)sp.q0 + which : sp.q0 + which] = big;
+            st.norms[keys ? a.Tq + kPlaces * (int64_t)sp.q0 + which : sp.q0 + which] = big;
         }
     }
 }
@@ -200,7 +209,7 @@ __device__ __forceinline__ float ds_lift(const Stat& st, const Span& sp, int64_t
         return 1.0f;
     } else {
         const int lane = threadIdx.x & 31;
-        const float *of_do = st.norms + sp.q0, *of_v = st.norms + Tq + 8 * (int64_t)sp.q0;
+        const float *of_do = st.norms + sp.q0, *of_v = st.norms + Tq + kPlaces * (int64_t)sp.q0;
         const int64_t n_do = (sp.lq + st.q_rows - 1) / st.q_rows, n_v = stat_places(sp, st.k_rows);
         float a = 0.0f, b = 0.0f;
         for (int64_t i = lane; i < n_do; i += 32) a = fmaxf(a, of_do[i]);
@@ -662,7 +671,7 @@ using namespace pmg;
 
 extern "C" size_t pmg_attention_grad_workspace_bytes(int64_t Tq, int32_t Hq) {
     if (Tq < 0 || Hq < 0) return 0;
-    return (size_t)Tq * (Hq * sizeof(float2) + 9 * sizeof(float));
+    return (size_t)Tq * (Hq * sizeof(float2) + (1 + kPlaces) * sizeof(float));
 }
 
 extern "C" int pmg_attention_grad(const void* dout, int64_t do_tok, int64_t do_head, const void* o, int64_t o_tok,
