@@ -352,8 +352,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
             const int tiles_k = w ? x.n1 : x.n0;
             const int i = x.r0 + 128 * w + (warp & 3) * 32 + lane;        // this thread's row in the document
             const int lim = last_key(a, x.sp, i);
-            // With a cap, rows behind the document count as masked: neither they nor hidden keys choose tanh's form.
-            const int warp_min = __reduce_min_sync(0xffffffffu, CAP || i < x.sp.lq ? lim : INT32_MAX);
+            const int warp_min = __reduce_min_sync(0xffffffffu, i < x.sp.lq ? lim : INT32_MAX);
             const float slope = BIAS ? a.slopes[x.head] * kLog2e : 0.0f;
             const float place = (float)(i + x.sp.lk - x.sp.lq);
             float m = -INFINITY;
@@ -367,20 +366,20 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
                 // registers to keep them.
                 float s[32];
                 bool fast = false;                        // the cap's polynomial serves (tanh_fast)
-                const bool masked = j0 + 63 > warp_min;
+                const bool masked = j0 + 63 > warp_min;   // something of these columns is hidden from a row of the warp
                 auto fetch = [&](int q) {
                     tmem_ld32(ts + 32 * q, reinterpret_cast<uint32_t*>(s));
                     tmem_wait_ld();
                 };
                 auto mask = [&](int q) {
-                    if (masked) {
+                    if (j0 + 32 * q + 31 > warp_min) {
 #pragma unroll
                         for (int k = 0; k < 32; ++k)
                             if (j0 + 32 * q + k > lim) s[k] = -INFINITY;
                     }
                 };
                 auto score = [&](int q) {                 // raw products to what the softmax takes
-                    if (CAP) tanh_scores<32>(a, s, BIAS ? !masked && tanh_fast(a, largest<32>(s)) : fast);
+                    if (CAP) tanh_scores<32>(a, s, BIAS ? j0 + 32 * q + 31 <= warp_min && tanh_fast(a, lim >= 0 ? largest<32>(s) : 0.0f) : fast);
                     if (BIAS) bias_scores<32>(s, CAP ? a.cap2 : a.scale2, slope, place - (float)(j0 + 32 * q));
                     mask(q);
                 };
@@ -400,7 +399,7 @@ __global__ void __launch_bounds__(Fwd<DP>::kThreads, Fwd<DP>::kCtas)
                 top = fmaxf(top, top2);
                 if (C::kHalves == 2) tell(top);
                 if (CAP && !BIAS) {
-                    fast = !masked && tanh_fast(a, big);
+                    fast = !masked && tanh_fast(a, lim >= 0 ? big : 0.0f);
                     score(1);
                 }
                 if (C::kHalves == 2) {

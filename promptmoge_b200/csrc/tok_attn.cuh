@@ -142,8 +142,9 @@ __device__ __forceinline__ float largest(const float (&s)[N]) {
 // Raw products to tanh(scale s / cap).  Scores mostly stay well below their cap: where `fast` (no |scale s / cap| of the
 // warp's above 1/2) a polynomial on the packed fp32 pipe takes 6 instructions a pair, against two trips through the
 // special function unit an element.  The two differ in the last bits, so the choice must not follow from what a row does not
-// see: a tile with anything masked takes the exact form (2 x 2560 tokens, capped: 119.6 -> 122.9 us; masking the products
-// before their largest is taken instead costs registers, and 125.8 to 134 us).
+// see: columns with anything masked take the exact form, and rows behind the document have no say (capped, 8 x 1200 tokens,
+// heads of 64: 126 -> 129 us; 2 x 2560 with prefix, heads of 128: 115 -> 119; masking the products before their largest is
+// taken instead costs registers, and 140 and 120).
 template <int N>
 __device__ __forceinline__ void tanh_scores(const Attn& a, float (&s)[N], bool fast) {
     if (fast) {
