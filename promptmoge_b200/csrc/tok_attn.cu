@@ -10,7 +10,7 @@
 //
 // What bounds it is neither the tensor core (30 % active for heads of 64) nor the special function unit (46 %) but the chain
 // of a step, scores -> maximum -> exponentials -> product -> next scores, with as many of them side by side as tensor memory
-// and registers hold.  Measured: 16 frames of up to 1200 tokens, 16 heads of 64, fp16: 95 us (525 TFLOP/s); 16,384 tokens,
+// and registers hold.  Measured: 16 frames of up to 1200 tokens, 16 heads of 64, fp16: 94 us (530 TFLOP/s); 16,384 tokens,
 // 9 heads: 690 (warm) to 830 TFLOP/s with heads of 64, 1190 to 1200 with heads of 128.
 #include <algorithm>
 #include <cmath>

@@ -101,23 +101,25 @@ class TokenCache:
 
     `lengths` (int32, on the device) says how many each holds and may be set, to 0 for a new stream.  `TokenBlock.step`
     raises before it writes where a stream has no room left.  It knows the lengths from its own steps and reads them anew
-    when they were set; what a replayed graph adds it does not see: a token without room then stays within its stream, on
-    the last row, and the status word tells (`tokens.check`)."""
+    when they were set (a tensor made in inference mode that was put in their place: only then).  What a replayed graph adds
+    it does not see: a token without room then stays within its stream, on the last row, and the status word tells
+    (`tokens.check`)."""
 
     def __init__(self, block: "TokenBlock", streams: int, room: int, device="cuda"):
         shape = (streams * room, block.key_heads, block.head)
         self.k, self.v = (torch.empty(shape, dtype=block.dtype, device=device) for _ in range(2))
         self.streams, self.room = streams, room
         self.offsets = torch.arange(streams + 1, dtype=torch.int32, device=device) * room
-        self.lengths = torch.zeros(streams, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):                  # so that it tells when it was set, in inference mode too
+            self.lengths = torch.zeros(streams, dtype=torch.int32, device=device)
         self._held, self._mark = [0] * streams, self._version()
 
     def _version(self):
-        return self.lengths, self.lengths._version
+        return self.lengths, None if self.lengths.is_inference() else self.lengths._version
 
     def after(self, packing: Packing) -> list:
         """The streams' lengths with the packing's tokens; ValueError where they have no room for them."""
-        known = self._mark is not None and self._mark[0] is self.lengths and self._mark[1] == self.lengths._version
+        known = self._mark is not None and self._mark[0] is self.lengths and self._mark[1] == self._version()[1]
         if not known and not torch.cuda.is_current_stream_capturing():
             self._held, self._mark = self.lengths.tolist(), self._version()
         lengths = [held + new for held, new in zip(self._held, packing.lengths)]
@@ -132,7 +134,7 @@ class TokenCache:
         at = torch.arange(total, device=self.lengths.device, dtype=torch.int32)
         stream = torch.searchsorted(packing_offsets, at, right=True) - 1
         place = at - packing_offsets[stream] + self.lengths[stream]
-        return stream * self.room + place.clamp(max=self.room - 1), place
+        return stream * self.room + place.clamp(0, self.room - 1), place
 
     def grow(self, packing: Packing, lengths: list) -> None:
         """Counts the packing's tokens in; lengths: what after() gave."""

@@ -103,3 +103,24 @@ def test_tokens_and_packing_have_to_agree():
         block.step(x, Packing([19]), TokenCache(block, 1, 32), cos, sin)
     with pytest.raises(ValueError, match="for this packing"):
         block(x[:, :64], Packing([20]), cos, sin, place)
+
+
+def test_serving_in_inference_mode():
+    from promptmoge_b200 import tokens
+    from promptmoge_b200.token_block import Packing, TokenCache
+    block = _block(causal=True)
+    cos, sin, _ = _frame()
+    x = torch.randn(4, 128, device="cuda")
+    cache = TokenCache(block, 2, 4)
+    want = block.step(x, Packing([3, 1]), cache, cos, sin)
+    with torch.inference_mode():
+        for made in (TokenCache(block, 2, 4), cache):
+            made.lengths.zero_()
+            assert torch.equal(block.step(x, Packing([3, 1]), made, cos, sin), want)
+            with pytest.raises(ValueError, match="do not fit"):
+                block.step(x[:2], Packing([2, 0]), made, cos, sin)
+            made.lengths = torch.zeros(2, dtype=torch.int32, device="cuda")
+            assert torch.equal(block.step(x, Packing([3, 1]), made, cos, sin), want)
+            with pytest.raises(ValueError, match="do not fit"):
+                block.step(x[:2], Packing([2, 0]), made, cos, sin)
+    tokens.check()
